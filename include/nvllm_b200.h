@@ -47,6 +47,7 @@ extern "C" {
 #endif
 
 #define NVLLM_BLOCK_SIZE 256 /* tokens per KV-cache block (nanovllm/engine/sequence.py:15) */
+#define NVLLM_SCALE_GROUP 16 /* slots of a block that share a scale in an 8-bit cache */
 
 /* host-side rejection codes */
 #define NVLLM_OK 0
@@ -265,6 +266,77 @@ NVLLM_API int nvllm_attention_prefill(const void* q, int64_t q_row_stride,
                          int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k,
                          int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
                          float scale, int64_t num_blocks, void* stream);
+
+/*
+ * K/V cache held in 8 bits.  No counterpart in the reference, whose cache is bf16: half the bytes that a decode step streams,
+ * twice the tokens that a GPU holds.
+ *   codes   k_cache / v_cache: e4m3 (1 byte), [num_blocks, 256, Hkv, D] contiguous, addressed as the bf16 planes are;
+ *   scales  k_scale / v_scale: fp32, [num_blocks, Hkv, 16] contiguous: one for every group of NVLLM_SCALE_GROUP slots of a
+ *           block and KV head.  Slot s, head h holds  code * scale[s / 256][h][s % 256 / 16].
+ * All four 16-byte aligned; num_blocks * 256 < 2^31.  D in {64,128}.  The readers take any positive finite scales, the stores
+ * write powers of two from 2^-64 to 2^120.
+ *
+ * nvllm_store_kvcache_fp8 stores rows as nvllm_store_kvcache does (row strides, skipped and flagged slots as there).  For every
+ * group that rows go to, and each head: f = the lowest offset in the group that is written, a = the largest finite magnitude
+ * of the rows written,
+ *     need  = the smallest power of two (from 2^-64 on) with a <= 448 * need
+ *     scale = need where f == 0, else max(need, the group's scale so far (rounded up to a power of two))
+ *     rows written: code = x / scale rounded to e4m3, nearest even;  infinities and NaN become NaN
+ *     rows of the group below f, if the scale has grown: code = code * old / scale, rounded likewise
+ * i.e. a group is filled from its first slot on, as sequences grow: a row at offset 0 starts it afresh, and rows above f that are
+ * not written are left as they are.  The rows of a launch that go to one group have to stand next to each other in
+ * slot_mapping (skipped rows may lie between them), as they do when sequences are listed one after the other; of rows with
+ * the same slot the last one stays.  Where they do not, the contents of that group (only) are unspecified.
+ */
+NVLLM_API int nvllm_store_kvcache_fp8(const void* key, int64_t key_row_stride, const void* value, int64_t value_row_stride,
+                            void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int32_t* slot_mapping,
+                            int64_t n_tokens, int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks, void* stream);
+
+/*
+ * nvllm_decode_paged over an 8-bit cache: same arguments, limits, workspace and rules, with the scales beside the codes.  Query
+ * and P are rounded to f16 (the query scaled by a power of two per head), sums are fp32.
+ */
+NVLLM_API int nvllm_decode_paged_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                           const float* k_scale, const float* v_scale, const int32_t* context_lens,
+                           const int32_t* block_tables, int64_t bt_row_stride, int32_t max_blocks,
+                           void* out, int64_t out_row_stride,
+                           int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                           float scale, int64_t num_blocks, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * nvllm_store_kvcache_fp8 of the new token of every sequence followed by nvllm_decode_paged_fp8, in one launch; cache, scales and
+ * output end up as those two would leave them.  The rules for slot_mapping are nvllm_decode_step's: the slot of position
+ * ctx_b - 1, or negative (nothing is stored); another slot is flagged and not stored; rows with ctx_b == 0 store nothing.
+ * No two sequences of a batch may have their new tokens in one group.
+ */
+NVLLM_API int nvllm_decode_step_fp8(const void* q, int64_t q_row_stride, const void* key, int64_t key_row_stride,
+                          const void* value, int64_t value_row_stride, const int32_t* slot_mapping,
+                          void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int32_t* context_lens,
+                          const int32_t* block_tables, int64_t bt_row_stride, int32_t max_blocks,
+                          void* out, int64_t out_row_stride,
+                          int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+                          float scale, int64_t num_blocks, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * What a step's launches are told about where its rows lie, built on the GPU from the requests' lengths (the device side of
+ * prepare_prefill / prepare_decode / prepare_block_tables, nanovllm/engine/model_runner.py:151-249).  Sequence b has
+ * cached_lens[b] tokens in the cache and seq_lens[b] with this step; the entries of its table row for the cached tokens,
+ * ceil(cached / 256) of them, are given.
+ *   block_tables: the entries from there to ceil(seq / 256) are taken from free_blocks, in order, sequence after sequence;
+ *       those behind become -1
+ *   cu_seqlens_q, cu_seqlens_k [batch + 1]: prefix sums of max(seq - cached, 0) and of seq
+ *   slot_mapping (int32), positions (int64) [num_rows]: of the new tokens, packed sequence after sequence; rows behind the
+ *       last one (the padding of a captured batch) get slot -1 and position 0
+ *   blocks_taken [1]: how many free blocks the step needs.  More than num_free: the entries without a block are -1, and so
+ *       are the slots in them.
+ * Lengths outside 0 to 256 * max_blocks are cut to that and flagged NVLLM_STATUS_BAD_BLOCK; more new tokens than num_rows are
+ * flagged NVLLM_STATUS_BAD_SLOT (the first num_rows are listed).  batch 1 to 4096; batch * max_blocks * 256 < 2^31.
+ * One launch; a second call with the same arguments leaves the same.
+ */
+NVLLM_API int nvllm_step_maps(const int32_t* seq_lens, const int32_t* cached_lens, int32_t batch, int32_t* block_tables,
+                    int64_t bt_row_stride, int32_t max_blocks, const int32_t* free_blocks, int32_t num_free,
+                    int32_t* cu_seqlens_q, int32_t* cu_seqlens_k, int32_t* slot_mapping, int64_t* positions,
+                    int64_t num_rows, int32_t* blocks_taken, void* stream);
 
 /*
  * Fused pre-attention step over the fused qkv activation [n_tokens, (Hq + 2*Hkv) * D] (bf16,

@@ -56,6 +56,16 @@ SIGNATURES = {
     "nvllm_decode_step_inputs_pinned": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int32,
                                                   c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                                   c_int64, c_void_p]),
+    "nvllm_store_kvcache_fp8": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                          c_int64, c_int32, c_int32, c_int64, c_void_p]),
+    "nvllm_decode_paged_fp8": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                         c_int32, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32, c_float, c_int64,
+                                         c_void_p, c_int64, c_void_p]),
+    "nvllm_decode_step_fp8": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32,
+                                        c_int32, c_int32, c_int32, c_float, c_int64, c_void_p, c_int64, c_void_p]),
+    "nvllm_step_maps": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+                                  c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "nvllm_ar_handle_bytes": (c_int64, []),
     "nvllm_ar_init": (c_int32, [c_int32, c_int32, c_int64, c_void_p]),
     "nvllm_ar_connect": (c_int32, [c_void_p]),

@@ -139,6 +139,36 @@ def prefill_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens
                                                 scale, block_tables, out)
 
 
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """``store_kvcache`` into a cache held in 8 bits: planes ``[num_blocks, 256, Hkv, D]`` of ``float8_e4m3fn`` codes and
+    fp32 scales ``[num_blocks, Hkv, 16]``, one for every 16 slots of a block and head; a code stands for code times scale.
+
+    The scale of a group is the smallest power of two (from 2^-64 on) that takes its largest value into e4m3's range.  A row
+    at a group's first slot starts it afresh; a later row that is too large for the scale makes it grow, and the rows before
+    it are coded anew.  The rows of a call that go to one group have to stand next to each other in ``slot_mapping`` (rows
+    with a negative slot, which are skipped, may lie between).  Infinities and NaN are stored as NaN.
+    """
+    (_host or _native(key)).store_kvcache_fp8(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+
+
+def decode_paged_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     context_lens: torch.Tensor, block_tables: torch.Tensor, scale: float,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """``decode_paged`` over a cache held in 8 bits (see ``store_kvcache_fp8``); q/out are ``[B, Hq, D]`` bf16."""
+    return (_host or _native(q)).decode_paged_fp8(q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, scale, out)
+
+
+def decode_step_fp8(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor, context_lens: torch.Tensor,
+                    block_tables: torch.Tensor, scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``store_kvcache_fp8(key, value, ...)`` followed by ``decode_paged_fp8`` as ONE launch, for a decode step.
+    ``slot_mapping[b]`` must be the slot of position ``context_lens[b] - 1`` or negative (nothing stored), as for
+    ``decode_step``; no two sequences may have their new tokens in one group of 16 slots."""
+    return (_host or _native(q)).decode_step_fp8(q, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, context_lens,
+                                                 block_tables, scale, out)
+
+
 def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_weight: torch.Tensor | None,
                        k_weight: torch.Tensor | None, cos_sin_cache: torch.Tensor, eps: float,
                        slot_mapping: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor,

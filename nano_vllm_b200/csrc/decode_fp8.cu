@@ -1,0 +1,779 @@
+// Paged GQA decode attention over the 8-bit cache (fp8.cuh), one query token per sequence, for sm_100a.
+//
+//   out[b,h] = sum_t softmax_t(scale q[b,h] . K[t,h/G]) V[t,h/G],  K, V = code * scale of the token's group and head
+//
+// The step variant also does what store_kvcache_fp8 does for the one new token of every sequence.
+//
+// Bound by the cached bytes, half of a bf16 cache's.  The launch is cut as the bf16 decode's is (decode_paged.cu): all
+// sequences' work units in one list, an equal stretch of it to each of two resident blocks per SM, partial results of
+// sequences that a cut divides merged by the last block to arrive.  What differs is what a tile costs:
+//   * K codes go from shared memory to registers 16 bytes a lane and become f16 pairs there (cvt, exact).  The four codes of a
+//     word are columns k = 2 tig .. and k = 2 tig + 8 .. of one m16n8k16 product: the order of the summed index is free, the
+//     query's columns follow it.
+//   * V codes go through ldmatrix.trans as pairs of neighbouring columns: a register then holds two columns of two tokens,
+//     one byte permutation away from (token, token) pairs of either column, rows gid and gid + 8 of V^T.
+//   * q is f16 too, scaled by a power of two to 2^14 <= max |q| < 2^15, so that it keeps all its bits down to 2^-29 of the
+//     largest.  The group's K scale multiplies the fp32 scores.  P is rounded to f16 (2^-11, of values up to 1), times the
+//     group's V scale over the warp's running unit: the sums O are held in that unit, which follows the scales (see `unit`).
+//   * 16 tokens share a scale, so a group lies in one warp's tile: the step variant's warp that streams the new token has
+//     its whole group at hand, codes the row, codes the rows before it anew where the scale grows, and writes them back.
+#include <cstdlib>
+
+#include "fp8.cuh"
+
+namespace nvllm {
+
+// Workspace: as nvllm_decode_paged's.  [arrival counters][partials O][partials (max, sum)]
+constexpr int kFp8CounterSlots = 16384;
+constexpr int64_t kFp8CounterBytes = static_cast<int64_t>(kFp8CounterSlots) * 4;
+constexpr int kFp8MaxCtas = 1024;
+
+struct DecodeFp8Params {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  unsigned char* k_cache;  // written by the step variant, as the scales are
+  unsigned char* v_cache;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* ctx_lens;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int max_blocks;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  int batch, hq, hkv, g;
+  float scale_log2e;
+  int64_t num_blocks;
+  const __nv_bfloat16* k_new;  // step variant
+  int64_t k_new_stride;
+  const __nv_bfloat16* v_new;
+  int64_t v_new_stride;
+  const int32_t* slot_mapping;
+  int n_ranges;
+  unsigned int* counters;  // [batch * hkv], zero between launches
+  float* ws_o;             // [n_ranges + batch][hq][D]
+  float* ws_ml;            // [n_ranges + batch][hq][2] = (running max in log2 units, sum)
+  int* status;
+};
+
+template <int D_, int TT_, int NST_, int NW_>
+struct DecodeFp8Cfg {
+  static constexpr int D = D_, TT = TT_, NST = NST_, NW = NW_;
+  static constexpr int UNIT = NW * TT;  // tokens of a work unit
+  static constexpr int MT = TT / 16;    // groups of a warp's tile
+  static constexpr int CPR = D / 16;    // 16-byte pieces of a row
+  static constexpr int TILE_BYTES = TT * D;
+  static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
+  static constexpr int WARP_BYTES = NST * STAGE_BYTES;
+  static constexpr int RING_BYTES = NW * WARP_BYTES;
+  static constexpr int SCALE_BYTES = 2 * MT * 4;  // of a stage: K's, V's
+  static constexpr int OFF_SCALES = RING_BYTES;
+  static constexpr int OFF_MERGE = OFF_SCALES + NW * NST * SCALE_BYTES;
+  static constexpr int SMEM = OFF_MERGE + NW * 8 * D * 4 + NW * 8 * 2 * 4;
+  static constexpr int KS = D / 16;  // products of a group's scores, and of its share of O
+  static_assert(TT % kScaleGroup == 0 && kBlockSize % TT == 0 && (MT & (MT - 1)) == 0 && MT <= 4, "whole groups, whole tiles");
+  static_assert((TT * CPR) % 32 == 0 && OFF_MERGE % 16 == 0, "a tile is copied evenly by a warp");
+};
+
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <int BYTES>
+__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int src_bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(BYTES), "r"(src_bytes));
+}
+__device__ __forceinline__ float ld_shared_f32(uint32_t a) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_f32(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(a), "f"(v) : "memory"); }
+__device__ __forceinline__ uint2 ld_shared8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared8(uint32_t a, const uint2& v) {
+  asm volatile("st.shared.v2.u32 [%0], {%1,%2};\n" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// Where piece c of row r of a tile lies: so that eight rows' pieces c, and two rows' pieces of one half, are in different banks.
+template <int D>
+__device__ __forceinline__ uint32_t tile_offset(int r, int c) {
+  const int x = D == 128 ? ((r & 1) << 2 | (r >> 1 & 3)) : (r >> 1 & 3);
+  return r * D + ((c ^ x) << 4);
+}
+
+struct Fp8Cursor {  // the sequence a block is working in: index, global index of its first unit, units, length
+  int b, first, units, ctx;
+  int slot;  // step variant: of the new token, -1: nothing is stored
+};
+struct Fp8Cut {  // a sequence whose units lie in several ranges: n of them, from r_first on
+  int b, r_first, n;
+};
+
+// Cost of a streamed unit over the cost of a merged partial (decode_paged.cu: the same trade).
+constexpr float kFp8SplitBalance = 16.f;
+
+template <class C, bool STEP>
+__global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeFp8Params p) {
+  constexpr int D = C::D, TT = C::TT, NST = C::NST, NW = C::NW, UNIT = C::UNIT, MT = C::MT, NT = NW * 32;
+  constexpr int QUADS = D / 4, GROUPS = NT / QUADS;  // lanes that hold a head four columns each; such groups in a block
+  constexpr int PIECES = D / 8;                      // lanes that hold a bf16 row, eight values each
+  constexpr unsigned ALL = 0xffffffffu;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int s_scan[NW];
+  __shared__ int s_start[3];
+  __shared__ int s_last_arrival[2];
+
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int gid = lane >> 2, tig = lane & 3;
+  const int kvh = blockIdx.x % p.hkv;
+  const int range = blockIdx.x / p.hkv;
+  const int ctx_cap = p.max_blocks * kBlockSize;
+  auto length_of = [&](int b) { return max(0, min(p.ctx_lens[b], ctx_cap)); };
+  auto units_of = [](int ctx) { return (ctx + UNIT - 1) / UNIT; };
+  auto write_zeros = [&](int b) {  // empty context: defined output, no cache access
+    if (b % p.n_ranges != range) return;
+    uint4* dst = reinterpret_cast<uint4*>(p.out + b * p.out_stride + static_cast<int64_t>(kvh * p.g) * D);
+    for (int i = 0; i < p.g * D / 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+  };
+
+  // ---- 1. units per sequence, block-wide scan, this block's range of the unit list ------
+  const int per_thread = (p.batch + NT - 1) / NT;
+  const int b_lo = min(tid * per_thread, p.batch), b_hi = min(b_lo + per_thread, p.batch);
+  // the first table line of every sequence on its way while the lengths are summed
+  if (p.batch <= NT && tid < p.batch) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.block_tables + tid * p.bt_stride));
+  int local = 0;
+  for (int b = b_lo; b < b_hi; ++b) {
+    const int c = length_of(b);
+    local += units_of(c);
+    if (c == 0) write_zeros(b);
+  }
+  int incl = local;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int v = __shfl_up_sync(ALL, incl, d);
+    if (lane >= d) incl += v;
+  }
+  if (lane == 31) s_scan[warp] = incl;
+  __syncthreads();
+  int before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w < warp) before += s_scan[w];
+    total += s_scan[w];
+  }
+  const int excl = before + incl - local;
+  // No more ranges than units, and where sequences are few no more than balance the two costs of a cut: a range streams
+  // total / n units and a sequence's merge reads n / batch partials.
+  const int n_ranges = max(1, min(min(p.n_ranges, total), static_cast<int>(sqrtf(kFp8SplitBalance * total * p.batch))));
+  if (range >= n_ranges || total == 0) return;  // block-uniform
+  const int per_range = total / n_ranges, longer = total - per_range * n_ranges;  // the first `longer` ranges hold one more
+  const int u0 = range * per_range + min(range, longer), u1 = u0 + per_range + (range < longer ? 1 : 0);
+  if (local > 0 && excl <= u0 && u0 < excl + local) {  // the one thread whose sequences hold unit u0
+    int first = excl;
+    for (int b = b_lo;; ++b) {
+      const int len = length_of(b), n = units_of(len);
+      if (u0 < first + n) {
+        s_start[0] = b;
+        s_start[1] = first;
+        s_start[2] = len;
+        break;
+      }
+      first += n;
+    }
+  }
+  __syncthreads();
+  auto range_of = [&](int u) {  // the range that holds global unit u
+    const int split = longer * (per_range + 1);
+    return u < split ? u / (per_range + 1) : longer + (u - split) / per_range;
+  };
+
+  auto slot_of = [&](int b) { return STEP ? p.slot_mapping[b] : -1; };
+  auto seek = [&](Fp8Cursor& c, int u) {  // u < total, so c.b stays inside the batch
+    if (u < c.first + c.units) return;
+    do {
+      c.first += c.units;
+      ++c.b;
+      c.ctx = length_of(c.b);
+      c.units = units_of(c.ctx);
+    } while (u >= c.first + c.units);
+    c.slot = slot_of(c.b);
+  };
+
+  // ---- the query: lane (gid, tig) holds columns 16 (tig + 4 j) .. + 15 of head gid ------------
+  constexpr int QW = D / 8;  // words of them
+  auto load_q = [&](uint32_t (&dst)[QW], int b) {
+    const uint4* row = reinterpret_cast<const uint4*>(p.q + b * p.q_stride + static_cast<int64_t>(kvh * p.g + gid) * D);
+#pragma unroll
+    for (int j = 0; j < D / 64; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint4 v = gid < p.g ? row[2 * (tig + 4 * j) + i] : make_uint4(0, 0, 0, 0);
+        uint32_t* to = dst + 8 * j + 4 * i;
+        to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+      }
+  };
+  uint32_t qb[QW];        // f16 pairs: word 2 ks + e is the B operand of product ks
+  float qk0 = 0.f, qk1 = 0.f;  // what takes the products of heads 2 tig and 2 tig + 1 to log2 units, K's scale apart
+  auto take_q = [&](const uint32_t (&raw)[QW]) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < QW; ++i) m = max_finite2(m, raw[i]);
+    m = max(m & 0xffffu, m >> 16);
+    m = max(m, __shfl_xor_sync(ALL, m, 1));
+    m = max(m, __shfl_xor_sync(ALL, m, 2));
+    const int e = max(static_cast<int>(m >> 7), 20) - 127;  // 2^e <= max |q| < 2^(e + 1)
+    const float f = power_of_two(14 - e);
+#pragma unroll
+    for (int i = 0; i < QW; ++i) qb[i] = pack_f16x2(__uint_as_float(raw[i] << 16) * f, __uint_as_float(raw[i] & 0xffff0000u) * f);
+    const float back = p.scale_log2e * power_of_two(e - 14);
+    qk0 = __shfl_sync(ALL, back, 8 * tig);
+    qk1 = __shfl_sync(ALL, back, 8 * tig + 4);
+  };
+
+  // ---- tiles: the warp's ring ------------------------------------------------------------------
+  const uint32_t warp_smem = smem_u32(smem) + warp * C::WARP_BYTES;
+  const uint32_t warp_scales = smem_u32(smem) + C::OFF_SCALES + warp * NST * C::SCALE_BYTES;
+  const int64_t row_bytes = static_cast<int64_t>(p.hkv) * D;
+  const bool is_v = lane >= 16;
+  const int sub = (lane & 15) / PIECES, piece = lane % PIECES;
+
+  int bad = 0;
+  unsigned fresh = 0;     // step variant: stages whose tile holds the new token's row
+  uint4 new_row[NST];     // and its row, K in the lower half of the warp, V in the upper: eight values a lane
+  Fp8Cursor cc, pc;       // compute side; load side, NST - 1 units ahead
+  auto load_unit = [&](int j) {  // the range's j-th unit
+    const int stage = j % NST;
+    seek(pc, u0 + j);
+    fresh &= ~(1u << stage);
+    const int t0 = (u0 + j - pc.first) * UNIT + warp * TT;
+    if (t0 >= pc.ctx) return;
+    int64_t blk = p.block_tables[pc.b * p.bt_stride + t0 / kBlockSize];
+    const bool blk_ok = blk >= 0 && blk < p.num_blocks;
+    if (!blk_ok) {
+      bad |= NVLLM_STATUS_BAD_BLOCK;
+      blk = 0;
+    }
+    const int64_t slot0 = blk * kBlockSize + t0 % kBlockSize;
+    int end = pc.ctx;  // rows from here on are zeros
+    if (STEP && pc.ctx - 1 < t0 + TT && pc.slot >= 0) {
+      if (blk_ok && pc.slot == slot0 + (pc.ctx - 1 - t0)) {
+        end = pc.ctx - 1;
+        fresh |= 1u << stage;
+        const __nv_bfloat16* src = (is_v ? p.v_new + pc.b * p.v_new_stride : p.k_new + pc.b * p.k_new_stride) + kvh * D + piece * 8;
+        const uint4 x = sub == 0 ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int s = 0; s < NST; ++s)
+          if (s == stage) new_row[s] = x;
+      } else {
+        bad |= NVLLM_STATUS_BAD_SLOT;
+      }
+    }
+    const uint32_t kdst = warp_smem + stage * C::STAGE_BYTES;
+#pragma unroll
+    for (int it = 0; it < TT * C::CPR / 32; ++it) {
+      const int idx = it * 32 + lane;
+      const int r = idx / C::CPR, col = idx % C::CPR;
+      const int bytes = blk_ok && t0 + r < end ? 16 : 0;
+      const int64_t off = bytes ? (slot0 + r) * row_bytes + kvh * D + col * 16 : 0;
+      const uint32_t dst = kdst + tile_offset<D>(r, col);
+      cp_async16(dst, p.k_cache + off, bytes);
+      cp_async16(dst + C::TILE_BYTES, p.v_cache + off, bytes);
+    }
+    if (lane < 2) {
+      const int64_t at = (blk * p.hkv + kvh) * kGroups + t0 % kBlockSize / kScaleGroup;
+      cp_async_small<MT * 4>(warp_scales + stage * C::SCALE_BYTES + lane * MT * 4, (lane ? p.v_scale : p.k_scale) + at, blk_ok ? MT * 4 : 0);
+    }
+  };
+
+  cc.b = s_start[0];
+  cc.first = s_start[1];
+  cc.ctx = s_start[2];
+  cc.units = units_of(cc.ctx);
+  cc.slot = slot_of(cc.b);
+  pc = cc;
+  uint32_t qn[QW];  // the next sequence's query, fetched early
+  {
+    uint32_t raw[QW];
+    load_q(raw, cc.b);
+    const int n_units0 = u1 - u0;
+#pragma unroll
+    for (int j = 0; j < NST - 1; ++j) {
+      if (j < n_units0) load_unit(j);
+      cp_async_commit();
+    }
+    take_q(raw);
+  }
+  int qn_b = min(cc.b + 1, p.batch - 1);
+  load_q(qn, qn_b);
+  const int n_units = u1 - u0;
+
+  float o[C::KS][4];     // columns 16 c + 2 gid (and + 1 in [2], [3]) of heads 2 tig ([0], [2]) and 2 tig + 1, in units of `unit`
+  float m0, m1, l0, l1;  // heads 2 tig and 2 tig + 1
+  // The power of two that O is held in (the same for all lanes of the warp): a group's P goes into its product times
+  // vscale / unit <= 1.  It grows at once to the largest scale of a tile and shrinks where that is 16 times smaller, so that
+  // a group's P loses four bits of f16's range at most; never by more than 2^-60, which keeps O finite whatever the scales.
+  float unit;
+  auto reset_state = [&]() {
+#pragma unroll
+    for (int c = 0; c < C::KS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
+    m0 = m1 = -INFINITY;
+    l0 = l1 = 0.f;
+    unit = 0.f;
+  };
+  reset_state();
+
+  float* sm_o = reinterpret_cast<float*>(smem + C::OFF_MERGE);  // [NW][8][D]
+  float* sm_ml = sm_o + NW * 8 * D;                             // [NW][8][2]
+  auto add_scaled = [](float4& acc, const float4& v, float f) {
+    acc.x += v.x * f;
+    acc.y += v.y * f;
+    acc.z += v.z * f;
+    acc.w += v.w * f;
+  };
+  auto write_quad = [&](int b, int h, int d4, const float4& acc, float L) {
+    const float inv = L > 0.f ? 1.f / L : L;  // no key: zeros; a sum that is NaN stays one
+    *reinterpret_cast<uint2*>(p.out + b * p.out_stride + static_cast<int64_t>(kvh * p.g + h) * D + d4 * 4) =
+        make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+  };
+
+  Fp8Cut cut0{}, cut1{};  // this range's sequences that other ranges share
+  int n_cut = 0;
+
+  // Leaves sequence cc.b: merges the NW warps' states and writes the output row or a partial.
+  auto flush = [&]() {
+#pragma unroll
+    for (int sh = 4; sh <= 16; sh <<= 1) {
+      l0 += __shfl_xor_sync(ALL, l0, sh);
+      l1 += __shfl_xor_sync(ALL, l1, sh);
+    }
+    __syncthreads();  // the previous merge has been read by everyone
+#pragma unroll
+    for (int c = 0; c < C::KS; ++c) {
+      float* dst = sm_o + (warp * 8 + 2 * tig) * D + c * 16 + 2 * gid;
+      *reinterpret_cast<float2*>(dst) = make_float2(o[c][0] * unit, o[c][2] * unit);
+      *reinterpret_cast<float2*>(dst + D) = make_float2(o[c][1] * unit, o[c][3] * unit);
+    }
+    if (gid == 0) {
+      *reinterpret_cast<float4*>(sm_ml + (warp * 8 + 2 * tig) * 2) = make_float4(m0, l0, m1, l1);
+    }
+    const int r_first = range_of(cc.first), r_last = range_of(cc.first + cc.units - 1);
+    const int n_parts = r_last - r_first + 1;  // ranges that hold a piece of this sequence
+    __syncthreads();
+    for (int quad = tid; quad < p.g * QUADS; quad += NT) {  // four columns of a head per thread
+      const int h = quad / QUADS, d4 = quad % QUADS;
+      float m[NW], mm = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        m[w] = sm_ml[(w * 8 + h) * 2];
+        mm = fmaxf(mm, m[w]);
+      }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = m[w] == -INFINITY ? 0.f : fast_exp2(m[w] - mm);
+        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * 8 + h) * D + d4 * 4);
+        L += sm_ml[(w * 8 + h) * 2 + 1] * f;
+        add_scaled(acc, v, f);
+      }
+      if (n_parts == 1) {
+        write_quad(cc.b, h, d4, acc, L);
+      } else {
+        // partial slot range + b: strictly increasing along the (range, sequence) pieces of the list
+        const int64_t row = static_cast<int64_t>(range + cc.b) * p.hq + kvh * p.g + h;
+        *reinterpret_cast<float4*>(p.ws_o + row * D + d4 * 4) = acc;
+        if (d4 == 0) *reinterpret_cast<float2*>(p.ws_ml + row * 2) = make_float2(mm, L);
+      }
+    }
+    if (n_parts > 1) {  // block-uniform
+      if (n_cut == 0) cut0 = {cc.b, r_first, n_parts};
+      else cut1 = {cc.b, r_first, n_parts};
+      ++n_cut;
+    }
+  };
+
+  // Merges the partials of a cut sequence, all of which are in the workspace, and writes its rows: QUADS lanes take a head,
+  // four columns each, and the statistics of a part each; eight parts to a trip; lane groups left over split the parts.
+  auto merge_cut = [&](const Fp8Cut& c) {
+    constexpr int AHEAD = 8;
+    const int group = tid / QUADS, gl = tid % QUADS;
+    const int n_split = max(1, GROUPS / p.g);
+    for (int h0 = 0; h0 < p.g; h0 += GROUPS) {
+      const bool narrow = p.g < GROUPS;
+      const int split = narrow ? group / p.g : 0, head = narrow ? group % p.g : min(h0 + group, p.g - 1);
+      const bool active = narrow ? split < n_split : h0 + group < p.g;
+      const int64_t row0 = static_cast<int64_t>(c.r_first + c.b) * p.hq + kvh * p.g + head;
+      auto row_of = [&](int j) { return __ldcg(reinterpret_cast<const float4*>(p.ws_o + (row0 + static_cast<int64_t>(j) * p.hq) * D) + gl); };
+      float mm = -INFINITY, L = 0.f;
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      auto rebase = [&](float m_new) {
+        const float keep = mm == -INFINITY ? 0.f : fast_exp2(mm - m_new);
+        L *= keep;
+        acc.x *= keep;
+        acc.y *= keep;
+        acc.z *= keep;
+        acc.w *= keep;
+        mm = m_new;
+      };
+      for (int j0 = 0; j0 < c.n; j0 += QUADS * n_split) {  // block-uniform; a group's parts are split + n_split * k
+        float4 rows[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const int j = j0 + k * n_split + split;
+          if (active && j < c.n) rows[k] = row_of(j);
+        }
+        const int mine = j0 + gl * n_split + split;
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (active && mine < c.n)
+          ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (row0 + static_cast<int64_t>(mine) * p.hq) * 2));
+        float m_new = fmaxf(mm, ml.x);
+#pragma unroll
+        for (int sh = QUADS / 2; sh > 0; sh >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(ALL, m_new, sh));
+        rebase(m_new);
+        const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - m_new);
+        float sum = ml.y * f;
+#pragma unroll
+        for (int sh = QUADS / 2; sh > 0; sh >>= 1) sum += __shfl_xor_sync(ALL, sum, sh);
+        L += sum;
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const float fk = __shfl_sync(ALL, f, k, QUADS);
+          if (active && j0 + k * n_split + split < c.n) add_scaled(acc, rows[k], fk);
+        }
+        const int n_here = min(QUADS, (c.n - j0 + n_split - 1) / n_split);
+#pragma unroll 1
+        for (int k0 = AHEAD; k0 < n_here; k0 += AHEAD) {
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const int j = j0 + (k0 + k) * n_split + split;
+            if (active && j < c.n) rows[k] = row_of(j);
+          }
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k) {
+            const float fk = __shfl_sync(ALL, f, k0 + k, QUADS);
+            if (active && j0 + (k0 + k) * n_split + split < c.n) add_scaled(acc, rows[k], fk);
+          }
+        }
+      }
+      if (n_split > 1) {  // block-uniform
+        float* patch = sm_o + group * (D + 4);
+        if (active && split > 0) {
+          *reinterpret_cast<float4*>(patch + gl * 4) = acc;
+          if (gl == 0) *reinterpret_cast<float2*>(patch + D) = make_float2(mm, L);
+        }
+        __syncthreads();
+        if (active && split == 0)
+          for (int k = 1; k < n_split; ++k) {
+            const float* other = sm_o + (group + k * p.g) * (D + 4);
+            const float2 ml = *reinterpret_cast<const float2*>(other + D);
+            rebase(fmaxf(mm, ml.x));
+            const float f = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - mm);
+            L += ml.y * f;
+            add_scaled(acc, *reinterpret_cast<const float4*>(other + gl * 4), f);
+          }
+        __syncthreads();
+      }
+      if (active && split == 0) write_quad(c.b, head, gl, acc, L);
+    }
+    if (tid == 0) p.counters[c.b * p.hkv + kvh] = 0u;  // ready for the next launch
+  };
+
+  // ---- 2. stream the range ------------------------------------------------------------------
+  for (int i = 0;; ++i) {
+    const int u = u0 + i;
+    if (i == n_units || u >= cc.first + cc.units) {  // block-uniform: the range leaves sequence cc.b
+      flush();
+      if (i == n_units) break;
+      seek(cc, u);
+      reset_state();
+      if (qn_b != cc.b) load_q(qn, cc.b);  // empty sequences in between
+      take_q(qn);
+      qn_b = min(cc.b + 1, p.batch - 1);
+      load_q(qn, qn_b);
+    }
+    cp_async_wait<NST - 2>();
+    if (!STEP) __syncthreads();  // the warps' tiles of a unit are fetched together
+    else __syncwarp();
+    if (i + NST - 1 < n_units) load_unit(i + NST - 1);
+    cp_async_commit();
+
+    const int t0 = (u - cc.first) * UNIT + warp * TT;
+    if (t0 >= cc.ctx) continue;
+    const uint32_t kbase = warp_smem + (i % NST) * C::STAGE_BYTES, vbase = kbase + C::TILE_BYTES;
+    const uint32_t scales = warp_scales + (i % NST) * C::SCALE_BYTES;
+
+    if (STEP && (fresh >> (i % NST) & 1u)) {  // the new token's row: to the tile and to the cache, its group with it
+      const int r = cc.ctx - 1 - t0, r0 = r & ~(kScaleGroup - 1);  // row of the tile; first of its group
+      uint4 x = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int s = 0; s < NST; ++s)
+        if (s == i % NST) x = new_row[s];
+      uint32_t most = max_finite2(max_finite2(max_finite2(max_finite2(0, x.x), x.y), x.z), x.w);
+      most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(ALL, most, d));
+      const uint32_t scale_smem = scales + (is_v ? MT * 4 : 0) + (r0 / kScaleGroup) * 4;
+      const float old = ld_shared_f32(scale_smem);
+      const int e = r > r0 ? max(exponent_for(most), exponent_of(old)) : exponent_for(most);
+      const float now = power_of_two(e), inv = power_of_two(-e);
+      const uint32_t tile = is_v ? vbase : kbase;
+      unsigned char* to = (is_v ? p.v_cache : p.k_cache) + (static_cast<int64_t>(cc.slot) - r) * row_bytes + kvh * D + piece * 8;
+      auto in_tile = [&](int row) { return tile + tile_offset<D>(row, piece >> 1) + (piece & 1) * 8; };
+      if (r > r0 && now != old) {
+        const float ratio = old * inv;
+#pragma unroll 1
+        for (int row = r0 + sub; row < r; row += 16 / PIECES) {
+          uint2 c = ld_shared8(in_tile(row));
+          c = make_uint2(recode4(c.x, ratio), recode4(c.y, ratio));
+          st_shared8(in_tile(row), c);
+          *reinterpret_cast<uint2*>(to + row * row_bytes) = c;
+        }
+      }
+      if (sub == 0) {
+        const uint2 c = encode8(x, inv);
+        st_shared8(in_tile(r), c);
+        *reinterpret_cast<uint2*>(to + r * row_bytes) = c;
+      }
+      __syncwarp();
+      if ((lane & 15) == 0) {
+        st_shared_f32(scale_smem, now);
+        const int64_t slot = cc.slot;
+        (is_v ? p.v_scale : p.k_scale)[(slot / kBlockSize * p.hkv + kvh) * kGroups + slot % kBlockSize / kScaleGroup] = now;
+      }
+      __syncwarp();
+    }
+
+    // S^T = K Q^T, in log2 units
+    float s[MT][4], vs[MT], most_vs = 0.f;
+    const bool tail = t0 + TT > cc.ctx;
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        const int ra = mt * 16 + gid;
+        const uint4 a = ld_shared16(kbase + tile_offset<D>(ra, tig + 4 * j)), b = ld_shared16(kbase + tile_offset<D>(ra + 8, tig + 4 * j));
+        const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          mma_f16_16816(s[mt], f16x2_of_low(wa[w]), f16x2_of_low(wb[w]), f16x2_of_high(wa[w]), f16x2_of_high(wb[w]),
+                        qb[8 * j + 2 * w], qb[8 * j + 2 * w + 1]);
+      }
+      const float ks = ld_shared_f32(scales + mt * 4);
+      vs[mt] = t0 + mt * 16 < cc.ctx ? ld_shared_f32(scales + (MT + mt) * 4) : 0.f;  // a group past the end: whatever is there
+      most_vs = fmaxf(most_vs, vs[mt]);
+      const float f0 = qk0 * ks, f1 = qk1 * ks;
+      s[mt][0] *= f0;
+      s[mt][1] *= f1;
+      s[mt][2] *= f0;
+      s[mt][3] *= f1;
+      if (tail) {
+        const int tr = t0 + mt * 16 + gid;
+        if (tr >= cc.ctx) s[mt][0] = s[mt][1] = -INFINITY;
+        if (tr + 8 >= cc.ctx) s[mt][2] = s[mt][3] = -INFINITY;
+      }
+      mx0 = fmaxf(mx0, fmaxf(s[mt][0], s[mt][2]));
+      mx1 = fmaxf(mx1, fmaxf(s[mt][1], s[mt][3]));
+    }
+#pragma unroll
+    for (int sh = 4; sh <= 16; sh <<= 1) {
+      mx0 = fmaxf(mx0, __shfl_xor_sync(ALL, mx0, sh));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(ALL, mx1, sh));
+    }
+    const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+    float alpha0 = fast_exp2(m0 - mn0), alpha1 = fast_exp2(m1 - mn1);
+    l0 *= alpha0;
+    l1 *= alpha1;
+    if (most_vs > unit || most_vs * 16.f < unit) {
+      const float next = fmaxf(most_vs, unit * 0x1p-60f), change = unit > 0.f ? unit / next : 0.f;
+      alpha0 *= change;
+      alpha1 *= change;
+      unit = next;
+    }
+    const float per_unit = unit > 0.f ? 1.f / unit : 0.f;
+    m0 = mn0;
+    m1 = mn1;
+    uint32_t pb[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      s[mt][0] = fast_exp2(s[mt][0] - mn0);
+      s[mt][1] = fast_exp2(s[mt][1] - mn1);
+      s[mt][2] = fast_exp2(s[mt][2] - mn0);
+      s[mt][3] = fast_exp2(s[mt][3] - mn1);
+      l0 += s[mt][0] + s[mt][2];  // per-lane partial sums; reduced over the token lanes at the flush
+      l1 += s[mt][1] + s[mt][3];
+      const float f = vs[mt] * per_unit;
+      pb[mt][0] = movmatrix_trans(pack_f16x2(s[mt][0] * f, s[mt][1] * f));
+      pb[mt][1] = movmatrix_trans(pack_f16x2(s[mt][2] * f, s[mt][3] * f));
+    }
+    if (__any_sync(ALL, alpha0 != 1.f || alpha1 != 1.f)) {
+#pragma unroll
+      for (int c = 0; c < C::KS; ++c) {
+        o[c][0] *= alpha0;
+        o[c][1] *= alpha1;
+        o[c][2] *= alpha0;
+        o[c][3] *= alpha1;
+      }
+    }
+
+    // O^T += V^T P^T
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int c = 0; c < C::KS; c += 2) {
+        const int r = mt * 16 + (lane & 15);
+        uint32_t v[4];  // tokens 0-7 and 8-15 of columns 16 c .., then of 16 (c + 1) ..
+        ldmatrix_x4_trans(v[0], v[1], v[2], v[3], vbase + tile_offset<D>(r, c + (lane >> 4)));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t lo = __byte_perm(v[2 * k], 0, 0x3120), hi = __byte_perm(v[2 * k + 1], 0, 0x3120);
+          mma_f16_16816(o[c + k], f16x2_of_low(lo), f16x2_of_high(lo), f16x2_of_low(hi), f16x2_of_high(hi), pb[mt][0], pb[mt][1]);
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  if (bad && lane == 0) atomicOr(p.status, bad);
+  if (n_cut == 0) return;  // block-uniform
+  __syncthreads();         // every thread's partials are written
+  if (tid < n_cut) {
+    const Fp8Cut& c = tid == 0 ? cut0 : cut1;
+    unsigned int arrived;  // releases the block's partials (the barrier ordered them before), acquires the others'
+    asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;"
+                 : "=r"(arrived) : "l"(p.counters + c.b * p.hkv + kvh) : "memory");
+    s_last_arrival[tid] = arrived == static_cast<unsigned int>(c.n - 1);
+  }
+  __syncthreads();
+  if (s_last_arrival[0]) merge_cut(cut0);
+  if (n_cut > 1 && s_last_arrival[1]) merge_cut(cut1);
+}
+
+// ---- host side -------------------------------------------------------------------------
+
+template <class C>
+static int launch_decode_fp8(const DecodeFp8Params& p, cudaStream_t stream) {
+  static bool attr_set[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
+    for (auto kernel : {decode_fp8_kernel<C, false>, decode_fp8_kernel<C, true>}) {
+      const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+      if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "decode_fp8: cannot reserve %d bytes of shared memory: %s", C::SMEM, cudaGetErrorString(e));
+    }
+    if (dev >= 0 && dev < 64) attr_set[dev] = true;
+  }
+  return launch_kernel("decode_fp8", p.k_new ? decode_fp8_kernel<C, true> : decode_fp8_kernel<C, false>,
+                       dim3(static_cast<unsigned>(p.n_ranges * p.hkv)), dim3(C::NW * 32), C::SMEM, stream, p);
+}
+
+struct Fp8Cache {
+  void *k, *v;
+  float *k_scale, *v_scale;
+};
+
+static int decode_fp8_common(const char* who, const void* q, int64_t q_row_stride, const void* k_new, int64_t k_new_row_stride,
+                             const void* v_new, int64_t v_new_row_stride, const int32_t* slot_mapping, bool with_store,
+                             const Fp8Cache& cache, const int32_t* context_lens, const int32_t* block_tables, int64_t bt_row_stride,
+                             int32_t max_blocks, void* out, int64_t out_row_stride, int32_t batch, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim, float scale, int64_t num_blocks, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
+  const int64_t need = nvllm_decode_workspace_bytes(batch, max_blocks, num_q_heads, num_kv_heads, head_dim);
+  if (need < 0) return static_cast<int>(need);
+  if (batch == 0) return NVLLM_OK;
+  const int rc = check_fp8_planes(who, cache.k, cache.v, cache.k_scale, cache.v_scale, num_kv_heads, head_dim, num_blocks);
+  if (rc) return rc;
+  if (!q || !context_lens || !block_tables || !out) return fail(NVLLM_E_NULL, "%s: NULL pointer argument", who);
+  const int64_t qrow = static_cast<int64_t>(num_q_heads) * head_dim, kvrow = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (q_row_stride < qrow || out_row_stride < qrow || bt_row_stride < max_blocks)
+    return fail(NVLLM_E_GEOMETRY, "%s: a row stride is smaller than its row", who);
+  if (q_row_stride % 8 || out_row_stride % 8 || !aligned16(q) || !aligned16(out))
+    return fail(NVLLM_E_ALIGN, "%s: q/out pointers and row strides must be 16-byte aligned", who);
+  if (with_store) {
+    if (!k_new || !v_new || !slot_mapping) return fail(NVLLM_E_NULL, "%s: NULL pointer argument", who);
+    if (k_new_row_stride < kvrow || v_new_row_stride < kvrow)
+      return fail(NVLLM_E_GEOMETRY, "%s: key/value row stride smaller than Hkv*D", who);
+    if (k_new_row_stride % 8 || v_new_row_stride % 8 || !aligned16(k_new) || !aligned16(v_new))
+      return fail(NVLLM_E_ALIGN, "%s: key/value pointers and row strides must be 16-byte aligned", who);
+  }
+  if (!workspace || workspace_bytes < need)
+    return fail(NVLLM_E_WORKSPACE, "%s: workspace of %lld bytes needed, %lld given", who, (long long)need,
+                (long long)(workspace ? workspace_bytes : 0));
+  if (!aligned16(workspace)) return fail(NVLLM_E_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  DecodeFp8Params p;
+  p.status = status_word();
+  if (!p.status) return fail(NVLLM_E_NO_DEVICE, "%s: no CUDA device is usable", who);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_row_stride;
+  p.k_cache = static_cast<unsigned char*>(cache.k);
+  p.v_cache = static_cast<unsigned char*>(cache.v);
+  p.k_scale = cache.k_scale;
+  p.v_scale = cache.v_scale;
+  p.ctx_lens = context_lens;
+  p.block_tables = block_tables;
+  p.bt_stride = bt_row_stride;
+  p.max_blocks = max_blocks;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride = out_row_stride;
+  p.batch = batch;
+  p.hq = num_q_heads;
+  p.hkv = num_kv_heads;
+  p.g = num_q_heads / num_kv_heads;
+  p.scale_log2e = scale * 1.4426950408889634f;
+  p.num_blocks = num_blocks;
+  p.k_new = with_store ? static_cast<const __nv_bfloat16*>(k_new) : nullptr;
+  p.k_new_stride = k_new_row_stride;
+  p.v_new = with_store ? static_cast<const __nv_bfloat16*>(v_new) : nullptr;
+  p.v_new_stride = v_new_row_stride;
+  p.slot_mapping = slot_mapping;
+  auto ranges_for = [&](int ctas) { return ctas / num_kv_heads > 1 ? ctas / num_kv_heads : 1; };
+  const int ctas = 2 * num_sms();
+  p.n_ranges = ranges_for(ctas > 0 && ctas <= kFp8MaxCtas ? ctas : kFp8MaxCtas);
+  const int64_t rows = (static_cast<int64_t>(ranges_for(kFp8MaxCtas)) + batch) * num_q_heads;
+  p.counters = static_cast<unsigned int*>(workspace);
+  p.ws_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kFp8CounterBytes);
+  p.ws_ml = p.ws_o + rows * head_dim;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128) return launch_decode_fp8<DecodeFp8Cfg<128, 32, 3, 4>>(p, st);
+  return launch_decode_fp8<DecodeFp8Cfg<64, 32, 4, 4>>(p, st);
+}
+
+}  // namespace nvllm
+
+extern "C" int nvllm_decode_paged_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                      const float* k_scale, const float* v_scale, const int32_t* context_lens,
+                                      const int32_t* block_tables, int64_t bt_row_stride, int32_t max_blocks, void* out,
+                                      int64_t out_row_stride, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                      int32_t head_dim, float scale, int64_t num_blocks, void* workspace,
+                                      int64_t workspace_bytes, void* stream) {
+  const nvllm::Fp8Cache cache = {const_cast<void*>(k_cache), const_cast<void*>(v_cache), const_cast<float*>(k_scale),
+                                 const_cast<float*>(v_scale)};
+  return nvllm::decode_fp8_common("decode_paged_fp8", q, q_row_stride, nullptr, 0, nullptr, 0, nullptr, false, cache, context_lens,
+                                  block_tables, bt_row_stride, max_blocks, out, out_row_stride, batch, num_q_heads, num_kv_heads,
+                                  head_dim, scale, num_blocks, workspace, workspace_bytes, stream);
+}
+
+extern "C" int nvllm_decode_step_fp8(const void* q, int64_t q_row_stride, const void* key, int64_t key_row_stride,
+                                     const void* value, int64_t value_row_stride, const int32_t* slot_mapping, void* k_cache,
+                                     void* v_cache, float* k_scale, float* v_scale, const int32_t* context_lens,
+                                     const int32_t* block_tables, int64_t bt_row_stride, int32_t max_blocks, void* out,
+                                     int64_t out_row_stride, int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, float scale, int64_t num_blocks, void* workspace, int64_t workspace_bytes,
+                                     void* stream) {
+  return nvllm::decode_fp8_common("decode_step_fp8", q, q_row_stride, key, key_row_stride, value, value_row_stride, slot_mapping,
+                                  true, {k_cache, v_cache, k_scale, v_scale}, context_lens, block_tables, bt_row_stride, max_blocks,
+                                  out, out_row_stride, batch, num_q_heads, num_kv_heads, head_dim, scale, num_blocks, workspace,
+                                  workspace_bytes, stream);
+}

@@ -1,0 +1,94 @@
+// The 8-bit K/V cache: e4m3 codes and one scale for every 16 slots of a block and KV head.
+//
+// A code c of slot s, head h stands for value(c) * scale[s / 256][h][s % 256 / 16].  Scales that the stores write are powers
+// of two: a floating-point code loses nothing by that (the same four significant bits in every binade, 448 / 2^-6 from end to
+// end), the quotient x / scale is exact, so that a row is rounded once, by its code, and a group whose scale has to grow is
+// coded anew without a second rounding except of values that fall below 2^-6 of the new scale.  Readers take any finite scale.
+#pragma once
+
+#include "common.cuh"
+
+namespace nvllm {
+
+constexpr int kScaleGroup = NVLLM_SCALE_GROUP;        // slots that share a scale
+constexpr int kGroups = kBlockSize / kScaleGroup;     // scales of a block and head
+constexpr int kMinExponent = -64, kMaxExponent = 120;  // of a scale that a store writes: 448 * 2^120 is the first beyond bf16
+static_assert(kScaleGroup == 16 && kGroups == 16, "a half warp holds a group's rows or a block's scales");
+
+// Argument checks shared by the entry points that take such a cache.
+inline int check_fp8_planes(const char* who, const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                            int32_t num_kv_heads, int32_t head_dim, int64_t num_blocks) {
+  if (head_dim != 64 && head_dim != 128) return fail(NVLLM_E_GEOMETRY, "%s: head_dim=%d unsupported (64 or 128)", who, head_dim);
+  if (num_kv_heads <= 0) return fail(NVLLM_E_GEOMETRY, "%s: Hkv=%d must be positive", who, num_kv_heads);
+  if (num_blocks <= 0 || num_blocks > 0x7fffffffLL / kBlockSize)
+    return fail(NVLLM_E_GEOMETRY, "%s: num_blocks=%lld must be positive and its slots fit 32 bits", who, (long long)num_blocks);
+  if (!k_cache || !v_cache || !k_scale || !v_scale) return fail(NVLLM_E_NULL, "%s: NULL pointer argument", who);
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_scale) || !aligned16(v_scale))
+    return fail(NVLLM_E_ALIGN, "%s: cache and scale pointers must be 16-byte aligned", who);
+  return NVLLM_OK;
+}
+
+#ifdef __CUDACC__
+
+// Two values to two codes, `lo` in the low byte: nearest, ties to even, beyond 448 to 448, NaN to 0x7f.
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Two codes (the low or the high half of x) to f16, exactly: every e4m3 value is one of f16.
+__device__ __forceinline__ uint32_t f16x2_of_low(uint32_t x) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t}" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2_of_high(uint32_t x) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, b;\n\t}" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ float2 float2_of_f16x2(uint32_t x) {
+  float2 r;
+  asm("{\n\t.reg .f16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.f32.f16 %0, a;\n\tcvt.f32.f16 %1, b;\n\t}" : "=f"(r.x), "=f"(r.y) : "r"(x));
+  return r;
+}
+
+__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
+
+// Largest magnitude (as bf16 bits) of two bf16 and `m`, infinities and NaN left out.
+__device__ __forceinline__ uint32_t max_finite2(uint32_t m, uint32_t x) {
+  x &= 0x7fff7fffu;
+  return __vmaxu2(m, x & ~__vcmpgeu2(x, 0x7f807f80u));
+}
+// Exponent of the smallest scale s that takes a magnitude of these bf16 bits: |x| <= 448 s, 448 = 1.75 * 2^8.
+__device__ __forceinline__ int exponent_for(uint32_t bf16_bits) {
+  const int e = static_cast<int>(bf16_bits >> 7) - 127 - 8 + ((bf16_bits & 0x7fu) > 0x60u);
+  return max(kMinExponent, e);
+}
+// Exponent of a scale read from memory, of the next power of two if it is none.
+__device__ __forceinline__ int exponent_of(float scale) {
+  const uint32_t b = __float_as_uint(scale);
+  return min(kMaxExponent, max(kMinExponent, static_cast<int>(b >> 23 & 255u) - 127 + ((b & 0x7fffffu) != 0)));
+}
+
+// Eight bf16 over a scale of 1 / inv to eight codes; what is not finite becomes NaN (e4m3 has no infinities).
+__device__ __forceinline__ uint2 encode8(const uint4& x, float inv) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  uint32_t h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo = __uint_as_float(w[i] << 16) * inv, hi = __uint_as_float(w[i] & 0xffff0000u) * inv;
+    lo = fabsf(lo) <= 448.f ? lo : NAN;
+    hi = fabsf(hi) <= 448.f ? hi : NAN;
+    h[i] = e4m3x2(lo, hi);
+  }
+  return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+}
+// Four codes whose scale changes by `ratio` <= 1.
+__device__ __forceinline__ uint32_t recode4(uint32_t c, float ratio) {
+  const float2 a = float2_of_f16x2(f16x2_of_low(c)), b = float2_of_f16x2(f16x2_of_high(c));
+  return e4m3x2(a.x * ratio, a.y * ratio) | e4m3x2(b.x * ratio, b.y * ratio) << 16;
+}
+
+#endif  // __CUDACC__
+}  // namespace nvllm

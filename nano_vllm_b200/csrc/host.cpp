@@ -25,6 +25,7 @@
 #include <limits>
 #include <memory>
 #include <string>
+#include <utility>
 #include <vector>
 
 #include "../../include/nvllm_b200.h"
@@ -53,6 +54,10 @@ struct Api {
   decltype(&nvllm_sample_tokens) sample_tokens;
   decltype(&nvllm_sample_candidates) sample_candidates;
   decltype(&nvllm_decode_step_inputs_pinned) decode_step_inputs_pinned;
+  decltype(&nvllm_store_kvcache_fp8) store_kvcache_fp8;
+  decltype(&nvllm_decode_paged_fp8) decode_paged_fp8;
+  decltype(&nvllm_decode_step_fp8) decode_step_fp8;
+  decltype(&nvllm_step_maps) step_maps;
 } api;
 PyObject* g_check = nullptr;  // _lib.check: raises NvllmError for a negative code
 
@@ -402,6 +407,179 @@ PyObject* prefill_varlen(PyObject* const* a) {
   return wrap(std::move(out));
 }
 
+// ---- the 8-bit cache ------------------------------------------------------------------------
+
+void require_on(const char* name, const at::Tensor& t, const at::Tensor& like) {
+  if (__builtin_expect(t.device() != like.device(), 0)) raise(PyExc_RuntimeError, std::string(name) + " is on another device");
+}
+
+struct Fp8Planes {  // codes [blocks, 256, Hkv, D], scales [blocks, Hkv, 16]
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t blocks, hkv, d;
+};
+
+Fp8Planes fp8_planes(const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale, const at::Tensor& v_scale,
+                     const at::Tensor& like) {
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"k_cache", &k_cache}, {"v_cache", &v_cache}}) {
+    if (!t->is_cuda()) raise(PyExc_RuntimeError, std::string(name) + " must be a CUDA tensor (nano_vllm_b200 has no CPU path)");
+    if (t->scalar_type() != at::kFloat8_e4m3fn)
+      raise(PyExc_RuntimeError, std::string(name) + " must be float8_e4m3fn, got " + std::string(c10::toString(t->scalar_type())));
+    require_on(name, *t, like);
+  }
+  require(k_cache.dim() == 4 && k_cache.size(1) == NVLLM_BLOCK_SIZE && k_cache.is_contiguous() && v_cache.is_contiguous() &&
+              v_cache.sizes() == k_cache.sizes(),
+          "k_cache and v_cache must be contiguous planes [blocks, 256, Hkv, D]");
+  const int64_t blocks = k_cache.size(0), hkv = k_cache.size(2);
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"k_scale", &k_scale}, {"v_scale", &v_scale}}) {
+    require_on(name, *t, like);
+    if (t->scalar_type() != at::kFloat) raise(PyExc_RuntimeError, std::string(name) + " must be float32");
+    require(t->dim() == 3 && t->size(0) == blocks && t->size(1) == hkv && t->size(2) == NVLLM_BLOCK_SIZE / NVLLM_SCALE_GROUP &&
+                t->is_contiguous(),
+            "k_scale and v_scale must be contiguous [blocks, Hkv, 16]");
+  }
+  return {k_cache.data_ptr(), v_cache.data_ptr(), ptr<float>(k_scale), ptr<float>(v_scale), blocks, hkv, k_cache.size(3)};
+}
+
+void store_fp8(const Rows& k, const Rows& v, const Fp8Planes& c, const at::Tensor& slots, void* stream) {
+  require(slots.numel() == k.n && v.n == k.n, "slot_mapping.numel() == N");
+  launch([&] {
+    return api.store_kvcache_fp8(k.p, k.stride, v.p, v.stride, c.k, c.v, c.k_scale, c.v_scale, ptr<int32_t>(slots), k.n,
+                                 static_cast<int32_t>(c.hkv), static_cast<int32_t>(c.d), c.blocks, stream);
+  });
+}
+
+void decode_fp8(const Rows& q, int64_t hq, const Fp8Planes& c, const at::Tensor& like, const at::Tensor& context_lens,
+                const at::Tensor& block_tables, double scale, const Rows& out, const Step* step) {
+  require_i32("context_lens", context_lens);
+  require_i32("block_tables", block_tables);
+  require_on("context_lens", context_lens, like);
+  require_on("block_tables", block_tables, like);
+  require(block_tables.dim() == 2 && block_tables.size(0) == q.n && context_lens.numel() == q.n,
+          "block_tables.dim() == 2 and block_tables.shape[0] == B and context_lens.numel() == B");
+  if (q.n == 0) return;
+  const int32_t B = static_cast<int32_t>(q.n), HQ = static_cast<int32_t>(hq), HKV = static_cast<int32_t>(c.hkv),
+                D = static_cast<int32_t>(c.d), width = static_cast<int32_t>(block_tables.size(1));
+  const int64_t need = api.decode_workspace_bytes(B, width, HQ, HKV, D);
+  check(need);
+  void* ws;
+  int64_t ws_size;
+  workspace(like, need, &ws, &ws_size);
+  void* st = stream_of(like);
+  launch([&] {
+    if (step)
+      return api.decode_step_fp8(q.p, q.stride, step->k.p, step->k.stride, step->v.p, step->v.stride, step->slots, c.k, c.v,
+                                 c.k_scale, c.v_scale, ptr<int32_t>(context_lens), ptr<int32_t>(block_tables),
+                                 block_tables.stride(0), width, out.p, out.stride, B, HQ, HKV, D, static_cast<float>(scale),
+                                 c.blocks, ws, ws_size, st);
+    return api.decode_paged_fp8(q.p, q.stride, c.k, c.v, c.k_scale, c.v_scale, ptr<int32_t>(context_lens),
+                                ptr<int32_t>(block_tables), block_tables.stride(0), width, out.p, out.stride, B, HQ, HKV, D,
+                                static_cast<float>(scale), c.blocks, ws, ws_size, st);
+  });
+}
+
+// K/V rows [N, Hkv, D] of a call that stores them.
+void check_rows_fp8(const at::Tensor& key, const at::Tensor& value, const Fp8Planes& c, const at::Tensor& slots) {
+  require(key.sizes() == value.sizes() && key.size(1) == c.hkv && key.size(2) == c.d, "key and value must be [N, Hkv, D] of the cache's Hkv and D");
+  require_on("value", value, key);
+  require_i32("slot_mapping", slots);
+  require_on("slot_mapping", slots, key);
+  require(slots.numel() == key.size(0) && slots.is_contiguous(), "slot_mapping.numel() == N");
+}
+
+PyObject* store_kvcache_fp8(PyObject* const* a) {  // key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping
+  const at::Tensor &key = tensor(a[0], "key"), &value = tensor(a[1], "value"), &slots = tensor(a[6], "slot_mapping");
+  require_dim("key", key, 3);
+  require_dim("value", value, 3);
+  require_cuda_bf16("key", key);
+  require_cuda_bf16("value", value);
+  const Rows k = rows3(key, "key.stride(-1) == 1 and key.stride(1) == D"), v = rows3(value, "value.stride(-1) == 1 and value.stride(1) == D");
+  const Fp8Planes c = fp8_planes(tensor(a[2], "k_cache"), tensor(a[3], "v_cache"), tensor(a[4], "k_scale"), tensor(a[5], "v_scale"), key);
+  check_rows_fp8(key, value, c, slots);
+  const c10::cuda::CUDAGuard guard(key.device());
+  store_fp8(k, v, c, slots, stream_of(key));
+  Py_RETURN_NONE;
+}
+
+// out of a call on q: of q's shape, type and device
+at::Tensor output_like(PyObject* o, const at::Tensor& q, Rows* rows) {
+  at::Tensor out = output_for(o, q, rows);
+  require_cuda_bf16("out", out);
+  require_on("out", out, q);
+  require(out.sizes() == q.sizes(), "out.shape == q.shape");
+  return out;
+}
+
+PyObject* decode_paged_fp8(PyObject* const* a) {  // q, k_cache, v_cache, k_scale, v_scale, context_lens, block_tables, scale, out
+  const at::Tensor& q = tensor(a[0], "q");
+  require_dim("q", q, 3);
+  require_cuda_bf16("q", q);
+  const Rows qr = rows3(q, "q.stride(-1) == 1 and q.stride(1) == D");
+  const Fp8Planes c = fp8_planes(tensor(a[1], "k_cache"), tensor(a[2], "v_cache"), tensor(a[3], "k_scale"), tensor(a[4], "v_scale"), q);
+  require(q.size(2) == c.d, "q.shape[2] == D of the cache");
+  const c10::cuda::CUDAGuard guard(q.device());
+  Rows o;
+  at::Tensor out = output_like(a[8], q, &o);
+  decode_fp8(qr, q.size(1), c, q, tensor(a[5], "context_lens"), tensor(a[6], "block_tables"), as_double(a[7]), o, nullptr);
+  return wrap(std::move(out));
+}
+
+PyObject* decode_step_fp8(PyObject* const* a) {
+  // q, key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping, context_lens, block_tables, scale, out
+  const at::Tensor &q = tensor(a[0], "q"), &key = tensor(a[1], "key"), &value = tensor(a[2], "value"), &slots = tensor(a[7], "slot_mapping");
+  require_dim("q", q, 3);
+  require_dim("key", key, 3);
+  require_dim("value", value, 3);
+  require_cuda_bf16("q", q);
+  require_cuda_bf16("key", key);
+  require_cuda_bf16("value", value);
+  require_on("key", key, q);
+  const Rows qr = rows3(q, "q.stride(-1) == 1 and q.stride(1) == D");
+  const Fp8Planes c = fp8_planes(tensor(a[3], "k_cache"), tensor(a[4], "v_cache"), tensor(a[5], "k_scale"), tensor(a[6], "v_scale"), q);
+  require(q.size(2) == c.d && key.size(0) == q.size(0), "q.shape[2] == D of the cache and a new row for each query");
+  check_rows_fp8(key, value, c, slots);
+  const Step step = {rows3(key, "key.stride(-1) == 1 and key.stride(1) == D"),
+                     rows3(value, "value.stride(-1) == 1 and value.stride(1) == D"), ptr<int32_t>(slots), true};
+  const c10::cuda::CUDAGuard guard(q.device());
+  Rows o;
+  at::Tensor out = output_like(a[11], q, &o);
+  decode_fp8(qr, q.size(1), c, q, tensor(a[8], "context_lens"), tensor(a[9], "block_tables"), as_double(a[10]), o, &step);
+  return wrap(std::move(out));
+}
+
+PyObject* step_maps(PyObject* const* a) {
+  // seq_lens, cached_lens, block_tables, free_blocks, num_tokens, cu_seqlens_q, cu_seqlens_k, slot_mapping, positions, blocks_taken
+  const at::Tensor &lens = tensor(a[0], "seq_lens"), &cached = tensor(a[1], "cached_lens"), &table = tensor(a[2], "block_tables"),
+                   &free = tensor(a[3], "free_blocks"), &cu_q = tensor(a[5], "cu_seqlens_q"), &cu_k = tensor(a[6], "cu_seqlens_k"),
+                   &slots = tensor(a[7], "slot_mapping"), &positions = tensor(a[8], "positions"), &taken = tensor(a[9], "blocks_taken");
+  const int64_t rows = as_i64(a[4]);
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"seq_lens", &lens}, {"cached_lens", &cached},
+                                {"block_tables", &table}, {"free_blocks", &free}, {"cu_seqlens_q", &cu_q}, {"cu_seqlens_k", &cu_k},
+                                {"slot_mapping", &slots}, {"blocks_taken", &taken}}) {
+    require_i32(name, *t);
+    require_on(name, *t, lens);
+  }
+  require(positions.is_cuda() && positions.scalar_type() == at::kLong && positions.is_contiguous(), "positions must be contiguous CUDA int64");
+  require_on("positions", positions, lens);
+  const int64_t batch = lens.numel();
+  require(lens.dim() == 1 && cached.dim() == 1 && cached.numel() == batch && table.dim() == 2 && table.size(0) == batch && free.dim() == 1,
+          "seq_lens [B], cached_lens [B], block_tables [B, blocks], free_blocks [F]");
+  require(rows >= 0 && cu_q.numel() == batch + 1 && cu_k.numel() == batch + 1 && slots.numel() == rows && positions.numel() == rows &&
+              taken.numel() == 1,
+          "outputs must have B + 1, B + 1, num_tokens, num_tokens and 1 elements");
+  require(table.size(1) <= std::numeric_limits<int32_t>::max() && free.numel() <= std::numeric_limits<int32_t>::max() &&
+              batch <= std::numeric_limits<int32_t>::max(),
+          "sizes must fit 32 bits");
+  const c10::cuda::CUDAGuard guard(lens.device());
+  launch([&] {
+    return api.step_maps(ptr<int32_t>(lens), ptr<int32_t>(cached), static_cast<int32_t>(batch), ptr<int32_t>(table), table.stride(0),
+                         static_cast<int32_t>(table.size(1)), ptr<int32_t>(free), static_cast<int32_t>(free.numel()),
+                         ptr<int32_t>(cu_q), ptr<int32_t>(cu_k), ptr<int32_t>(slots), ptr<int64_t>(positions), rows,
+                         ptr<int32_t>(taken), stream_of(lens));
+  });
+  Py_RETURN_NONE;
+}
+
 struct Ref {  // owned reference
   PyObject* o;
   explicit Ref(PyObject* p) : o(p) {
@@ -747,6 +925,10 @@ PyObject* bind(PyObject* const* a) {  // library path, check
   RESOLVE(sample_tokens);
   RESOLVE(sample_candidates);
   RESOLVE(decode_step_inputs_pinned);
+  RESOLVE(store_kvcache_fp8);
+  RESOLVE(decode_paged_fp8);
+  RESOLVE(decode_step_fp8);
+  RESOLVE(step_maps);
 #undef RESOLVE
   Py_INCREF(a[1]);
   Py_XSETREF(g_check, a[1]);
@@ -796,6 +978,10 @@ PyMethodDef methods[] = {
     METHOD(pack, 4),
     METHOD(make_stager, 5),
     METHOD(stage, 10),
+    METHOD(store_kvcache_fp8, 7),
+    METHOD(decode_paged_fp8, 9),
+    METHOD(decode_step_fp8, 12),
+    METHOD(step_maps, 10),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of nano_vllm_b200's entry points.", -1, methods,
