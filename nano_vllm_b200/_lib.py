@@ -64,6 +64,9 @@ SIGNATURES = {
     "nvllm_decode_step_fp8": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                         c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_int32,
                                         c_int32, c_int32, c_int32, c_float, c_int64, c_void_p, c_int64, c_void_p]),
+    "nvllm_prefill_varlen_fp8": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
+                                           c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
+                                           c_int32, c_int32, c_float, c_int64, c_void_p]),
     "nvllm_step_maps": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "nvllm_ar_handle_bytes": (c_int64, []),

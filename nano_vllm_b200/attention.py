@@ -169,6 +169,15 @@ def decode_step_fp8(q: torch.Tensor, key: torch.Tensor, value: torch.Tensor, k_c
                                                  block_tables, scale, out)
 
 
+def prefill_varlen_fp8(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                       cu_seqlens_q: torch.Tensor, cu_seqlens_k: torch.Tensor, max_seqlen_q: int, max_seqlen_k: int, scale: float,
+                       block_tables: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
+    """``prefill_varlen`` through the block table of a cache held in 8 bits (see ``store_kvcache_fp8``): the new tokens' rows
+    have been stored, and are read back like the cached ones.  q/out: ``[N, Hq, D]`` bf16."""
+    return (_host or _native(q)).prefill_varlen_fp8(q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k,
+                                                    int(max_seqlen_q), int(max_seqlen_k), scale, block_tables, out)
+
+
 def qk_norm_rope_store(qkv: torch.Tensor, positions: torch.Tensor, q_weight: torch.Tensor | None,
                        k_weight: torch.Tensor | None, cos_sin_cache: torch.Tensor, eps: float,
                        slot_mapping: torch.Tensor | None, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -219,7 +228,11 @@ def sample_unpack(candidates: torch.Tensor, out: torch.Tensor | None = None) -> 
 # ---- the layer --------------------------------------------------------------------------
 
 class Attention(nn.Module):
-    """Drop-in for nanovllm/layers/attention.py:42-79 (same constructor, attributes, forward)."""
+    """Drop-in for nanovllm/layers/attention.py:42-79 (same constructor, attributes, forward).
+
+    A cache held in 8 bits: bind ``k_cache`` / ``v_cache`` to ``float8_e4m3fn`` planes and ``k_scale`` / ``v_scale`` to their
+    scales (see ``store_kvcache_fp8``).  A decode step is then one launch (``decode_step_fp8``), a prefill without cached
+    prefixes attends this step's own rows in bf16 and stores them, one with them reads the cache."""
 
     def __init__(self, num_heads, head_dim, scale, num_kv_heads):
         super().__init__()
@@ -228,6 +241,7 @@ class Attention(nn.Module):
         self.scale = scale
         self.num_kv_heads = num_kv_heads
         self.k_cache = self.v_cache = torch.tensor([])
+        self.k_scale = self.v_scale = torch.tensor([])
 
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, kv_stored: bool = False):
         """``kv_stored=True``: the caller has already written this step's K/V rows into the cache

@@ -324,14 +324,15 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
   float m0, m1, l0, l1;  // heads 2 tig and 2 tig + 1
   // The power of two that O is held in (the same for all lanes of the warp): a group's P goes into its product times
   // vscale / unit <= 1.  It grows at once to the largest scale of a tile and shrinks where that is 16 times smaller, so that
-  // a group's P loses four bits of f16's range at most; never by more than 2^-60, which keeps O finite whatever the scales.
-  float unit;
+  // a group's P loses four bits of f16's range at most; not below 2^-60 of what it has been, which keeps O finite whatever the
+  // scales.
+  float unit, most_unit;
   auto reset_state = [&]() {
 #pragma unroll
     for (int c = 0; c < C::KS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
     m0 = m1 = -INFINITY;
     l0 = l1 = 0.f;
-    unit = 0.f;
+    unit = most_unit = 0.f;
   };
   reset_state();
 
@@ -597,11 +598,12 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
     float alpha0 = fast_exp2(m0 - mn0), alpha1 = fast_exp2(m1 - mn1);
     l0 *= alpha0;
     l1 *= alpha1;
-    if (most_vs > unit || most_vs * 16.f < unit) {
-      const float next = fmaxf(most_vs, unit * 0x1p-60f), change = unit > 0.f ? unit / next : 0.f;
+    if (most_vs > unit || (most_vs > 0.f && most_vs * 16.f < unit)) {
+      const float next = fmaxf(most_vs, most_unit * 0x1p-60f), change = unit > 0.f ? unit / next : 0.f;
       alpha0 *= change;
       alpha1 *= change;
       unit = next;
+      most_unit = fmaxf(most_unit, next);
     }
     const float per_unit = unit > 0.f ? 1.f / unit : 0.f;
     m0 = mn0;
@@ -692,6 +694,7 @@ static int decode_fp8_common(const char* who, const void* q, int64_t q_row_strid
                              int64_t workspace_bytes, void* stream) {
   const int64_t need = nvllm_decode_workspace_bytes(batch, max_blocks, num_q_heads, num_kv_heads, head_dim);
   if (need < 0) return static_cast<int>(need);
+  if (!(scale >= 0.f && scale < INFINITY)) return fail(NVLLM_E_GEOMETRY, "%s: scale must be finite and not negative", who);
   if (batch == 0) return NVLLM_OK;
   const int rc = check_fp8_planes(who, cache.k, cache.v, cache.k_scale, cache.v_scale, num_kv_heads, head_dim, num_blocks);
   if (rc) return rc;

@@ -57,12 +57,13 @@ struct Api {
   decltype(&nvllm_store_kvcache_fp8) store_kvcache_fp8;
   decltype(&nvllm_decode_paged_fp8) decode_paged_fp8;
   decltype(&nvllm_decode_step_fp8) decode_step_fp8;
+  decltype(&nvllm_prefill_varlen_fp8) prefill_varlen_fp8;
   decltype(&nvllm_step_maps) step_maps;
 } api;
 PyObject* g_check = nullptr;  // _lib.check: raises NvllmError for a negative code
 
 struct Names {
-  PyObject *num_heads, *head_dim, *scale, *num_kv_heads, *k_cache, *v_cache, *is_prefill, *cu_seqlens_q, *cu_seqlens_k,
+  PyObject *num_heads, *head_dim, *scale, *num_kv_heads, *k_cache, *v_cache, *k_scale, *v_scale, *is_prefill, *cu_seqlens_q, *cu_seqlens_k,
       *max_seqlen_q, *max_seqlen_k, *slot_mapping, *context_lens, *block_tables, *last_token, *num_tokens, *temperature,
       *block_table;
 } names;
@@ -547,6 +548,42 @@ PyObject* decode_step_fp8(PyObject* const* a) {
   return wrap(std::move(out));
 }
 
+void prefill_fp8(const Rows& q, int64_t hq, const Fp8Planes& c, const at::Tensor& like, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                 int64_t max_q, int64_t max_k, double scale, const at::Tensor& table, const Rows& out) {
+  for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"cu_seqlens_q", &cu_q}, {"cu_seqlens_k", &cu_k}, {"block_tables", &table}}) {
+    require_i32(name, *t);
+    require_on(name, *t, like);
+  }
+  const int64_t batch = cu_q.numel() - 1;
+  require(batch >= 0 && cu_k.numel() == batch + 1, "cu_seqlens_k.numel() == batch + 1");
+  require(table.dim() == 2 && table.size(0) == batch, "block_tables.dim() == 2 and block_tables.shape[0] == batch");
+  constexpr int64_t most = std::numeric_limits<int32_t>::max();
+  require(batch <= most && max_q <= most && max_k <= most, "sizes must fit 32 bits");
+  launch([&] {
+    return api.prefill_varlen_fp8(q.p, q.stride, c.k, c.v, c.k_scale, c.v_scale, ptr<int32_t>(table), table.stride(0),
+                                  static_cast<int32_t>(table.size(1)), out.p, out.stride, ptr<int32_t>(cu_q), ptr<int32_t>(cu_k), q.n,
+                                  static_cast<int32_t>(batch), static_cast<int32_t>(max_q), static_cast<int32_t>(max_k),
+                                  static_cast<int32_t>(hq), static_cast<int32_t>(c.hkv), static_cast<int32_t>(c.d),
+                                  static_cast<float>(scale), c.blocks, stream_of(like));
+  });
+}
+
+PyObject* prefill_varlen_fp8(PyObject* const* a) {
+  // q, k_cache, v_cache, k_scale, v_scale, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, block_tables, out
+  const at::Tensor& q = tensor(a[0], "q");
+  require_dim("q", q, 3);
+  require_cuda_bf16("q", q);
+  const Rows qr = rows3(q, "q.stride(-1) == 1 and q.stride(1) == D");
+  const Fp8Planes c = fp8_planes(tensor(a[1], "k_cache"), tensor(a[2], "v_cache"), tensor(a[3], "k_scale"), tensor(a[4], "v_scale"), q);
+  require(q.size(2) == c.d, "q.shape[2] == D of the cache");
+  const c10::cuda::CUDAGuard guard(q.device());
+  Rows o;
+  at::Tensor out = output_like(a[11], q, &o);
+  prefill_fp8(qr, q.size(1), c, q, tensor(a[5], "cu_seqlens_q"), tensor(a[6], "cu_seqlens_k"), as_i64(a[7]), as_i64(a[8]),
+              as_double(a[9]), tensor(a[10], "block_tables"), o);
+  return wrap(std::move(out));
+}
+
 PyObject* step_maps(PyObject* const* a) {
   // seq_lens, cached_lens, block_tables, free_blocks, num_tokens, cu_seqlens_q, cu_seqlens_k, slot_mapping, positions, blocks_taken
   const at::Tensor &lens = tensor(a[0], "seq_lens"), &cached = tensor(a[1], "cached_lens"), &table = tensor(a[2], "block_tables"),
@@ -625,6 +662,39 @@ PyObject* attention_forward(PyObject* const* a) {
   require_cuda_bf16("q", q);
   const c10::cuda::CUDAGuard guard(q.device());
   Ref slots(PyObject_GetAttr(ctx, names.slot_mapping));
+  if (k_cache.scalar_type() == at::kFloat8_e4m3fn) {  // a cache held in 8 bits, its scales beside it
+    Ref ks(PyObject_GetAttr(layer, names.k_scale)), vs(PyObject_GetAttr(layer, names.v_scale));
+    const Fp8Planes c = fp8_planes(k_cache, v_cache, tensor(ks.o, "k_scale"), tensor(vs.o, "v_scale"), q);
+    require(c.hkv == hkv && c.d == d, "the cache's Hkv and D are the layer's");
+    const at::Tensor* sm = do_store ? &tensor(slots.o, "slot_mapping") : nullptr;
+    if (sm) {
+      require_i32("slot_mapping", *sm);
+      require_on("slot_mapping", *sm, q);
+      require_on("k", k, q);
+      require_on("v", v, q);
+    }
+    at::Tensor out = new_tensor({qr.n, hq * d}, q.options());
+    const Rows o = {out.data_ptr(), qr.n, hq * d};
+    if (prefill_phase) {
+      Ref cq(PyObject_GetAttr(ctx, names.cu_seqlens_q)), ck(PyObject_GetAttr(ctx, names.cu_seqlens_k));
+      const int64_t mq = attr_i64(ctx, names.max_seqlen_q), mk = attr_i64(ctx, names.max_seqlen_k);
+      if (sm) store_fp8(kr, vr, c, *sm, stream_of(q));
+      if (const at::Tensor* table = maybe_tensor(bt.o, "block_tables"))
+        prefill_fp8(qr, hq, c, q, tensor(cq.o, "cu_seqlens_q"), tensor(ck.o, "cu_seqlens_k"), mq, mk, scale, *table, o);
+      else  // no cached prefix: this step's own rows, as they are
+        prefill(qr, hq, d, KV{kr, vr, hkv, nullptr, 0}, tensor(cq.o, "cu_seqlens_q"), tensor(ck.o, "cu_seqlens_k"), mq, mk, scale, o,
+                stream_of(q));
+    } else {
+      Ref lens(PyObject_GetAttr(ctx, names.context_lens));
+      Step step{kr, vr, nullptr, true};
+      if (sm) {
+        require(sm->numel() == qr.n && kr.n == qr.n && vr.n == qr.n, "slot_mapping.numel() == N");
+        step.slots = ptr<int32_t>(*sm);
+      }
+      decode_fp8(qr, hq, c, q, tensor(lens.o, "context_lens"), tensor(bt.o, "block_tables"), scale, o, sm ? &step : nullptr);
+    }
+    return wrap(std::move(out));
+  }
   Step step{};
   const Step* with_store = nullptr;
   if (do_store) {
@@ -928,13 +998,15 @@ PyObject* bind(PyObject* const* a) {  // library path, check
   RESOLVE(store_kvcache_fp8);
   RESOLVE(decode_paged_fp8);
   RESOLVE(decode_step_fp8);
+  RESOLVE(prefill_varlen_fp8);
   RESOLVE(step_maps);
 #undef RESOLVE
   Py_INCREF(a[1]);
   Py_XSETREF(g_check, a[1]);
 #define NAME(x) \
   if (!names.x) names.x = PyUnicode_InternFromString(#x)
-  NAME(num_heads); NAME(head_dim); NAME(scale); NAME(num_kv_heads); NAME(k_cache); NAME(v_cache); NAME(is_prefill);
+  NAME(num_heads); NAME(head_dim); NAME(scale); NAME(num_kv_heads); NAME(k_cache); NAME(v_cache); NAME(k_scale);
+  NAME(v_scale); NAME(is_prefill);
   NAME(cu_seqlens_q); NAME(cu_seqlens_k); NAME(max_seqlen_q); NAME(max_seqlen_k); NAME(slot_mapping); NAME(context_lens);
   NAME(block_tables); NAME(last_token); NAME(num_tokens); NAME(temperature); NAME(block_table);
 #undef NAME
@@ -981,6 +1053,7 @@ PyMethodDef methods[] = {
     METHOD(store_kvcache_fp8, 7),
     METHOD(decode_paged_fp8, 9),
     METHOD(decode_step_fp8, 12),
+    METHOD(prefill_varlen_fp8, 12),
     METHOD(step_maps, 10),
     {nullptr, nullptr, 0, nullptr},
 };

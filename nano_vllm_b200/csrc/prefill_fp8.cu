@@ -1,0 +1,772 @@
+// Varlen causal GQA prefill over the 8-bit cache (fp8.cuh) on the 5th-generation tensor cores, head_dim 64 or 128.
+//
+//   query i of a sequence with Lq new tokens of Lk sees keys j <= i + Lk - Lq;  K, V = code * scale of the token's group
+//
+// Tiles of 128 query rows (128 / n tokens x n heads that share a KV head) and 64 keys, four groups of scales:
+//   * S = Q K^T with the codes as they come by TMA (kind::f8f6f4).  A row of Q, scaled by a power of two to 128 <= max < 256, is
+//     the sum of two e4m3 numbers: the nearest, and what is left of bf16's eight bits, which has four at most.  Exact down to
+//     2^-10 of the row's largest value, below that within 2^-17 of it.  Two products at twice the rate of a 16-bit one: the
+//     same time, and no key has to be converted.
+//   * The K scale of a group and the row's power of two enter the multiply-add in front of the exponential, four factors a tile.
+//   * O += P V in f16 (kind::f16): P from TMEM, rounded to f16 (2^-11); V's codes are converted to f16, exactly, once a tile by
+//     the warps that also write results.  P carries the group's V scale over a running unit, a power of two that O is held
+//     in: it grows at once with the largest scale of a tile and shrinks where that is 16 times smaller.
+//   * Keys past the end: their scores are masked, their V rows converted to zeros whatever the codes are.
+//
+// Twelve warps, two blocks to an SM for the whole launch: 0-3 softmax (thread = query row), 4-7 query rows in, V conversion and
+// results out, 8 = TMA of K and of the scales, 9 = MMA issuer, 10 = TMA of V.  The three warp groups trade registers at
+// start-up.  Items (query tile of a sequence, head group) are ordered by their key tiles, most first, over all sequences, and
+// dealt out in turn, there and back again, so that all blocks have about the same to do; no counter in memory, so nothing is
+// shared by launches.
+#include <algorithm>
+
+#include "fp8.cuh"
+#include "prefill_tc.cuh"
+#include "sm100.cuh"
+
+namespace nvllm {
+using namespace sm100;
+
+namespace f8 {
+constexpr int BM = 128, BN = 64, KST = 2;
+constexpr int MAX_BATCH = 1024;  // sequences of a launch
+constexpr int NTHREADS = 384;
+constexpr int REGS_LAUNCH = 80, REGS_SOFTMAX = 136, REGS_ROWS = 64, REGS_OTHER = 40;
+static_assert(128 * (REGS_SOFTMAX + REGS_ROWS + REGS_OTHER) <= NTHREADS * REGS_LAUNCH, "register pool of a block");
+constexpr int TMEM_COLS = 256, TMEM_O = 128;  // S / P buffers [0,64) and [64,128), O [128,256)
+constexpr float kRescaleThreshold = 8.f;      // log2 units
+enum Bar {
+  Q_FULL, K_FULL0, K_FULL1, RAW_FULL0, RAW_FULL1, RAW_FREE0, RAW_FREE1, V_FULL0, V_FULL1, QK_DONE0, QK_DONE1, PV_DONE0, PV_DONE1,
+  P_FULL0, P_FULL1, ITEM_FULL0, ITEM_FULL1, ITEM_FREE0, ITEM_FREE1, O_FREE, EPI_FULL0, EPI_FULL1,
+  SCALES0, SCALES1, SCALES2, SCALES3, FACTOR0, FACTOR1, DRAIN, NUM_BARS
+};
+static_assert(NUM_BARS <= 32, "a barrier per lane");
+
+template <int D_>
+struct Geo {
+  static constexpr int D = D_;
+  static constexpr int Q_PART = BM * D, Q_BYTES = 2 * Q_PART;      // high and low e4m3 parts
+  static constexpr int K_BYTES = BN * D;                           // codes
+  static constexpr int V_SUB = BN * 128, V_BYTES = D / 64 * V_SUB;  // f16, 64 columns to a sub-tile
+  static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_RAW = OFF_K + KST * K_BYTES, OFF_V = OFF_RAW + KST * K_BYTES;
+  static constexpr int OFF_STAGE = OFF_V + KST * V_BYTES;          // 4 warps x 32 rows x 64 B of output
+  static constexpr int OFF_CTRL = OFF_STAGE + 4 * 2048;            // barriers
+  static constexpr int OFF_SLOTS = OFF_CTRL + 256;                 // two item descriptors of 8 ints
+  static constexpr int OFF_MISC = OFF_SLOTS + 64;                  // TMEM address, abort flag
+  static constexpr int OFF_SCALES = OFF_MISC + 64;                 // 4 tiles x (4 of K, 4 of V)
+  static constexpr int OFF_ROW = OFF_SCALES + 128;                 // 2 items x 128 rows: the query row's power of two
+  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: unit / row sum
+  static constexpr int SMEM = OFF_INV + 2 * 128 * 4 + 1024;
+  static constexpr int SBO = D == 128 ? 1024 : 512;                // eight rows of codes
+  static constexpr int OCH = D / 32;
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two blocks to an SM");
+};
+}  // namespace f8
+
+struct PrefillFp8Params {
+  const __nv_bfloat16* q;
+  int64_t q_stride;
+  const float* k_scale;
+  const float* v_scale;
+  const int32_t* block_tables;
+  int64_t bt_stride;
+  int max_blocks;
+  __nv_bfloat16* out;
+  int64_t out_stride;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int batch, hq, hkv, g;
+  int pack, tile_tokens, inv_pack;  // query heads in a tile, its tokens, 2^16 / heads
+  float scale_log2e;
+  int64_t num_blocks;
+  int* status;
+};
+
+// Shared-memory descriptor of e4m3 rows as TMA leaves them: 128-byte rows under the 128-byte swizzle, or 64 under the 64-byte one.
+template <int D>
+__device__ __forceinline__ uint64_t codes_desc(uint32_t smem_addr) {
+  uint64_t d = static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4);
+  d |= static_cast<uint64_t>(1) << 16;
+  d |= static_cast<uint64_t>(f8::Geo<D>::SBO >> 4) << 32;
+  d |= 1ull << 46;
+  d |= (D == 128 ? 2ull : 4ull) << 61;
+  return d;
+}
+// Byte of 16-byte piece c of row r in such a tile.
+template <int D>
+__device__ __forceinline__ uint32_t code_piece(int r, int c) {
+  return D == 128 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ (r >> 1 & 3)) << 4);
+}
+__device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// e4m3 x e4m3 -> fp32, both K-major; f16 x f16 -> fp32, B MN-major.
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
+__host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return idesc_f8(m, n) | (1u << 16); }
+
+__device__ __forceinline__ void bulk_copy16(uint32_t dst, const void* src, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst), "l"(src), "r"(bar)
+               : "memory");
+}
+
+struct Fp8Item {
+  int b, h, m0, q0, Lq, Lk, n_kv;  // n_kv < 0: no more work
+};
+
+// Key tiles that the first `tokens` query tokens of a sequence see.
+__device__ __forceinline__ int fp8_key_tiles(int tokens, int Lq, int Lk) {
+  const int end = min(Lk, min(tokens, Lq) + (Lk - Lq));
+  return end > 0 ? (end + f8::BN - 1) / f8::BN : 0;
+}
+// Query tiles of a sequence that see more than x key tiles (they are its last ones).
+__device__ __forceinline__ int fp8_tiles_above(int x, int Lq, int Lk, int bmt) {
+  const int tiles = (Lq + bmt - 1) / bmt, off = Lk - Lq;
+  if (Lq <= 0 || Lk <= x * f8::BN) return 0;  // the last one sees the most
+  // tile m sees more than x where off + (m + 1) bmt > 64 x
+  const int least = x * f8::BN - off;  // tokens that see no more
+  return least < 0 ? tiles : tiles - min(tiles - 1, least / bmt);
+}
+
+template <int D>
+__global__ void __launch_bounds__(f8::NTHREADS, 2)
+prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v) {
+  using namespace f8;
+  using G = Geo<D>;
+  constexpr unsigned ALL = 0xffffffffu;
+  extern __shared__ unsigned char smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  auto bar = [&](int i) { return base + G::OFF_CTRL + 8u * i; };
+  volatile int* slots = reinterpret_cast<volatile int*>(base_ptr + G::OFF_SLOTS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + G::OFF_MISC);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + G::OFF_MISC + 8);
+  float* row_factor = reinterpret_cast<float*>(base_ptr + G::OFF_ROW);
+  float* inv_buf = reinterpret_cast<float*>(base_ptr + G::OFF_INV);
+  const int pack = p.pack, BMT = p.tile_tokens;
+  auto token_of = [&](int row) { return row * p.inv_pack >> 16; };  // row / pack, row < 128
+
+  pdl_trigger();
+  if (warp == 9 && lane < NUM_BARS) {
+    // by the four warps of a group: query rows, V, P, normalisers, O; an item slot is free when the softmax (4), the row (4)
+    // warps, the MMA issuer and the V producer are done with it
+    const bool by_four = lane == Q_FULL || lane == RAW_FREE0 || lane == RAW_FREE1 || lane == V_FULL0 || lane == V_FULL1 ||
+                         lane == P_FULL0 || lane == P_FULL1 || lane == O_FREE || lane == EPI_FULL0 || lane == EPI_FULL1 ||
+                         lane == FACTOR0 || lane == FACTOR1;
+    mbar_init(bar(lane), by_four ? 4u : lane == ITEM_FREE0 || lane == ITEM_FREE1 ? 10u : 1u);
+    if (lane == 0) {
+      *abort_flag = 0;
+      prefetch_tmap(&tmap_k);
+      prefetch_tmap(&tmap_v);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 10) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+  pdl_wait();
+  auto lens = [&](int b) { return make_int2(p.cu_q[b + 1] - p.cu_q[b], p.cu_k[b + 1] - p.cu_k[b]); };  // Lq, Lk
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot, tmem_o = tmem + TMEM_O;
+  auto tmem_s = [&](int st) { return tmem + st * 64; };
+
+  auto read_item = [&](int it) {
+    volatile int* s = slots + (it & 1) * 8;
+    Fp8Item x;
+    x.b = s[0]; x.h = s[1]; x.m0 = s[2]; x.q0 = s[3];
+    x.Lq = s[4]; x.Lk = s[5]; x.n_kv = s[6];
+    return x;
+  };
+  auto block_of = [&](const Fp8Item& x, int j) -> int64_t {  // of key tile j
+    const int i = j * BN / kBlockSize;
+    const int64_t blk = i < p.max_blocks ? p.block_tables[x.b * p.bt_stride + i] : -1;
+    if (blk >= 0 && blk < p.num_blocks) return blk;
+    atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
+    return 0;
+  };
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
+    if (warp == 8) {
+      // ---------------------------------------------------------------- items; TMA of K and the scales
+      const int hgroups = p.hq / pack;
+      // Query tiles of all sequences that see more than x key tiles.
+      auto above = [&](int x) {
+        int n = 0;
+#pragma unroll 1
+        for (int b = lane; b < p.batch; b += 32) n += fp8_tiles_above(x, lens(b).x, lens(b).y, BMT);
+        return __reduce_add_sync(ALL, static_cast<unsigned>(n));
+      };
+      int longest = 0;
+#pragma unroll 1
+      for (int b = lane; b < p.batch; b += 32) longest = max(longest, lens(b).y);
+      longest = (__reduce_max_sync(ALL, longest) + BN - 1) / BN;
+      const unsigned total = above(0) * hgroups;  // items; tiles that see no key are none
+      int T = 0, loaded = 0;
+      bool ok = true;
+#pragma unroll 1
+      for (int it = 0;; ++it) {
+        const unsigned drawn = it * gridDim.x + (it & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        Fp8Item x{};
+        x.n_kv = -1;
+        if (drawn < total) {
+          const unsigned rank = drawn / hgroups;
+          x.h = (drawn - rank * hgroups) * pack;
+          int lo = 1, hi = longest;  // its key tiles: the least n with above(n) <= rank (above(longest) = 0)
+#pragma unroll 1
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (above(mid) <= rank) hi = mid;
+            else lo = mid + 1;
+          }
+          x.n_kv = lo;
+          unsigned k = rank - above(lo);  // its number among the tiles with as many
+#pragma unroll 1
+          for (int b0 = 0; b0 < p.batch; b0 += 32) {
+            const int b = b0 + lane;
+            unsigned n = 0;
+            if (b < p.batch) {
+              const int2 len = lens(b);
+              n = fp8_tiles_above(lo - 1, len.x, len.y, BMT) - fp8_tiles_above(lo, len.x, len.y, BMT);
+            }
+            unsigned incl = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+              const unsigned v = __shfl_up_sync(ALL, incl, d);
+              if (lane >= d) incl += v;
+            }
+            const unsigned hit = __ballot_sync(ALL, incl > k);
+            if (hit) {
+              const int src = __ffs(hit) - 1;
+              x.b = b0 + src;
+              k -= __shfl_sync(ALL, incl - n, src);
+              break;
+            }
+            k -= __shfl_sync(ALL, incl, 31);
+          }
+          x.Lq = lens(x.b).x;
+          x.Lk = lens(x.b).y;
+          x.q0 = p.cu_q[x.b];
+          x.m0 = ((x.Lq + BMT - 1) / BMT - 1 - fp8_tiles_above(lo, x.Lq, x.Lk, BMT) - static_cast<int>(k)) * BMT;
+        }
+        if (it >= 2) ok = wait_or_abort(bar(ITEM_FREE0 + (it & 1)), ((it >> 1) - 1) & 1, abort_flag);
+        if (!__all_sync(ALL, ok)) break;
+        if (lane == 0) {
+          volatile int* s = slots + (it & 1) * 8;
+          s[0] = x.b; s[1] = x.h; s[2] = x.m0; s[3] = x.q0;
+          s[4] = x.Lq; s[5] = x.Lk; s[6] = x.n_kv;
+          mbar_arrive(bar(ITEM_FULL0 + (it & 1)));
+        }
+        __syncwarp();
+        if (x.n_kv < 0) break;
+        if (elect_one()) {
+          const int kvh = x.h / p.g;
+#pragma unroll 1
+          for (int j = 0; j < x.n_kv; ++j) {
+            const int t = T + j, st = t & 1, use = t >> 1;
+            const int64_t blk = block_of(x, j);
+            if (use > 0 && !(ok = wait_or_abort(bar(QK_DONE0 + st), (use - 1) & 1, abort_flag))) break;
+            // K's stage is free, and so are the scales of tile t - 4: its softmax came before the scores of tile t - 2
+            const int64_t at = (blk * p.hkv + kvh) * kGroups + j * BN % kBlockSize / kScaleGroup;
+            const uint32_t sc = base + G::OFF_SCALES + (t & 3) * 32;
+            mbar_expect_tx(bar(SCALES0 + (t & 3)), 32);
+            bulk_copy16(sc, p.k_scale + at, bar(SCALES0 + (t & 3)));
+            bulk_copy16(sc + 16, p.v_scale + at, bar(SCALES0 + (t & 3)));
+            mbar_expect_tx(bar(K_FULL0 + st), G::K_BYTES);
+            tma_load_3d(base + G::OFF_K + st * G::K_BYTES, &tmap_k, bar(K_FULL0 + st), 0, kvh, static_cast<int>(blk * kBlockSize + j * BN % kBlockSize));
+            ++loaded;
+          }
+          if (!ok) {  // gave up: no copy is in flight when the block ends
+#pragma unroll 1
+            for (int t = max(loaded - 4, 0); t < loaded; ++t) {
+              if (t >= loaded - 2) (void)mbar_wait(bar(K_FULL0 + (t & 1)), (t >> 1) & 1);
+              (void)mbar_wait(bar(SCALES0 + (t & 3)), (t >> 2) & 1);
+            }
+          }
+        }
+        if (!__all_sync(ALL, ok)) break;
+        T += x.n_kv;
+      }
+    } else if (warp == 10) {
+      // ---------------------------------------------------------------- TMA of V
+      if (elect_one()) {
+        int T = 0, loaded = 0;
+        bool ok = true;
+#pragma unroll 1
+        for (int it = 0; ok; ++it) {
+          if (!(ok = wait_or_abort(bar(ITEM_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
+          const Fp8Item x = read_item(it);
+          if (x.n_kv < 0) break;
+          const int kvh = x.h / p.g;
+#pragma unroll 1
+          for (int j = 0; j < x.n_kv; ++j) {
+            const int t = T + j, st = t & 1, use = t >> 1;
+            const int64_t blk = block_of(x, j);
+            if (use > 0 && !(ok = wait_or_abort(bar(RAW_FREE0 + st), (use - 1) & 1, abort_flag))) break;
+            mbar_expect_tx(bar(RAW_FULL0 + st), G::K_BYTES);
+            tma_load_3d(base + G::OFF_RAW + st * G::K_BYTES, &tmap_v, bar(RAW_FULL0 + st), 0, kvh, static_cast<int>(blk * kBlockSize + j * BN % kBlockSize));
+            ++loaded;
+          }
+          if (!ok) break;
+          T += x.n_kv;
+          mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
+        }
+        if (!ok) {
+#pragma unroll 1
+          for (int t = max(loaded - 2, 0); t < loaded; ++t) (void)mbar_wait(bar(RAW_FULL0 + (t & 1)), (t >> 1) & 1);
+        }
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------------- MMA issuer
+      if (elect_one()) {
+        constexpr uint32_t idesc_qk = idesc_f8(BM, BN), idesc_pv = idesc_f16(BM, D);
+        const uint64_t q_desc = codes_desc<D>(base + G::OFF_Q), k_desc = codes_desc<D>(base + G::OFF_K);
+        const uint64_t v_desc = umma_desc(base + G::OFF_V, G::V_SUB, 1024);
+        auto issue_qk = [&](int t) -> bool {
+          const int st = t & 1;
+          if (!wait_or_abort(bar(K_FULL0 + st), (t >> 1) & 1, abort_flag)) return false;
+          tc_fence_after();
+          const uint64_t kd = k_desc + static_cast<uint64_t>(st * (G::K_BYTES >> 4));
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int ks = 0; ks < D / 32; ++ks)
+              umma_f8_ss(tmem_s(st), q_desc + ((part * G::Q_PART + ks * 32) >> 4), kd + ((ks * 32) >> 4), idesc_qk, part > 0 || ks > 0);
+          umma_commit(bar(QK_DONE0 + st));
+          return true;
+        };
+        int T = 0;
+        bool ok = true;
+#pragma unroll 1
+        for (int it = 0; ok; ++it) {
+          if (!(ok = wait_or_abort(bar(ITEM_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
+          const Fp8Item x = read_item(it);
+          if (x.n_kv < 0) break;
+          if (!(ok = wait_or_abort(bar(Q_FULL), it & 1, abort_flag))) break;
+#pragma unroll 1
+          for (int j = -1; j < x.n_kv; ++j) {
+            const int t = T + j, st = t & 1, ph = (t >> 1) & 1;
+            if (j + 1 < x.n_kv && !(ok = issue_qk(t + 1))) break;  // the next scores run under this tile's softmax
+            if (j < 0) continue;
+            if (!(ok = wait_or_abort(bar(V_FULL0 + st), ph, abort_flag))) break;
+            if (!(ok = wait_or_abort(bar(P_FULL0 + st), ph, abort_flag))) break;
+            // the first product of an item overwrites O: the previous item's must have been read
+            if (j == 0 && it > 0 && !(ok = wait_or_abort(bar(O_FREE), (it - 1) & 1, abort_flag))) break;
+            tc_fence_after();
+            const uint64_t vd = v_desc + static_cast<uint64_t>(st * (G::V_BYTES >> 4));
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks)
+              umma_ts(tmem_o, tmem_s(st) + ks * 8, vd + static_cast<uint64_t>((ks * 2048) >> 4), idesc_pv, (j > 0 || ks > 0) ? 1u : 0u);
+            umma_commit(bar(PV_DONE0 + st));
+          }
+          if (!ok) break;
+          T += x.n_kv;
+          mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
+        }
+        if (!ok) {  // make sure nothing is still running on TMEM before it is freed
+          umma_commit(bar(DRAIN));
+          (void)mbar_wait(bar(DRAIN), 0);
+        }
+      }
+    } else {
+      // ---------------------------------------------------------------- rows of tiles that see no key: zeros
+#pragma unroll 1
+      for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+        const int Lq = lens(b).x, Lk = lens(b).y, dead = Lk <= 0 ? Lq : Lk < Lq ? (Lq - Lk) / BMT * BMT : 0;
+        const int per_row = p.hq * (D / 8);
+        const int64_t q0 = p.cu_q[b];
+#pragma unroll 1
+        for (int t = 0; t < dead; ++t)
+#pragma unroll 1
+          for (int i = lane; i < per_row; i += 32)
+            reinterpret_cast<uint4*>(p.out + (q0 + t) * p.out_stride)[i] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ softmax rows
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    const int r = warp * 32 + lane;
+    const int r_tok = token_of(r);
+    const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
+    int T = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int it = 0; ok; ++it) {
+      if (!(ok = wait_or_abort(bar(ITEM_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
+      const Fp8Item x = read_item(it);
+      if (x.n_kv < 0) break;
+      if (!(ok = wait_or_abort(bar(FACTOR0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
+      const float factor = row_factor[(it & 1) * 128 + r];
+      const int qi = x.m0 + r_tok, off = x.Lk - x.Lq;
+      float m_used = -INFINITY, l = 0.f, unit = 0.f, most_unit = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < x.n_kv; ++j) {
+        const int t = T + j, st = t & 1, ph = (t >> 1) & 1;
+        const uint32_t scores = tmem_s(st) + lane_addr;
+        if (!(ok = wait_or_abort(bar(SCALES0 + (t & 3)), (t >> 2) & 1, abort_flag))) break;
+        const float* sc = reinterpret_cast<const float*>(base_ptr + G::OFF_SCALES + (t & 3) * 32);
+        const int j0 = j * BN;
+        float ks[4], vs[4];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          // A group behind the end may hold anything: a number, then.  Never zero, which -inf of a masked score must not meet.
+          const bool live = j0 + g * kScaleGroup < x.Lk;
+          ks[g] = fmaxf((live ? sc[g] : 1.f) * factor, 0x1p-126f);
+          vs[g] = live ? sc[4 + g] : 0.f;
+        }
+        if (!(ok = wait_or_abort(bar(QK_DONE0 + st), ph, abort_flag))) break;
+        tc_fence_after();
+        uint32_t s[64];
+        tmem_ld32(scores, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_ld32(scores + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+        tmem_wait_ld();
+        if ((j0 + BN - 1 > x.m0 + off) || (j0 + BN > x.Lk)) {  // tile touches the diagonal or the end
+          const int limit = min(qi + off, x.Lk - 1) - j0;        // columns c <= limit are visible
+#pragma unroll
+          for (int c = 0; c < 64; ++c)
+            if (c > limit) s[c] = 0xff800000u;  // -inf
+        }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          float m2[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = g * 16; c < g * 16 + 16; c += 4) {
+            m2[0] = fmax3(m2[0], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+            m2[1] = fmax3(m2[1], __uint_as_float(s[c + 2]), __uint_as_float(s[c + 3]));
+          }
+          mx = fmaxf(mx, fmaxf(m2[0], m2[1]) * ks[g]);
+        }
+        const float m_new = fmaxf(m_used, mx);
+        // lazy rescale: keep the old reference maximum unless it has been outgrown by 2^8; and the unit, see above
+        const bool grow = m_new > m_used + kRescaleThreshold;
+        const float most_vs = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+        const bool other_unit = most_vs > unit || (most_vs > 0.f && most_vs * 16.f < unit);  // the same for all rows
+        if (other_unit || __any_sync(ALL, grow)) {
+          float alpha = 1.f;
+          if (grow) {
+            alpha = (m_used == -INFINITY) ? 0.f : fast_exp2(m_used - m_new);
+            m_used = m_new;
+            l *= alpha;
+          }
+          if (other_unit) {
+            const float next = fmaxf(most_vs, most_unit * 0x1p-60f);
+            alpha *= unit > 0.f ? unit / next : 0.f;
+            unit = next;
+            most_unit = fmaxf(most_unit, next);
+          }
+          if (j > 0 && __any_sync(ALL, alpha != 1.f)) {  // O holds tiles 0..j-1 of this item once the previous product has finished
+            if (!(ok = wait_or_abort(bar(PV_DONE0 + ((t - 1) & 1)), ((t - 1) >> 1) & 1, abort_flag))) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < G::OCH; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tmem_o + lane_addr + c * 32, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st32(tmem_o + lane_addr + c * 32, o);
+            }
+          }
+        }
+        const float msub = (m_used == -INFINITY) ? 0.f : m_used;
+        const float per_unit = unit > 0.f ? 1.f / unit : 0.f;
+        // p = 2^(s * scale - m), times V's scale for the product: two lanes at a time
+        const uint64_t nmsub2 = pack2(-msub, -msub);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint64_t scale2 = pack2(ks[g], ks[g]), vs2 = pack2(vs[g] * per_unit, vs[g] * per_unit);
+#pragma unroll
+          for (int c = g * 8; c < g * 8 + 8; ++c) {  // P is packed in place: s[c] <- (p[2c], p[2c+1])
+            float a0, a1;
+            unpack2(fma2(pack2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, nmsub2), a0, a1);
+            const uint64_t p2 = pack2(fast_exp2(a0), fast_exp2(a1));
+            sum2[c & 1] = add2(sum2[c & 1], p2);
+            unpack2(mul2(p2, vs2), a0, a1);
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(s[c]) : "f"(a1), "f"(a0));
+          }
+        }
+        {
+          float t0, t1, t2, t3;
+          unpack2(sum2[0], t0, t1);
+          unpack2(sum2[1], t2, t3);
+          l += (t0 + t1) + (t2 + t3);
+        }
+        tmem_st32(scores, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(P_FULL0 + st));
+      }
+      if (!ok) break;
+      T += x.n_kv;
+      // the row's normaliser goes to the row warps; no key: zeros; a sum that is NaN stays one
+      inv_buf[(it & 1) * 128 + r] = l > 0.f ? unit / l : l;
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(EPI_FULL0 + (it & 1)));
+        mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ query rows in, V to f16, results out
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ROWS));
+    const int ew = warp - 4, r = ew * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>(ew * 32) << 16;
+    unsigned char* stage = base_ptr + G::OFF_STAGE + ew * 2048;
+    // Thread = query row: its power of two, then high and low parts piece by piece.
+    auto take_rows = [&](const Fp8Item& x, int it) {
+      const int tok = token_of(r), hh = r - tok * pack;
+      const bool live = tok < min(BMT, x.Lq - x.m0);
+      const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(x.q0 + x.m0 + (live ? tok : 0)) * p.q_stride + (x.h + hh) * D);
+      uint32_t m = 0;
+      if (live) {
+#pragma unroll 2
+        for (int c = 0; c < D / 16; ++c) {
+          const uint4 a = __ldg(src + 2 * c), b = __ldg(src + 2 * c + 1);
+          m = max_finite2(max_finite2(max_finite2(max_finite2(m, a.x), a.y), a.z), a.w);
+          m = max_finite2(max_finite2(max_finite2(max_finite2(m, b.x), b.y), b.z), b.w);
+        }
+      }
+      m = max(m & 0xffffu, m >> 16);
+      const int e = max(static_cast<int>(m >> 7), 20) - 127;  // 2^e <= max |q| < 2^(e + 1)
+      const float f = power_of_two(7 - e);
+      row_factor[(it & 1) * 128 + r] = p.scale_log2e * power_of_two(e - 7);
+#pragma unroll 1
+      for (int c = 0; c < D / 16; ++c) {
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint4 a = live ? __ldg(src + 2 * c + half) : make_uint4(0, 0, 0, 0);
+          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float y0 = __uint_as_float(w[i] << 16) * f, y1 = __uint_as_float(w[i] & 0xffff0000u) * f;
+            y0 = fabsf(y0) <= 448.f ? y0 : NAN;  // infinities: the row is NaN
+            y1 = fabsf(y1) <= 448.f ? y1 : NAN;
+            const uint32_t h = e4m3x2(y0, y1);
+            const float2 back = float2_of_f16x2(f16x2_of_low(h));
+            const uint32_t l2 = e4m3x2(y0 - back.x, y1 - back.y);
+            const int at = 2 * half + (i >> 1);
+            if (i & 1) hi[at] |= h << 16, lo[at] |= l2 << 16;
+            else hi[at] = h, lo[at] = l2;
+          }
+        }
+        unsigned char* to = base_ptr + G::OFF_Q + code_piece<D>(r, c);
+        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(to + G::Q_PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(Q_FULL));
+        mbar_arrive(bar(FACTOR0 + (it & 1)));
+      }
+    };
+    // Tile t (the j-th of item x) of V: 16 codes at a time to two 16-byte pieces of f16.
+    auto convert = [&](const Fp8Item& x, int j, int t) {
+      const int st = t & 1, use = t >> 1;
+      if (!wait_or_abort(bar(RAW_FULL0 + st), use & 1, abort_flag)) return false;
+      if (use > 0 && !wait_or_abort(bar(PV_DONE0 + st), (use - 1) & 1, abort_flag)) return false;
+      const unsigned char* raw = base_ptr + G::OFF_RAW + st * G::K_BYTES;
+      unsigned char* vt = base_ptr + G::OFF_V + st * G::V_BYTES;
+      const int rows = x.Lk - j * BN;  // that hold a token
+      constexpr int PIECES = D / 16;
+      uint4 code[BN * PIECES / 128];
+#pragma unroll
+      for (int i = 0; i < BN * PIECES / 128; ++i) {
+        const int idx = i * 128 + r, row = idx / PIECES, c = idx % PIECES;
+        code[i] = *reinterpret_cast<const uint4*>(raw + code_piece<D>(row, c));
+        if (row >= rows) code[i] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < BN * PIECES / 128; ++i) {
+        const int idx = i * 128 + r, row = idx / PIECES, c = idx % PIECES;
+        unsigned char* sub = vt + (c >> 2) * G::V_SUB + row * 128;
+        const int c0 = (c & 3) * 2;
+        *reinterpret_cast<uint4*>(sub + ((c0 ^ (row & 7)) << 4)) =
+            make_uint4(f16x2_of_low(code[i].x), f16x2_of_high(code[i].x), f16x2_of_low(code[i].y), f16x2_of_high(code[i].y));
+        *reinterpret_cast<uint4*>(sub + (((c0 + 1) ^ (row & 7)) << 4)) =
+            make_uint4(f16x2_of_low(code[i].z), f16x2_of_high(code[i].z), f16x2_of_low(code[i].w), f16x2_of_high(code[i].w));
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(V_FULL0 + st));
+        mbar_arrive(bar(RAW_FREE0 + st));
+      }
+      return true;
+    };
+    int T = 0;
+    bool ok = wait_or_abort(bar(ITEM_FULL0), 0, abort_flag);
+    Fp8Item x;
+    x.n_kv = -1;
+    if (ok) x = read_item(0);
+    if (ok && x.n_kv > 0) {
+      take_rows(x, 0);
+      ok = convert(x, 0, 0);
+    }
+#pragma unroll 1
+    for (int it = 0; ok && x.n_kv > 0; ++it) {
+#pragma unroll 1
+      for (int j = 1; ok && j < x.n_kv; ++j) ok = convert(x, j, T + j);
+      if (!ok) break;
+      // the next item's rows and first tile before this one's results, so that its products run under their writing
+      const int last = T + x.n_kv - 1;
+      if (!(ok = wait_or_abort(bar(ITEM_FULL0 + ((it + 1) & 1)), ((it + 1) >> 1) & 1, abort_flag))) break;
+      const Fp8Item next = read_item(it + 1);
+      if (next.n_kv > 0) {
+        if (!(ok = wait_or_abort(bar(QK_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag))) break;
+        take_rows(next, it + 1);
+        if (!(ok = convert(next, 0, last + 1))) break;
+      }
+      T += x.n_kv;
+      if (!(ok = wait_or_abort(bar(EPI_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
+      const float inv = inv_buf[(it & 1) * 128 + r];
+      if (!(ok = wait_or_abort(bar(PV_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag))) break;
+      tc_fence_after();
+      // O / l -> bf16, 32 columns at a time through this warp's patch of shared memory
+      const int srow = lane >> 2, spiece = lane & 3;
+      __nv_bfloat16* out_tile = p.out + static_cast<int64_t>(x.q0 + x.m0) * p.out_stride + x.h * D;
+      const int toks_valid = min(BMT, x.Lq - x.m0);
+#pragma unroll 1
+      for (int c = 0; c < G::OCH; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + lane_addr + c * 32, o);
+        tmem_wait_ld();
+        if (c == G::OCH - 1) {  // O is in registers: the next item's first product may overwrite it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(O_FREE));
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint4 v;
+          v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
+          v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
+          v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
+          v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = v;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int lr = i * 8 + srow, row = ew * 32 + lr;
+          const int tok = token_of(row), hh = row - tok * pack;
+          const uint4 v = *reinterpret_cast<const uint4*>(stage + lr * 64 + ((spiece ^ ((lr >> 1) & 3)) << 4));
+          if (tok < toks_valid)
+            *reinterpret_cast<uint4*>(out_tile + static_cast<int64_t>(tok) * p.out_stride + hh * D + c * 32 + spiece * 8) = v;
+        }
+        __syncwarp();
+      }
+      if (lane == 0) mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
+      x = next;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(p.status, NVLLM_STATUS_TIMEOUT);
+  if (warp == 10) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------------
+
+// Heads packed into a query tile: the largest divisor of the group size that is at most 8.
+static int heads_in_tile(int g) {
+  int pack = 1;
+  for (int n = 2; n <= 8; ++n)
+    if (g % n == 0) pack = n;
+  return pack;
+}
+
+template <int D>
+static int launch_prefill_fp8(PrefillFp8Params& p, const void* k_cache, const void* v_cache, int max_seqlen_q, cudaStream_t stream) {
+  using G = f8::Geo<D>;
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return fail(NVLLM_E_NO_DEVICE, "prefill_fp8: device index %d out of range", dev);
+  if (!ready[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
+    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "prefill_fp8: set-up failed: %s", cudaGetErrorString(e));
+    // The warp groups trade registers inside the pool the block gets at launch: a build with fewer could never satisfy the
+    // softmax group's request, and that request waits without a bound.
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, prefill_fp8_kernel<D>);
+    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "prefill_fp8: set-up failed: %s", cudaGetErrorString(e));
+    if (attr.numRegs < f8::REGS_LAUNCH)
+      return fail(NVLLM_E_CUDA, "prefill_fp8: built with %d registers per thread, the warp groups' hand-over needs %d", attr.numRegs,
+                  f8::REGS_LAUNCH);
+    ready[dev] = true;
+  }
+  p.pack = heads_in_tile(p.g);
+  p.tile_tokens = f8::BM / p.pack;
+  p.inv_pack = 65536 / p.pack + 1;  // exact for rows of a tile
+  CUtensorMap mk, mv;
+  const uint64_t slots = static_cast<uint64_t>(p.num_blocks) * kBlockSize;
+  if (!make_tmap_codes(&mk, k_cache, D, p.hkv, slots, f8::BN) || !make_tmap_codes(&mv, v_cache, D, p.hkv, slots, f8::BN)) return NVLLM_E_CUDA;
+  const int64_t items = static_cast<int64_t>((max_seqlen_q + p.tile_tokens - 1) / p.tile_tokens) * (p.hq / p.pack) * p.batch;  // at most
+  const int grid = static_cast<int>(std::min<int64_t>(2ll * num_sms(), items));
+  return launch_kernel("prefill_fp8", prefill_fp8_kernel<D>, dim3(grid), dim3(f8::NTHREADS), G::SMEM, stream, p, mk, mv);
+}
+
+}  // namespace nvllm
+
+extern "C" int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
+                                        const float* k_scale, const float* v_scale, const int32_t* block_tables,
+                                        int64_t bt_row_stride, int32_t max_blocks, void* out, int64_t out_row_stride,
+                                        const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t total_q, int32_t batch,
+                                        int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_q_heads, int32_t num_kv_heads,
+                                        int32_t head_dim, float scale, int64_t num_blocks, void* stream) {
+  using namespace nvllm;
+  const char* who = "prefill_varlen_fp8";
+  if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || total_q < 0)
+    return fail(NVLLM_E_GEOMETRY, "%s: negative batch, max_seqlen or total_q", who);
+  if (batch > f8::MAX_BATCH) return fail(NVLLM_E_GEOMETRY, "%s: batch=%d exceeds the %d sequences of one launch", who, batch, f8::MAX_BATCH);
+  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || num_q_heads > 65535)
+    return fail(NVLLM_E_GEOMETRY, "%s: Hq=%d must be a positive multiple of Hkv=%d, at most 65535", who, num_q_heads, num_kv_heads);
+  if (!(scale >= 0.f && scale < INFINITY)) return fail(NVLLM_E_GEOMETRY, "%s: scale must be finite and not negative", who);
+  if (batch == 0 || max_seqlen_q == 0 || total_q == 0) return NVLLM_OK;
+  const int rc = check_fp8_planes(who, k_cache, v_cache, k_scale, v_scale, num_kv_heads, head_dim, num_blocks);
+  if (rc) return rc;
+  if (!q || !out || !cu_seqlens_q || !cu_seqlens_k || !block_tables) return fail(NVLLM_E_NULL, "%s: NULL pointer argument", who);
+  const int64_t qrow = static_cast<int64_t>(num_q_heads) * head_dim;
+  if (q_row_stride < qrow || out_row_stride < qrow || max_blocks <= 0 || bt_row_stride < max_blocks)
+    return fail(NVLLM_E_GEOMETRY, "%s: a row stride is smaller than its row", who);
+  if (static_cast<int64_t>(max_blocks) * kBlockSize > 0x7fffffffLL)
+    return fail(NVLLM_E_GEOMETRY, "%s: max_blocks=%d too large", who, max_blocks);
+  if (q_row_stride % 8 || out_row_stride % 8 || !aligned16(q) || !aligned16(out))
+    return fail(NVLLM_E_ALIGN, "%s: q/out pointers and row strides must be 16-byte aligned", who);
+  PrefillFp8Params p;
+  p.status = status_word();
+  if (!p.status) return fail(NVLLM_E_NO_DEVICE, "%s: no CUDA device is usable", who);
+  p.q = static_cast<const __nv_bfloat16*>(q);
+  p.q_stride = q_row_stride;
+  p.k_scale = k_scale;
+  p.v_scale = v_scale;
+  p.block_tables = block_tables;
+  p.bt_stride = bt_row_stride;
+  p.max_blocks = max_blocks;
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.out_stride = out_row_stride;
+  p.cu_q = cu_seqlens_q;
+  p.cu_k = cu_seqlens_k;
+  p.batch = batch;
+  p.hq = num_q_heads;
+  p.hkv = num_kv_heads;
+  p.g = num_q_heads / num_kv_heads;
+  p.scale_log2e = scale * 1.4426950408889634f;
+  p.num_blocks = num_blocks;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128) return launch_prefill_fp8<128>(p, k_cache, v_cache, max_seqlen_q, st);
+  return launch_prefill_fp8<64>(p, k_cache, v_cache, max_seqlen_q, st);
+}

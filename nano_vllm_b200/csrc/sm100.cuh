@@ -20,6 +20,10 @@ namespace sm100 {
 bool make_tmap_3d(CUtensorMap* map, const void* base, uint64_t head_dim, uint64_t heads, uint64_t rows,
                   uint64_t head_stride_elems, uint64_t row_stride_elems, uint32_t box_rows, uint32_t box_heads = 1);
 
+// The same of 8-bit codes [rows, heads, head_dim] (64 or 128), contiguous, with a {head_dim, 1, box_rows} box: rows of 128 bytes
+// under the 128-byte swizzle, or of 64 under the 64-byte one.
+bool make_tmap_codes(CUtensorMap* map, const void* base, uint32_t head_dim, uint64_t heads, uint64_t rows, uint32_t box_rows);
+
 #ifdef __CUDACC__
 
 constexpr long long kWaitLimitCycles = 2000000000ll;  // a wait gives up after ~1 s of SM clocks

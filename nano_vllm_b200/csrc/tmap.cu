@@ -50,5 +50,24 @@ bool make_tmap_3d(CUtensorMap* map, const void* base, uint64_t head_dim, uint64_
   return true;
 }
 
+bool make_tmap_codes(CUtensorMap* map, const void* base, uint32_t head_dim, uint64_t heads, uint64_t rows, uint32_t box_rows) {
+  EncodeTiledFn enc = encoder();
+  if (!enc) {
+    fail(NVLLM_E_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+    return false;
+  }
+  const cuuint64_t dims[3] = {head_dim, heads, rows};
+  const cuuint64_t strides[2] = {head_dim, heads * head_dim};
+  const cuuint32_t box[3] = {head_dim, 1, box_rows};
+  const cuuint32_t elem_strides[3] = {1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, elem_strides,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return true;
+  fail(NVLLM_E_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d (codes, %llu x %llu x %llu)", (int)r, (unsigned long long)head_dim,
+       (unsigned long long)heads, (unsigned long long)rows);
+  return false;
+}
+
 }  // namespace sm100
 }  // namespace nvllm

@@ -62,3 +62,17 @@ def assert_within(out, ref, bound, what=""):
     over = (out - ref).abs() / bound.clamp(min=1e-30)
     over[(out == ref)] = 0
     assert over.max() <= 1, f"{what}: {over.max():.3g} times the bound at {tuple((over == over.max()).nonzero()[0].tolist())}"
+
+
+def prefill_reference(q, planes, cu_q, cu_k, tables, scale):
+    """The definition, and the bound with what the query's two e4m3 parts may add: values below 2^-10 of a row's largest are
+    off by 2^-17 of it at most, so a score by scale * 2^-17 * max|q| * sum |k|, and a weight by as much of itself."""
+    out, bound = F8.prefill_fp8_ref(q, *planes, cu_q, cu_k, scale, tables)
+    k, v, ks, vs = planes
+    most = 0.0
+    for b in range(len(cu_q) - 1):
+        n = int(cu_k[b + 1] - cu_k[b])
+        if n and cu_q[b + 1] > cu_q[b]:
+            most = max(most, float(F8.gather(k, ks, tables[b], n).abs().sum(-1).max()) * float(q[cu_q[b]:cu_q[b + 1]].abs().max()))
+    extra = 2 * scale * 2.0 ** -17 * most
+    return out, bound * (1 + extra / (1.5 * 2.0 ** -11))

@@ -20,6 +20,7 @@ def test_there_is_no_cpu_fallback():
     for call in (lambda: A.store_kvcache_fp8(q[:, :2], q[:, :2], c, c, s, s, i),
                  lambda: A.decode_paged_fp8(q, c, c, s, s, i, i.view(2, 1), 0.1),
                  lambda: A.decode_step_fp8(q, q[:, :2], q[:, :2], c, c, s, s, i, i, i.view(2, 1), 0.1),
+                 lambda: A.prefill_varlen_fp8(q, c, c, s, s, i, i, 2, 2, 0.1, i.view(2, 1)),
                  lambda: step_maps(i, i, i.view(2, 1), i, 4)):
         with pytest.raises(RuntimeError, match="CUDA"):
             call()
@@ -41,7 +42,7 @@ def test_store_refuses(lib, change, code):
     ({"q": NULL}, -1), ({"kc": NULL}, -1), ({"ks": NULL}, -1), ({"lens": NULL}, -1), ({"bt": NULL}, -1), ({"out": NULL}, -1),
     ({"q": P8}, -2), ({"out_stride": 2052}, -2), ({"q_stride": 1024}, -3), ({"bt_stride": 8}, -3), ({"vs": P8}, -2), ({"d": 96}, -3),
     ({"hq": 12}, -3), ({"hq": 128}, -3), ({"blocks": 0}, -3), ({"ws": NULL}, -4), ({"ws_bytes": 100}, -4), ({"ws": P8}, -2),
-    ({"batch": 4096}, -3), ({"batch": 0}, 0)])
+    ({"batch": 4096}, -3), ({"batch": 0}, 0), ({"scale": ctypes.c_float(-0.1)}, -3)])
 def test_decode_refuses(lib, change, code):
     a = dict(q=P16, q_stride=2048, kc=P16, vc=P16, ks=P16, vs=P16, lens=P16, bt=P16, bt_stride=16, width=16, out=P16, out_stride=2048,
              batch=2, hq=16, hkv=8, d=128, scale=F, blocks=100, ws=P16, ws_bytes=1 << 30)
@@ -60,6 +61,18 @@ def test_step_refuses(lib, change, code):
              ws_bytes=1 << 30)
     a.update(change)
     assert lib.nvllm_decode_step_fp8(*a.values(), None) == code
+
+
+@pytest.mark.parametrize("change,code", [
+    ({"q": NULL}, -1), ({"vc": NULL}, -1), ({"ks": NULL}, -1), ({"bt": NULL}, -1), ({"cu_k": NULL}, -1), ({"out": NULL}, -1), ({"q": P8}, -2),
+    ({"ks": P8}, -2), ({"q_stride": 2052}, -2), ({"out_stride": 8}, -3), ({"bt_stride": 1}, -3), ({"width": 0}, -3), ({"batch": 1025}, -3),
+    ({"batch": -1}, -3), ({"hq": 15}, -3), ({"d": 32}, -3), ({"blocks": 0}, -3), ({"scale": ctypes.c_float(-1)}, -3),
+    ({"scale": ctypes.c_float(float("nan"))}, -3), ({"batch": 0}, 0), ({"total": 0}, 0), ({"max_q": 0}, 0)])
+def test_prefill_refuses(lib, change, code):
+    a = dict(q=P16, q_stride=2048, kc=P16, vc=P16, ks=P16, vs=P16, bt=P16, bt_stride=4, width=4, out=P16, out_stride=2048, cu_q=P16, cu_k=P16,
+             total=100, batch=2, max_q=60, max_k=600, hq=16, hkv=8, d=128, scale=F, blocks=10)
+    a.update(change)
+    assert lib.nvllm_prefill_varlen_fp8(*a.values(), None) == code
 
 
 @pytest.mark.parametrize("change,code", [
