@@ -96,15 +96,6 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t a) {
   return v;
 }
 __device__ __forceinline__ void st_shared_f32(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(a), "f"(v) : "memory"); }
-__device__ __forceinline__ uint2 ld_shared8(uint32_t a) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ void st_shared8(uint32_t a, const uint2& v) {
-  asm volatile("st.shared.v2.u32 [%0], {%1,%2};\n" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
-}
-
 // Where piece c of row r of a tile lies: so that eight rows' pieces c, and two rows' pieces of one half, are in different banks.
 template <int D>
 __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
@@ -322,10 +313,10 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
 
   float o[C::KS][4];     // columns 16 c + 2 gid (and + 1 in [2], [3]) of heads 2 tig ([0], [2]) and 2 tig + 1, in units of `unit`
   float m0, m1, l0, l1;  // heads 2 tig and 2 tig + 1
-  // The power of two that O is held in (the same for all lanes of the warp): a group's P goes into its product times
-  // vscale / unit <= 1.  It grows at once to the largest scale of a tile and shrinks where that is 16 times smaller, so that
-  // a group's P loses four bits of f16's range at most; not below 2^-60 of what it has been, which keeps O finite whatever the
-  // scales.
+  // What O is held in (the same for all lanes of the warp): a group's P goes into its product times vscale / unit.  It is the
+  // largest scale of the first tile, changed where a tile's largest is more than 64 times larger or 16 times smaller, so that
+  // P stays below f16's end and loses four bits of its range at most; not below 2^-60 of what it has been, which keeps O
+  // finite whatever the scales.
   float unit, most_unit;
   auto reset_state = [&]() {
 #pragma unroll
@@ -598,7 +589,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
     float alpha0 = fast_exp2(m0 - mn0), alpha1 = fast_exp2(m1 - mn1);
     l0 *= alpha0;
     l1 *= alpha1;
-    if (most_vs > unit || (most_vs > 0.f && most_vs * 16.f < unit)) {
+    if (most_vs > unit * 64.f || (most_vs > 0.f && most_vs * 16.f < unit)) {
       const float next = fmaxf(most_vs, most_unit * 0x1p-60f), change = unit > 0.f ? unit / next : 0.f;
       alpha0 *= change;
       alpha1 *= change;

@@ -8,14 +8,16 @@
 //     2^-10 of the row's largest value, below that within 2^-17 of it.  Two products at twice the rate of a 16-bit one: the
 //     same time, and no key has to be converted.
 //   * The K scale of a group and the row's power of two enter the multiply-add in front of the exponential, four factors a tile.
-//   * O += P V in f16 (kind::f16): P from TMEM, rounded to f16 (2^-11); V's codes are converted to f16, exactly, once a tile by
-//     the warps that also write results.  P carries the group's V scale over a running unit, a power of two that O is held
-//     in: it grows at once with the largest scale of a tile and shrinks where that is 16 times smaller.
+//   * O += P V in f16 (kind::f16): P from TMEM, rounded to f16 (2^-11); V's codes become f16 once a tile, by the warps that also
+//     write results, times the group's scale over the unit that O is held in: the largest scale of an item's first tile,
+//     changed (and O with it) where a tile's largest is more than 2^7 times larger or 2^14 times smaller, which keeps every
+//     V / unit an f16 number; not below 2^-60 of what it has been, which keeps O finite whatever the scales.  Exact for scales
+//     that are powers of two, two more roundings to f16 for others.
 //   * Keys past the end: their scores are masked, their V rows converted to zeros whatever the codes are.
 //
 // Twelve warps, two blocks to an SM for the whole launch: 0-3 softmax (thread = query row), 4-7 query rows in, V conversion and
-// results out, 8 = TMA of K and of the scales, 9 = MMA issuer, 10 = TMA of V.  The three warp groups trade registers at
-// start-up.  Items (query tile of a sequence, head group) are ordered by their key tiles, most first, over all sequences, and
+// results out, 8 = TMA of the query rows, K and the scales, 9 = MMA issuer, 10 = TMA of V.  The three warp groups trade registers at
+// start-up; 11 works out the items, one ahead.  Items (query tile of a sequence, head group) are ordered by their key tiles, most first, over all sequences, and
 // dealt out in turn, there and back again, so that all blocks have about the same to do; no counter in memory, so nothing is
 // shared by launches.
 #include <algorithm>
@@ -34,11 +36,11 @@ constexpr int NTHREADS = 384;
 constexpr int REGS_LAUNCH = 80, REGS_SOFTMAX = 136, REGS_ROWS = 64, REGS_OTHER = 40;
 static_assert(128 * (REGS_SOFTMAX + REGS_ROWS + REGS_OTHER) <= NTHREADS * REGS_LAUNCH, "register pool of a block");
 constexpr int TMEM_COLS = 256, TMEM_O = 128;  // S / P buffers [0,64) and [64,128), O [128,256)
-constexpr float kRescaleThreshold = 8.f;      // log2 units
+constexpr float kRescaleThreshold = 14.f;     // log2 units: P stays below 2^15, f16 goes to 2^16
 enum Bar {
   Q_FULL, K_FULL0, K_FULL1, RAW_FULL0, RAW_FULL1, RAW_FREE0, RAW_FREE1, V_FULL0, V_FULL1, QK_DONE0, QK_DONE1, PV_DONE0, PV_DONE1,
   P_FULL0, P_FULL1, ITEM_FULL0, ITEM_FULL1, ITEM_FREE0, ITEM_FREE1, O_FREE, EPI_FULL0, EPI_FULL1,
-  SCALES0, SCALES1, SCALES2, SCALES3, FACTOR0, FACTOR1, DRAIN, NUM_BARS
+  INFO0, INFO1, INFO2, INFO3, FACTOR0, FACTOR1, ROWS_FULL, DRAIN, NUM_BARS
 };
 static_assert(NUM_BARS <= 32, "a barrier per lane");
 
@@ -50,12 +52,14 @@ struct Geo {
   static constexpr int V_SUB = BN * 128, V_BYTES = D / 64 * V_SUB;  // f16, 64 columns to a sub-tile
   static constexpr int OFF_Q = 0, OFF_K = OFF_Q + Q_BYTES, OFF_RAW = OFF_K + KST * K_BYTES, OFF_V = OFF_RAW + KST * K_BYTES;
   static constexpr int OFF_STAGE = OFF_V + KST * V_BYTES;          // 4 warps x 32 rows x 64 B of output
-  static constexpr int OFF_CTRL = OFF_STAGE + 4 * 2048;            // barriers
+  // query rows as they are: D = 128 where their parts go (there is no room), D = 64 in a place of their own
+  static constexpr int OFF_ROWS = D == 128 ? OFF_Q : OFF_STAGE + 4 * 2048;
+  static constexpr int OFF_CTRL = OFF_STAGE + 4 * 2048 + (D == 128 ? 0 : BM * 128);  // barriers
   static constexpr int OFF_SLOTS = OFF_CTRL + 256;                 // two item descriptors of 8 ints
   static constexpr int OFF_MISC = OFF_SLOTS + 64;                  // TMEM address, abort flag
-  static constexpr int OFF_SCALES = OFF_MISC + 64;                 // 4 tiles x (4 of K, 4 of V)
-  static constexpr int OFF_ROW = OFF_SCALES + 128;                 // 2 items x 128 rows: the query row's power of two
-  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: unit / row sum
+  static constexpr int OFF_TILES = OFF_MISC + 64;                  // 4 tiles: see Fp8Tile
+  static constexpr int OFF_ROW = OFF_TILES + 256;                  // 2 items x 128 rows: the query row's power of two
+  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: 1 / row sum
   static constexpr int SMEM = OFF_INV + 2 * 128 * 4 + 1024;
   static constexpr int SBO = D == 128 ? 1024 : 512;                // eight rows of codes
   static constexpr int OCH = D / 32;
@@ -108,9 +112,27 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uin
 __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return idesc_f8(m, n) | (1u << 16); }
 
-__device__ __forceinline__ void bulk_copy16(uint32_t dst, const void* src, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst), "l"(src), "r"(bar)
-               : "memory");
+__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
+
+// A tile's scales: K's; V's over the unit, as f16 pairs; what O is multiplied by (where the unit changes); the unit.
+struct __align__(16) Fp8Tile {
+  float k[4];
+  uint32_t v[4];
+  float change, unit, pad[2];
+};
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// The larger of the magnitudes of two bf16, twice; the sign bits are anything.  NaN wins.
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 struct Fp8Item {
@@ -133,7 +155,8 @@ __device__ __forceinline__ int fp8_tiles_above(int x, int Lq, int Lk, int bmt) {
 
 template <int D>
 __global__ void __launch_bounds__(f8::NTHREADS, 2)
-prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v) {
+prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                   const __grid_constant__ CUtensorMap tmap_v) {
   using namespace f8;
   using G = Geo<D>;
   constexpr unsigned ALL = 0xffffffffu;
@@ -153,13 +176,13 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
   pdl_trigger();
   if (warp == 9 && lane < NUM_BARS) {
     // by the four warps of a group: query rows, V, P, normalisers, O; an item slot is free when the softmax (4), the row (4)
-    // warps, the MMA issuer and the V producer are done with it
-    const bool by_four = lane == Q_FULL || lane == RAW_FREE0 || lane == RAW_FREE1 || lane == V_FULL0 || lane == V_FULL1 ||
-                         lane == P_FULL0 || lane == P_FULL1 || lane == O_FREE || lane == EPI_FULL0 || lane == EPI_FULL1 ||
-                         lane == FACTOR0 || lane == FACTOR1;
-    mbar_init(bar(lane), by_four ? 4u : lane == ITEM_FREE0 || lane == ITEM_FREE1 ? 10u : 1u);
+    // warps, the MMA issuer and the two producers are done with it
+    const bool by_four = lane == Q_FULL || lane == RAW_FREE0 || lane == RAW_FREE1 || lane == V_FULL0 || lane == V_FULL1 || lane == P_FULL0 ||
+                         lane == P_FULL1 || lane == O_FREE || lane == EPI_FULL0 || lane == EPI_FULL1 || lane == FACTOR0 || lane == FACTOR1;
+    mbar_init(bar(lane), by_four ? 4u : lane == ITEM_FREE0 || lane == ITEM_FREE1 ? 11u : 1u);
     if (lane == 0) {
       *abort_flag = 0;
+      prefetch_tmap(&tmap_q);
       prefetch_tmap(&tmap_k);
       prefetch_tmap(&tmap_v);
     }
@@ -185,111 +208,87 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
     const int i = j * BN / kBlockSize;
     const int64_t blk = i < p.max_blocks ? p.block_tables[x.b * p.bt_stride + i] : -1;
     if (blk >= 0 && blk < p.num_blocks) return blk;
-    atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
+    if (lane == 0) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
     return 0;
   };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
     if (warp == 8) {
-      // ---------------------------------------------------------------- items; TMA of K and the scales
-      const int hgroups = p.hq / pack;
-      // Query tiles of all sequences that see more than x key tiles.
-      auto above = [&](int x) {
-        int n = 0;
-#pragma unroll 1
-        for (int b = lane; b < p.batch; b += 32) n += fp8_tiles_above(x, lens(b).x, lens(b).y, BMT);
-        return __reduce_add_sync(ALL, static_cast<unsigned>(n));
-      };
-      int longest = 0;
-#pragma unroll 1
-      for (int b = lane; b < p.batch; b += 32) longest = max(longest, lens(b).y);
-      longest = (__reduce_max_sync(ALL, longest) + BN - 1) / BN;
-      const unsigned total = above(0) * hgroups;  // items; tiles that see no key are none
-      int T = 0, loaded = 0;
+      // ---------------------------------------------------------------- TMA of the query rows and K; the scales
+      const int g = lane & 3;
+      int T = 0, loaded = 0, rows_loaded = 0;
+      float most_unit = 0.f, unit = 0.f;
       bool ok = true;
 #pragma unroll 1
-      for (int it = 0;; ++it) {
-        const unsigned drawn = it * gridDim.x + (it & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        Fp8Item x{};
-        x.n_kv = -1;
-        if (drawn < total) {
-          const unsigned rank = drawn / hgroups;
-          x.h = (drawn - rank * hgroups) * pack;
-          int lo = 1, hi = longest;  // its key tiles: the least n with above(n) <= rank (above(longest) = 0)
-#pragma unroll 1
-          while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (above(mid) <= rank) hi = mid;
-            else lo = mid + 1;
-          }
-          x.n_kv = lo;
-          unsigned k = rank - above(lo);  // its number among the tiles with as many
-#pragma unroll 1
-          for (int b0 = 0; b0 < p.batch; b0 += 32) {
-            const int b = b0 + lane;
-            unsigned n = 0;
-            if (b < p.batch) {
-              const int2 len = lens(b);
-              n = fp8_tiles_above(lo - 1, len.x, len.y, BMT) - fp8_tiles_above(lo, len.x, len.y, BMT);
-            }
-            unsigned incl = n;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-              const unsigned v = __shfl_up_sync(ALL, incl, d);
-              if (lane >= d) incl += v;
-            }
-            const unsigned hit = __ballot_sync(ALL, incl > k);
-            if (hit) {
-              const int src = __ffs(hit) - 1;
-              x.b = b0 + src;
-              k -= __shfl_sync(ALL, incl - n, src);
-              break;
-            }
-            k -= __shfl_sync(ALL, incl, 31);
-          }
-          x.Lq = lens(x.b).x;
-          x.Lk = lens(x.b).y;
-          x.q0 = p.cu_q[x.b];
-          x.m0 = ((x.Lq + BMT - 1) / BMT - 1 - fp8_tiles_above(lo, x.Lq, x.Lk, BMT) - static_cast<int>(k)) * BMT;
-        }
-        if (it >= 2) ok = wait_or_abort(bar(ITEM_FREE0 + (it & 1)), ((it >> 1) - 1) & 1, abort_flag);
-        if (!__all_sync(ALL, ok)) break;
-        if (lane == 0) {
-          volatile int* s = slots + (it & 1) * 8;
-          s[0] = x.b; s[1] = x.h; s[2] = x.m0; s[3] = x.q0;
-          s[4] = x.Lq; s[5] = x.Lk; s[6] = x.n_kv;
-          mbar_arrive(bar(ITEM_FULL0 + (it & 1)));
-        }
-        __syncwarp();
+      for (int it = 0; ok; ++it) {
+        ok = __all_sync(ALL, wait_or_abort(bar(ITEM_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag));
+        if (!ok) break;
+        const Fp8Item x = read_item(it);
         if (x.n_kv < 0) break;
-        if (elect_one()) {
-          const int kvh = x.h / p.g;
+        const int kvh = x.h / p.g;
+        int64_t blk = block_of(x, 0);
+        auto scale_at = [&](int j) { return (blk * p.hkv + kvh) * kGroups + j * BN % kBlockSize / kScaleGroup + g; };
+        float k = p.k_scale[scale_at(0)], v = p.v_scale[scale_at(0)];  // of tile j, group g
 #pragma unroll 1
-          for (int j = 0; j < x.n_kv; ++j) {
-            const int t = T + j, st = t & 1, use = t >> 1;
-            const int64_t blk = block_of(x, j);
-            if (use > 0 && !(ok = wait_or_abort(bar(QK_DONE0 + st), (use - 1) & 1, abort_flag))) break;
-            // K's stage is free, and so are the scales of tile t - 4: its softmax came before the scores of tile t - 2
-            const int64_t at = (blk * p.hkv + kvh) * kGroups + j * BN % kBlockSize / kScaleGroup;
-            const uint32_t sc = base + G::OFF_SCALES + (t & 3) * 32;
-            mbar_expect_tx(bar(SCALES0 + (t & 3)), 32);
-            bulk_copy16(sc, p.k_scale + at, bar(SCALES0 + (t & 3)));
-            bulk_copy16(sc + 16, p.v_scale + at, bar(SCALES0 + (t & 3)));
-            mbar_expect_tx(bar(K_FULL0 + st), G::K_BYTES);
-            tma_load_3d(base + G::OFF_K + st * G::K_BYTES, &tmap_k, bar(K_FULL0 + st), 0, kvh, static_cast<int>(blk * kBlockSize + j * BN % kBlockSize));
-            ++loaded;
+        for (int j = 0; j < x.n_kv; ++j) {
+          const int t = T + j, st = t & 1, use = t >> 1;
+          const int row = static_cast<int>(blk * kBlockSize + j * BN % kBlockSize);
+          float k_next = 0.f, v_next = 0.f;
+          if (j + 1 < x.n_kv) {
+            if ((j + 1) % (kBlockSize / BN) == 0) blk = block_of(x, j + 1);
+            k_next = p.k_scale[scale_at(j + 1)], v_next = p.v_scale[scale_at(j + 1)];
           }
-          if (!ok) {  // gave up: no copy is in flight when the block ends
-#pragma unroll 1
-            for (int t = max(loaded - 4, 0); t < loaded; ++t) {
-              if (t >= loaded - 2) (void)mbar_wait(bar(K_FULL0 + (t & 1)), (t >> 1) & 1);
-              (void)mbar_wait(bar(SCALES0 + (t & 3)), (t >> 2) & 1);
+          ok = __all_sync(ALL, use == 0 || wait_or_abort(bar(QK_DONE0 + st), (use - 1) & 1, abort_flag));
+          if (!ok) break;
+          // K's stage is free, and so is the record of tile t - 4: its softmax came before the scores of tile t - 2
+          if (lane == 0) {
+            mbar_expect_tx(bar(K_FULL0 + st), G::K_BYTES);
+            tma_load_3d(base + G::OFF_K + st * G::K_BYTES, &tmap_k, bar(K_FULL0 + st), 0, kvh, row);
+          }
+          ++loaded;
+          if (j * BN + g * kScaleGroup >= x.Lk) k = 1.f, v = 0.f;  // a group behind the end may hold anything
+          float most = fmaxf(v, __shfl_xor_sync(ALL, v, 1));
+          most = fmaxf(most, __shfl_xor_sync(ALL, most, 2));
+          const float before = unit;
+          if (j == 0) unit = most_unit = most;
+          else if (most > unit * 128.f || (most > 0.f && most * 0x1p14f < unit)) unit = fmaxf(most, most_unit * 0x1p-60f);
+          most_unit = fmaxf(most_unit, unit);
+          Fp8Tile& tile = *reinterpret_cast<Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile));
+          if (lane < 4) {
+            const float ratio = unit > 0.f ? v / unit : 0.f;
+            tile.k[g] = k;
+            asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(tile.v[g]) : "f"(ratio));
+            if (g == 0) {
+              tile.change = j > 0 && unit != before ? before / unit : 1.f;
+              tile.unit = unit;
             }
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(INFO0 + (t & 3)));
+          k = k_next, v = v_next;
+          if (j == 0) {
+            // The query rows, as they are: their place is free once the previous item's last scores are there, or, in a place of
+            // their own, once its rows have been taken.
+            if constexpr (D == 128) ok = __all_sync(ALL, t == 0 || wait_or_abort(bar(QK_DONE0 + ((t - 1) & 1)), ((t - 1) >> 1) & 1, abort_flag));
+            else ok = __all_sync(ALL, it == 0 || wait_or_abort(bar(FACTOR0 + ((it - 1) & 1)), ((it - 1) >> 1) & 1, abort_flag));
+            if (!ok) break;
+            if (lane == 0) {
+              mbar_expect_tx(bar(ROWS_FULL), D / 64 * pack * BMT * 128);
+              tma_load_3d(base + G::OFF_ROWS, &tmap_q, bar(ROWS_FULL), 0, x.h, x.q0 + x.m0);
+              if constexpr (D == 128) tma_load_3d(base + G::OFF_ROWS + BM * 128, &tmap_q, bar(ROWS_FULL), 64, x.h, x.q0 + x.m0);
+            }
+            ++rows_loaded;
+          }
         }
-        if (!__all_sync(ALL, ok)) break;
+        if (!ok) break;
         T += x.n_kv;
+        if (lane == 0) mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
+      }
+      if (!ok) {  // gave up: no copy is in flight when the block ends
+#pragma unroll 1
+        for (int t = max(loaded - 2, 0); t < loaded; ++t) (void)mbar_wait(bar(K_FULL0 + (t & 1)), (t >> 1) & 1);
+        if (rows_loaded > 0) (void)mbar_wait(bar(ROWS_FULL), (rows_loaded - 1) & 1);
       }
     } else if (warp == 10) {
       // ---------------------------------------------------------------- TMA of V
@@ -302,10 +301,11 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           const Fp8Item x = read_item(it);
           if (x.n_kv < 0) break;
           const int kvh = x.h / p.g;
+          int64_t blk = 0;
 #pragma unroll 1
           for (int j = 0; j < x.n_kv; ++j) {
             const int t = T + j, st = t & 1, use = t >> 1;
-            const int64_t blk = block_of(x, j);
+            if (j % (kBlockSize / BN) == 0) blk = block_of(x, j);
             if (use > 0 && !(ok = wait_or_abort(bar(RAW_FREE0 + st), (use - 1) & 1, abort_flag))) break;
             mbar_expect_tx(bar(RAW_FULL0 + st), G::K_BYTES);
             tma_load_3d(base + G::OFF_RAW + st * G::K_BYTES, &tmap_v, bar(RAW_FULL0 + st), 0, kvh, static_cast<int>(blk * kBlockSize + j * BN % kBlockSize));
@@ -373,7 +373,86 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         }
       }
     } else {
-      // ---------------------------------------------------------------- rows of tiles that see no key: zeros
+      // ---------------------------------------------------------------- items, one ahead of the others; rows that see no key
+      const int hgroups = p.hq / pack;
+      // Query tiles of all sequences that see more than x key tiles.
+      const int2 mine = lane < p.batch ? lens(lane) : make_int2(0, 0);
+      auto length = [&](int b) { return b == lane ? mine : lens(b); };
+      auto above = [&](int x) {
+        int n = fp8_tiles_above(x, mine.x, mine.y, BMT);
+#pragma unroll 1
+        for (int b = lane + 32; b < p.batch; b += 32) {
+          const int2 len = lens(b);
+          n += fp8_tiles_above(x, len.x, len.y, BMT);
+        }
+        return __reduce_add_sync(ALL, static_cast<unsigned>(n));
+      };
+      int longest = 0;
+#pragma unroll 1
+      for (int b = lane; b < p.batch; b += 32) longest = max(longest, length(b).y);
+      longest = (__reduce_max_sync(ALL, longest) + BN - 1) / BN;
+      const unsigned total = above(0) * hgroups;  // items; tiles that see no key are none
+      bool ok = true;
+#pragma unroll 1
+      for (int it = 0;; ++it) {
+        const unsigned drawn = it * gridDim.x + (it & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        Fp8Item x{};
+        x.n_kv = -1;
+        if (drawn < total) {
+          const unsigned rank = drawn / hgroups;
+          x.h = (drawn - rank * hgroups) * pack;
+          int lo = 1, hi = longest;  // its key tiles: the least n with above(n) <= rank (above(longest) = 0)
+#pragma unroll 1
+          while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (above(mid) <= rank) hi = mid;
+            else lo = mid + 1;
+          }
+          x.n_kv = lo;
+          unsigned k = rank - above(lo);  // its number among the tiles with as many
+#pragma unroll 1
+          for (int b0 = 0; b0 < p.batch; b0 += 32) {
+            const int b = b0 + lane;
+            unsigned n = 0;
+            if (b < p.batch) {
+              const int2 len = length(b);
+              n = fp8_tiles_above(lo - 1, len.x, len.y, BMT) - fp8_tiles_above(lo, len.x, len.y, BMT);
+            }
+            unsigned incl = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+              const unsigned v = __shfl_up_sync(ALL, incl, d);
+              if (lane >= d) incl += v;
+            }
+            const unsigned hit = __ballot_sync(ALL, incl > k);
+            if (hit) {
+              const int src = __ffs(hit) - 1;
+              x.b = b0 + src;
+              k -= __shfl_sync(ALL, incl - n, src);
+              break;
+            }
+            k -= __shfl_sync(ALL, incl, 31);
+          }
+          x.Lq = lens(x.b).x;
+          x.Lk = lens(x.b).y;
+          x.q0 = p.cu_q[x.b];
+          x.m0 = ((x.Lq + BMT - 1) / BMT - 1 - fp8_tiles_above(lo, x.Lq, x.Lk, BMT) - static_cast<int>(k)) * BMT;
+        }
+        if (it >= 2) ok = wait_or_abort(bar(ITEM_FREE0 + (it & 1)), ((it >> 1) - 1) & 1, abort_flag);
+        if (!__all_sync(ALL, ok)) break;
+        if (lane == 0) {
+          volatile int* s = slots + (it & 1) * 8;
+          s[0] = x.b; s[1] = x.h; s[2] = x.m0; s[3] = x.q0;
+          s[4] = x.Lq; s[5] = x.Lk; s[6] = x.n_kv;
+          mbar_arrive(bar(ITEM_FULL0 + (it & 1)));
+          if (x.n_kv > 0) {  // its query rows are on the path from the item before: to L2
+            prefetch_tile(&tmap_q, 0, x.h, x.q0 + x.m0);
+            if constexpr (D == 128) prefetch_tile(&tmap_q, 64, x.h, x.q0 + x.m0);
+          }
+        }
+        __syncwarp();
+        if (x.n_kv < 0) break;
+      }
 #pragma unroll 1
       for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
         const int Lq = lens(b).x, Lk = lens(b).y, dead = Lk <= 0 ? Lq : Lk < Lq ? (Lq - Lk) / BMT * BMT : 0;
@@ -402,27 +481,24 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       if (!(ok = wait_or_abort(bar(FACTOR0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
       const float factor = row_factor[(it & 1) * 128 + r];
       const int qi = x.m0 + r_tok, off = x.Lk - x.Lq;
-      float m_used = -INFINITY, l = 0.f, unit = 0.f, most_unit = 0.f;
+      float m_used = -INFINITY, l = 0.f;
 #pragma unroll 1
       for (int j = 0; j < x.n_kv; ++j) {
         const int t = T + j, st = t & 1, ph = (t >> 1) & 1;
         const uint32_t scores = tmem_s(st) + lane_addr;
-        if (!(ok = wait_or_abort(bar(SCALES0 + (t & 3)), (t >> 2) & 1, abort_flag))) break;
-        const float* sc = reinterpret_cast<const float*>(base_ptr + G::OFF_SCALES + (t & 3) * 32);
-        const int j0 = j * BN;
-        float ks[4], vs[4];
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          // A group behind the end may hold anything: a number, then.  Never zero, which -inf of a masked score must not meet.
-          const bool live = j0 + g * kScaleGroup < x.Lk;
-          ks[g] = fmaxf((live ? sc[g] : 1.f) * factor, 0x1p-126f);
-          vs[g] = live ? sc[4 + g] : 0.f;
-        }
         if (!(ok = wait_or_abort(bar(QK_DONE0 + st), ph, abort_flag))) break;
         tc_fence_after();
         uint32_t s[64];
         tmem_ld32(scores, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
         tmem_ld32(scores + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
+        if (!(ok = wait_or_abort(bar(INFO0 + (t & 3)), (t >> 2) & 1, abort_flag))) break;
+        const Fp8Tile& tile = *reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile));
+        float ks[4];
+        *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(tile.k);
+        const float change = tile.change;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) ks[g] = fmaxf(ks[g] * factor, 0x1p-126f);  // not zero, which -inf of a masked score must not meet
+        const int j0 = j * BN;
         tmem_wait_ld();
         if ((j0 + BN - 1 > x.m0 + off) || (j0 + BN > x.Lk)) {  // tile touches the diagonal or the end
           const int limit = min(qi + off, x.Lk - 1) - j0;        // columns c <= limit are visible
@@ -442,24 +518,17 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           mx = fmaxf(mx, fmaxf(m2[0], m2[1]) * ks[g]);
         }
         const float m_new = fmaxf(m_used, mx);
-        // lazy rescale: keep the old reference maximum unless it has been outgrown by 2^8; and the unit, see above
+        // lazy rescale: keep the old reference maximum unless it has been outgrown by 2^14
         const bool grow = m_new > m_used + kRescaleThreshold;
-        const float most_vs = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-        const bool other_unit = most_vs > unit || (most_vs > 0.f && most_vs * 16.f < unit);  // the same for all rows
-        if (other_unit || __any_sync(ALL, grow)) {
+        if (change != 1.f || __any_sync(ALL, grow)) {
           float alpha = 1.f;
           if (grow) {
             alpha = (m_used == -INFINITY) ? 0.f : fast_exp2(m_used - m_new);
             m_used = m_new;
             l *= alpha;
           }
-          if (other_unit) {
-            const float next = fmaxf(most_vs, most_unit * 0x1p-60f);
-            alpha *= unit > 0.f ? unit / next : 0.f;
-            unit = next;
-            most_unit = fmaxf(most_unit, next);
-          }
-          if (j > 0 && __any_sync(ALL, alpha != 1.f)) {  // O holds tiles 0..j-1 of this item once the previous product has finished
+          alpha *= change;
+          if (j > 0) {  // O holds tiles 0..j-1 of this item once the previous product has finished
             if (!(ok = wait_or_abort(bar(PV_DONE0 + ((t - 1) & 1)), ((t - 1) >> 1) & 1, abort_flag))) break;
             tc_fence_after();
 #pragma unroll 1
@@ -474,21 +543,19 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           }
         }
         const float msub = (m_used == -INFINITY) ? 0.f : m_used;
-        const float per_unit = unit > 0.f ? 1.f / unit : 0.f;
-        // p = 2^(s * scale - m), times V's scale for the product: two lanes at a time
+        // p = 2^(s * scale - m): the multiply-subtract and the row sum run two lanes at a time
         const uint64_t nmsub2 = pack2(-msub, -msub);
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const uint64_t scale2 = pack2(ks[g], ks[g]), vs2 = pack2(vs[g] * per_unit, vs[g] * per_unit);
+          const uint64_t scale2 = pack2(ks[g], ks[g]);
 #pragma unroll
           for (int c = g * 8; c < g * 8 + 8; ++c) {  // P is packed in place: s[c] <- (p[2c], p[2c+1])
             float a0, a1;
             unpack2(fma2(pack2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, nmsub2), a0, a1);
-            const uint64_t p2 = pack2(fast_exp2(a0), fast_exp2(a1));
-            sum2[c & 1] = add2(sum2[c & 1], p2);
-            unpack2(mul2(p2, vs2), a0, a1);
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(s[c]) : "f"(a1), "f"(a0));
+            const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
+            sum2[c & 1] = add2(sum2[c & 1], pack2(p0, p1));
+            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(s[c]) : "f"(p1), "f"(p0));
           }
         }
         {
@@ -506,7 +573,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       if (!ok) break;
       T += x.n_kv;
       // the row's normaliser goes to the row warps; no key: zeros; a sum that is NaN stays one
-      inv_buf[(it & 1) * 128 + r] = l > 0.f ? unit / l : l;
+      inv_buf[(it & 1) * 128 + r] = l > 0.f ? 1.f / l : l;
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(bar(EPI_FULL0 + (it & 1)));
@@ -519,47 +586,54 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
     const int ew = warp - 4, r = ew * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>(ew * 32) << 16;
     unsigned char* stage = base_ptr + G::OFF_STAGE + ew * 2048;
-    // Thread = query row: its power of two, then high and low parts piece by piece.
-    auto take_rows = [&](const Fp8Item& x, int it) {
-      const int tok = token_of(r), hh = r - tok * pack;
-      const bool live = tok < min(BMT, x.Lq - x.m0);
-      const uint4* src = reinterpret_cast<const uint4*>(p.q + static_cast<int64_t>(x.q0 + x.m0 + (live ? tok : 0)) * p.q_stride + (x.h + hh) * D);
-      uint32_t m = 0;
-      if (live) {
-#pragma unroll 2
-        for (int c = 0; c < D / 16; ++c) {
-          const uint4 a = __ldg(src + 2 * c), b = __ldg(src + 2 * c + 1);
-          m = max_finite2(max_finite2(max_finite2(max_finite2(m, a.x), a.y), a.z), a.w);
-          m = max_finite2(max_finite2(max_finite2(max_finite2(m, b.x), b.y), b.z), b.w);
-        }
+    // Thread = query row: its power of two, then its two parts, eight values at a time (f16 holds them: 128 <= max < 256): the
+    // nearest codes, and the nearest ones of what is left.  Run once an item, so short: code that is not in the instruction
+    // cache comes at 25 cycles an instruction (unrolled, this took 8000 cycles).
+    // D = 128: TMA has brought the bf16 values into the place of the parts, in two sub-tiles of 64 columns, rows of 128 bytes as
+    // the parts have; a thread stays within its own rows' bytes and writes none before what lies there has been read: pieces
+    // 0 to 7, then 15 down to 8, the first half's low parts by way of this thread's 64 bytes of the patch for results.
+    auto take_rows = [&](const Fp8Item& x, int it, int last) {  // last: the last tile of the item before
+      if (!wait_or_abort(bar(ROWS_FULL), it & 1, abort_flag)) return false;
+      const bool live = token_of(r) < BMT;  // rows behind a sequence's end hold something that nobody looks at
+      const uint32_t from = base + G::OFF_ROWS + r * 128 + ((r & 7) << 4);  // piece i, eight values: the sub-tile's, ^ i * 16
+      auto piece = [&](int i) { return ld_shared16((from + (i >> 3) * (BM * 128)) ^ ((i & 7) << 4)); };
+      uint32_t m = 0;  // the largest magnitudes, two columns at a time; infinities and NaN stay what they are
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        const uint4 a = piece(i);
+        m = max_magnitude(max_magnitude(a.x, a.y), max_magnitude(max_magnitude(a.z, a.w), m));
       }
-      m = max(m & 0xffffu, m >> 16);
-      const int e = max(static_cast<int>(m >> 7), 20) - 127;  // 2^e <= max |q| < 2^(e + 1)
+      m &= 0x7fff7fffu;
+      m = live ? max(m & 0xffffu, m >> 16) : 0;
+      const uint32_t spoilt = m >= 0x7f80u ? 0x7fu : 0u;  // an infinity or NaN: so is the row, by its first code
+      const int e = min(max(static_cast<int>(m >> 7), 20), 254) - 127;  // 2^e <= max |q| < 2^(e + 1)
       const float f = power_of_two(7 - e);
       row_factor[(it & 1) * 128 + r] = p.scale_log2e * power_of_two(e - 7);
+      if (D == 64 && it > 0 && !wait_or_abort(bar(QK_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag)) return false;
+      // pieces of the parts, two of these to one: the high part's row and swizzle, the low part's, the patch's
+      const uint32_t to_high = base + G::OFF_Q + code_piece<D>(r, 0), to_low = to_high + G::Q_PART;
+      const uint32_t to_aside = smem_u32(stage) + lane * 64 + ((lane >> 1 & 3) << 4);
 #pragma unroll 1
-      for (int c = 0; c < D / 16; ++c) {
-        uint32_t hi[4], lo[4];
+      for (int n = 0; n < D / 8; ++n) {
+        const int i = n < 8 ? n : 23 - n;
+        const uint4 a = piece(i);
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w}, at = (i >> 1) << 4, half = (i & 1) * 8;
+        uint32_t h[4], l[4];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint4 a = live ? __ldg(src + 2 * c + half) : make_uint4(0, 0, 0, 0);
-          const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float y0 = __uint_as_float(w[i] << 16) * f, y1 = __uint_as_float(w[i] & 0xffff0000u) * f;
-            y0 = fabsf(y0) <= 448.f ? y0 : NAN;  // infinities: the row is NaN
-            y1 = fabsf(y1) <= 448.f ? y1 : NAN;
-            const uint32_t h = e4m3x2(y0, y1);
-            const float2 back = float2_of_f16x2(f16x2_of_low(h));
-            const uint32_t l2 = e4m3x2(y0 - back.x, y1 - back.y);
-            const int at = 2 * half + (i >> 1);
-            if (i & 1) hi[at] |= h << 16, lo[at] |= l2 << 16;
-            else hi[at] = h, lo[at] = l2;
-          }
+        for (int k = 0; k < 4; ++k) {
+          uint32_t y, rest;
+          asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(__uint_as_float(w[k] & 0xffff0000u) * f), "f"(__uint_as_float(w[k] << 16) * f));
+          h[k] = e4m3x2_of_f16x2(y);
+          asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(rest) : "r"(y), "r"(f16x2_of_low(h[k])));
+          l[k] = e4m3x2_of_f16x2(rest);
         }
-        unsigned char* to = base_ptr + G::OFF_Q + code_piece<D>(r, c);
-        *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4*>(to + G::Q_PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        if (n == 0) h[0] |= spoilt;
+        st_shared8((to_high ^ at) + half, make_uint2(__byte_perm(h[0], h[1], 0x5410), __byte_perm(h[2], h[3], 0x5410)));
+        st_shared8((D == 128 && n < 8 ? to_aside ^ at : to_low ^ at) + half, make_uint2(__byte_perm(l[0], l[1], 0x5410), __byte_perm(l[2], l[3], 0x5410)));
+      }
+      if constexpr (D == 128) {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) st_shared16(to_low ^ c << 4, ld_shared16(to_aside ^ c << 4));
       }
       fence_proxy_async();
       __syncwarp();
@@ -567,32 +641,41 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         mbar_arrive(bar(Q_FULL));
         mbar_arrive(bar(FACTOR0 + (it & 1)));
       }
+      return true;
     };
-    // Tile t (the j-th of item x) of V: 16 codes at a time to two 16-byte pieces of f16.
+    // Tile t (the j-th of item x) of V: 16 codes at a time to two 16-byte pieces of f16, times the group's scale over the unit.
+    // Eight lanes take two rows' halves whose pieces are in different banks both where they come from and where they go: at
+    // D = 64 neighbouring rows, at D = 128 rows whose numbers differ by the bits of 5.  The next of a thread's pieces lie 16
+    // (D = 128) or 32 rows on, so in places a constant apart.
+    constexpr int STEPS = D / 32, STEP_ROWS = BN / STEPS;  // pieces of a thread
+    const int v_row = D == 64 ? r >> 2 : (r >> 6) * 8 + ((r >> 4 & 3) ^ (r & 4 ? 5 : 0)), v_piece = D == 64 ? r & 3 : (r & 3) | (r & 8) >> 1;
+    const unsigned char* v_from = base_ptr + G::OFF_RAW + code_piece<D>(v_row, v_piece);
+    unsigned char* v_to = base_ptr + G::OFF_V + (v_piece >> 2) * G::V_SUB + v_row * 128 + (((v_piece & 3) * 2 ^ (v_row & 7)) << 4);
     auto convert = [&](const Fp8Item& x, int j, int t) {
-      const int st = t & 1, use = t >> 1;
+      const int st = t & 1, use = t >> 1, rows = x.Lk - j * BN;
+      if (!wait_or_abort(bar(INFO0 + (t & 3)), (t >> 2) & 1, abort_flag)) return false;
+      uint32_t by[4];
+      *reinterpret_cast<uint4*>(by) = *reinterpret_cast<const uint4*>(reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile))->v);
       if (!wait_or_abort(bar(RAW_FULL0 + st), use & 1, abort_flag)) return false;
       if (use > 0 && !wait_or_abort(bar(PV_DONE0 + st), (use - 1) & 1, abort_flag)) return false;
-      const unsigned char* raw = base_ptr + G::OFF_RAW + st * G::K_BYTES;
-      unsigned char* vt = base_ptr + G::OFF_V + st * G::V_BYTES;
-      const int rows = x.Lk - j * BN;  // that hold a token
-      constexpr int PIECES = D / 16;
-      uint4 code[BN * PIECES / 128];
+      uint4 code[STEPS];
 #pragma unroll
-      for (int i = 0; i < BN * PIECES / 128; ++i) {
-        const int idx = i * 128 + r, row = idx / PIECES, c = idx % PIECES;
-        code[i] = *reinterpret_cast<const uint4*>(raw + code_piece<D>(row, c));
-        if (row >= rows) code[i] = make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < STEPS; ++i)
+        code[i] = *reinterpret_cast<const uint4*>(v_from + st * G::K_BYTES + i * (STEP_ROWS * D));
+      if (rows < BN) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i)
+          if (i * STEP_ROWS + v_row >= rows) code[i] = make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
-      for (int i = 0; i < BN * PIECES / 128; ++i) {
-        const int idx = i * 128 + r, row = idx / PIECES, c = idx % PIECES;
-        unsigned char* sub = vt + (c >> 2) * G::V_SUB + row * 128;
-        const int c0 = (c & 3) * 2;
-        *reinterpret_cast<uint4*>(sub + ((c0 ^ (row & 7)) << 4)) =
-            make_uint4(f16x2_of_low(code[i].x), f16x2_of_high(code[i].x), f16x2_of_low(code[i].y), f16x2_of_high(code[i].y));
-        *reinterpret_cast<uint4*>(sub + (((c0 + 1) ^ (row & 7)) << 4)) =
-            make_uint4(f16x2_of_low(code[i].z), f16x2_of_high(code[i].z), f16x2_of_low(code[i].w), f16x2_of_high(code[i].w));
+      for (int i = 0; i < STEPS; ++i) {
+        const uint32_t f = D == 128 ? by[i] : r < 64 ? by[2 * i] : by[2 * i + 1];  // of rows 16 i .. or 32 i ..: their groups
+        unsigned char* to = v_to + st * G::V_BYTES + i * (STEP_ROWS * 128);
+        *reinterpret_cast<uint4*>(to) = make_uint4(
+            mul_f16x2(f16x2_of_low(code[i].x), f), mul_f16x2(f16x2_of_high(code[i].x), f), mul_f16x2(f16x2_of_low(code[i].y), f), mul_f16x2(f16x2_of_high(code[i].y), f));
+        to = reinterpret_cast<unsigned char*>(reinterpret_cast<uintptr_t>(to) ^ 16);  // the odd neighbour: pieces 2 c and 2 c + 1
+        *reinterpret_cast<uint4*>(to) = make_uint4(
+            mul_f16x2(f16x2_of_low(code[i].z), f), mul_f16x2(f16x2_of_high(code[i].z), f), mul_f16x2(f16x2_of_low(code[i].w), f), mul_f16x2(f16x2_of_high(code[i].w), f));
       }
       fence_proxy_async();
       __syncwarp();
@@ -602,33 +685,11 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       }
       return true;
     };
-    int T = 0;
-    bool ok = wait_or_abort(bar(ITEM_FULL0), 0, abort_flag);
-    Fp8Item x;
-    x.n_kv = -1;
-    if (ok) x = read_item(0);
-    if (ok && x.n_kv > 0) {
-      take_rows(x, 0);
-      ok = convert(x, 0, 0);
-    }
-#pragma unroll 1
-    for (int it = 0; ok && x.n_kv > 0; ++it) {
-#pragma unroll 1
-      for (int j = 1; ok && j < x.n_kv; ++j) ok = convert(x, j, T + j);
-      if (!ok) break;
-      // the next item's rows and first tile before this one's results, so that its products run under their writing
-      const int last = T + x.n_kv - 1;
-      if (!(ok = wait_or_abort(bar(ITEM_FULL0 + ((it + 1) & 1)), ((it + 1) >> 1) & 1, abort_flag))) break;
-      const Fp8Item next = read_item(it + 1);
-      if (next.n_kv > 0) {
-        if (!(ok = wait_or_abort(bar(QK_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag))) break;
-        take_rows(next, it + 1);
-        if (!(ok = convert(next, 0, last + 1))) break;
-      }
-      T += x.n_kv;
-      if (!(ok = wait_or_abort(bar(EPI_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
-      const float inv = inv_buf[(it & 1) * 128 + r];
-      if (!(ok = wait_or_abort(bar(PV_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag))) break;
+    // Results of item number `done`, whose last tile was `last`.
+    auto results = [&](const Fp8Item& x, int done, int last) {
+      if (!wait_or_abort(bar(EPI_FULL0 + (done & 1)), (done >> 1) & 1, abort_flag)) return false;
+      const float inv = inv_buf[(done & 1) * 128 + r] * reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (last & 3) * sizeof(Fp8Tile))->unit;
+      if (!wait_or_abort(bar(PV_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag)) return false;
       tc_fence_after();
       // O / l -> bf16, 32 columns at a time through this warp's patch of shared memory
       const int srow = lane >> 2, spiece = lane & 3;
@@ -664,8 +725,26 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         }
         __syncwarp();
       }
-      if (lane == 0) mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
-      x = next;
+      if (lane == 0) mbar_arrive(bar(ITEM_FREE0 + (done & 1)));
+      return true;
+    };
+    // An item's results are written when the next one's rows and first tile are there, whose products run meanwhile.
+    Fp8Item before{};
+    int T = 0;
+    bool ok = true;
+#pragma unroll 1
+    for (int it = 0; ok; ++it) {
+      if (!(ok = wait_or_abort(bar(ITEM_FULL0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
+      const Fp8Item x = read_item(it);
+      if (x.n_kv > 0 && !(ok = take_rows(x, it, T - 1))) break;
+#pragma unroll 1
+      for (int j = 0; ok && j < max(x.n_kv, 1); ++j) {
+        if (x.n_kv > 0 && !(ok = convert(x, j, T + j))) break;
+        if (j == 0 && it > 0) ok = results(before, it - 1, T - 1);
+      }
+      if (x.n_kv < 0) break;
+      T += x.n_kv;
+      before = x;
     }
   }
 
@@ -689,7 +768,8 @@ static int heads_in_tile(int g) {
 }
 
 template <int D>
-static int launch_prefill_fp8(PrefillFp8Params& p, const void* k_cache, const void* v_cache, int max_seqlen_q, cudaStream_t stream) {
+static int launch_prefill_fp8(PrefillFp8Params& p, const void* k_cache, const void* v_cache, int64_t total_q, int max_seqlen_q,
+                              cudaStream_t stream) {
   using G = f8::Geo<D>;
   static bool ready[64] = {false};
   int dev = 0;
@@ -711,12 +791,13 @@ static int launch_prefill_fp8(PrefillFp8Params& p, const void* k_cache, const vo
   p.pack = heads_in_tile(p.g);
   p.tile_tokens = f8::BM / p.pack;
   p.inv_pack = 65536 / p.pack + 1;  // exact for rows of a tile
-  CUtensorMap mk, mv;
+  CUtensorMap mq, mk, mv;
+  if (!make_tmap_3d(&mq, p.q, D, p.hq, total_q, D, p.q_stride, p.tile_tokens, p.pack)) return NVLLM_E_CUDA;
   const uint64_t slots = static_cast<uint64_t>(p.num_blocks) * kBlockSize;
   if (!make_tmap_codes(&mk, k_cache, D, p.hkv, slots, f8::BN) || !make_tmap_codes(&mv, v_cache, D, p.hkv, slots, f8::BN)) return NVLLM_E_CUDA;
   const int64_t items = static_cast<int64_t>((max_seqlen_q + p.tile_tokens - 1) / p.tile_tokens) * (p.hq / p.pack) * p.batch;  // at most
   const int grid = static_cast<int>(std::min<int64_t>(2ll * num_sms(), items));
-  return launch_kernel("prefill_fp8", prefill_fp8_kernel<D>, dim3(grid), dim3(f8::NTHREADS), G::SMEM, stream, p, mk, mv);
+  return launch_kernel("prefill_fp8", prefill_fp8_kernel<D>, dim3(grid), dim3(f8::NTHREADS), G::SMEM, stream, p, mq, mk, mv);
 }
 
 }  // namespace nvllm
@@ -767,6 +848,6 @@ extern "C" int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, con
   p.scale_log2e = scale * 1.4426950408889634f;
   p.num_blocks = num_blocks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_prefill_fp8<128>(p, k_cache, v_cache, max_seqlen_q, st);
-  return launch_prefill_fp8<64>(p, k_cache, v_cache, max_seqlen_q, st);
+  if (head_dim == 128) return launch_prefill_fp8<128>(p, k_cache, v_cache, total_q, max_seqlen_q, st);
+  return launch_prefill_fp8<64>(p, k_cache, v_cache, total_q, max_seqlen_q, st);
 }

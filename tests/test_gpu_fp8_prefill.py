@@ -75,7 +75,10 @@ def test_scales_of_every_size(cuda, d):
     q = (q.float() * 2.0 ** -20 * torch.exp2(torch.randint(-8, 1, q.shape, generator=g))).bfloat16()
     for f in (1.0, 1e-30, 0.0):
         x = (q.float() * f).bfloat16()
-        assert_within(run(cuda, x, planes, *rest, 0.1), *prefill_reference(x, planes, *rest, 0.1), f"queries times {f}")
+        ref, bound = prefill_reference(x, planes, *rest, 0.1)
+        # scales that are no powers of two: V times scale over unit is rounded to f16 twice, 2^-10 A more, where the bound
+        # holds 1.5 * 2^-11 A: 4 / 3 of it
+        assert_within(run(cuda, x, planes, *rest, 0.1), ref, bound * (1 + 4 / 3), f"queries times {f}")
 
 
 def test_a_group_of_tiny_values_behind_large_ones(cuda):
