@@ -4,12 +4,16 @@
 //
 // The step variant also does what store_kvcache_fp8 does for the one new token of every sequence.
 //
-// Bound by the cached bytes, half of a bf16 cache's.  The launch is cut as the bf16 decode's is (decode_paged.cu): all
-// sequences' work units in one list, an equal stretch of it to each of two resident blocks per SM, partial results of
-// sequences that a cut divides merged by the last block to arrive.  What differs is what a tile costs:
-//   * K codes go from shared memory to registers 16 bytes a lane and become f16 pairs there (cvt, exact).  The four codes of a
-//     word are columns k = 2 tig .. and k = 2 tig + 8 .. of one m16n8k16 product: the order of the summed index is free, the
-//     query's columns follow it.
+// Bound by the cached bytes, half of a bf16 cache's: 128 sequences of 1024-8192 tokens (32 / 8 heads of 128) 184 us, 6.4 TB/s
+// (bf16: 363), 180 with nothing computed.  The launch is cut as the bf16 decode's is (decode_paged.cu): all sequences' work units
+// in one list, an equal stretch of it to each of two resident blocks per SM, partial results of sequences that a cut
+// divides merged by the last block to arrive.  What differs is what a tile costs:
+//   * A warp of its own loads: table entries, tiles by TMA (a box for every warp's tile that holds a token), scales.  When the
+//     four others did that themselves, with cp.async, they spent half of their instructions on it; a barrier of the block
+//     for every unit instead was slower (128 sequences 199 -> 214 us, loading warp 184; 60 of 100-1024 21.5, 23.3, 18.3).
+//   * K codes go from shared memory to registers 16 bytes a lane and become f16 pairs there (cvt, exact, two cycles).  The four
+//     codes of a word are columns k = 2 tig .. and k = 2 tig + 8 .. of one m16n8k16 product: the order of the summed index
+//     is free, the query's columns follow it.
 //   * V codes go through ldmatrix.trans as pairs of neighbouring columns: a register then holds two columns of two tokens,
 //     one byte permutation away from (token, token) pairs of either column, rows gid and gid + 8 of V^T.
 //   * q is f16 too, scaled by a power of two to 2^14 <= max |q| < 2^15, so that it keeps all its bits down to 2^-29 of the
@@ -17,9 +21,12 @@
 //     group's V scale over the warp's running unit: the sums O are held in that unit, which follows the scales (see `unit`).
 //   * 16 tokens share a scale, so a group lies in one warp's tile: the step variant's warp that streams the new token has
 //     its whole group at hand, codes the row, codes the rows before it anew where the scale grows, and writes them back.
-#include <cstdlib>
-
+//
+// Small batches are bound by trips one after the other: lengths and split (0.7 us), table entry, tiles, the products of a tile
+// (0.7), flush (0.6), arrival (0.8), merge.  The first three run ahead of the wait for the previous kernel and are verified
+// behind it (a sequence of 317 tokens 7.1 -> 6.7 us in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6).
 #include "fp8.cuh"
+#include "sm100.cuh"
 
 namespace nvllm {
 
@@ -56,23 +63,28 @@ struct DecodeFp8Params {
   int* status;
 };
 
-template <int D_, int TT_, int NST_, int NW_>
+template <int D_, int TT_, int NST_, int NW_, int BLOCKS_>
 struct DecodeFp8Cfg {
-  static constexpr int D = D_, TT = TT_, NST = NST_, NW = NW_;
+  static constexpr int D = D_, TT = TT_, NST = NST_, NW = NW_, BLOCKS = BLOCKS_;  // blocks to an SM
   static constexpr int UNIT = NW * TT;  // tokens of a work unit
   static constexpr int MT = TT / 16;    // groups of a warp's tile
   static constexpr int CPR = D / 16;    // 16-byte pieces of a row
-  static constexpr int TILE_BYTES = TT * D;
-  static constexpr int STAGE_BYTES = 2 * TILE_BYTES;
-  static constexpr int WARP_BYTES = NST * STAGE_BYTES;
-  static constexpr int RING_BYTES = NW * WARP_BYTES;
-  static constexpr int SCALE_BYTES = 2 * MT * 4;  // of a stage: K's, V's
+  static constexpr int TILE_BYTES = TT * D;       // a warp's part of a unit
+  static constexpr int UNIT_BYTES = UNIT * D;
+  static constexpr int STAGE_BYTES = 2 * UNIT_BYTES;
+  static constexpr int RING_BYTES = NST * STAGE_BYTES;
+  static constexpr int UNIT_GROUPS = UNIT / kScaleGroup;
+  static constexpr int SCALE_BYTES = 2 * UNIT_GROUPS * 4;  // of a stage: K's, V's
   static constexpr int OFF_SCALES = RING_BYTES;
-  static constexpr int OFF_MERGE = OFF_SCALES + NW * NST * SCALE_BYTES;
-  static constexpr int SMEM = OFF_MERGE + NW * 8 * D * 4 + NW * 8 * 2 * 4;
+  static constexpr int OFF_MERGE = OFF_SCALES + NST * SCALE_BYTES;
+  static constexpr int OROW = D + 4;    // floats of a head's row: sums, maximum, sum; heads written together lie in different banks
+  static constexpr int OFF_CTRL = OFF_MERGE + NW * 8 * OROW * 4;  // barriers, then a few words
+  static constexpr int SMEM = OFF_CTRL + 2 * NST * 8 + (NST + NW + 3 + 2) * 4;
+  static constexpr int NTHREADS = (NW + 1) * 32;  // and a warp that loads
   static constexpr int KS = D / 16;  // products of a group's scores, and of its share of O
-  static_assert(TT % kScaleGroup == 0 && kBlockSize % TT == 0 && (MT & (MT - 1)) == 0 && MT <= 4, "whole groups, whole tiles");
-  static_assert((TT * CPR) % 32 == 0 && OFF_MERGE % 16 == 0, "a tile is copied evenly by a warp");
+  static_assert(TT % kScaleGroup == 0 && kBlockSize % UNIT == 0 && (MT & (MT - 1)) == 0 && MT <= 4, "whole groups, units within a block");
+  static_assert(TILE_BYTES % 1024 == 0 && OFF_MERGE % 16 == 0, "a warp's tile starts where the swizzle does");
+  static_assert(BLOCKS * (SMEM + 1024) <= 228 * 1024, "as many blocks to an SM");
 };
 
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -86,21 +98,22 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-template <int BYTES>
-__device__ __forceinline__ void cp_async_small(uint32_t dst, const void* src, int src_bytes) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(BYTES), "r"(src_bytes));
-}
 __device__ __forceinline__ float ld_shared_f32(uint32_t a) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(a) : "memory");
   return v;
 }
 __device__ __forceinline__ void st_shared_f32(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;\n" ::"r"(a), "f"(v) : "memory"); }
-// Where piece c of row r of a tile lies: so that eight rows' pieces c, and two rows' pieces of one half, are in different banks.
+// Where TMA's swizzle puts piece c of row r of a tile (128-byte rows; or 64-byte ones, two to a line).
 template <int D>
 __device__ __forceinline__ uint32_t tile_offset(int r, int c) {
-  const int x = D == 128 ? ((r & 1) << 2 | (r >> 1 & 3)) : (r >> 1 & 3);
-  return r * D + ((c ^ x) << 4);
+  return r * D + ((c ^ (D == 128 ? r & 7 : r >> 1 & 3)) << 4);
+}
+// The token of row i < 8 of a matrix operand.  Neighbouring rows of K are read together, a half of 64 bytes each: at D = 128
+// tokens four apart lie in different banks.  The order is free as long as V's is the same.
+template <int D>
+__device__ __forceinline__ int token_of_row(int i) {
+  return D == 128 ? (i >> 1) | (i & 1) << 2 : i;
 }
 
 struct Fp8Cursor {  // the sequence a block is working in: index, global index of its first unit, units, length
@@ -115,18 +128,30 @@ struct Fp8Cut {  // a sequence whose units lie in several ranges: n of them, fro
 constexpr float kFp8SplitBalance = 16.f;
 
 template <class C, bool STEP>
-__global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeFp8Params p) {
+__global__ void __launch_bounds__(C::NTHREADS, C::BLOCKS)
+decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap tmap_k, const __grid_constant__ CUtensorMap tmap_v) {
   constexpr int D = C::D, TT = C::TT, NST = C::NST, NW = C::NW, UNIT = C::UNIT, MT = C::MT, NT = NW * 32;
   constexpr int QUADS = D / 4, GROUPS = NT / QUADS;  // lanes that hold a head four columns each; such groups in a block
   constexpr int PIECES = D / 8;                      // lanes that hold a bf16 row, eight values each
   constexpr unsigned ALL = 0xffffffffu;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int s_scan[NW];
-  __shared__ int s_start[3];
-  __shared__ int s_last_arrival[2];
+  extern __shared__ __align__(1024) unsigned char smem[];
+  // in the dynamic part, which would start 1024 bytes later behind any other: two blocks to an SM need all but 900 bytes
+  uint64_t* s_full = reinterpret_cast<uint64_t*>(smem + C::OFF_CTRL);
+  uint64_t* s_free = s_full + NST;
+  int *s_row = reinterpret_cast<int*>(s_free + NST), *s_scan = s_row + NST;
+  int *s_start = s_scan + NW, *s_last_arrival = s_start + 3;
 
   pdl_trigger();
-  pdl_wait();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 0; i < NST; ++i) {
+      sm100::mbar_init(smem_u32(s_full + i), 2);  // the tiles; the scales
+      sm100::mbar_init(smem_u32(s_free + i), NW);
+    }
+    sm100::mbar_fence_init();
+    sm100::prefetch_tmap(&tmap_k);
+    sm100::prefetch_tmap(&tmap_v);
+  }
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int gid = lane >> 2, tig = lane & 3;
   const int kvh = blockIdx.x % p.hkv;
@@ -141,51 +166,99 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
   };
 
   // ---- 1. units per sequence, block-wide scan, this block's range of the unit list ------
-  const int per_thread = (p.batch + NT - 1) / NT;
+  const bool loader = warp == NW;
+  const int per_thread = loader ? 0 : (p.batch + NT - 1) / NT;
   const int b_lo = min(tid * per_thread, p.batch), b_hi = min(b_lo + per_thread, p.batch);
-  // the first table line of every sequence on its way while the lengths are summed
-  if (p.batch <= NT && tid < p.batch) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.block_tables + tid * p.bt_stride));
-  int local = 0;
-  for (int b = b_lo; b < b_hi; ++b) {
-    const int c = length_of(b);
-    local += units_of(c);
-    if (c == 0) write_zeros(b);
-  }
-  int incl = local;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(ALL, incl, d);
-    if (lane >= d) incl += v;
-  }
-  if (lane == 31) s_scan[warp] = incl;
-  __syncthreads();
-  int before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    if (w < warp) before += s_scan[w];
-    total += s_scan[w];
-  }
-  const int excl = before + incl - local;
-  // No more ranges than units, and where sequences are few no more than balance the two costs of a cut: a range streams
-  // total / n units and a sequence's merge reads n / batch partials.
-  const int n_ranges = max(1, min(min(p.n_ranges, total), static_cast<int>(sqrtf(kFp8SplitBalance * total * p.batch))));
-  if (range >= n_ranges || total == 0) return;  // block-uniform
-  const int per_range = total / n_ranges, longer = total - per_range * n_ranges;  // the first `longer` ranges hold one more
-  const int u0 = range * per_range + min(range, longer), u1 = u0 + per_range + (range < longer ? 1 : 0);
-  if (local > 0 && excl <= u0 && u0 < excl + local) {  // the one thread whose sequences hold unit u0
-    int first = excl;
-    for (int b = b_lo;; ++b) {
-      const int len = length_of(b), n = units_of(len);
-      if (u0 < first + n) {
-        s_start[0] = b;
-        s_start[1] = first;
-        s_start[2] = len;
-        break;
-      }
-      first += n;
+  int total, n_ranges, per_range, longer, u0, u1, len_lo;
+  int2* seqs = reinterpret_cast<int2*>(smem + C::OFF_MERGE);  // ahead: first unit and length of every sequence
+  static_assert(NT * 8 <= C::OFF_CTRL - C::OFF_MERGE, "room for them until the first merge");
+  auto split = [&](bool ahead) {  // whether this block has a range
+    int local = 0;
+    len_lo = 0;
+    for (int b = b_lo; b < b_hi; ++b) {
+      const int c = ahead ? max(0, min(__ldcg(p.ctx_lens + b), ctx_cap)) : length_of(b);
+      if (b == b_lo) len_lo = c;
+      local += units_of(c);
     }
+    int incl = local;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(ALL, incl, d);
+      if (lane >= d) incl += v;
+    }
+    if (lane == 31 && !loader) s_scan[warp] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w < warp) before += s_scan[w];
+      total += s_scan[w];
+    }
+    const int excl = before + incl - local;
+    if (ahead && !loader) seqs[tid] = make_int2(excl, len_lo);
+    // No more ranges than units, and where sequences are few no more than balance the two costs of a cut: a range streams
+    // total / n units and a sequence's merge reads n / batch partials.
+    n_ranges = max(1, min(min(p.n_ranges, total), static_cast<int>(sqrtf(kFp8SplitBalance * total * p.batch))));
+    if (p.batch == 1 && total <= 4) n_ranges = 1;  // a unit more takes less than a merge: 317 tokens 6.7 -> 6.4 us
+    if (range >= n_ranges || total == 0) return false;  // block-uniform
+    per_range = total / n_ranges, longer = total - per_range * n_ranges;  // the first `longer` ranges hold one more
+    u0 = range * per_range + min(range, longer), u1 = u0 + per_range + (range < longer ? 1 : 0);
+    if (local > 0 && excl <= u0 && u0 < excl + local) {  // the one thread whose sequences hold unit u0
+      int first = excl;
+      for (int b = b_lo;; ++b) {
+        const int len = b == b_lo ? len_lo : length_of(b), n = units_of(len);
+        if (u0 < first + n) {
+          s_start[0] = b;
+          s_start[1] = first;
+          s_start[2] = len;
+          break;
+        }
+        first += n;
+      }
+    }
+    __syncthreads();
+    return true;
+  };
+  // Batches of a sequence to a thread at most: the split is made, and the first units' table entries are read and their tiles
+  // brought to L2, while the previous kernel still runs.  It may change lengths and tables: when it is done they are read
+  // again, in one trip, and if one has changed the split is made anew.  What is read before the wait goes round L1, is held
+  // to the bounds of the table and the cache, and serves the guess alone.
+  int n_listed = 0, listed_blk = -1;  // the loading warp: units whose entries are known, one to a lane
+  bool mine;
+#pragma unroll 1
+  for (bool ahead = p.batch <= NT;; ahead = false) {
+    if (!ahead) pdl_wait();
+    mine = split(ahead);
+    if (!ahead) break;
+    const int32_t* at = nullptr;
+    if (mine && loader) {
+      n_listed = min(u1 - u0, NST);
+      int row = -1;
+      if (lane < n_listed) {
+        const int u = u0 + lane;
+        int b = s_start[0];
+        while (b + 1 < p.batch && u >= seqs[b].x + units_of(seqs[b].y)) ++b;
+        const int unit0 = (u - seqs[b].x) * UNIT;
+        at = p.block_tables + b * p.bt_stride + unit0 / kBlockSize;
+        listed_blk = __ldcg(at);
+        if (listed_blk >= 0 && listed_blk < p.num_blocks) row = listed_blk * kBlockSize + unit0 % kBlockSize;
+      }
+#pragma unroll 1
+      for (int k0 = 0; k0 < n_listed * 2 * NW; k0 += 32) {
+        const int k = k0 + lane, from = __shfl_sync(ALL, row, min(k / (2 * NW), 31));
+        if (k < n_listed * 2 * NW && from >= 0) sm100::tma_prefetch_3d(k & 1 ? &tmap_v : &tmap_k, 0, kvh, from + k % (2 * NW) / 2 * TT);
+      }
+    }
+    pdl_wait();
+    const bool changed = (!loader && tid < p.batch && length_of(tid) != len_lo) || (at && *at != listed_blk);
+    if (!__syncthreads_or(changed)) break;
+    n_listed = 0;
   }
-  __syncthreads();
+  for (int b = b_lo; b < b_hi; ++b)
+    if (length_of(b) == 0) write_zeros(b);
+  if (!mine) return;
+
   auto range_of = [&](int u) {  // the range that holds global unit u
     const int split = longer * (per_range + 1);
     return u < split ? u / (per_range + 1) : longer + (u - split) / per_range;
@@ -202,6 +275,69 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
     } while (u >= c.first + c.units);
     c.slot = slot_of(c.b);
   };
+
+  const int n_units = u1 - u0;
+  const uint32_t ring = smem_u32(smem), scale_ring = ring + C::OFF_SCALES;
+  auto full = [&](int i) { return smem_u32(s_full + i % NST); };
+  auto free = [&](int i) { return smem_u32(s_free + i % NST); };
+  auto sync_warps = [&]() { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); };  // of those that compute
+  Fp8Cursor cc;
+  cc.b = s_start[0];
+  cc.first = s_start[1];
+  cc.ctx = s_start[2];
+  cc.units = units_of(cc.ctx);
+  cc.slot = slot_of(cc.b);
+  int bad = 0;
+
+  // ---- 2. the loading warp: units by TMA (a box to a warp's tile that holds a token), their scales a group to a lane ----
+  if (loader) {
+    const bool of_v = lane >= C::UNIT_GROUPS;
+    const float* scales = of_v ? p.v_scale : p.k_scale;
+    auto block_at = [&](int j) -> int64_t {  // of the range's j-th unit; the cursor goes along
+      seek(cc, u0 + j);
+      const int64_t blk = j < n_listed ? __shfl_sync(ALL, listed_blk, j) : p.block_tables[cc.b * p.bt_stride + (u0 + j - cc.first) * UNIT / kBlockSize];
+      if (blk >= 0 && blk < p.num_blocks) return blk;
+      bad |= NVLLM_STATUS_BAD_BLOCK;
+      return p.num_blocks;  // rows behind the cache: zeros
+    };
+    auto scale_of = [&](int64_t blk, int unit0) {
+      if (blk >= p.num_blocks || lane >= 2 * C::UNIT_GROUPS) return 0.f;
+      return scales[(blk * p.hkv + kvh) * kGroups + unit0 % kBlockSize / kScaleGroup + lane % C::UNIT_GROUPS];
+    };
+    int64_t blk = block_at(0);
+    float scale = scale_of(blk, (u0 - cc.first) * UNIT);
+#pragma unroll 1
+    for (int j = 0; j < n_units; ++j) {
+      const int unit0 = (u0 + j - cc.first) * UNIT;
+      if (j >= NST && !sm100::mbar_wait(free(j), (j / NST - 1) & 1)) {
+        bad |= NVLLM_STATUS_TIMEOUT;
+        break;
+      }
+      const int row = static_cast<int>(blk * kBlockSize + unit0 % kBlockSize);
+      if (lane == 0) {
+        const uint32_t dst = ring + j % NST * C::STAGE_BYTES;
+        const int tiles = min((cc.ctx - unit0 + TT - 1) / TT, NW);
+        sm100::mbar_expect_tx(full(j), tiles * 2 * C::TILE_BYTES);
+#pragma unroll 1
+        for (int w = 0; w < tiles; ++w) {
+          sm100::tma_load_3d(dst + w * C::TILE_BYTES, &tmap_k, full(j), 0, kvh, row + w * TT);
+          sm100::tma_load_3d(dst + C::UNIT_BYTES + w * C::TILE_BYTES, &tmap_v, full(j), 0, kvh, row + w * TT);
+        }
+        s_row[j % NST] = row;
+      }
+      // the next unit's entry and scales, on their way while this one's tiles are
+      const float scale_now = scale;
+      if (j + 1 < n_units) {
+        blk = block_at(j + 1);
+        scale = scale_of(blk, (u0 + j + 1 - cc.first) * UNIT);
+      }
+      if (lane < 2 * C::UNIT_GROUPS) st_shared_f32(scale_ring + j % NST * C::SCALE_BYTES + lane * 4, scale_now);
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(full(j));
+    }
+    if (bad && lane == 0) atomicOr(p.status, bad);
+    return;
+  }
 
   // ---- the query: lane (gid, tig) holds columns 16 (tig + 4 j) .. + 15 of head gid ------------
   constexpr int QW = D / 8;  // words of them
@@ -234,82 +370,24 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
     qk1 = __shfl_sync(ALL, back, 8 * tig + 4);
   };
 
-  // ---- tiles: the warp's ring ------------------------------------------------------------------
-  const uint32_t warp_smem = smem_u32(smem) + warp * C::WARP_BYTES;
-  const uint32_t warp_scales = smem_u32(smem) + C::OFF_SCALES + warp * NST * C::SCALE_BYTES;
+  // ---- 3. the other warps: a tile of every unit -------------------------------------------------
+  const uint32_t warp_tile = ring + warp * C::TILE_BYTES, warp_scales = scale_ring + warp * MT * 4;
   const int64_t row_bytes = static_cast<int64_t>(p.hkv) * D;
   const bool is_v = lane >= 16;
   const int sub = (lane & 15) / PIECES, piece = lane % PIECES;
-
-  int bad = 0;
-  unsigned fresh = 0;     // step variant: stages whose tile holds the new token's row
-  uint4 new_row[NST];     // and its row, K in the lower half of the warp, V in the upper: eight values a lane
-  Fp8Cursor cc, pc;       // compute side; load side, NST - 1 units ahead
-  auto load_unit = [&](int j) {  // the range's j-th unit
-    const int stage = j % NST;
-    seek(pc, u0 + j);
-    fresh &= ~(1u << stage);
-    const int t0 = (u0 + j - pc.first) * UNIT + warp * TT;
-    if (t0 >= pc.ctx) return;
-    int64_t blk = p.block_tables[pc.b * p.bt_stride + t0 / kBlockSize];
-    const bool blk_ok = blk >= 0 && blk < p.num_blocks;
-    if (!blk_ok) {
-      bad |= NVLLM_STATUS_BAD_BLOCK;
-      blk = 0;
-    }
-    const int64_t slot0 = blk * kBlockSize + t0 % kBlockSize;
-    int end = pc.ctx;  // rows from here on are zeros
-    if (STEP && pc.ctx - 1 < t0 + TT && pc.slot >= 0) {
-      if (blk_ok && pc.slot == slot0 + (pc.ctx - 1 - t0)) {
-        end = pc.ctx - 1;
-        fresh |= 1u << stage;
-        const __nv_bfloat16* src = (is_v ? p.v_new + pc.b * p.v_new_stride : p.k_new + pc.b * p.k_new_stride) + kvh * D + piece * 8;
-        const uint4 x = sub == 0 ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
-#pragma unroll
-        for (int s = 0; s < NST; ++s)
-          if (s == stage) new_row[s] = x;
-      } else {
-        bad |= NVLLM_STATUS_BAD_SLOT;
-      }
-    }
-    const uint32_t kdst = warp_smem + stage * C::STAGE_BYTES;
-#pragma unroll
-    for (int it = 0; it < TT * C::CPR / 32; ++it) {
-      const int idx = it * 32 + lane;
-      const int r = idx / C::CPR, col = idx % C::CPR;
-      const int bytes = blk_ok && t0 + r < end ? 16 : 0;
-      const int64_t off = bytes ? (slot0 + r) * row_bytes + kvh * D + col * 16 : 0;
-      const uint32_t dst = kdst + tile_offset<D>(r, col);
-      cp_async16(dst, p.k_cache + off, bytes);
-      cp_async16(dst + C::TILE_BYTES, p.v_cache + off, bytes);
-    }
-    if (lane < 2) {
-      const int64_t at = (blk * p.hkv + kvh) * kGroups + t0 % kBlockSize / kScaleGroup;
-      cp_async_small<MT * 4>(warp_scales + stage * C::SCALE_BYTES + lane * MT * 4, (lane ? p.v_scale : p.k_scale) + at, blk_ok ? MT * 4 : 0);
-    }
+  // Step variant: the new token's row of a sequence, K in the lower half of the warp, V in the upper, eight values a lane.
+  auto load_new = [&](int b) {
+    const __nv_bfloat16* src = (is_v ? p.v_new + b * p.v_new_stride : p.k_new + b * p.k_new_stride) + kvh * D + piece * 8;
+    return sub == 0 ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
   };
-
-  cc.b = s_start[0];
-  cc.first = s_start[1];
-  cc.ctx = s_start[2];
-  cc.units = units_of(cc.ctx);
-  cc.slot = slot_of(cc.b);
-  pc = cc;
-  uint32_t qn[QW];  // the next sequence's query, fetched early
-  {
-    uint32_t raw[QW];
-    load_q(raw, cc.b);
-    const int n_units0 = u1 - u0;
-#pragma unroll
-    for (int j = 0; j < NST - 1; ++j) {
-      if (j < n_units0) load_unit(j);
-      cp_async_commit();
-    }
-    take_q(raw);
-  }
+  uint4 new_row = make_uint4(0, 0, 0, 0), next_row = new_row;
+  uint32_t qn[QW];  // the next sequence's query, and its row, fetched early
+  load_q(qn, cc.b);
+  if (STEP) new_row = load_new(cc.b);
+  take_q(qn);
   int qn_b = min(cc.b + 1, p.batch - 1);
   load_q(qn, qn_b);
-  const int n_units = u1 - u0;
+  if (STEP) next_row = load_new(qn_b);
 
   float o[C::KS][4];     // columns 16 c + 2 gid (and + 1 in [2], [3]) of heads 2 tig ([0], [2]) and 2 tig + 1, in units of `unit`
   float m0, m1, l0, l1;  // heads 2 tig and 2 tig + 1
@@ -327,8 +405,8 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
   };
   reset_state();
 
-  float* sm_o = reinterpret_cast<float*>(smem + C::OFF_MERGE);  // [NW][8][D]
-  float* sm_ml = sm_o + NW * 8 * D;                             // [NW][8][2]
+  constexpr int OROW = C::OROW;
+  float* sm_o = reinterpret_cast<float*>(smem + C::OFF_MERGE);  // [NW][8][OROW]
   auto add_scaled = [](float4& acc, const float4& v, float f) {
     acc.x += v.x * f;
     acc.y += v.y * f;
@@ -351,33 +429,38 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
       l0 += __shfl_xor_sync(ALL, l0, sh);
       l1 += __shfl_xor_sync(ALL, l1, sh);
     }
-    __syncthreads();  // the previous merge has been read by everyone
+    sync_warps();  // the previous merge has been read by everyone
 #pragma unroll
     for (int c = 0; c < C::KS; ++c) {
-      float* dst = sm_o + (warp * 8 + 2 * tig) * D + c * 16 + 2 * gid;
+      float* dst = sm_o + (warp * 8 + 2 * tig) * OROW + c * 16 + 2 * gid;
       *reinterpret_cast<float2*>(dst) = make_float2(o[c][0] * unit, o[c][2] * unit);
-      *reinterpret_cast<float2*>(dst + D) = make_float2(o[c][1] * unit, o[c][3] * unit);
+      *reinterpret_cast<float2*>(dst + OROW) = make_float2(o[c][1] * unit, o[c][3] * unit);
     }
     if (gid == 0) {
-      *reinterpret_cast<float4*>(sm_ml + (warp * 8 + 2 * tig) * 2) = make_float4(m0, l0, m1, l1);
+      float* dst = sm_o + (warp * 8 + 2 * tig) * OROW + D;
+      *reinterpret_cast<float2*>(dst) = make_float2(m0, l0);
+      *reinterpret_cast<float2*>(dst + OROW) = make_float2(m1, l1);
     }
-    const int r_first = range_of(cc.first), r_last = range_of(cc.first + cc.units - 1);
-    const int n_parts = r_last - r_first + 1;  // ranges that hold a piece of this sequence
-    __syncthreads();
+    int r_first = range, n_parts = 1;  // ranges that hold a piece of this sequence
+    if (cc.first < u0 || cc.first + cc.units > u1) {
+      r_first = range_of(cc.first);
+      n_parts = range_of(cc.first + cc.units - 1) - r_first + 1;
+    }
+    sync_warps();
     for (int quad = tid; quad < p.g * QUADS; quad += NT) {  // four columns of a head per thread
       const int h = quad / QUADS, d4 = quad % QUADS;
       float m[NW], mm = -INFINITY, L = 0.f;
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        m[w] = sm_ml[(w * 8 + h) * 2];
+        m[w] = sm_o[(w * 8 + h) * OROW + D];
         mm = fmaxf(mm, m[w]);
       }
       float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
         const float f = m[w] == -INFINITY ? 0.f : fast_exp2(m[w] - mm);
-        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * 8 + h) * D + d4 * 4);
-        L += sm_ml[(w * 8 + h) * 2 + 1] * f;
+        const float4 v = *reinterpret_cast<const float4*>(sm_o + (w * 8 + h) * OROW + d4 * 4);
+        L += sm_o[(w * 8 + h) * OROW + D + 1] * f;
         add_scaled(acc, v, f);
       }
       if (n_parts == 1) {
@@ -399,7 +482,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
   // Merges the partials of a cut sequence, all of which are in the workspace, and writes its rows: QUADS lanes take a head,
   // four columns each, and the statistics of a part each; eight parts to a trip; lane groups left over split the parts.
   auto merge_cut = [&](const Fp8Cut& c) {
-    constexpr int AHEAD = 8;
+    constexpr int AHEAD = D == 64 ? 16 : 8;
     const int group = tid / QUADS, gl = tid % QUADS;
     const int n_split = max(1, GROUPS / p.g);
     for (int h0 = 0; h0 < p.g; h0 += GROUPS) {
@@ -465,7 +548,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
           *reinterpret_cast<float4*>(patch + gl * 4) = acc;
           if (gl == 0) *reinterpret_cast<float2*>(patch + D) = make_float2(mm, L);
         }
-        __syncthreads();
+        sync_warps();
         if (active && split == 0)
           for (int k = 1; k < n_split; ++k) {
             const float* other = sm_o + (group + k * p.g) * (D + 4);
@@ -475,14 +558,13 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
             L += ml.y * f;
             add_scaled(acc, *reinterpret_cast<const float4*>(other + gl * 4), f);
           }
-        __syncthreads();
+        sync_warps();
       }
       if (active && split == 0) write_quad(c.b, head, gl, acc, L);
     }
     if (tid == 0) p.counters[c.b * p.hkv + kvh] = 0u;  // ready for the next launch
   };
 
-  // ---- 2. stream the range ------------------------------------------------------------------
   for (int i = 0;; ++i) {
     const int u = u0 + i;
     if (i == n_units || u >= cc.first + cc.units) {  // block-uniform: the range leaves sequence cc.b
@@ -490,33 +572,41 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
       if (i == n_units) break;
       seek(cc, u);
       reset_state();
-      if (qn_b != cc.b) load_q(qn, cc.b);  // empty sequences in between
+      if (qn_b != cc.b) {  // empty sequences in between
+        load_q(qn, cc.b);
+        if (STEP) next_row = load_new(cc.b);
+      }
       take_q(qn);
+      new_row = next_row;
       qn_b = min(cc.b + 1, p.batch - 1);
       load_q(qn, qn_b);
+      if (STEP) next_row = load_new(qn_b);
     }
-    cp_async_wait<NST - 2>();
-    if (!STEP) __syncthreads();  // the warps' tiles of a unit are fetched together
-    else __syncwarp();
-    if (i + NST - 1 < n_units) load_unit(i + NST - 1);
-    cp_async_commit();
-
+    if (!sm100::mbar_wait(full(i), (i / NST) & 1)) {
+      bad |= NVLLM_STATUS_TIMEOUT;
+      break;
+    }
     const int t0 = (u - cc.first) * UNIT + warp * TT;
-    if (t0 >= cc.ctx) continue;
-    const uint32_t kbase = warp_smem + (i % NST) * C::STAGE_BYTES, vbase = kbase + C::TILE_BYTES;
+    if (t0 >= cc.ctx) {
+      if (lane == 0) sm100::mbar_arrive(free(i));
+      continue;
+    }
+    const uint32_t kbase = warp_tile + (i % NST) * C::STAGE_BYTES, vbase = kbase + C::UNIT_BYTES;
     const uint32_t scales = warp_scales + (i % NST) * C::SCALE_BYTES;
 
-    if (STEP && (fresh >> (i % NST) & 1u)) {  // the new token's row: to the tile and to the cache, its group with it
-      const int r = cc.ctx - 1 - t0, r0 = r & ~(kScaleGroup - 1);  // row of the tile; first of its group
-      uint4 x = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int s = 0; s < NST; ++s)
-        if (s == i % NST) x = new_row[s];
+    const int r = cc.ctx - 1 - t0, r0 = r & ~(kScaleGroup - 1);  // the newest token's row of the tile, the first one of its group
+    bool fresh = STEP && r < TT && cc.slot >= 0;
+    if (fresh) {  // its place by the table, too
+      fresh = cc.slot == s_row[i % NST] + warp * TT + r && cc.slot < p.num_blocks * kBlockSize;
+      if (!fresh) bad |= NVLLM_STATUS_BAD_SLOT;
+    }
+    if (fresh) {  // the new token's row: to the tile and to the cache, its group with it
+      const uint4 x = new_row;
       uint32_t most = max_finite2(max_finite2(max_finite2(max_finite2(0, x.x), x.y), x.z), x.w);
       most = max(most & 0xffffu, most >> 16);
 #pragma unroll
       for (int d = 8; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(ALL, most, d));
-      const uint32_t scale_smem = scales + (is_v ? MT * 4 : 0) + (r0 / kScaleGroup) * 4;
+      const uint32_t scale_smem = scales + (is_v ? C::UNIT_GROUPS * 4 : 0) + (r0 / kScaleGroup) * 4;
       const float old = ld_shared_f32(scale_smem);
       const int e = r > r0 ? max(exponent_for(most), exponent_of(old)) : exponent_for(most);
       const float now = power_of_two(e), inv = power_of_two(-e);
@@ -538,6 +628,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
         st_shared8(in_tile(r), c);
         *reinterpret_cast<uint2*>(to + r * row_bytes) = c;
       }
+      sm100::fence_proxy_async();  // TMA writes here again
       __syncwarp();
       if ((lane & 15) == 0) {
         st_shared_f32(scale_smem, now);
@@ -547,16 +638,23 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
       __syncwarp();
     }
 
+    const bool tail = t0 + TT > cc.ctx;
+    if (tail) {  // V rows behind the end hold anything: zeros, which their weights leave what they are
+      for (int x = (cc.ctx - t0) * C::CPR + lane; x < TT * C::CPR; x += 32)
+        st_shared16(vbase + tile_offset<D>(x / C::CPR, x % C::CPR), make_uint4(0, 0, 0, 0));
+      sm100::fence_proxy_async();
+      __syncwarp();
+    }
+
     // S^T = K Q^T, in log2 units
     float s[MT][4], vs[MT], most_vs = 0.f;
-    const bool tail = t0 + TT > cc.ctx;
     float mx0 = -INFINITY, mx1 = -INFINITY;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       s[mt][0] = s[mt][1] = s[mt][2] = s[mt][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 64; ++j) {
-        const int ra = mt * 16 + gid;
+        const int ra = mt * 16 + token_of_row<D>(gid);
         const uint4 a = ld_shared16(kbase + tile_offset<D>(ra, tig + 4 * j)), b = ld_shared16(kbase + tile_offset<D>(ra + 8, tig + 4 * j));
         const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
@@ -565,7 +663,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
                         qb[8 * j + 2 * w], qb[8 * j + 2 * w + 1]);
       }
       const float ks = ld_shared_f32(scales + mt * 4);
-      vs[mt] = t0 + mt * 16 < cc.ctx ? ld_shared_f32(scales + (MT + mt) * 4) : 0.f;  // a group past the end: whatever is there
+      vs[mt] = t0 + mt * 16 < cc.ctx ? ld_shared_f32(scales + (C::UNIT_GROUPS + mt) * 4) : 0.f;  // a group past the end: whatever is there
       most_vs = fmaxf(most_vs, vs[mt]);
       const float f0 = qk0 * ks, f1 = qk1 * ks;
       s[mt][0] *= f0;
@@ -573,7 +671,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
       s[mt][2] *= f0;
       s[mt][3] *= f1;
       if (tail) {
-        const int tr = t0 + mt * 16 + gid;
+        const int tr = t0 + mt * 16 + token_of_row<D>(gid);
         if (tr >= cc.ctx) s[mt][0] = s[mt][1] = -INFINITY;
         if (tr + 8 >= cc.ctx) s[mt][2] = s[mt][3] = -INFINITY;
       }
@@ -627,7 +725,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
     for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
       for (int c = 0; c < C::KS; c += 2) {
-        const int r = mt * 16 + (lane & 15);
+        const int r = mt * 16 + (lane & 8) + token_of_row<D>(lane & 7);
         uint32_t v[4];  // tokens 0-7 and 8-15 of columns 16 c .., then of 16 (c + 1) ..
         ldmatrix_x4_trans(v[0], v[1], v[2], v[3], vbase + tile_offset<D>(r, c + (lane >> 4)));
 #pragma unroll
@@ -637,11 +735,12 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
         }
       }
     }
+    __syncwarp();  // everything of the unit is in registers
+    if (lane == 0) sm100::mbar_arrive(free(i));
   }
-  cp_async_wait<0>();
   if (bad && lane == 0) atomicOr(p.status, bad);
   if (n_cut == 0) return;  // block-uniform
-  __syncthreads();         // every thread's partials are written
+  sync_warps();            // every thread's partials are written
   if (tid < n_cut) {
     const Fp8Cut& c = tid == 0 ? cut0 : cut1;
     unsigned int arrived;  // releases the block's partials (the barrier ordered them before), acquires the others'
@@ -649,7 +748,7 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
                  : "=r"(arrived) : "l"(p.counters + c.b * p.hkv + kvh) : "memory");
     s_last_arrival[tid] = arrived == static_cast<unsigned int>(c.n - 1);
   }
-  __syncthreads();
+  sync_warps();
   if (s_last_arrival[0]) merge_cut(cut0);
   if (n_cut > 1 && s_last_arrival[1]) merge_cut(cut1);
 }
@@ -658,6 +757,10 @@ __global__ void __launch_bounds__(C::NW * 32, 2) decode_fp8_kernel(const DecodeF
 
 template <class C>
 static int launch_decode_fp8(const DecodeFp8Params& p, cudaStream_t stream) {
+  CUtensorMap mk, mv;
+  const uint64_t slots = static_cast<uint64_t>(p.num_blocks) * kBlockSize;
+  if (!sm100::make_tmap_codes(&mk, p.k_cache, C::D, p.hkv, slots, C::TT) || !sm100::make_tmap_codes(&mv, p.v_cache, C::D, p.hkv, slots, C::TT))
+    return NVLLM_E_CUDA;
   static bool attr_set[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -669,7 +772,7 @@ static int launch_decode_fp8(const DecodeFp8Params& p, cudaStream_t stream) {
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
   return launch_kernel("decode_fp8", p.k_new ? decode_fp8_kernel<C, true> : decode_fp8_kernel<C, false>,
-                       dim3(static_cast<unsigned>(p.n_ranges * p.hkv)), dim3(C::NW * 32), C::SMEM, stream, p);
+                       dim3(static_cast<unsigned>(p.n_ranges * p.hkv)), dim3(C::NTHREADS), C::SMEM, stream, p, mk, mv);
 }
 
 struct Fp8Cache {
@@ -733,15 +836,19 @@ static int decode_fp8_common(const char* who, const void* q, int64_t q_row_strid
   p.v_new_stride = v_new_row_stride;
   p.slot_mapping = slot_mapping;
   auto ranges_for = [&](int ctas) { return ctas / num_kv_heads > 1 ? ctas / num_kv_heads : 1; };
-  const int ctas = 2 * num_sms();
-  p.n_ranges = ranges_for(ctas > 0 && ctas <= kFp8MaxCtas ? ctas : kFp8MaxCtas);
+  auto ranges_of = [&](int blocks) {
+    const int ctas = blocks * num_sms();
+    return ranges_for(ctas > 0 && ctas <= kFp8MaxCtas ? ctas : kFp8MaxCtas);
+  };
   const int64_t rows = (static_cast<int64_t>(ranges_for(kFp8MaxCtas)) + batch) * num_q_heads;
   p.counters = static_cast<unsigned int*>(workspace);
   p.ws_o = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + kFp8CounterBytes);
   p.ws_ml = p.ws_o + rows * head_dim;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_decode_fp8<DecodeFp8Cfg<128, 32, 3, 4>>(p, st);
-  return launch_decode_fp8<DecodeFp8Cfg<64, 32, 4, 4>>(p, st);
+  using Wide = DecodeFp8Cfg<128, 32, 3, 4, 2>;
+  using Narrow = DecodeFp8Cfg<64, 64, 2, 4, 2>;
+  p.n_ranges = ranges_of(head_dim == 128 ? Wide::BLOCKS : Narrow::BLOCKS);
+  return head_dim == 128 ? launch_decode_fp8<Wide>(p, st) : launch_decode_fp8<Narrow>(p, st);
 }
 
 }  // namespace nvllm

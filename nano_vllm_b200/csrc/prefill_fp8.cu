@@ -112,10 +112,6 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uin
 __host__ __device__ constexpr uint32_t idesc_f8(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return idesc_f8(m, n) | (1u << 16); }
 
-__device__ __forceinline__ void prefetch_tile(const CUtensorMap* map, int c0, int c1, int c2) {
-  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(map), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
-
 // A tile's scales: K's; V's over the unit, as f16 pairs; what O is multiplied by (where the unit changes); the unit.
 struct __align__(16) Fp8Tile {
   float k[4];
@@ -446,8 +442,8 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           s[4] = x.Lq; s[5] = x.Lk; s[6] = x.n_kv;
           mbar_arrive(bar(ITEM_FULL0 + (it & 1)));
           if (x.n_kv > 0) {  // its query rows are on the path from the item before: to L2
-            prefetch_tile(&tmap_q, 0, x.h, x.q0 + x.m0);
-            if constexpr (D == 128) prefetch_tile(&tmap_q, 64, x.h, x.q0 + x.m0);
+            tma_prefetch_3d(&tmap_q, 0, x.h, x.q0 + x.m0);
+            if constexpr (D == 128) tma_prefetch_3d(&tmap_q, 64, x.h, x.q0 + x.m0);
           }
         }
         __syncwarp();
