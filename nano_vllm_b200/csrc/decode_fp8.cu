@@ -624,7 +624,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
         }
       }
       if (sub == 0) {
-        const uint2 c = encode8(x, inv);
+        const uint2 c = make_uint2(encode4(make_uint2(x.x, x.y), inv), encode4(make_uint2(x.z, x.w), inv));
         st_shared8(in_tile(r), c);
         *reinterpret_cast<uint2*>(to + r * row_bytes) = c;
       }

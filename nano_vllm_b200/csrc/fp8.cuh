@@ -74,6 +74,12 @@ __device__ __forceinline__ uint32_t max_finite2(uint32_t m, uint32_t x) {
   x &= 0x7fff7fffu;
   return __vmaxu2(m, x & ~__vcmpgeu2(x, 0x7f807f80u));
 }
+// The larger of the magnitudes of two bf16, twice; the sign bits are anything.  NaN wins.
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 // Exponent of the smallest scale s that takes a magnitude of these bf16 bits: |x| <= 448 s, 448 = 1.75 * 2^8.
 __device__ __forceinline__ int exponent_for(uint32_t bf16_bits) {
   const int e = static_cast<int>(bf16_bits >> 7) - 127 - 8 + ((bf16_bits & 0x7fu) > 0x60u);
@@ -85,18 +91,21 @@ __device__ __forceinline__ int exponent_of(float scale) {
   return min(kMaxExponent, max(kMinExponent, static_cast<int>(b >> 23 & 255u) - 127 + ((b & 0x7fffffu) != 0)));
 }
 
-// Eight bf16 over a scale of 1 / inv to eight codes; what is not finite becomes NaN (e4m3 has no infinities).
-__device__ __forceinline__ uint2 encode8(const uint4& x, float inv) {
-  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-  uint32_t h[4];
+// Four bf16 over a scale of 1 / inv to four codes; what is not finite becomes NaN (e4m3 has no infinities).
+__device__ __forceinline__ uint32_t encode4(const uint2& x, float inv) {
+  float y[4] = {__uint_as_float(x.x << 16) * inv, __uint_as_float(x.x & 0xffff0000u) * inv, __uint_as_float(x.y << 16) * inv,
+                __uint_as_float(x.y & 0xffff0000u) * inv};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float lo = __uint_as_float(w[i] << 16) * inv, hi = __uint_as_float(w[i] & 0xffff0000u) * inv;
-    lo = fabsf(lo) <= 448.f ? lo : NAN;
-    hi = fabsf(hi) <= 448.f ? hi : NAN;
-    h[i] = e4m3x2(lo, hi);
-  }
-  return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+  for (int i = 0; i < 4; ++i) y[i] = fabsf(y[i]) <= 448.f ? y[i] : NAN;
+  return e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16;
+}
+// The same of finite values, inv = 2^-e twice in bf16 (a power of two leaves all bits of a bf16 product).
+__device__ __forceinline__ uint32_t encode4_finite(const uint2& x, uint32_t inv) {
+  uint32_t a, b;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(x.x), "r"(inv));
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(x.y), "r"(inv));
+  return __byte_perm(e4m3x2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)),
+                     e4m3x2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), 0x5410);
 }
 // Four codes whose scale changes by `ratio` <= 1.
 __device__ __forceinline__ uint32_t recode4(uint32_t c, float ratio) {

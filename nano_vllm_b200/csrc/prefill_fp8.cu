@@ -124,13 +124,6 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// The larger of the magnitudes of two bf16, twice; the sign bits are anything.  NaN wins.
-__device__ __forceinline__ uint32_t max_magnitude(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
 struct Fp8Item {
   int b, h, m0, q0, Lq, Lk, n_kv;  // n_kv < 0: no more work
 };

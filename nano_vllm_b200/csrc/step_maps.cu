@@ -10,12 +10,14 @@
 // Every thread block sums the lengths itself (two words a sequence, a scan in shared memory) and then fills its share of the
 // tables and rows, so one launch does it without any block waiting for another.  A token finds its sequence by bisection of
 // the sums; a fresh block's id is read from the free list and not from the table that another block fills.
+#include <algorithm>
+
 #include "common.cuh"
 
 namespace nvllm {
 
 constexpr int kMapsThreads = 256;
-constexpr int kMapsMaxBatch = 4096;  // two sums a sequence in shared memory
+constexpr int kMapsMaxBatch = 4096;  // 16 bytes a sequence in shared memory
 
 struct StepMapsParams {
   const int32_t* seq_lens;
@@ -36,14 +38,12 @@ struct StepMapsParams {
 };
 
 __global__ void __launch_bounds__(kMapsThreads) step_maps_kernel(const StepMapsParams p) {
-  __shared__ int s_q[kMapsMaxBatch + 1], s_first[kMapsMaxBatch + 1];
+  extern __shared__ int4 s_seq[];  // of every sequence: first packed token, first fresh block, cached tokens, all tokens; then the sums
   __shared__ int s_warp[3][kMapsThreads / 32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int most = p.width * kBlockSize;
   pdl_wait();
   pdl_trigger();
-  auto cached_of = [&](int b) { return max(0, min(p.cached_lens[b], most)); };
-  auto length_of = [&](int b) { return max(0, min(p.seq_lens[b], most)); };
   auto blocks = [](int tokens) { return (tokens + kBlockSize - 1) / kBlockSize; };
 
   // per thread a run of sequences; their sums, a scan over the threads, then the run again
@@ -52,8 +52,10 @@ __global__ void __launch_bounds__(kMapsThreads) step_maps_kernel(const StepMapsP
   int sum[3] = {0, 0, 0};  // new tokens, fresh blocks, all tokens
   bool bad = false;
   for (int b = lo; b < hi; ++b) {
-    const int cached = cached_of(b), len = length_of(b);
-    bad |= cached != p.cached_lens[b] || len != p.seq_lens[b];
+    const int raw_cached = p.cached_lens[b], raw_len = p.seq_lens[b];
+    const int cached = max(0, min(raw_cached, most)), len = max(0, min(raw_len, most));
+    bad |= cached != raw_cached || len != raw_len;
+    s_seq[b] = make_int4(sum[0], sum[1], cached, len);
     sum[0] += max(len - cached, 0);
     sum[1] += max(blocks(len) - blocks(cached), 0);
     sum[2] += len;
@@ -72,55 +74,58 @@ __global__ void __launch_bounds__(kMapsThreads) step_maps_kernel(const StepMapsP
   }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < 3; ++k)
-    for (int w = 0; w < warp; ++w) before[k] += s_warp[k][w];
+  for (int w = 0; w < kMapsThreads / 32; ++w)
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      if (w < warp) before[k] += s_warp[k][w];
   const bool first_block = blockIdx.x == 0;
+  int keys = before[2];
   for (int b = lo; b < hi; ++b) {
-    const int cached = cached_of(b), len = length_of(b);
-    s_q[b] = before[0];
-    s_first[b] = before[1];
+    int4 x = s_seq[b];
+    x.x += before[0];
+    x.y += before[1];
+    s_seq[b] = x;
     if (first_block) {
-      p.cu_q[b] = before[0];
-      p.cu_k[b] = before[2];
+      p.cu_q[b] = x.x;
+      p.cu_k[b] = keys;
     }
-    before[0] += max(len - cached, 0);
-    before[1] += max(blocks(len) - blocks(cached), 0);
-    before[2] += len;
+    keys += x.w;
   }
   if (hi == p.batch && lo < hi) {  // one thread: the last run's
-    s_q[p.batch] = before[0];
-    s_first[p.batch] = before[1];
+    const int total = before[0] + sum[0], taken = before[1] + sum[1];
+    s_seq[p.batch] = make_int4(total, taken, 0, 0);
     if (first_block) {
-      p.cu_q[p.batch] = before[0];
-      p.cu_k[p.batch] = before[2];
-      *p.taken = before[1];
-      if (before[0] > p.rows) atomicOr(p.status, NVLLM_STATUS_BAD_SLOT);
+      p.cu_q[p.batch] = total;
+      p.cu_k[p.batch] = keys;
+      *p.taken = taken;
+      if (total > p.rows) atomicOr(p.status, NVLLM_STATUS_BAD_SLOT);
     }
   }
   if (first_block && bad) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
   __syncthreads();
 
   auto fresh = [&](int k) { return k < p.n_free ? p.free_blocks[k] : -1; };
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kMapsThreads, start = static_cast<int64_t>(blockIdx.x) * kMapsThreads + tid;
-  for (int64_t i = start; i < static_cast<int64_t>(p.batch) * p.width; i += step) {
-    const int b = static_cast<int>(i / p.width), col = static_cast<int>(i - static_cast<int64_t>(b) * p.width);
-    const int held = blocks(cached_of(b));
-    if (col < held) continue;
-    p.block_tables[b * p.bt_stride + col] = col < blocks(length_of(b)) ? fresh(s_first[b] + col - held) : -1;
+  const unsigned step = gridDim.x * kMapsThreads, start = blockIdx.x * kMapsThreads + tid;
+  for (unsigned i = start; i < static_cast<unsigned>(p.batch) * p.width; i += step) {  // below 2^23
+    const int b = i / p.width, col = i - b * p.width;
+    const int4 x = s_seq[b];
+    const int held = blocks(x.z);
+    if (col >= held) p.block_tables[b * p.bt_stride + col] = col < blocks(x.w) ? fresh(x.y + col - held) : -1;
   }
-  const int total = s_q[p.batch];
-  for (int64_t t = start; t < p.rows; t += step) {
+  const int total = s_seq[p.batch].x;
+  for (unsigned t = start; t < static_cast<unsigned>(p.rows); t += step) {
     int slot = -1;
     int64_t position = 0;
-    if (t < total) {
-      int b = 0, end = p.batch;  // the last sequence with s_q[b] <= t, so one that has a token here
+    if (static_cast<int>(t) < total) {
+      int b = 0, end = p.batch;  // the last sequence that starts at t or before, so one that has a token here
       while (end - b > 1) {
         const int mid = (b + end) >> 1;
-        if (s_q[mid] <= t) b = mid;
+        if (s_seq[mid].x <= static_cast<int>(t)) b = mid;
         else end = mid;
       }
-      const int cached = cached_of(b), pos = cached + static_cast<int>(t) - s_q[b], col = pos / kBlockSize, held = blocks(cached);
-      const int blk = col < held ? p.block_tables[b * p.bt_stride + col] : fresh(s_first[b] + col - held);
+      const int4 x = s_seq[b];
+      const int pos = x.z + static_cast<int>(t) - x.x, col = pos / kBlockSize, held = blocks(x.z);
+      const int blk = col < held ? p.block_tables[b * p.bt_stride + col] : fresh(x.y + col - held);
       if (blk >= 0 && blk <= 0x7fffffff / kBlockSize - 1) slot = blk * kBlockSize + pos % kBlockSize;
       position = pos;
     }
@@ -164,11 +169,18 @@ extern "C" int nvllm_step_maps(const int32_t* seq_lens, const int32_t* cached_le
   p.positions = positions;
   p.rows = static_cast<int>(num_rows);
   p.taken = blocks_taken;
-  // a few entries to a thread, so that the sum at the start is paid by few blocks
+  const size_t smem = (static_cast<size_t>(batch) + 1) * sizeof(int4);
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (smem > (48u << 10) && (dev < 0 || dev >= 64 || !ready[dev])) {
+    const cudaError_t e = cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMapsMaxBatch + 1) * sizeof(int4));
+    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "step_maps: cannot reserve shared memory: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  // an entry and a row to a thread, as long as there are SMs: every block makes the sums itself
   const int64_t items = num_rows > static_cast<int64_t>(batch) * max_blocks ? num_rows : static_cast<int64_t>(batch) * max_blocks;
-  int64_t grid = (items + 4 * kMapsThreads - 1) / (4 * kMapsThreads);
-  const int most = 2 * num_sms();
-  if (grid > most) grid = most;
-  return launch_kernel("step_maps", step_maps_kernel, dim3(static_cast<unsigned>(grid > 0 ? grid : 1)), dim3(kMapsThreads), 0,
+  const int64_t grid = std::min<int64_t>((items + kMapsThreads - 1) / kMapsThreads, 2ll * num_sms());
+  return launch_kernel("step_maps", step_maps_kernel, dim3(static_cast<unsigned>(std::max<int64_t>(grid, 1))), dim3(kMapsThreads), smem,
                        static_cast<cudaStream_t>(stream), p);
 }

@@ -7,10 +7,12 @@
 // f == 0 starts a group afresh (whatever an earlier owner of the block left in it counts for nothing); rows above f that are
 // not written stay as they are, they belong to nobody yet.
 //
-// A warp owns a group and head: it reads the group's rows once into registers (16 rows of K by one half of the warp, of V by
-// the other), takes the maximum by shuffles, and writes codes and scale, so no group is touched by two warps and nothing
-// depends on their order.  The rows of a group stand next to each other in slot_mapping (rows that are skipped may lie between);
+// A warp owns a group and head of K or of V: it reads the group's rows once into registers (four values a lane: 16 rows take 32
+// registers, so that 24 warps of an SM have 100 KB on the way), takes the maximum by shuffles, and writes codes and scale, so
+// no group is touched by two warps and nothing depends on their order.  The rows of a group stand next to each other in slot_mapping (rows that are skipped may lie between);
 // the warp that the first of them falls to takes them all.
+#include <algorithm>
+
 #include "fp8.cuh"
 
 namespace nvllm {
@@ -30,47 +32,58 @@ struct StoreFp8Params {
 constexpr int kStoreFp8Threads = 256;
 
 template <int D>
-__global__ void __launch_bounds__(kStoreFp8Threads) store_fp8_kernel(const StoreFp8Params p) {
-  constexpr int PIECES = D / 8;       // lanes that hold a row, eight values each
-  constexpr int ROWS = 16 / PIECES;   // rows that a half of the warp takes at a time
+__global__ void __launch_bounds__(kStoreFp8Threads, 3) store_fp8_kernel(const StoreFp8Params p) {
+  constexpr int LANES = D / 4;       // lanes that hold a row, four values each
+  constexpr int ROWS = 32 / LANES;   // rows that a warp takes at a time
   constexpr int HELD = kScaleGroup / ROWS;
   constexpr unsigned ALL = 0xffffffffu;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const bool is_v = lane >= 16;
-  const int sub = (lane & 15) / PIECES, piece = lane % PIECES;
-  const __nv_bfloat16* rows = is_v ? p.rows[1] : p.rows[0];
+  const int sub = lane / LANES, col = lane % LANES * 4;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_block;
+  const bool is_v = blockIdx.y;
+  const __nv_bfloat16* rows = (is_v ? p.rows[1] : p.rows[0]) + col;
   const int64_t stride = is_v ? p.stride[1] : p.stride[0];
-  unsigned char* cache = is_v ? p.cache[1] : p.cache[0];
-  float* scales = is_v ? p.scale[1] : p.scale[0];
+  auto load = [&](int64_t r, int head) { return __ldg(reinterpret_cast<const uint2*>(rows + r * stride + head * D)); };
 
   pdl_wait();
   pdl_trigger();
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.rows_per_block;
-  const int n_here = static_cast<int>(min(static_cast<int64_t>(p.rows_per_block), p.n - r0));
-  auto slot_at = [&](int64_t r) -> int {  // -1: nothing is stored
-    if (r < 0 || r >= p.n) return -1;
-    const int s = p.slots[r];
-    return s < p.num_slots ? max(s, -1) : -1;
-  };
-  const int slot = lane < n_here ? slot_at(r0 + lane) : -1;
-  if (warp == 0 && lane < n_here && p.slots[r0 + lane] >= p.num_slots) atomicOr(p.status, NVLLM_STATUS_BAD_SLOT);
+  // The slots of this block's rows and of those behind them, a row to a lane, and of the 32 before; where a block has one row
+  // its values come in the same trip.
+  const int64_t n_here = p.n - r0;
+  const int raw = lane < n_here ? p.slots[r0 + lane] : -1, raw_before = r0 + lane >= 32 ? p.slots[r0 + lane - 32] : -1;
+  const bool alone = p.rows_per_block == 1;
+  uint2 early = make_uint2(0, 0);
+  if (alone && sub == 0 && warp < p.hkv) early = load(r0, warp);
+  if (!alone) {  // the block's rows to L2 while it finds out which of them go together
+    for (int head = warp; head < p.hkv; head += warps) {
+      constexpr int LINES = D / 64;  // of a row: 16 rows are 16 or 32 lines
+      const int r = lane / LINES;
+      if (r < min(static_cast<int64_t>(p.rows_per_block), n_here))
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(rows - col + (r0 + r) * stride + head * D + lane % LINES * 64));
+    }
+  }
+  auto stored = [&](int s) { return s < p.num_slots ? max(s, -1) : -1; };  // -1: nothing is stored
+  const int slot = stored(raw);
+  const bool own = lane < p.rows_per_block;
+  if (warp == 0 && !is_v && own && raw >= p.num_slots) atomicOr(p.status, NVLLM_STATUS_BAD_SLOT);
   const unsigned live = __ballot_sync(ALL, slot >= 0);
-  if (!live) return;
+  if (!__ballot_sync(ALL, own && slot >= 0)) return;
   // the group of the last stored row before this block's
-  int before = -1;
+  auto slot_at = [&](int64_t r) { return r >= 0 && r < p.n ? stored(p.slots[r]) : -1; };
+  int before = -1, seen = stored(raw_before);
 #pragma unroll 1
   for (int64_t r = r0 - 32; r > -32; r -= 32) {
-    const int s = slot_at(r + lane);
-    const unsigned m = __ballot_sync(ALL, s >= 0);
+    const unsigned m = __ballot_sync(ALL, seen >= 0);
     if (m) {
-      before = __shfl_sync(ALL, s, 31 - __clz(m)) / kScaleGroup;
+      before = __shfl_sync(ALL, seen, 31 - __clz(m)) / kScaleGroup;
       break;
     }
+    seen = slot_at(r - 32 + lane);
   }
   const int group = slot >= 0 ? slot / kScaleGroup : -1;
   const unsigned below = live & ((1u << lane) - 1);
   const int previous = __shfl_sync(ALL, group, below ? 31 - __clz(below) : lane);
-  const unsigned leaders = __ballot_sync(ALL, slot >= 0 && group != (below ? previous : before));
+  const unsigned leaders = __ballot_sync(ALL, own && slot >= 0 && group != (below ? previous : before));
 
 #pragma unroll 1
   for (int u = warp; u < __popc(leaders) * p.hkv; u += warps) {
@@ -80,15 +93,6 @@ __global__ void __launch_bounds__(kStoreFp8Threads) store_fp8_kernel(const Store
     const int at = __ffs(left) - 1;
     const int g = __shfl_sync(ALL, group, at);
     const int64_t i = r0 + at;
-    const __nv_bfloat16* src = rows + head * D + piece * 8;
-    // Rows i + b, b < 32, of this group: bits b.  `ended`: a row of another group follows, or none.
-    auto window = [&](int64_t from, int& s, bool& ended) {
-      s = slot_at(from + lane);
-      const unsigned same = __ballot_sync(ALL, s >= 0 && s / kScaleGroup == g);
-      const unsigned other = __ballot_sync(ALL, s >= 0 && s / kScaleGroup != g);
-      ended = other != 0 || from + 32 >= p.n;
-      return other ? same & ((other & -other) - 1) : same;
-    };
     // This lane's row of the next ROWS set bits of m, -1 if there is none.
     auto next_rows = [&](unsigned& m) {
       int b = -1;
@@ -100,99 +104,113 @@ __global__ void __launch_bounds__(kStoreFp8Threads) store_fp8_kernel(const Store
       }
       return b;
     };
-    auto load = [&](int64_t r) { return __ldg(reinterpret_cast<const uint4*>(src + r * stride)); };
-
-    int s;
-    bool ended;
-    const unsigned run = window(i, s, ended);
-    const bool held = ended && __popc(run) <= kScaleGroup;  // all rows of the group in registers
-    int first = __reduce_min_sync(ALL, run >> lane & 1u ? s % kScaleGroup : kScaleGroup);
-    uint4 x[HELD];
-    uint32_t most = 0;
-    auto fold = [&](const uint4& v) {
-      most = max_finite2(max_finite2(max_finite2(max_finite2(most, v.x), v.y), v.z), v.w);
-    };
-    float* scale_at = scales + (static_cast<int64_t>(g / kGroups) * p.hkv + head) * kGroups + g % kGroups;
-    float old = 0.f;
-    if (held) {
-      unsigned m = run;
-#pragma unroll
-      for (int j = 0; j < HELD; ++j) {
-        const int b = next_rows(m);
-        x[j] = b >= 0 ? load(i + b) : make_uint4(0, 0, 0, 0);
-      }
-      if (first > 0) old = *scale_at;
-#pragma unroll
-      for (int j = 0; j < HELD; ++j) fold(x[j]);
-    } else {  // the same slots over and over
-      int64_t from = i;
-#pragma unroll 1
-      while (true) {
-        int s2;
-        bool end2;
-        unsigned m = window(from, s2, end2);
-        first = min(first, __reduce_min_sync(ALL, m >> lane & 1u ? s2 % kScaleGroup : kScaleGroup));
-#pragma unroll 1
-        while (m) {
-          const int b = next_rows(m);
-          if (b >= 0) fold(load(from + b));
-        }
-        if (end2) break;
-        from += 32;
-      }
-      if (first > 0) old = *scale_at;
-    }
-    most = max(most & 0xffffu, most >> 16);
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(ALL, most, d));
-    const int e = first > 0 ? max(exponent_for(most), exponent_of(old)) : exponent_for(most);
-    const float now = power_of_two(e), inv = power_of_two(-e);
-    if (first > 0 && now != old) {  // a half warp at most: no shuffles in here
-      const float ratio = old * inv;
-#pragma unroll 1
-      for (int r = sub; r < first; r += ROWS) {
-        uint2* c = reinterpret_cast<uint2*>(cache + ((static_cast<int64_t>(g) * kScaleGroup + r) * p.hkv + head) * D + piece * 8);
-        const uint2 v = *c;
-        *c = make_uint2(recode4(v.x, ratio), recode4(v.y, ratio));
-      }
-    }
-    __syncwarp();
-    auto store = [&](const uint4& v, int to) {
-      *reinterpret_cast<uint2*>(cache + (static_cast<int64_t>(to) * p.hkv + head) * D + piece * 8) = encode8(v, inv);
-    };
-    // Rows in order, so that of two with the same slot the later one stays; of two at a time the first only where they differ.
+    // Where row b of the slots `sl` goes: rows in order, so that of two with the same slot the later one stays; of two at a time
+    // the first only where they differ.
     auto destination = [&](int sl, int b) {
       const int to = __shfl_sync(ALL, sl, max(b, 0));
-      const int later = ROWS == 2 ? __shfl_down_sync(ALL, b >= 0 ? to : -1, PIECES) : -1;
+      const int later = ROWS == 2 ? __shfl_down_sync(ALL, b >= 0 ? to : -1, LANES) : -1;
       return b < 0 || (ROWS == 2 && sub == 0 && later == to) ? -1 : to;
     };
-    if (held) {
-      unsigned m = run;
+    float* scale_at = (is_v ? p.scale[1] : p.scale[0]) + (static_cast<int64_t>(g / kGroups) * p.hkv + head) * kGroups + g % kGroups;
+    unsigned char* cache = (is_v ? p.cache[1] : p.cache[0]) + head * D + col;
+    const int64_t row_bytes = static_cast<int64_t>(p.hkv) * D;
+    auto code_at = [&](int to) { return reinterpret_cast<uint32_t*>(cache + to * row_bytes); };
+    // The group's scale from the largest magnitude written (over the warp) and the scale so far, and the rows below `first` if it
+    // has grown.  Returns its exponent.
+    auto settle = [&](uint32_t most, int first, float old) {
+      most = max(most & 0xffffu, most >> 16);
 #pragma unroll
-      for (int j = 0; j < HELD; ++j) {
-        const int to = destination(s, next_rows(m));
-        if (to >= 0) store(x[j], to);
-        __syncwarp();
+      for (int d = 16; d > 0; d >>= 1) most = max(most, __shfl_xor_sync(ALL, most, d));
+      const int e = first > 0 ? max(exponent_for(most), exponent_of(old)) : exponent_for(most);
+      const float now = power_of_two(e);
+      if (first > 0 && now != old) {
+        const float ratio = old * power_of_two(-e);
+#pragma unroll 1
+        for (int r0 = sub; r0 < first; r0 += 4 * ROWS) {
+          uint32_t c[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (r0 + k * ROWS < first) c[k] = *code_at(g * kScaleGroup + r0 + k * ROWS);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (r0 + k * ROWS < first) *code_at(g * kScaleGroup + r0 + k * ROWS) = recode4(c[k], ratio);
+        }
       }
-    } else {
+      if (lane == 0) *scale_at = now;
+      return e;
+    };
+
+    // Rows at + b of this group: bits b.
+    const int behind = __shfl_sync(ALL, slot, (at + lane) & 31), sl = at + lane < 32 ? behind : -1;
+    const unsigned same = __ballot_sync(ALL, sl >= 0 && sl / kScaleGroup == g), other = __ballot_sync(ALL, sl >= 0 && sl / kScaleGroup != g);
+    const unsigned run = other ? same & ((other & -other) - 1) : same;
+    const bool ended = other != 0 || r0 + 32 >= p.n;  // a row of another group follows, or none
+    const int first = __reduce_min_sync(ALL, run >> lane & 1u ? sl % kScaleGroup : kScaleGroup);
+    // Rows one after the other to slots one after the other, as sequences have them: all of them in registers.
+    const int count = __popc(run), slot0 = __shfl_sync(ALL, slot, at);
+    if (ended && run == (2u << (count - 1)) - 1 && !__any_sync(ALL, lane < count && sl != slot0 + lane)) {
+      float old = 0.f;
+      if (first > 0) old = *scale_at;
+      uint2 x[HELD];
+      x[0] = make_uint2(0, 0);
+      if (alone && u < warps) x[0] = early;
+      else if (sub < count) x[0] = load(i + sub, head);
+      if (ROWS == 2 && alone && sub == 1 && count > 1) x[0] = load(i + 1, head);
+      if (count > ROWS) {
+#pragma unroll
+        for (int j = 1; j < HELD; ++j) x[j] = j * ROWS + sub < count ? load(i + j * ROWS + sub, head) : make_uint2(0, 0);
+      }
+      uint32_t most = max_magnitude(x[0].x, x[0].y);  // two columns at a time; infinities and NaN stay what they are
+      if (count > ROWS) {
+#pragma unroll
+        for (int j = 1; j < HELD; ++j) most = max_magnitude(max_magnitude(x[j].x, x[j].y), most);
+      }
+      most &= 0x7fff7fffu;
+      if (!__any_sync(ALL, max(most & 0xffffu, most >> 16) >= 0x7f80u)) {
+        const uint32_t inv = static_cast<uint32_t>(127 - settle(most, first, old)) * 0x00800080u;  // 2^-e as bf16, twice: exact
+        unsigned char* to = cache + static_cast<int64_t>(slot0 + sub) * row_bytes;
+        if (sub < count) *reinterpret_cast<uint32_t*>(to) = encode4_finite(x[0], inv);
+        if (count > ROWS) {
+#pragma unroll
+          for (int j = 1; j < HELD; ++j)
+            if (j * ROWS + sub < count) *reinterpret_cast<uint32_t*>(to + j * ROWS * row_bytes) = encode4_finite(x[j], inv);
+        }
+        continue;
+      }
+    }
+    // Gaps, the same slots over and over, or something that is not finite: row by row, 32 slots at a time, as often as it takes.
+    auto windows = [&](auto each) {
       int64_t from = i;
 #pragma unroll 1
       while (true) {
-        int s2;
-        bool end2;
-        unsigned m = window(from, s2, end2);
-#pragma unroll 1
-        while (m) {
-          const int b = next_rows(m);
-          const int to = destination(s2, b);
-          if (to >= 0) store(load(from + b), to);
-          __syncwarp();
-        }
-        if (end2) break;
+        const int w = slot_at(from + lane);
+        const unsigned in = __ballot_sync(ALL, w >= 0 && w / kScaleGroup == g), out = __ballot_sync(ALL, w >= 0 && w / kScaleGroup != g);
+        unsigned m = out ? in & ((out & -out) - 1) : in;
+        each(from, w, m);
+        if (out != 0 || from + 32 >= p.n) break;
         from += 32;
       }
-    }
-    if ((lane & 15) == 0) *scale_at = now;
+    };
+    uint32_t most = 0;
+    int lowest = kScaleGroup;
+    windows([&](int64_t from, int w, unsigned m) {
+      lowest = min(lowest, __reduce_min_sync(ALL, m >> lane & 1u ? w % kScaleGroup : kScaleGroup));
+#pragma unroll 1
+      while (m) {
+        const int b = next_rows(m);
+        const uint2 v = b >= 0 ? load(from + b, head) : make_uint2(0, 0);
+        most = max_finite2(max_finite2(most, v.x), v.y);
+      }
+    });
+    const float inv = power_of_two(-settle(most, lowest, lowest > 0 ? *scale_at : 0.f));
+    windows([&](int64_t from, int w, unsigned m) {
+#pragma unroll 1
+      while (m) {
+        const int b = next_rows(m), to = destination(w, b);
+        if (to >= 0) *code_at(to) = encode4(load(from + b, head), inv);
+        __syncwarp();
+      }
+    });
   }
 }
 
@@ -229,10 +247,10 @@ extern "C" int nvllm_store_kvcache_fp8(const void* key, int64_t key_row_stride, 
   p.n = n_tokens;
   p.num_slots = num_blocks * kBlockSize;
   p.hkv = num_kv_heads;
-  p.rows_per_block = n_tokens <= 4096 ? 1 : kScaleGroup;
+  p.rows_per_block = n_tokens <= 1024 ? 1 : kScaleGroup;
   const int64_t blocks = (n_tokens + p.rows_per_block - 1) / p.rows_per_block;
   if (blocks > 0x7fffffffLL) return fail(NVLLM_E_GEOMETRY, "store_kvcache_fp8: too many tokens for one launch");
-  const int threads = 32 * (num_kv_heads < kStoreFp8Threads / 32 ? num_kv_heads : kStoreFp8Threads / 32);
+  const int threads = 32 * std::min(num_kv_heads, kStoreFp8Threads / 32);
   return launch_kernel("store_kvcache_fp8", head_dim == 128 ? store_fp8_kernel<128> : store_fp8_kernel<64>,
-                       dim3(static_cast<unsigned>(blocks)), dim3(threads), 0, static_cast<cudaStream_t>(stream), p);
+                       dim3(static_cast<unsigned>(blocks), 2), dim3(threads), 0, static_cast<cudaStream_t>(stream), p);
 }
