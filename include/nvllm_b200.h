@@ -321,14 +321,20 @@ NVLLM_API int nvllm_decode_step_fp8(const void* q, int64_t q_row_stride, const v
  * nvllm_prefill_varlen over an 8-bit cache, through the block table: same masks, same rules for rows without a key and for what lies
  * behind a sequence's end.  total_q: rows of q and out.  max_seqlen_q / max_seqlen_k: at least the longest.  Queries are
  * taken as sums of two e4m3 numbers (all of bf16's bits down to 2^-10 of a row's largest value, an error of at most 2^-17 of
- * that below), P is rounded to f16, sums are fp32.  batch <= 1024; scale >= 0.  No workspace.
+ * that below), P is rounded to f16, sums are fp32.  batch <= 1024; scale >= 0.
+ * `workspace`: nvllm_prefill_fp8_workspace_bytes(...) bytes for the same sizes on the current device, 16-byte aligned; it may be
+ * nvllm_decode_paged's (calls that share one must not overlap).  With it, few new tokens behind long prefixes have their keys
+ * split over the GPU; without (NULL) they have not, and the results are as good.
  */
+NVLLM_API int64_t nvllm_prefill_fp8_workspace_bytes(int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_q_heads,
+                             int32_t num_kv_heads, int32_t head_dim);
 NVLLM_API int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                              const float* k_scale, const float* v_scale, const int32_t* block_tables, int64_t bt_row_stride,
                              int32_t max_blocks, void* out, int64_t out_row_stride,
                              const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t total_q, int32_t batch,
                              int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_q_heads, int32_t num_kv_heads,
-                             int32_t head_dim, float scale, int64_t num_blocks, void* stream);
+                             int32_t head_dim, float scale, int64_t num_blocks, void* workspace, int64_t workspace_bytes,
+                             void* stream);
 
 /*
  * What a step's launches are told about where its rows lie, built on the GPU from the requests' lengths (the device side of

@@ -66,7 +66,8 @@ SIGNATURES = {
                                         c_int32, c_int32, c_int32, c_float, c_int64, c_void_p, c_int64, c_void_p]),
     "nvllm_prefill_varlen_fp8": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
                                            c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int32, c_int32, c_int32,
-                                           c_int32, c_int32, c_float, c_int64, c_void_p]),
+                                           c_int32, c_int32, c_float, c_int64, c_void_p, c_int64, c_void_p]),
+    "nvllm_prefill_fp8_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "nvllm_step_maps": (c_int32, [c_void_p, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
                                   c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
     "nvllm_ar_handle_bytes": (c_int64, []),

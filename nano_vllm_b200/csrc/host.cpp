@@ -58,6 +58,7 @@ struct Api {
   decltype(&nvllm_decode_paged_fp8) decode_paged_fp8;
   decltype(&nvllm_decode_step_fp8) decode_step_fp8;
   decltype(&nvllm_prefill_varlen_fp8) prefill_varlen_fp8;
+  decltype(&nvllm_prefill_fp8_workspace_bytes) prefill_fp8_workspace_bytes;
   decltype(&nvllm_step_maps) step_maps;
 } api;
 PyObject* g_check = nullptr;  // _lib.check: raises NvllmError for a negative code
@@ -559,12 +560,18 @@ void prefill_fp8(const Rows& q, int64_t hq, const Fp8Planes& c, const at::Tensor
   require(table.dim() == 2 && table.size(0) == batch, "block_tables.dim() == 2 and block_tables.shape[0] == batch");
   constexpr int64_t most = std::numeric_limits<int32_t>::max();
   require(batch <= most && max_q <= most && max_k <= most, "sizes must fit 32 bits");
+  const int64_t need = api.prefill_fp8_workspace_bytes(static_cast<int32_t>(batch), static_cast<int32_t>(max_q), static_cast<int32_t>(max_k),
+                                                       static_cast<int32_t>(hq), static_cast<int32_t>(c.hkv), static_cast<int32_t>(c.d));
+  check(need);
+  void* ws;
+  int64_t ws_size;
+  workspace(like, need, &ws, &ws_size);
   launch([&] {
     return api.prefill_varlen_fp8(q.p, q.stride, c.k, c.v, c.k_scale, c.v_scale, ptr<int32_t>(table), table.stride(0),
                                   static_cast<int32_t>(table.size(1)), out.p, out.stride, ptr<int32_t>(cu_q), ptr<int32_t>(cu_k), q.n,
                                   static_cast<int32_t>(batch), static_cast<int32_t>(max_q), static_cast<int32_t>(max_k),
                                   static_cast<int32_t>(hq), static_cast<int32_t>(c.hkv), static_cast<int32_t>(c.d),
-                                  static_cast<float>(scale), c.blocks, stream_of(like));
+                                  static_cast<float>(scale), c.blocks, ws, ws_size, stream_of(like));
   });
 }
 
@@ -999,6 +1006,7 @@ PyObject* bind(PyObject* const* a) {  // library path, check
   RESOLVE(decode_paged_fp8);
   RESOLVE(decode_step_fp8);
   RESOLVE(prefill_varlen_fp8);
+  RESOLVE(prefill_fp8_workspace_bytes);
   RESOLVE(step_maps);
 #undef RESOLVE
   Py_INCREF(a[1]);

@@ -17,9 +17,11 @@
 //
 // Twelve warps, two blocks to an SM for the whole launch: 0-3 softmax (thread = query row), 4-7 query rows in, V conversion and
 // results out, 8 = TMA of the query rows, K and the scales, 9 = MMA issuer, 10 = TMA of V.  The three warp groups trade registers at
-// start-up; 11 works out the items, one ahead.  Items (query tile of a sequence, head group) are ordered by their key tiles, most first, over all sequences, and
+// start-up; 11 works out the items, one ahead.  Items (query tile of a sequence, head group) are ordered by their key tiles,
+// most first, over all sequences, and
 // dealt out in turn, there and back again, so that all blocks have about the same to do; no counter in memory, so nothing is
-// shared by launches.
+// shared by launches.  Where there are two blocks or more to an item (few new tokens behind a long prefix) an item's keys go to
+// several of them (SPLIT), and prefill_fp8_join sums the parts up from the workspace.
 #include <algorithm>
 
 #include "fp8.cuh"
@@ -84,6 +86,11 @@ struct PrefillFp8Params {
   float scale_log2e;
   int64_t num_blocks;
   int* status;
+  // few items: their keys in parts, a block to each (item * parts + part)
+  int parts, items;
+  int4* ws_items;  // [items]: first token, head, rows (0: nothing to sum up), parts
+  float2* ws_ml;   // [blocks][128]: running maximum in log2 units, sum
+  float4* ws_o;    // [blocks][D / 4][128]
 };
 
 // Shared-memory descriptor of e4m3 rows as TMA leaves them: 128-byte rows under the 128-byte swizzle, or 64 under the 64-byte one.
@@ -109,7 +116,9 @@ __device__ __forceinline__ void umma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 // e4m3 x e4m3 -> fp32, both K-major; f16 x f16 -> fp32, B MN-major.
-__host__ __device__ constexpr uint32_t idesc_f8(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
+__host__ __device__ constexpr uint32_t idesc_f8(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
 __host__ __device__ constexpr uint32_t idesc_f16(int m, int n) { return idesc_f8(m, n) | (1u << 16); }
 
 // A tile's scales: K's; V's over the unit, as f16 pairs; what O is multiplied by (where the unit changes); the unit.
@@ -125,7 +134,8 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 }
 
 struct Fp8Item {
-  int b, h, m0, q0, Lq, Lk, n_kv;  // n_kv < 0: no more work
+  int b, h, m0, q0, Lq, Lk, n_kv;  // n_kv key tiles, < 0: no more work
+  int first;                       // of a part of an item's keys: its first tile
 };
 
 // Key tiles that the first `tokens` query tokens of a sequence see.
@@ -142,7 +152,7 @@ __device__ __forceinline__ int fp8_tiles_above(int x, int Lq, int Lk, int bmt) {
   return least < 0 ? tiles : tiles - min(tiles - 1, least / bmt);
 }
 
-template <int D>
+template <int D, bool SPLIT>
 __global__ void __launch_bounds__(f8::NTHREADS, 2)
 prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                    const __grid_constant__ CUtensorMap tmap_v) {
@@ -157,6 +167,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
   volatile int* slots = reinterpret_cast<volatile int*>(base_ptr + G::OFF_SLOTS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + G::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + G::OFF_MISC + 8);
+  volatile int* parts_of_item = reinterpret_cast<volatile int*>(base_ptr + G::OFF_MISC + 16);  // SPLIT: whose part this block has
   float* row_factor = reinterpret_cast<float*>(base_ptr + G::OFF_ROW);
   float* inv_buf = reinterpret_cast<float*>(base_ptr + G::OFF_INV);
   const int pack = p.pack, BMT = p.tile_tokens;
@@ -186,11 +197,13 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
   const uint32_t tmem = *tmem_slot, tmem_o = tmem + TMEM_O;
   auto tmem_s = [&](int st) { return tmem + st * 64; };
 
+  auto tile_of = [&](int t) { return reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile)); };
   auto read_item = [&](int it) {
     volatile int* s = slots + (it & 1) * 8;
     Fp8Item x;
     x.b = s[0]; x.h = s[1]; x.m0 = s[2]; x.q0 = s[3];
     x.Lq = s[4]; x.Lk = s[5]; x.n_kv = s[6];
+    x.first = SPLIT ? s[7] : 0;
     return x;
   };
   auto block_of = [&](const Fp8Item& x, int j) -> int64_t {  // of key tile j
@@ -216,17 +229,17 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         const Fp8Item x = read_item(it);
         if (x.n_kv < 0) break;
         const int kvh = x.h / p.g;
-        int64_t blk = block_of(x, 0);
+        int64_t blk = block_of(x, x.first);
         auto scale_at = [&](int j) { return (blk * p.hkv + kvh) * kGroups + j * BN % kBlockSize / kScaleGroup + g; };
-        float k = p.k_scale[scale_at(0)], v = p.v_scale[scale_at(0)];  // of tile j, group g
+        float k = p.k_scale[scale_at(x.first)], v = p.v_scale[scale_at(x.first)];  // of tile j, group g
 #pragma unroll 1
         for (int j = 0; j < x.n_kv; ++j) {
-          const int t = T + j, st = t & 1, use = t >> 1;
-          const int row = static_cast<int>(blk * kBlockSize + j * BN % kBlockSize);
+          const int t = T + j, st = t & 1, use = t >> 1, tile_no = x.first + j;
+          const int row = static_cast<int>(blk * kBlockSize + tile_no * BN % kBlockSize);
           float k_next = 0.f, v_next = 0.f;
           if (j + 1 < x.n_kv) {
-            if ((j + 1) % (kBlockSize / BN) == 0) blk = block_of(x, j + 1);
-            k_next = p.k_scale[scale_at(j + 1)], v_next = p.v_scale[scale_at(j + 1)];
+            if ((tile_no + 1) % (kBlockSize / BN) == 0) blk = block_of(x, tile_no + 1);
+            k_next = p.k_scale[scale_at(tile_no + 1)], v_next = p.v_scale[scale_at(tile_no + 1)];
           }
           ok = __all_sync(ALL, use == 0 || wait_or_abort(bar(QK_DONE0 + st), (use - 1) & 1, abort_flag));
           if (!ok) break;
@@ -236,7 +249,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
             tma_load_3d(base + G::OFF_K + st * G::K_BYTES, &tmap_k, bar(K_FULL0 + st), 0, kvh, row);
           }
           ++loaded;
-          if (j * BN + g * kScaleGroup >= x.Lk) k = 1.f, v = 0.f;  // a group behind the end may hold anything
+          if (tile_no * BN + g * kScaleGroup >= x.Lk) k = 1.f, v = 0.f;  // a group behind the end may hold anything
           float most = fmaxf(v, __shfl_xor_sync(ALL, v, 1));
           most = fmaxf(most, __shfl_xor_sync(ALL, most, 2));
           const float before = unit;
@@ -293,11 +306,12 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           int64_t blk = 0;
 #pragma unroll 1
           for (int j = 0; j < x.n_kv; ++j) {
-            const int t = T + j, st = t & 1, use = t >> 1;
-            if (j % (kBlockSize / BN) == 0) blk = block_of(x, j);
+            const int t = T + j, st = t & 1, use = t >> 1, tile_no = x.first + j;
+            if (j == 0 || tile_no % (kBlockSize / BN) == 0) blk = block_of(x, tile_no);
             if (use > 0 && !(ok = wait_or_abort(bar(RAW_FREE0 + st), (use - 1) & 1, abort_flag))) break;
             mbar_expect_tx(bar(RAW_FULL0 + st), G::K_BYTES);
-            tma_load_3d(base + G::OFF_RAW + st * G::K_BYTES, &tmap_v, bar(RAW_FULL0 + st), 0, kvh, static_cast<int>(blk * kBlockSize + j * BN % kBlockSize));
+            tma_load_3d(base + G::OFF_RAW + st * G::K_BYTES, &tmap_v, bar(RAW_FULL0 + st), 0, kvh,
+                        static_cast<int>(blk * kBlockSize + tile_no * BN % kBlockSize));
             ++loaded;
           }
           if (!ok) break;
@@ -384,7 +398,8 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       bool ok = true;
 #pragma unroll 1
       for (int it = 0;; ++it) {
-        const unsigned drawn = it * gridDim.x + (it & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+        const unsigned drawn = SPLIT ? (it == 0 ? blockIdx.x / p.parts : total)
+                                     : it * gridDim.x + (it & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
         Fp8Item x{};
         x.n_kv = -1;
         if (drawn < total) {
@@ -427,12 +442,24 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           x.q0 = p.cu_q[x.b];
           x.m0 = ((x.Lq + BMT - 1) / BMT - 1 - fp8_tiles_above(lo, x.Lq, x.Lk, BMT) - static_cast<int>(k)) * BMT;
         }
+        if (SPLIT && x.n_kv > 0) {
+          const int parts = max(1, min(p.parts, x.n_kv / 2)), part = blockIdx.x % p.parts;
+          x.first = static_cast<int>(static_cast<int64_t>(x.n_kv) * part / parts);
+          x.n_kv = part < parts ? static_cast<int>(static_cast<int64_t>(x.n_kv) * (part + 1) / parts) - x.first : -1;
+          if (lane == 0) {
+            *parts_of_item = parts;
+            if (part == 0) p.ws_items[drawn] = make_int4(x.q0 + x.m0, x.h, parts > 1 ? min(BMT, x.Lq - x.m0) * pack : 0, parts);
+          }
+        } else if (SPLIT && lane == 0 && it == 0 && blockIdx.x % p.parts == 0) {
+          p.ws_items[drawn] = make_int4(0, 0, 0, 0);  // no such item
+        }
         if (it >= 2) ok = wait_or_abort(bar(ITEM_FREE0 + (it & 1)), ((it >> 1) - 1) & 1, abort_flag);
         if (!__all_sync(ALL, ok)) break;
         if (lane == 0) {
           volatile int* s = slots + (it & 1) * 8;
           s[0] = x.b; s[1] = x.h; s[2] = x.m0; s[3] = x.q0;
           s[4] = x.Lq; s[5] = x.Lk; s[6] = x.n_kv;
+          if (SPLIT) s[7] = x.first;
           mbar_arrive(bar(ITEM_FULL0 + (it & 1)));
           if (x.n_kv > 0) {  // its query rows are on the path from the item before: to L2
             tma_prefetch_3d(&tmap_q, 0, x.h, x.q0 + x.m0);
@@ -481,13 +508,13 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         tmem_ld32(scores, *reinterpret_cast<uint32_t(*)[32]>(&s[0]));
         tmem_ld32(scores + 32, *reinterpret_cast<uint32_t(*)[32]>(&s[32]));
         if (!(ok = wait_or_abort(bar(INFO0 + (t & 3)), (t >> 2) & 1, abort_flag))) break;
-        const Fp8Tile& tile = *reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile));
+        const Fp8Tile& tile = *tile_of(t);
         float ks[4];
         *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(tile.k);
         const float change = tile.change;
 #pragma unroll
         for (int g = 0; g < 4; ++g) ks[g] = fmaxf(ks[g] * factor, 0x1p-126f);  // not zero, which -inf of a masked score must not meet
-        const int j0 = j * BN;
+        const int j0 = (x.first + j) * BN;
         tmem_wait_ld();
         if ((j0 + BN - 1 > x.m0 + off) || (j0 + BN > x.Lk)) {  // tile touches the diagonal or the end
           const int limit = min(qi + off, x.Lk - 1) - j0;        // columns c <= limit are visible
@@ -562,6 +589,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       if (!ok) break;
       T += x.n_kv;
       // the row's normaliser goes to the row warps; no key: zeros; a sum that is NaN stays one
+      if (SPLIT && *parts_of_item > 1) p.ws_ml[static_cast<int64_t>(blockIdx.x) * BM + r] = make_float2(m_used, l);
       inv_buf[(it & 1) * 128 + r] = l > 0.f ? 1.f / l : l;
       __syncwarp();
       if (lane == 0) {
@@ -641,10 +669,10 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
     const unsigned char* v_from = base_ptr + G::OFF_RAW + code_piece<D>(v_row, v_piece);
     unsigned char* v_to = base_ptr + G::OFF_V + (v_piece >> 2) * G::V_SUB + v_row * 128 + (((v_piece & 3) * 2 ^ (v_row & 7)) << 4);
     auto convert = [&](const Fp8Item& x, int j, int t) {
-      const int st = t & 1, use = t >> 1, rows = x.Lk - j * BN;
+      const int st = t & 1, use = t >> 1, rows = x.Lk - (x.first + j) * BN;
       if (!wait_or_abort(bar(INFO0 + (t & 3)), (t >> 2) & 1, abort_flag)) return false;
       uint32_t by[4];
-      *reinterpret_cast<uint4*>(by) = *reinterpret_cast<const uint4*>(reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile))->v);
+      *reinterpret_cast<uint4*>(by) = *reinterpret_cast<const uint4*>(tile_of(t)->v);
       if (!wait_or_abort(bar(RAW_FULL0 + st), use & 1, abort_flag)) return false;
       if (use > 0 && !wait_or_abort(bar(PV_DONE0 + st), (use - 1) & 1, abort_flag)) return false;
       uint4 code[STEPS];
@@ -674,12 +702,31 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       }
       return true;
     };
+    // A part of an item's keys: O in 32 bits goes to the workspace, four columns of all rows side by side.
+    auto set_aside = [&](const Fp8Item& x, float unit) {
+      const int rows = min(BMT, x.Lq - x.m0) * pack;
+      float4* mine = p.ws_o + static_cast<int64_t>(blockIdx.x) * (D / 4) * BM + r;
+#pragma unroll 1
+      for (int c = 0; c < G::OCH; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + lane_addr + c * 32, o);
+        tmem_wait_ld();
+        if (r < rows) {
+#pragma unroll
+          for (int k = 0; k < 32; k += 4)
+            mine[(c * 8 + k / 4) * BM] = make_float4(__uint_as_float(o[k]) * unit, __uint_as_float(o[k + 1]) * unit,
+                                                     __uint_as_float(o[k + 2]) * unit, __uint_as_float(o[k + 3]) * unit);
+        }
+      }
+      return true;
+    };
     // Results of item number `done`, whose last tile was `last`.
     auto results = [&](const Fp8Item& x, int done, int last) {
       if (!wait_or_abort(bar(EPI_FULL0 + (done & 1)), (done >> 1) & 1, abort_flag)) return false;
-      const float inv = inv_buf[(done & 1) * 128 + r] * reinterpret_cast<const Fp8Tile*>(base_ptr + G::OFF_TILES + (last & 3) * sizeof(Fp8Tile))->unit;
+      const float inv = inv_buf[(done & 1) * 128 + r] * tile_of(last)->unit;
       if (!wait_or_abort(bar(PV_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag)) return false;
       tc_fence_after();
+      if (SPLIT && *parts_of_item > 1) return set_aside(x, tile_of(last)->unit);
       // O / l -> bf16, 32 columns at a time through this warp's patch of shared memory
       const int srow = lane >> 2, spiece = lane & 3;
       __nv_bfloat16* out_tile = p.out + static_cast<int64_t>(x.q0 + x.m0) * p.out_stride + x.h * D;
@@ -746,6 +793,54 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
   }
 }
 
+// What an item's parts add up to: a thread has a row's four columns of all parts, `1 << log_rows` rows side by side.  It loads
+// eight parts at a time, before it is known how many there are (the workspace holds as many for every item): one latency.
+// (The block that reports an item's last part as the one that sums them up has only its own loads to hide the latency
+// with: 20 us for 50 rows in 5 parts.)
+template <int D>
+__global__ void __launch_bounds__(256) prefill_fp8_join_kernel(const PrefillFp8Params p, int log_rows) {
+  using namespace f8;
+  const int t = blockIdx.x * 256 + threadIdx.x, row = t & ((1 << log_rows) - 1), c = (t >> log_rows) & (D / 4 - 1);
+  const int item = (t >> log_rows) / (D / 4);
+  pdl_prologue();
+  if (item >= p.items) return;
+  const int4 what = p.ws_items[item];
+  const float2* ml = p.ws_ml + static_cast<int64_t>(item) * p.parts * BM + row;
+  const float4* from = p.ws_o + (static_cast<int64_t>(item) * p.parts * (D / 4) + c) * BM + row;
+  float top = -INFINITY, sum = 0.f;
+  float4 acc{};
+#pragma unroll 1
+  for (int i0 = 0; i0 < p.parts; i0 += 8) {
+    float2 s[8];
+    float4 o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i0 + i < p.parts) s[i] = ml[(i0 + i) * BM], o[i] = from[static_cast<int64_t>(i0 + i) * (D / 4) * BM];
+    float high = top;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (i0 + i >= what.w) s[i] = make_float2(-INFINITY, 0.f);
+      high = fmaxf(high, s[i].x);
+    }
+    const float old = top == -INFINITY ? 0.f : fast_exp2(top - high);
+    sum *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+    top = high;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (s[i].x != -INFINITY) {
+        const float w = fast_exp2(s[i].x - top);
+        sum = fmaf(s[i].y, w, sum);
+        acc.x = fmaf(o[i].x, w, acc.x), acc.y = fmaf(o[i].y, w, acc.y);
+        acc.z = fmaf(o[i].z, w, acc.z), acc.w = fmaf(o[i].w, w, acc.w);
+      }
+  }
+  if (row >= what.z) return;
+  const float by = sum > 0.f ? 1.f / sum : sum;  // no key: zeros; a sum that is NaN stays one
+  const int tok = row * p.inv_pack >> 16, hh = row - tok * p.pack;
+  *reinterpret_cast<uint2*>(p.out + static_cast<int64_t>(what.x + tok) * p.out_stride + (what.y + hh) * D + c * 4) =
+      make_uint2(pack_bf16x2(acc.x * by, acc.y * by), pack_bf16x2(acc.z * by, acc.w * by));
+}
+
 // ---- host side ---------------------------------------------------------------------------
 
 // Heads packed into a query tile: the largest divisor of the group size that is at most 8.
@@ -756,25 +851,56 @@ static int heads_in_tile(int g) {
   return pack;
 }
 
+template <int D, bool SPLIT>
+static int prepare_prefill_fp8() {
+  cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<D, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, f8::Geo<D>::SMEM);
+  // The warp groups trade registers inside the pool the block gets at launch: a build with fewer could never satisfy the
+  // softmax group's request, and that request waits without a bound.
+  cudaFuncAttributes attr;
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, prefill_fp8_kernel<D, SPLIT>);
+  if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "prefill_fp8: set-up failed: %s", cudaGetErrorString(e));
+  if (attr.numRegs < f8::REGS_LAUNCH)
+    return fail(NVLLM_E_CUDA, "prefill_fp8: built with %d registers per thread, the warp groups' hand-over needs %d", attr.numRegs,
+                f8::REGS_LAUNCH);
+  return NVLLM_OK;
+}
+
+// Items of a launch at most, as far as the host knows.
+static int64_t prefill_fp8_items(int hq, int g, int max_seqlen_q, int batch) {
+  const int pack = heads_in_tile(g), tokens = f8::BM / pack;
+  return static_cast<int64_t>((max_seqlen_q + tokens - 1) / tokens) * (hq / pack) * batch;
+}
+// The parts that an item's keys go into; 1: whole items.  A tile takes a block 0.9 us, which is latency, a part more 0.1 us of
+// summing up, and a split at all 2 to 4 us (one sequence, 16 heads over 8 of dim 128, 600 cached tokens and 25 new ones: whole
+// 15.6, 5 parts 12.7, 24 parts 16.6 us; 16000 and 16: whole 191, 12 parts 35.5, 32 parts 26.8; 5000 and 1: 65.7, 12 parts 19.3,
+// 32 parts 23.3; 700 new ones alone: whole 18.4, 3 parts 21.8; 400 and 300: whole 18.5, 2 parts 17.9).  So none where an item has
+// fewer than 9 tiles, and about 2 sqrt(tiles) parts, two tiles to each at least, as many as there are blocks for.
+static int prefill_fp8_parts(int64_t items, int max_seqlen_q, int max_seqlen_k, int blocks) {
+  const int64_t tiles = (max_seqlen_k - max_seqlen_q / 2 + int64_t{f8::BN - 1}) / f8::BN;  // of an item in the middle of its queries
+  if (tiles < 9) return 1;
+  const int64_t most = std::min<int64_t>(tiles / 2, 32);
+  int parts = 1;
+  while (parts < most && (parts + 1) * items <= blocks && parts * parts < 4 * tiles) ++parts;
+  return parts;
+}
+static int prefill_fp8_blocks() {
+  const int sms = num_sms();
+  return sms > 0 ? 2 * sms : 512;  // no device: as if there were more than any has
+}
+constexpr int64_t kFp8CounterArea = 16384 * 4;  // at the workspace's head, left as it is: the decode's, whose workspace this may be
+
 template <int D>
 static int launch_prefill_fp8(PrefillFp8Params& p, const void* k_cache, const void* v_cache, int64_t total_q, int max_seqlen_q,
-                              cudaStream_t stream) {
+                              int max_seqlen_k, void* workspace, cudaStream_t stream) {
   using G = f8::Geo<D>;
   static bool ready[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return fail(NVLLM_E_NO_DEVICE, "prefill_fp8: device index %d out of range", dev);
-  if (!ready[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(prefill_fp8_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, G::SMEM);
-    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "prefill_fp8: set-up failed: %s", cudaGetErrorString(e));
-    // The warp groups trade registers inside the pool the block gets at launch: a build with fewer could never satisfy the
-    // softmax group's request, and that request waits without a bound.
-    cudaFuncAttributes attr;
-    e = cudaFuncGetAttributes(&attr, prefill_fp8_kernel<D>);
-    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "prefill_fp8: set-up failed: %s", cudaGetErrorString(e));
-    if (attr.numRegs < f8::REGS_LAUNCH)
-      return fail(NVLLM_E_CUDA, "prefill_fp8: built with %d registers per thread, the warp groups' hand-over needs %d", attr.numRegs,
-                  f8::REGS_LAUNCH);
+  if (!ready[dev]) {  // both: another's first launch may be captured
+    int rc = prepare_prefill_fp8<D, false>();
+    if (rc == NVLLM_OK) rc = prepare_prefill_fp8<D, true>();
+    if (rc) return rc;
     ready[dev] = true;
   }
   p.pack = heads_in_tile(p.g);
@@ -784,19 +910,48 @@ static int launch_prefill_fp8(PrefillFp8Params& p, const void* k_cache, const vo
   if (!make_tmap_3d(&mq, p.q, D, p.hq, total_q, D, p.q_stride, p.tile_tokens, p.pack)) return NVLLM_E_CUDA;
   const uint64_t slots = static_cast<uint64_t>(p.num_blocks) * kBlockSize;
   if (!make_tmap_codes(&mk, k_cache, D, p.hkv, slots, f8::BN) || !make_tmap_codes(&mv, v_cache, D, p.hkv, slots, f8::BN)) return NVLLM_E_CUDA;
-  const int64_t items = static_cast<int64_t>((max_seqlen_q + p.tile_tokens - 1) / p.tile_tokens) * (p.hq / p.pack) * p.batch;  // at most
-  const int grid = static_cast<int>(std::min<int64_t>(2ll * num_sms(), items));
-  return launch_kernel("prefill_fp8", prefill_fp8_kernel<D>, dim3(grid), dim3(f8::NTHREADS), G::SMEM, stream, p, mq, mk, mv);
+  const int64_t items = prefill_fp8_items(p.hq, p.g, max_seqlen_q, p.batch);
+  p.parts = workspace ? prefill_fp8_parts(items, max_seqlen_q, max_seqlen_k, prefill_fp8_blocks()) : 1;
+  if (p.parts == 1) {
+    const int grid = static_cast<int>(std::min<int64_t>(prefill_fp8_blocks(), items));
+    return launch_kernel("prefill_fp8", prefill_fp8_kernel<D, false>, dim3(grid), dim3(f8::NTHREADS), G::SMEM, stream, p, mq, mk, mv);
+  }
+  const int grid = static_cast<int>(items) * p.parts;
+  p.items = static_cast<int>(items);
+  p.ws_items = reinterpret_cast<int4*>(static_cast<unsigned char*>(workspace) + kFp8CounterArea);
+  p.ws_ml = reinterpret_cast<float2*>(p.ws_items + items);
+  p.ws_o = reinterpret_cast<float4*>(p.ws_ml + static_cast<int64_t>(grid) * f8::BM);
+  const int rc = launch_kernel("prefill_fp8", prefill_fp8_kernel<D, true>, dim3(grid), dim3(f8::NTHREADS), G::SMEM, stream, p, mq, mk, mv);
+  if (rc) return rc;
+  int log_rows = 0;  // of a tile, as far as they are there
+  while ((1 << log_rows) < std::min(p.tile_tokens, max_seqlen_q) * p.pack) ++log_rows;
+  const int64_t threads = (items * (D / 4)) << log_rows;
+  return launch_kernel("prefill_fp8_join", prefill_fp8_join_kernel<D>, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream,
+                       p, log_rows);
 }
 
 }  // namespace nvllm
+
+extern "C" int64_t nvllm_prefill_fp8_workspace_bytes(int32_t batch, int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_q_heads,
+                                                     int32_t num_kv_heads, int32_t head_dim) {
+  using namespace nvllm;
+  if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads ||
+      num_q_heads > 65535 || (head_dim != 64 && head_dim != 128))
+    return fail(NVLLM_E_GEOMETRY, "prefill_fp8_workspace_bytes: batch=%d max_seqlen=%d / %d Hq=%d Hkv=%d head_dim=%d invalid", batch,
+                max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim);
+  if (batch == 0 || max_seqlen_q == 0) return 0;
+  const int64_t items = prefill_fp8_items(num_q_heads, num_q_heads / num_kv_heads, max_seqlen_q, batch);
+  const int parts = prefill_fp8_parts(items, max_seqlen_q, max_seqlen_k, prefill_fp8_blocks());
+  return parts == 1 ? 0 : kFp8CounterArea + items * 16 + items * parts * f8::BM * (head_dim + 2) * 4;
+}
 
 extern "C" int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                                         const float* k_scale, const float* v_scale, const int32_t* block_tables,
                                         int64_t bt_row_stride, int32_t max_blocks, void* out, int64_t out_row_stride,
                                         const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int64_t total_q, int32_t batch,
                                         int32_t max_seqlen_q, int32_t max_seqlen_k, int32_t num_q_heads, int32_t num_kv_heads,
-                                        int32_t head_dim, float scale, int64_t num_blocks, void* stream) {
+                                        int32_t head_dim, float scale, int64_t num_blocks, void* workspace, int64_t workspace_bytes,
+                                        void* stream) {
   using namespace nvllm;
   const char* who = "prefill_varlen_fp8";
   if (batch < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 || total_q < 0)
@@ -816,7 +971,13 @@ extern "C" int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, con
     return fail(NVLLM_E_GEOMETRY, "%s: max_blocks=%d too large", who, max_blocks);
   if (q_row_stride % 8 || out_row_stride % 8 || !aligned16(q) || !aligned16(out))
     return fail(NVLLM_E_ALIGN, "%s: q/out pointers and row strides must be 16-byte aligned", who);
-  PrefillFp8Params p;
+  if (workspace) {
+    const int64_t need = nvllm_prefill_fp8_workspace_bytes(batch, max_seqlen_q, max_seqlen_k, num_q_heads, num_kv_heads, head_dim);
+    if (workspace_bytes < need)
+      return fail(NVLLM_E_WORKSPACE, "%s: workspace of %lld bytes needed, %lld given", who, (long long)need, (long long)workspace_bytes);
+    if (!aligned16(workspace)) return fail(NVLLM_E_ALIGN, "%s: workspace must be 16-byte aligned", who);
+  }
+  PrefillFp8Params p{};
   p.status = status_word();
   if (!p.status) return fail(NVLLM_E_NO_DEVICE, "%s: no CUDA device is usable", who);
   p.q = static_cast<const __nv_bfloat16*>(q);
@@ -837,6 +998,6 @@ extern "C" int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, con
   p.scale_log2e = scale * 1.4426950408889634f;
   p.num_blocks = num_blocks;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) return launch_prefill_fp8<128>(p, k_cache, v_cache, total_q, max_seqlen_q, st);
-  return launch_prefill_fp8<64>(p, k_cache, v_cache, total_q, max_seqlen_q, st);
+  if (head_dim == 128) return launch_prefill_fp8<128>(p, k_cache, v_cache, total_q, max_seqlen_q, max_seqlen_k, workspace, st);
+  return launch_prefill_fp8<64>(p, k_cache, v_cache, total_q, max_seqlen_q, max_seqlen_k, workspace, st);
 }

@@ -67,10 +67,10 @@ def test_step_refuses(lib, change, code):
     ({"q": NULL}, -1), ({"vc": NULL}, -1), ({"ks": NULL}, -1), ({"bt": NULL}, -1), ({"cu_k": NULL}, -1), ({"out": NULL}, -1), ({"q": P8}, -2),
     ({"ks": P8}, -2), ({"q_stride": 2052}, -2), ({"out_stride": 8}, -3), ({"bt_stride": 1}, -3), ({"width": 0}, -3), ({"batch": 1025}, -3),
     ({"batch": -1}, -3), ({"hq": 15}, -3), ({"d": 32}, -3), ({"blocks": 0}, -3), ({"scale": ctypes.c_float(-1)}, -3),
-    ({"scale": ctypes.c_float(float("nan"))}, -3), ({"batch": 0}, 0), ({"total": 0}, 0), ({"max_q": 0}, 0)])
+    ({"scale": ctypes.c_float(float("nan"))}, -3), ({"ws": P8}, -2), ({"ws_bytes": 1000}, -4), ({"batch": 0}, 0), ({"total": 0}, 0), ({"max_q": 0}, 0)])
 def test_prefill_refuses(lib, change, code):
     a = dict(q=P16, q_stride=2048, kc=P16, vc=P16, ks=P16, vs=P16, bt=P16, bt_stride=4, width=4, out=P16, out_stride=2048, cu_q=P16, cu_k=P16,
-             total=100, batch=2, max_q=60, max_k=600, hq=16, hkv=8, d=128, scale=F, blocks=10)
+             total=100, batch=2, max_q=60, max_k=600, hq=16, hkv=8, d=128, scale=F, blocks=10, ws=P16, ws_bytes=1 << 30)
     a.update(change)
     assert lib.nvllm_prefill_varlen_fp8(*a.values(), None) == code
 

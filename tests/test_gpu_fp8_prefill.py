@@ -167,6 +167,66 @@ def test_captured_and_replayed_with_other_lengths(cuda):
     assert _lib.read_status() == 0
 
 
+FEW = {
+    "one token": [(5000, 1)], "a block in part": [(2817, 3)], "two lengths": [(3, 2), (4000, 30)], "one more than blocks": [(2047, 2)],
+    "tiles of all": [(1000, 130)], "shorter than parts": [(7000, 4), (0, 1), (0, 0), (100, 3)], "no key in some": [(-40, 60), (3000, 9)],
+}
+
+
+@pytest.mark.parametrize("lens", FEW.values(), ids=FEW)
+@pytest.mark.parametrize("hq,hkv,d", HEADS)
+def test_few_tokens_behind_long_prefixes(cuda, hq, hkv, d, lens):
+    """An item's keys in parts, and the same without a workspace; a workspace that is as it was (counters at zero) behind each."""
+    g = torch.Generator().manual_seed(hq + 31 * len(lens))
+    q, planes, cu_q, cu_k, tables = case(g, lens, hq, hkv, d)
+    ref, bound = prefill_reference(q, planes, cu_q, cu_k, tables, d ** -0.5)
+    dev, qd = planes_on(cuda, *planes), q.to(cuda)
+    cq, ck, bt = cu_q.to(cuda), cu_k.to(cuda), tables.to(cuda)
+    lib, lq, lk = _lib.load(), int(cu_q.diff().max()), int(cu_k.diff().max())
+    need = lib.nvllm_prefill_fp8_workspace_bytes(len(lens), lq, lk, hq, hkv, d)
+    ws = torch.zeros(max(need, 1), dtype=torch.uint8, device=cuda)
+    for w, size in ((ws.data_ptr(), need), (ws.data_ptr(), need), (0, 0)):
+        out = torch.full_like(qd, 9.0)
+        k, v, ks, vs = (t.data_ptr() for t in dev)
+        rc = lib.nvllm_prefill_varlen_fp8(qd.data_ptr(), hq * d, k, v, ks, vs, bt.data_ptr(), bt.stride(0), bt.shape[1], out.data_ptr(),
+                                          hq * d, cq.data_ptr(), ck.data_ptr(), q.shape[0], len(lens), lq, lk, hq, hkv, d,
+                                          d ** -0.5, dev[0].shape[0], w, size, torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        assert_within(out, ref, bound, f"workspace of {size}")
+    assert (ws[:65536] == 0).all()
+    assert _lib.read_status() == 0
+
+
+def test_split_in_graphs_that_share_the_scratch(cuda):
+    """Graphs of a prefill behind a long prefix, of a decode over the same cache and of both, replayed in turn."""
+    g = torch.Generator().manual_seed(12)
+    hq, hkv, d = 8, 2, 128
+    q, planes, cu_q, cu_k, tables = case(g, [(3000, 20)], hq, hkv, d)
+    dev, qd, ctx = planes_on(cuda, *planes), q.to(cuda), torch.tensor([3020], dtype=torch.int32, device=cuda)
+    cq, ck, bt = cu_q.to(cuda), cu_k.to(cuda), tables.to(cuda)
+    pre = lambda: A.prefill_varlen_fp8(qd, *dev, cq, ck, 20, 3020, 0.1, bt)  # noqa: E731
+    dec = lambda: A.decode_paged_fp8(qd[19:], *dev, ctx, bt, 0.1)  # noqa: E731
+    want = [pre().clone(), dec().clone()]
+    ref, bound = prefill_reference(q, planes, cu_q, cu_k, tables, 0.1)
+    assert_within(want[0], ref, bound)
+    torch.cuda.synchronize()
+    graphs = []
+    for calls in ((pre,), (dec,), (pre, dec, dec, pre, pre)):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [c() for c in calls]
+        graphs.append((graph, calls, outs))
+    for n in (0, 1, 2, 1, 0, 2):
+        graph, calls, outs = graphs[n]
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        pre()
+        for c, o in zip(calls, outs):
+            assert torch.equal(o, want[0 if c is pre else 1])
+    assert _lib.read_status() == 0
+
+
 def test_refusals(cuda):
     bf = dict(dtype=torch.bfloat16, device=cuda)
     q, c = torch.zeros(4, 4, 64, **bf), torch.zeros(3, 256, 2, 64, device=cuda).to(torch.float8_e4m3fn)
