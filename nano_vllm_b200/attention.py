@@ -18,6 +18,7 @@ from . import _lib
 from . import context as _own_context
 
 BLOCK_SIZE = 256
+SCALE_GROUP = 16  # slots of a block that share a scale, in a cache held in 8 bits
 
 _get_context: Callable[[], object] = _own_context.get_context
 

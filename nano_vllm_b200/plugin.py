@@ -9,6 +9,7 @@ nanovllm/layers/attention.py:32-79) and makes the layer read nano-vllm's own per
 
 Optional steps after ``install()``, each replacing one method of the engine by a version that
 calls this package: ``fuse_pre_attention()`` (q/k norm + rotary + KV store in one launch),
+``fp8_kv_cache()`` (the KV cache in 8 bits, nearly twice the blocks),
 ``fuse_sampler()`` (one-pass token sampling), ``fuse_decode_inputs()`` (decode-step inputs in
 one launch) and, for tensor-parallel runs, ``fuse_all_reduce()`` (peer-memory sum
 behind the row-parallel projections) and ``fuse_lm_head()`` (every rank samples its own slice of
@@ -30,17 +31,20 @@ def _fused_attention_forward(has_qk_norm: bool):
     (nanovllm/models/qwen3.py:77-113, qwen2.py:77-97): same projections, but q/k norm, rotary
     embedding and the KV-cache store run as one launch on the fused qkv activation."""
 
+    import torch
+
     def forward(self, positions, hidden_states):
         qkv = self.qkv_proj(hidden_states)
         attn = self.attn
         ctx = _attention._get_context()
+        eight = attn.k_cache.dtype == torch.float8_e4m3fn  # the layer stores these itself
         _attention.qk_norm_rope_store(
             qkv, positions,
             self.q_norm.weight if has_qk_norm else None, self.k_norm.weight if has_qk_norm else None,
             self.rotary_emb.cos_sin_cache, self.q_norm.eps if has_qk_norm else 0.0,
-            ctx.slot_mapping, attn.k_cache, attn.v_cache, self.num_heads, self.num_kv_heads, self.head_dim)
+            None if eight else ctx.slot_mapping, attn.k_cache, attn.v_cache, self.num_heads, self.num_kv_heads, self.head_dim)
         q, k, v = qkv.split([self.q_size, self.kv_size, self.kv_size], dim=-1)
-        return self.o_proj(attn(q, k, v, kv_stored=True))
+        return self.o_proj(attn(q, k, v, kv_stored=not eight))
 
     return forward
 
@@ -52,6 +56,42 @@ def fuse_pre_attention() -> None:
     qwen2 = importlib.import_module("nanovllm.models.qwen2")
     qwen3.Qwen3Attention.forward = _fused_attention_forward(True)
     qwen2.Qwen2Attention.forward = _fused_attention_forward(False)
+
+
+def fp8_kv_cache() -> None:
+    """Optional step: the engine's KV cache in 8 bits.  ``ModelRunner.allocate_kv_cache`` (nanovllm/engine/model_runner.py:110-149)
+    sizes and binds its cache as ever; what it got is then laid out as e4m3 planes and scales, nearly twice the blocks in
+    the same memory, and bound to the layers (``Attention.k_cache``, ``v_cache``, ``k_scale``, ``v_scale``), and
+    ``config.num_kvcache_blocks`` says how many there are.  Attention over it differs from the bf16 cache's by the rounding of
+    K and V to 4 significant bits."""
+    runner = importlib.import_module("nanovllm.engine.model_runner")
+    import torch
+    stock = runner.ModelRunner.allocate_kv_cache
+
+    def allocate_kv_cache(self):
+        stock(self)
+        _, layers, blocks, block_size, heads, head_dim = self.kv_cache.shape
+        if block_size != 256 or head_dim not in (64, 128):
+            raise RuntimeError(f"a cache in 8 bits has blocks of 256 slots and heads of 64 or 128, not {block_size} and {head_dim}")
+        device, total = self.kv_cache.device, self.kv_cache.nbytes
+        attn = [m for m in self.model.modules() if hasattr(m, "k_cache") and hasattr(m, "v_cache")]
+        if not all(isinstance(m, _attention.Attention) for m in attn):
+            raise RuntimeError("fp8_kv_cache() needs this package's attention layer: call install() before nanovllm.models is imported")
+        self.kv_cache = None
+        for m in attn:
+            m.k_cache = m.v_cache = torch.tensor([])
+        if device.type == "cuda":
+            torch.cuda.empty_cache()
+        groups = block_size // _attention.SCALE_GROUP
+        blocks = total // (2 * layers * heads * (block_size * head_dim + groups * 4))
+        self.kv_cache = torch.zeros(2, layers, blocks, block_size, heads, head_dim, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        self.kv_scale = torch.ones(2, layers, blocks, heads, groups, dtype=torch.float32, device=device)
+        for i, m in enumerate(attn):
+            m.k_cache, m.v_cache = self.kv_cache[0, i], self.kv_cache[1, i]
+            m.k_scale, m.v_scale = self.kv_scale[0, i], self.kv_scale[1, i]
+        self.config.num_kvcache_blocks = blocks
+
+    runner.ModelRunner.allocate_kv_cache = allocate_kv_cache
 
 
 def fuse_sampler(seed: int | None = None) -> None:
