@@ -99,13 +99,20 @@ __device__ __forceinline__ uint32_t encode4(const uint2& x, float inv) {
   for (int i = 0; i < 4; ++i) y[i] = fabsf(y[i]) <= 448.f ? y[i] : NAN;
   return e4m3x2(y[0], y[1]) | e4m3x2(y[2], y[3]) << 16;
 }
-// The same of finite values, inv = 2^-e twice in bf16 (a power of two leaves all bits of a bf16 product).
+// The same of finite values, inv = 2^-e twice in bf16 (a power of two leaves all bits of a bf16 product).  A magnitude below 2^9
+// times 2^-112 has in bf16 the exponent that it has in f16 without, its bits three places further right (subnormal ones too;
+// of those f16 has more bits, which only values below 2^-14 have, and they are zeros in e4m3).  The signs go around: this takes
+// five instructions of the integer unit for four values, which is what bounds the store; by way of fp32 it were nine.
 __device__ __forceinline__ uint32_t encode4_finite(const uint2& x, uint32_t inv) {
-  uint32_t a, b;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(x.x), "r"(inv));
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(x.y), "r"(inv));
-  return __byte_perm(e4m3x2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)),
-                     e4m3x2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)), 0x5410);
+  auto code2 = [&](uint32_t v) {
+    uint32_t y, z;
+    unsigned short c;
+    asm("{.reg .b32 m; abs.bf16x2 m, %1; mul.rn.bf16x2 %0, m, %2;}" : "=r"(y) : "r"(v), "r"(inv));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(z) : "r"(y), "r"(0x07800780u));  // 2^-112, twice
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(c) : "r"(z * 8));
+    return static_cast<uint32_t>(c);
+  };
+  return __byte_perm(code2(x.x), code2(x.y), 0x5410) | (__byte_perm(x.x, x.y, 0x7531) & 0x80808080u);
 }
 // Four codes whose scale changes by `ratio` <= 1.
 __device__ __forceinline__ uint32_t recode4(uint32_t c, float ratio) {
