@@ -7,8 +7,9 @@
  *
  * Conventions shared by every entry point
  *   - All tensors are bf16 (2-byte elements), a cache held in 8 bits and its fp32 scales apart (the
- *     `_fp8` calls); metadata is int32.  Strides and extents are in ELEMENTS, never bytes.  Every data pointer and every row stride must be 16-byte aligned
- *     (8 elements); an entry point rejects anything else instead of taking a slow path.
+ *     `_fp8` calls); metadata is int32.  Strides and extents are in ELEMENTS, never bytes.  Every
+ *     data pointer and every row stride must be 16-byte aligned (8 elements); an entry point
+ *     rejects anything else instead of taking a slow path.
  *   - The caller owns every buffer.  No entry point allocates, frees or synchronises, and
  *     every kernel is launched on the `stream` that is passed in (a `cudaStream_t` given as
  *     `void*`; NULL is the legacy default stream), on the device that is current.  That makes

@@ -309,7 +309,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
 #pragma unroll 1
     for (int j = 0; j < n_units; ++j) {
       const int unit0 = (u0 + j - cc.first) * UNIT;
-      if (j >= NST && !sm100::mbar_wait(free(j), (j / NST - 1) & 1)) {
+      if (j >= NST && !__all_sync(ALL, sm100::mbar_wait(free(j), (j / NST - 1) & 1))) {
         bad |= NVLLM_STATUS_TIMEOUT;
         break;
       }
@@ -565,6 +565,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     if (tid == 0) p.counters[c.b * p.hkv + kvh] = 0u;  // ready for the next launch
   };
 
+  bool gave_up = false;
   for (int i = 0;; ++i) {
     const int u = u0 + i;
     if (i == n_units || u >= cc.first + cc.units) {  // block-uniform: the range leaves sequence cc.b
@@ -582,9 +583,11 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       load_q(qn, qn_b);
       if (STEP) next_row = load_new(qn_b);
     }
-    if (!sm100::mbar_wait(full(i), (i / NST) & 1)) {
-      bad |= NVLLM_STATUS_TIMEOUT;
-      break;
+    // A wait that ran out: no more of this warp's waits and tiles, but all barriers that the other warps count on.
+    if (!gave_up) gave_up = !__all_sync(ALL, sm100::mbar_wait(full(i), (i / NST) & 1));
+    if (gave_up) {
+      if (lane == 0) sm100::mbar_arrive(free(i));
+      continue;
     }
     const int t0 = (u - cc.first) * UNIT + warp * TT;
     if (t0 >= cc.ctx) {
@@ -738,6 +741,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     __syncwarp();  // everything of the unit is in registers
     if (lane == 0) sm100::mbar_arrive(free(i));
   }
+  if (gave_up) bad |= NVLLM_STATUS_TIMEOUT;
   if (bad && lane == 0) atomicOr(p.status, bad);
   if (n_cut == 0) return;  // block-uniform
   sync_warps();            // every thread's partials are written

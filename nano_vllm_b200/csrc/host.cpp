@@ -563,15 +563,15 @@ void prefill_fp8(const Rows& q, int64_t hq, const Fp8Planes& c, const at::Tensor
   const int64_t need = api.prefill_fp8_workspace_bytes(static_cast<int32_t>(batch), static_cast<int32_t>(max_q), static_cast<int32_t>(max_k),
                                                        static_cast<int32_t>(hq), static_cast<int32_t>(c.hkv), static_cast<int32_t>(c.d));
   check(need);
-  void* ws;
-  int64_t ws_size;
-  workspace(like, need, &ws, &ws_size);
+  // Of the call: nothing in it has to be zero or outlives it, and calls on several streams and captured ones have their own.
+  at::Tensor parts;
+  if (need > 0) parts = unlocked([&] { return at::empty({need}, like.options().dtype(at::kByte)); });
   launch([&] {
     return api.prefill_varlen_fp8(q.p, q.stride, c.k, c.v, c.k_scale, c.v_scale, ptr<int32_t>(table), table.stride(0),
                                   static_cast<int32_t>(table.size(1)), out.p, out.stride, ptr<int32_t>(cu_q), ptr<int32_t>(cu_k), q.n,
                                   static_cast<int32_t>(batch), static_cast<int32_t>(max_q), static_cast<int32_t>(max_k),
                                   static_cast<int32_t>(hq), static_cast<int32_t>(c.hkv), static_cast<int32_t>(c.d),
-                                  static_cast<float>(scale), c.blocks, ws, ws_size, stream_of(like));
+                                  static_cast<float>(scale), c.blocks, need > 0 ? parts.data_ptr() : nullptr, need, stream_of(like));
   });
 }
 

@@ -18,10 +18,13 @@
 // Twelve warps, two blocks to an SM for the whole launch: 0-3 softmax (thread = query row), 4-7 query rows in, V conversion and
 // results out, 8 = TMA of the query rows, K and the scales, 9 = MMA issuer, 10 = TMA of V.  The three warp groups trade registers at
 // start-up; 11 works out the items, one ahead.  Items (query tile of a sequence, head group) are ordered by their key tiles,
-// most first, over all sequences, and
-// dealt out in turn, there and back again, so that all blocks have about the same to do; no counter in memory, so nothing is
-// shared by launches.  Where there are two blocks or more to an item (few new tokens behind a long prefix) an item's keys go to
-// several of them (SPLIT), and prefill_fp8_join sums the parts up from the workspace.
+// most first, over all sequences, and dealt out in turn, there and back again, so that all blocks have about the same to do; no
+// counter in memory, so nothing is shared by launches.  Where there are two blocks or more to an item (few new tokens behind a
+// long prefix) an item's keys go to several of them (SPLIT), and prefill_fp8_join sums the parts up from the workspace.
+//
+// 4 x 4096 tokens (16 heads over 8 of 128): 318 us at full clocks, 860 TFLOP/s; 12 sequences of 100-2000 tokens behind 256-4096 (14
+// over 2 of 64): 200.  Bound by the chain scores - softmax - P - product of a block, of which two to an SM overlap: without
+// the exponentials 8 % less, without V's conversion 11 and 9, without rescaling O 5 and 6; the tensor cores are busy 42 % of the time.
 #include <algorithm>
 
 #include "fp8.cuh"

@@ -10,6 +10,10 @@
 // Every thread block sums the lengths itself (two words a sequence, a scan in shared memory) and then fills its share of the
 // tables and rows, so one launch does it without any block waiting for another.  A token finds its sequence by bisection of
 // the sums; a fresh block's id is read from the free list and not from the table that another block fills.
+//
+// Bound by trips one after the other (lengths, sums, entries): 2.9 us in a chain of launches for a decode step of 256 sequences
+// with tables 16 wide, 4.1 for 512 prompts; three arrays of sums instead of one of 16 bytes a sequence, lengths read twice
+// and 64-bit indexes were 4.3 for the former.
 #include <algorithm>
 
 #include "common.cuh"

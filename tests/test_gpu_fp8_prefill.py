@@ -197,7 +197,7 @@ def test_few_tokens_behind_long_prefixes(cuda, hq, hkv, d, lens):
     assert _lib.read_status() == 0
 
 
-def test_split_in_graphs_that_share_the_scratch(cuda):
+def test_split_in_graphs(cuda):
     """Graphs of a prefill behind a long prefix, of a decode over the same cache and of both, replayed in turn."""
     g = torch.Generator().manual_seed(12)
     hq, hkv, d = 8, 2, 128
@@ -224,6 +224,27 @@ def test_split_in_graphs_that_share_the_scratch(cuda):
         pre()
         for c, o in zip(calls, outs):
             assert torch.equal(o, want[0 if c is pre else 1])
+    assert _lib.read_status() == 0
+
+
+def test_split_on_two_streams_at_once(cuda):
+    """Every call has a scratch of its own: calls that overlap do not meet."""
+    g = torch.Generator().manual_seed(13)
+    jobs = []
+    for lens in ([(6000, 30)], [(4000, 9), (2500, 64)]):
+        q, planes, cu_q, cu_k, tables = case(g, lens, 14, 2, 64)
+        args = (q.to(cuda), *planes_on(cuda, *planes), cu_q.to(cuda), cu_k.to(cuda), int(cu_q.diff().max()), int(cu_k.diff().max()), 0.1, tables.to(cuda))
+        jobs.append((torch.cuda.Stream(), args, prefill_reference(q, planes, cu_q, cu_k, tables, 0.1)))
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for o, (stream, args, _) in zip(outs, jobs):
+            with torch.cuda.stream(stream):
+                o.append(A.prefill_varlen_fp8(*args))
+    torch.cuda.synchronize()
+    for o, (_, _, (ref, bound)) in zip(outs, jobs):
+        assert_within(o[0], ref, bound)
+        assert all(torch.equal(x, o[0]) for x in o)
     assert _lib.read_status() == 0
 
 
