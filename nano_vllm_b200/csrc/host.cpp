@@ -592,11 +592,35 @@ PyObject* prefill_varlen_fp8(PyObject* const* a) {
 }
 
 PyObject* step_maps(PyObject* const* a) {
-  // seq_lens, cached_lens, block_tables, free_blocks, num_tokens, cu_seqlens_q, cu_seqlens_k, slot_mapping, positions, blocks_taken
+  // seq_lens, cached_lens, block_tables, free_blocks, num_tokens, None or (cu_seqlens_q, cu_seqlens_k, slot_mapping, positions,
+  // blocks_taken); returns those
   const at::Tensor &lens = tensor(a[0], "seq_lens"), &cached = tensor(a[1], "cached_lens"), &table = tensor(a[2], "block_tables"),
-                   &free = tensor(a[3], "free_blocks"), &cu_q = tensor(a[5], "cu_seqlens_q"), &cu_k = tensor(a[6], "cu_seqlens_k"),
-                   &slots = tensor(a[7], "slot_mapping"), &positions = tensor(a[8], "positions"), &taken = tensor(a[9], "blocks_taken");
-  const int64_t rows = as_i64(a[4]);
+                   &free = tensor(a[3], "free_blocks");
+  const int64_t rows = as_i64(a[4]), batch = lens.numel();
+  require(rows >= 0, "num_tokens must not be negative");
+  require(lens.is_cuda(), "seq_lens must be a CUDA tensor");
+  at::Tensor out[5];
+  if (a[5] == Py_None) {
+    unlocked([&] {
+      const at::TensorOptions i32 = lens.options().dtype(at::kInt);
+      const int64_t sizes[5] = {batch + 1, batch + 1, rows, rows, 1};
+      for (int i = 0; i < 5; ++i) out[i] = at::empty({sizes[i]}, i == 3 ? i32.dtype(at::kLong) : i32);
+      return 0;
+    });
+  } else {
+    const char* of[5] = {"cu_seqlens_q", "cu_seqlens_k", "slot_mapping", "positions", "blocks_taken"};
+    if (!PySequence_Check(a[5]) || PySequence_Size(a[5]) != 5) raise(PyExc_ValueError, "out must be the five tensors of a step's maps");
+    for (int i = 0; i < 5; ++i) {
+      PyObject* item = PySequence_GetItem(a[5], i);
+      if (!item) throw PyErrorSet{};
+      struct Drop {
+        PyObject* o;
+        ~Drop() { Py_DECREF(o); }
+      } drop{item};
+      out[i] = tensor(item, of[i]);
+    }
+  }
+  const at::Tensor &cu_q = out[0], &cu_k = out[1], &slots = out[2], &positions = out[3], &taken = out[4];
   for (const auto& [name, t] : {std::pair<const char*, const at::Tensor*>{"seq_lens", &lens}, {"cached_lens", &cached},
                                 {"block_tables", &table}, {"free_blocks", &free}, {"cu_seqlens_q", &cu_q}, {"cu_seqlens_k", &cu_k},
                                 {"slot_mapping", &slots}, {"blocks_taken", &taken}}) {
@@ -605,10 +629,9 @@ PyObject* step_maps(PyObject* const* a) {
   }
   require(positions.is_cuda() && positions.scalar_type() == at::kLong && positions.is_contiguous(), "positions must be contiguous CUDA int64");
   require_on("positions", positions, lens);
-  const int64_t batch = lens.numel();
   require(lens.dim() == 1 && cached.dim() == 1 && cached.numel() == batch && table.dim() == 2 && table.size(0) == batch && free.dim() == 1,
           "seq_lens [B], cached_lens [B], block_tables [B, blocks], free_blocks [F]");
-  require(rows >= 0 && cu_q.numel() == batch + 1 && cu_k.numel() == batch + 1 && slots.numel() == rows && positions.numel() == rows &&
+  require(cu_q.numel() == batch + 1 && cu_k.numel() == batch + 1 && slots.numel() == rows && positions.numel() == rows &&
               taken.numel() == 1,
           "outputs must have B + 1, B + 1, num_tokens, num_tokens and 1 elements");
   require(table.size(1) <= std::numeric_limits<int32_t>::max() && free.numel() <= std::numeric_limits<int32_t>::max() &&
@@ -621,7 +644,10 @@ PyObject* step_maps(PyObject* const* a) {
                          ptr<int32_t>(cu_q), ptr<int32_t>(cu_k), ptr<int32_t>(slots), ptr<int64_t>(positions), rows,
                          ptr<int32_t>(taken), stream_of(lens));
   });
-  Py_RETURN_NONE;
+  PyObject* result = PyTuple_New(5);
+  if (!result) throw PyErrorSet{};
+  for (int i = 0; i < 5; ++i) PyTuple_SET_ITEM(result, i, wrap(out[i]));
+  return result;
 }
 
 struct Ref {  // owned reference
@@ -1062,7 +1088,7 @@ PyMethodDef methods[] = {
     METHOD(decode_paged_fp8, 9),
     METHOD(decode_step_fp8, 12),
     METHOD(prefill_varlen_fp8, 12),
-    METHOD(step_maps, 10),
+    METHOD(step_maps, 6),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of nano_vllm_b200's entry points.", -1, methods,

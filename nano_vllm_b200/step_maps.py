@@ -32,11 +32,4 @@ def step_maps(seq_lens: torch.Tensor, cached_lens: torch.Tensor, block_tables: t
     More blocks needed than there are free shows in ``blocks_taken``; entries without a block are -1 and the slots in them
     too, so nothing is stored there.  ``out``: the five result tensors of an earlier call or of a graph, else they are made.
     One launch, no synchronisation; the same call again leaves the same."""
-    native = _native(seq_lens)
-    if out is None:
-        B, i32 = seq_lens.numel(), dict(dtype=torch.int32, device=seq_lens.device)
-        out = (torch.empty(B + 1, **i32), torch.empty(B + 1, **i32), torch.empty(num_tokens, **i32),
-               torch.empty(num_tokens, dtype=torch.int64, device=seq_lens.device), torch.empty(1, **i32))
-    maps = StepMaps(*out)
-    native.step_maps(seq_lens, cached_lens, block_tables, free_blocks, num_tokens, *maps)
-    return maps
+    return StepMaps._make(_native(seq_lens).step_maps(seq_lens, cached_lens, block_tables, free_blocks, num_tokens, out))
