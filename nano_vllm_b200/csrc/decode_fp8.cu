@@ -23,8 +23,8 @@
 //     its whole group at hand, codes the row, codes the rows before it anew where the scale grows, and writes them back.
 //
 // Small batches are bound by trips one after the other: lengths and split (0.7 us), table entry, tiles, the products of a tile
-// (0.7), flush (0.6), arrival (0.8), merge.  The first three run ahead of the wait for the previous kernel and are verified
-// behind it (a sequence of 317 tokens 7.1 -> 6.7 us in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6).
+// (0.7), flush (0.6), arrival (0.8), merge (of two to four parts 1.5 us by short code of its own, by that for any number 3).  The first three run ahead of the wait for the previous kernel and are verified
+// behind it (a sequence of 317 tokens 7.1 -> 6.7 us in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6; now 5.9, 17.6 and 18.2).
 #include "fp8.cuh"
 #include "sm100.cuh"
 
@@ -480,9 +480,10 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
   };
 
   // Merges the partials of a cut sequence, all of which are in the workspace, and writes its rows: QUADS lanes take a head,
-  // four columns each, and the statistics of a part each; eight parts to a trip; lane groups left over split the parts.
+  // four columns each, and the statistics of a part each; sixteen parts to a trip; lane groups left over split the parts.
   auto merge_cut = [&](const Fp8Cut& c) {
-    constexpr int AHEAD = D == 64 ? 16 : 8;
+    constexpr int AHEAD = 16;
+    static_assert(AHEAD <= QUADS, "a lane for each part's statistics");
     const int group = tid / QUADS, gl = tid % QUADS;
     const int n_split = max(1, GROUPS / p.g);
     for (int h0 = 0; h0 < p.g; h0 += GROUPS) {
@@ -502,7 +503,8 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
         acc.w *= keep;
         mm = m_new;
       };
-      for (int j0 = 0; j0 < c.n; j0 += QUADS * n_split) {  // block-uniform; a group's parts are split + n_split * k
+#pragma unroll 1
+      for (int j0 = 0; j0 < c.n; j0 += AHEAD * n_split) {  // block-uniform; a group's parts are split + n_split * k
         float4 rows[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
@@ -511,7 +513,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
         }
         const int mine = j0 + gl * n_split + split;
         float2 ml = make_float2(-INFINITY, 0.f);
-        if (active && mine < c.n)
+        if (active && gl < AHEAD && mine < c.n)
           ml = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + (row0 + static_cast<int64_t>(mine) * p.hq) * 2));
         float m_new = fmaxf(mm, ml.x);
 #pragma unroll
@@ -526,20 +528,6 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
         for (int k = 0; k < AHEAD; ++k) {
           const float fk = __shfl_sync(ALL, f, k, QUADS);
           if (active && j0 + k * n_split + split < c.n) add_scaled(acc, rows[k], fk);
-        }
-        const int n_here = min(QUADS, (c.n - j0 + n_split - 1) / n_split);
-#pragma unroll 1
-        for (int k0 = AHEAD; k0 < n_here; k0 += AHEAD) {
-#pragma unroll
-          for (int k = 0; k < AHEAD; ++k) {
-            const int j = j0 + (k0 + k) * n_split + split;
-            if (active && j < c.n) rows[k] = row_of(j);
-          }
-#pragma unroll
-          for (int k = 0; k < AHEAD; ++k) {
-            const float fk = __shfl_sync(ALL, f, k0 + k, QUADS);
-            if (active && j0 + (k0 + k) * n_split + split < c.n) add_scaled(acc, rows[k], fk);
-          }
         }
       }
       if (n_split > 1) {  // block-uniform
@@ -561,6 +549,40 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
         sync_warps();
       }
       if (active && split == 0) write_quad(c.b, head, gl, acc, L);
+    }
+    if (tid == 0) p.counters[c.b * p.hkv + kvh] = 0u;  // ready for the next launch
+  };
+
+  // The same of a few parts, which is what a batch's sequences are cut into as a rule: a thread its columns of all of them.  A merge
+  // is the last thing that a block does and runs once, so its instructions come from L2, at 25 cycles each: short code it is.
+  constexpr int FEW = 4;
+  auto merge_few = [&](const Fp8Cut& c) {
+    const int64_t row0 = static_cast<int64_t>(c.r_first + c.b) * p.hq + kvh * p.g;
+#pragma unroll 1
+    for (int x = tid; x < p.g * QUADS; x += NT) {
+      const int64_t row = row0 + x / QUADS;
+      float2 ml[FEW];
+      float4 v[FEW], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      float top = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int j = 0; j < FEW; ++j) {
+        const int64_t at = row + static_cast<int64_t>(min(j, c.n - 1)) * p.hq;
+        ml[j] = __ldcg(reinterpret_cast<const float2*>(p.ws_ml + at * 2));
+        v[j] = __ldcg(reinterpret_cast<const float4*>(p.ws_o + at * D) + x % QUADS);
+      }
+#pragma unroll
+      for (int j = 0; j < FEW; ++j) {
+        if (j >= c.n) ml[j] = make_float2(-INFINITY, 0.f);
+        top = fmaxf(top, ml[j].x);
+      }
+#pragma unroll
+      for (int j = 0; j < FEW; ++j) {
+        if (j >= c.n || ml[j].x == -INFINITY) continue;
+        const float f = fast_exp2(ml[j].x - top);
+        L += ml[j].y * f;
+        add_scaled(acc, v[j], f);
+      }
+      write_quad(c.b, x / QUADS, x % QUADS, acc, L);
     }
     if (tid == 0) p.counters[c.b * p.hkv + kvh] = 0u;  // ready for the next launch
   };
@@ -752,8 +774,13 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     s_last_arrival[tid] = arrived == static_cast<unsigned int>(c.n - 1);
   }
   sync_warps();
-  if (s_last_arrival[0]) merge_cut(cut0);
-  if (n_cut > 1 && s_last_arrival[1]) merge_cut(cut1);
+#pragma unroll 1
+  for (int k = 0; k < n_cut; ++k) {
+    if (!s_last_arrival[k]) continue;
+    const Fp8Cut c = k == 0 ? cut0 : cut1;
+    if (c.n <= FEW) merge_few(c);
+    else merge_cut(c);
+  }
 }
 
 // ---- host side -------------------------------------------------------------------------
