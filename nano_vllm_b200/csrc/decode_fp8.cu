@@ -23,8 +23,9 @@
 //     its whole group at hand, codes the row, codes the rows before it anew where the scale grows, and writes them back.
 //
 // Small batches are bound by trips one after the other: lengths and split (0.7 us), table entry, tiles, the products of a tile
-// (0.7), flush (0.6), arrival (0.8), merge (of two to four parts 1.5 us by short code of its own, by that for any number 3).  The first three run ahead of the wait for the previous kernel and are verified
-// behind it (a sequence of 317 tokens 7.1 -> 6.7 us in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6; now 5.9, 17.6 and 18.2).
+// (0.7), flush (0.6), arrival (0.8), merge (of two to four parts 1.5 us by short code of its own, by that for any number 3).  The
+// first three run ahead of the wait for the previous kernel and are verified behind it (a sequence of 317 tokens 7.1 -> 6.7 us
+// in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6; now 5.9, 17.6 and 18.2).
 #include "fp8.cuh"
 #include "sm100.cuh"
 
@@ -295,7 +296,8 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     const float* scales = of_v ? p.v_scale : p.k_scale;
     auto block_at = [&](int j) -> int64_t {  // of the range's j-th unit; the cursor goes along
       seek(cc, u0 + j);
-      const int64_t blk = j < n_listed ? __shfl_sync(ALL, listed_blk, j) : p.block_tables[cc.b * p.bt_stride + (u0 + j - cc.first) * UNIT / kBlockSize];
+      const int64_t blk = j < n_listed ? __shfl_sync(ALL, listed_blk, j)
+                                       : p.block_tables[cc.b * p.bt_stride + (u0 + j - cc.first) * UNIT / kBlockSize];
       if (blk >= 0 && blk < p.num_blocks) return blk;
       bad |= NVLLM_STATUS_BAD_BLOCK;
       return p.num_blocks;  // rows behind the cache: zeros
