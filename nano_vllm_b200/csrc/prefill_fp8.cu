@@ -64,7 +64,7 @@ struct Geo {
   static constexpr int OFF_MISC = OFF_SLOTS + 64;                  // TMEM address, abort flag
   static constexpr int OFF_TILES = OFF_MISC + 64;                  // 4 tiles: see Fp8Tile
   static constexpr int OFF_ROW = OFF_TILES + 256;                  // 2 items x 128 rows: the query row's power of two
-  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: 1 / row sum
+  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: O's last unit / row sum
   static constexpr int SMEM = OFF_INV + 2 * 128 * 4 + 1024;
   static constexpr int SBO = D == 128 ? 1024 : 512;                // eight rows of codes
   static constexpr int OCH = D / 32;
@@ -246,7 +246,8 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           }
           ok = __all_sync(ALL, use == 0 || wait_or_abort(bar(QK_DONE0 + st), (use - 1) & 1, abort_flag));
           if (!ok) break;
-          // K's stage is free, and so is the record of tile t - 4: its softmax came before the scores of tile t - 2
+          // K's stage is free, and so is the record of tile t - 4: the scores of tile t - 2 were issued behind that tile's product,
+          // so behind its softmax and its V.  Nobody may read a record after he has reported his part of its tile.
           if (lane == 0) {
             mbar_expect_tx(bar(K_FULL0 + st), G::K_BYTES);
             tma_load_3d(base + G::OFF_K + st * G::K_BYTES, &tmap_k, bar(K_FULL0 + st), 0, kvh, row);
@@ -500,7 +501,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       if (!(ok = wait_or_abort(bar(FACTOR0 + (it & 1)), (it >> 1) & 1, abort_flag))) break;
       const float factor = row_factor[(it & 1) * 128 + r];
       const int qi = x.m0 + r_tok, off = x.Lk - x.Lq;
-      float m_used = -INFINITY, l = 0.f;
+      float m_used = -INFINITY, l = 0.f, unit = 0.f;
 #pragma unroll 1
       for (int j = 0; j < x.n_kv; ++j) {
         const int t = T + j, st = t & 1, ph = (t >> 1) & 1;
@@ -515,6 +516,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         float ks[4];
         *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(tile.k);
         const float change = tile.change;
+        unit = tile.unit;  // goes on with the row's sum: the record is the next tiles' once P is reported
 #pragma unroll
         for (int g = 0; g < 4; ++g) ks[g] = fmaxf(ks[g] * factor, 0x1p-126f);  // not zero, which -inf of a masked score must not meet
         const int j0 = (x.first + j) * BN;
@@ -591,9 +593,13 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       }
       if (!ok) break;
       T += x.n_kv;
-      // the row's normaliser goes to the row warps; no key: zeros; a sum that is NaN stays one
-      if (SPLIT && *parts_of_item > 1) p.ws_ml[static_cast<int64_t>(blockIdx.x) * BM + r] = make_float2(m_used, l);
-      inv_buf[(it & 1) * 128 + r] = l > 0.f ? 1.f / l : l;
+      // what takes O to the result, or to its part of it, goes to the row warps; no key: zeros; a sum that is NaN stays one
+      float by = l > 0.f ? 1.f / l : l;
+      if (SPLIT && *parts_of_item > 1) {
+        p.ws_ml[static_cast<int64_t>(blockIdx.x) * BM + r] = make_float2(m_used, l);
+        by = 1.f;
+      }
+      inv_buf[(it & 1) * 128 + r] = by * unit;
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(bar(EPI_FULL0 + (it & 1)));
@@ -723,13 +729,14 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       }
       return true;
     };
-    // Results of item number `done`, whose last tile was `last`.
+    // Results of item number `done`, whose last tile was `last`.  Its record may be another tile's by now: what is needed of it came
+    // with the row's sum.
     auto results = [&](const Fp8Item& x, int done, int last) {
       if (!wait_or_abort(bar(EPI_FULL0 + (done & 1)), (done >> 1) & 1, abort_flag)) return false;
-      const float inv = inv_buf[(done & 1) * 128 + r] * tile_of(last)->unit;
+      const float inv = inv_buf[(done & 1) * 128 + r];
       if (!wait_or_abort(bar(PV_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag)) return false;
       tc_fence_after();
-      if (SPLIT && *parts_of_item > 1) return set_aside(x, tile_of(last)->unit);
+      if (SPLIT && *parts_of_item > 1) return set_aside(x, inv);
       // O / l -> bf16, 32 columns at a time through this warp's patch of shared memory
       const int srow = lane >> 2, spiece = lane & 3;
       __nv_bfloat16* out_tile = p.out + static_cast<int64_t>(x.q0 + x.m0) * p.out_stride + x.h * D;
