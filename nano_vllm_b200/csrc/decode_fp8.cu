@@ -17,8 +17,11 @@
 //   * V codes go through ldmatrix.trans as pairs of neighbouring columns: a register then holds two columns of two tokens,
 //     one byte permutation away from (token, token) pairs of either column, rows gid and gid + 8 of V^T.
 //   * q is f16 too, scaled by a power of two to 2^14 <= max |q| < 2^15, so that it keeps all its bits down to 2^-29 of the
-//     largest.  The group's K scale multiplies the fp32 scores.  P is rounded to f16 (2^-11, of values up to 1), times the
-//     group's V scale over the warp's running unit: the sums O are held in that unit, which follows the scales (see `unit`).
+//     largest.  The group's K scale multiplies the fp32 scores.  P, times 2^12 and the group's V scale over the warp's running
+//     unit, is rounded to f16: the sums O are held in that unit, which follows the scales (see `unit`).  2^12 takes P to
+//     f16's upper end: weights down to 2^-24 of the largest keep all its bits, and what those below lose is 2^-35 of the largest
+//     each, in all 2^-18 of it over 131072 keys.  (Without it the keys that shared a warp with a first key 18 nats above them, 32768
+//     to a sequence, were lost: the result came out at 86 % of its value.)
 //   * 16 tokens share a scale, so a group lies in one warp's tile: the step variant's warp that streams the new token has
 //     its whole group at hand, codes the row, codes the rows before it anew where the scale grows, and writes them back.
 //
@@ -129,6 +132,8 @@ struct Fp8Cut {  // a sequence whose units lie in several ranges: n of them, fro
 // 8192 tokens (32 / 8 heads of 128) 9.9, 9.6, 8.8, 9.4 us, two of 2000 (16 / 8) 7.4, 7.5, 6.6, 6.6, two of 110000 (14 / 2 of 64) 20, 16.6,
 // 16.1, 16.1.
 constexpr float kFp8SplitBalance = 16.f;
+// P's largest in log2 units, and how far V's scales may go from the unit of O: their product stays in f16, which ends at 2^16.
+constexpr float kFp8WeightBits = 12.f, kFp8UnitUp = 8.f, kFp8UnitDown = 4.f;
 
 template <class C, bool STEP>
 __global__ void __launch_bounds__(C::NTHREADS, C::BLOCKS)
@@ -396,9 +401,9 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
   float o[C::KS][4];     // columns 16 c + 2 gid (and + 1 in [2], [3]) of heads 2 tig ([0], [2]) and 2 tig + 1, in units of `unit`
   float m0, m1, l0, l1;  // heads 2 tig and 2 tig + 1
   // What O is held in (the same for all lanes of the warp): a group's P goes into its product times vscale / unit.  It is the
-  // largest scale of the first tile, changed where a tile's largest is more than 64 times larger or 16 times smaller, so that
-  // P stays below f16's end and loses four bits of its range at most; not below 2^-60 of what it has been, which keeps O
-  // finite whatever the scales.
+  // largest scale of the first tile, changed where a tile's largest is more than 8 times larger or 4 times smaller, so that P,
+  // up to 2^12, stays below f16's end and loses two bits of its range at most; not below 2^-60 of what it has been, which keeps
+  // O finite whatever the scales.
   float unit, most_unit;
   auto reset_state = [&]() {
 #pragma unroll
@@ -715,7 +720,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     float alpha0 = fast_exp2(m0 - mn0), alpha1 = fast_exp2(m1 - mn1);
     l0 *= alpha0;
     l1 *= alpha1;
-    if (most_vs > unit * 64.f || (most_vs > 0.f && most_vs * 16.f < unit)) {
+    if (most_vs > unit * kFp8UnitUp || (most_vs > 0.f && most_vs * kFp8UnitDown < unit)) {
       const float next = fmaxf(most_vs, most_unit * 0x1p-60f), change = unit > 0.f ? unit / next : 0.f;
       alpha0 *= change;
       alpha1 *= change;
@@ -725,13 +730,14 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     const float per_unit = unit > 0.f ? 1.f / unit : 0.f;
     m0 = mn0;
     m1 = mn1;
+    const float top0 = mn0 - kFp8WeightBits, top1 = mn1 - kFp8WeightBits;  // sums of P carry 2^12 as O does: nothing to take off again
     uint32_t pb[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      s[mt][0] = fast_exp2(s[mt][0] - mn0);
-      s[mt][1] = fast_exp2(s[mt][1] - mn1);
-      s[mt][2] = fast_exp2(s[mt][2] - mn0);
-      s[mt][3] = fast_exp2(s[mt][3] - mn1);
+      s[mt][0] = fast_exp2(s[mt][0] - top0);
+      s[mt][1] = fast_exp2(s[mt][1] - top1);
+      s[mt][2] = fast_exp2(s[mt][2] - top0);
+      s[mt][3] = fast_exp2(s[mt][3] - top1);
       l0 += s[mt][0] + s[mt][2];  // per-lane partial sums; reduced over the token lanes at the flush
       l1 += s[mt][1] + s[mt][3];
       const float f = vs[mt] * per_unit;

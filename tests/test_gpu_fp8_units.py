@@ -51,3 +51,43 @@ def test_items_whose_scales_differ(cuda, hq, hkv, d, batch, cached, new):
         ref, bound = prefill_reference(q[:, heads], by_head(planes, h), cu_q, cu_k, tables, d ** -0.5)
         assert_within(first[:, heads], ref, bound, f"KV head {h}")
     assert _lib.read_status() == 0
+
+
+def sink(gen, hkv, d, n, nats, apart):
+    """Planes of one sequence of ``n`` tokens whose first key is ``nats`` above all others, with V = 0, in a group whose scale is
+    2^``apart`` of the others'; and the output of a query of ones in column 0.  V is an e4m3 number in every column."""
+    blocks = -(-n // 256)
+    k = torch.zeros(blocks, 256, hkv, d, dtype=torch.uint8)
+    v = torch.randint(0x30, 0x38, (1, 1, hkv, d), generator=gen, dtype=torch.uint8).repeat(blocks, 256, 1, 1)  # 0.5 to 0.94
+    ks, vs = torch.ones(blocks, hkv, 16), torch.ones(blocks, hkv, 16)
+    k[0, 0, :, 0], v[0, 0] = {14: 0x56, 16: 0x58, 18: 0x59}[nats], 0
+    vs[0, :, 0] = 2.0 ** apart
+    values = v[0, 1].view(torch.float8_e4m3fn).double()  # [hkv, d]
+    p = torch.exp(torch.tensor(-float(nats), dtype=torch.float64))
+    total = 1 + (n - 1) * p
+    own = min(15, n - 1)  # of the first key's group
+    out = p * (own * 2.0 ** apart + (n - 1 - own)) / total * values
+    # half a step of the result's rounding to bf16, of every weight's to f16, as much again for half of it for sums and
+    # exponentials in 32 bits; and for weights below f16's normal range 2^-25 of the unit, which is 4 times a tile's largest
+    # scale at most, over 2^12: n 2^-35 max |v| / total
+    bound = (2.0 ** -8 + 1.5 * 2.0 ** -11) * out + 2.0 ** -35 * n * values.amax() * 2.0 ** max(apart, 0) / total
+    return (k, v, ks, vs), out, bound
+
+
+SINKS = [(16384, 14), (32768, 16), (32768, 18), (131072, 18)]
+
+
+@pytest.mark.parametrize("apart", [-4, -1, 0, 1, 2, 3, 4])
+@pytest.mark.parametrize("n,nats", SINKS)
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 64), (4, 1, 128)])
+def test_decode_of_small_weights_in_great_number(cuda, hq, hkv, d, n, nats, apart):
+    """One such sequence, cut into parts with maxima of their own, and 300 of them (the same blocks), a range to each or so."""
+    planes, out, bound = sink(torch.Generator().manual_seed(n + nats), hkv, d, n, nats, apart)
+    dev = planes_on(cuda, *planes)
+    for batch in (1, 300):
+        q = torch.zeros(batch, hq, d, dtype=torch.bfloat16, device=cuda)
+        q[:, :, 0] = 1
+        table = torch.arange(n // 256, dtype=torch.int32, device=cuda).expand(batch, -1).contiguous()
+        got = A.decode_paged_fp8(q, *dev, torch.full((batch,), n, dtype=torch.int32, device=cuda), table, 1.0)
+        assert_within(got, out.expand(batch, hq, d), bound.expand(batch, hq, d), f"{batch} sequences")
+    assert _lib.read_status() == 0
