@@ -8,7 +8,8 @@
 //     2^-10 of the row's largest value, below that within 2^-17 of it.  Two products at twice the rate of a 16-bit one: the
 //     same time, and no key has to be converted.
 //   * The K scale of a group and the row's power of two enter the multiply-add in front of the exponential, four factors a tile.
-//   * O += P V in f16 (kind::f16): P from TMEM, rounded to f16 (2^-11); V's codes become f16 once a tile, by the warps that also
+//   * O += P V in f16 (kind::f16): P from TMEM, 2^8 to 2^15 at a row's largest score, rounded to f16: weights down to 2^-22 of the
+//     largest keep all its bits, those below lose 2^-33 of it each.  V's codes become f16 once a tile, by the warps that also
 //     write results, times the group's scale over the unit that O is held in: the largest scale of an item's first tile,
 //     changed (and O with it) where a tile's largest is more than 2^7 times larger or 2^14 times smaller, which keeps every
 //     V / unit an f16 number; not below 2^-60 of what it has been, which keeps O finite whatever the scales.  Exact for scales
@@ -41,7 +42,11 @@ constexpr int NTHREADS = 384;
 constexpr int REGS_LAUNCH = 80, REGS_SOFTMAX = 136, REGS_ROWS = 64, REGS_OTHER = 40;
 static_assert(128 * (REGS_SOFTMAX + REGS_ROWS + REGS_OTHER) <= NTHREADS * REGS_LAUNCH, "register pool of a block");
 constexpr int TMEM_COLS = 256, TMEM_O = 128;  // S / P buffers [0,64) and [64,128), O [128,256)
-constexpr float kRescaleThreshold = 14.f;     // log2 units: P stays below 2^15, f16 goes to 2^16
+// Log2 units: P is 2^8 where a score is the maximum in use, which is kept until one is 2^7 times larger; f16 goes to 2^16.  (P from 1 on,
+// and 2^14, lost all that 131072 keys 18 nats below a first one have.)  Where a row outgrows its maximum, its warp's other rows go to
+// theirs too: 4 x 4096 tokens (16 heads over 8 of 128, scores of 2.2 nats) one call after the other 380 -> 365 us; thresholds of 8, 6 and 5
+// are 362, 370 and 367, 14 is 349.  (14 for an item's first 1024 keys alone is 358, and loses 2^-26 of the largest on each of those.)
+constexpr float kWeightBits = 8.f, kRescaleThreshold = 7.f;
 enum Bar {
   Q_FULL, K_FULL0, K_FULL1, RAW_FULL0, RAW_FULL1, RAW_FREE0, RAW_FREE1, V_FULL0, V_FULL1, QK_DONE0, QK_DONE1, PV_DONE0, PV_DONE1,
   P_FULL0, P_FULL1, ITEM_FULL0, ITEM_FULL1, ITEM_FREE0, ITEM_FREE1, O_FREE, EPI_FULL0, EPI_FULL1,
@@ -539,11 +544,10 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           mx = fmaxf(mx, fmaxf(m2[0], m2[1]) * ks[g]);
         }
         const float m_new = fmaxf(m_used, mx);
-        // lazy rescale: keep the old reference maximum unless it has been outgrown by 2^14
-        const bool grow = m_new > m_used + kRescaleThreshold;
-        if (change != 1.f || __any_sync(ALL, grow)) {
+        // lazy rescale: the old reference maxima stay until one of the warp has been outgrown by the threshold; then all follow
+        if (change != 1.f || __any_sync(ALL, m_new > m_used + kRescaleThreshold)) {
           float alpha = 1.f;
-          if (grow) {
+          if (m_new > m_used) {
             alpha = (m_used == -INFINITY) ? 0.f : fast_exp2(m_used - m_new);
             m_used = m_new;
             l *= alpha;
@@ -563,8 +567,8 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
             }
           }
         }
-        const float msub = (m_used == -INFINITY) ? 0.f : m_used;
-        // p = 2^(s * scale - m): the multiply-subtract and the row sum run two lanes at a time
+        const float msub = (m_used == -INFINITY) ? 0.f : m_used - kWeightBits;
+        // p = 2^(s * scale - m + 8), and so are l and O: the multiply-subtract and the row sum run two lanes at a time
         const uint64_t nmsub2 = pack2(-msub, -msub);
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll

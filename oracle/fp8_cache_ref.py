@@ -106,8 +106,11 @@ def attend(q, k, v, scale, seen):
       2^-8 |out|            the output's rounding, half a step
       (2^-11 + 2^-12) A     A = sum p |v| / sum p: every weight's rounding to f16 (half a step, 2^-11), and as much again
                             for half of it: scores and exponentials in 32 bits (their errors are some 2^-18 at |s| < 100)
-      2^-20 n max|v| / L    L = sum p / max p: weights below f16's normal range are off by 2^-25 of the unit of a tile's V,
-                            which is at most 16 times the largest scale in it, and that 2 times what max|v| calls for
+      2^-33 n max|v| / L    L = sum p / max p: weights below f16's normal range are off by 2^-25.  Prefill: of a largest weight of
+                            2^8 at least; decode: of one of 2^12, in a unit at most 4 times the largest scale of a tile,
+                            which is 2 times what max|v| calls for at most: 2^-34
+      2^-24 max|v|          prefill: a group's scale over the unit is rounded to f16, off by 2^-25 where it is far smaller, times
+                            a code of 448 at most; the unit is a tile's largest scale, max|v| / 224 at most
     """
     lq, hq, d = q.shape
     lk, hkv, _ = k.shape
@@ -120,7 +123,7 @@ def attend(q, k, v, scale, seen):
     div = torch.where(total > 0, total, 1.0)
     out = torch.einsum("hqk,khd->qhd", p, v) / div.T[..., None]
     a = torch.einsum("hqk,khd->qhd", p, v.abs()) / div.T[..., None]
-    bound = 2.0 ** -8 * out.abs() + 1.5 * 2.0 ** -11 * a + 2.0 ** -20 * lk * v.abs().amax() / div.T[..., None]
+    bound = 2.0 ** -8 * out.abs() + 1.5 * 2.0 ** -11 * a + (2.0 ** -33 * lk / div.T[..., None] + 2.0 ** -24) * v.abs().amax()
     return out, bound
 
 

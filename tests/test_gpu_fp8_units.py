@@ -53,7 +53,7 @@ def test_items_whose_scales_differ(cuda, hq, hkv, d, batch, cached, new):
     assert _lib.read_status() == 0
 
 
-def sink(gen, hkv, d, n, nats, apart):
+def sink(gen, hkv, d, n, nats, apart, bits=35):
     """Planes of one sequence of ``n`` tokens whose first key is ``nats`` above all others, with V = 0, in a group whose scale is
     2^``apart`` of the others'; and the output of a query of ones in column 0.  V is an e4m3 number in every column."""
     blocks = -(-n // 256)
@@ -68,9 +68,9 @@ def sink(gen, hkv, d, n, nats, apart):
     own = min(15, n - 1)  # of the first key's group
     out = p * (own * 2.0 ** apart + (n - 1 - own)) / total * values
     # half a step of the result's rounding to bf16, of every weight's to f16, as much again for half of it for sums and
-    # exponentials in 32 bits; and for weights below f16's normal range 2^-25 of the unit, which is 4 times a tile's largest
-    # scale at most, over 2^12: n 2^-35 max |v| / total
-    bound = (2.0 ** -8 + 1.5 * 2.0 ** -11) * out + 2.0 ** -35 * n * values.amax() * 2.0 ** max(apart, 0) / total
+    # exponentials in 32 bits; and for weights below f16's normal range n 2^-bits max |v| / total: 2^-25 of the unit, which is 4
+    # times a tile's largest scale at most, over a largest weight of 2^12 (decode, 35), or 2^-25 over one of 2^8 (prefill, 33)
+    bound = (2.0 ** -8 + 1.5 * 2.0 ** -11) * out + 2.0 ** -bits * n * values.amax() * 2.0 ** max(apart, 0) / total
     return (k, v, ks, vs), out, bound
 
 
@@ -89,5 +89,22 @@ def test_decode_of_small_weights_in_great_number(cuda, hq, hkv, d, n, nats, apar
         q[:, :, 0] = 1
         table = torch.arange(n // 256, dtype=torch.int32, device=cuda).expand(batch, -1).contiguous()
         got = A.decode_paged_fp8(q, *dev, torch.full((batch,), n, dtype=torch.int32, device=cuda), table, 1.0)
+        assert_within(got, out.expand(batch, hq, d), bound.expand(batch, hq, d), f"{batch} sequences")
+    assert _lib.read_status() == 0
+
+
+@pytest.mark.parametrize("apart", [-4, 0, 3, 7])
+@pytest.mark.parametrize("n,nats", SINKS)
+@pytest.mark.parametrize("hq,hkv,d", [(2, 1, 64), (4, 1, 128)])
+def test_prefill_of_small_weights_in_great_number(cuda, hq, hkv, d, n, nats, apart):
+    """One query token behind such a sequence, its keys in parts, and 300 of them, whole."""
+    planes, out, bound = sink(torch.Generator().manual_seed(n + nats), hkv, d, n, nats, apart, 33)
+    dev = planes_on(cuda, *planes)
+    for batch in (1, 300):
+        q = torch.zeros(batch, hq, d, dtype=torch.bfloat16, device=cuda)
+        q[:, :, 0] = 1
+        table = torch.arange(n // 256, dtype=torch.int32, device=cuda).expand(batch, -1).contiguous()
+        cu = torch.arange(batch + 1, dtype=torch.int32, device=cuda)
+        got = A.prefill_varlen_fp8(q, *dev, cu, cu * n, 1, n, 1.0, table)
         assert_within(got, out.expand(batch, hq, d), bound.expand(batch, hq, d), f"{batch} sequences")
     assert _lib.read_status() == 0
