@@ -586,8 +586,8 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       }
 #pragma unroll
       for (int j = 0; j < FEW; ++j) {
-        if (j >= c.n || ml[j].x == -INFINITY) continue;
-        const float f = fast_exp2(ml[j].x - top);
+        if (j >= c.n) continue;
+        const float f = ml[j].x == -INFINITY ? 0.f : fast_exp2(ml[j].x - top);  // no maximum but a sum: NaN, which zero times it stays
         L += ml[j].y * f;
         add_scaled(acc, v[j], f);
       }

@@ -5,6 +5,7 @@ import torch
 
 from fp8_cases import assert_within, planes_on, prefill_reference, random_planes, tables_for
 from nano_vllm_b200 import _lib, attention as A
+from oracle import fp8_cache_ref as F8
 
 pytestmark = pytest.mark.gpu
 
@@ -107,4 +108,27 @@ def test_prefill_of_small_weights_in_great_number(cuda, hq, hkv, d, n, nats, apa
         cu = torch.arange(batch + 1, dtype=torch.int32, device=cuda)
         got = A.prefill_varlen_fp8(q, *dev, cu, cu * n, 1, n, 1.0, table)
         assert_within(got, out.expand(batch, hq, d), bound.expand(batch, hq, d), f"{batch} sequences")
+    assert _lib.read_status() == 0
+
+
+@pytest.mark.parametrize("n", [300, 500, 1500])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (4, 2, 64)])
+def test_nan_in_cut_sequences(cuda, hq, hkv, d, n):
+    """Sequences whose keys several blocks share, in parts of few and of many: a query of NaN, a head whose every key is NaN in one
+    part alone, and in all of them."""
+    g = torch.Generator().manual_seed(n + d)
+    lens = [n] * 4
+    blocks = 4 * -(-n // 256)
+    planes, tables = random_planes(g, blocks, hkv, d), tables_for(g, lens, blocks)
+    q = torch.randn(4, hq, d, generator=g).bfloat16()
+    q[0, 1] = float("nan")
+    planes[0][int(tables[1, 0]), 128:256, 0, 5] = 0x7F
+    planes[0][tables[2].long(), :, 1, 7] = 0xFF
+    ctx = torch.tensor(lens, dtype=torch.int32)
+    got = A.decode_paged_fp8(q.to(cuda), *planes_on(cuda, *planes), ctx.to(cuda), tables.to(cuda), 0.1).cpu()
+    ref, bound = F8.decode_fp8_ref(q, *planes, ctx, tables, 0.1)
+    assert ref[0, 1].isnan().all() and ref[1, :2].isnan().all() and ref[2, 2:].isnan().all() and ref.isnan().sum() == 5 * d
+    assert torch.equal(got.isnan(), ref.isnan())
+    whole = ~ref.isnan()
+    assert_within(got[whole], ref[whole], bound.nan_to_num(float("inf"))[whole])
     assert _lib.read_status() == 0
