@@ -840,13 +840,14 @@ __global__ void __launch_bounds__(256) prefill_fp8_join_kernel(const PrefillFp8P
     sum *= old, acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
     top = high;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      const float w = s[i].x == -INFINITY ? 0.f : fast_exp2(s[i].x - top);
+      sum = fmaf(s[i].y, w, sum);  // no maximum but a sum: NaN, which zero times it stays
       if (s[i].x != -INFINITY) {
-        const float w = fast_exp2(s[i].x - top);
-        sum = fmaf(s[i].y, w, sum);
         acc.x = fmaf(o[i].x, w, acc.x), acc.y = fmaf(o[i].y, w, acc.y);
         acc.z = fmaf(o[i].z, w, acc.z), acc.w = fmaf(o[i].w, w, acc.w);
       }
+    }
   }
   if (row >= what.z) return;
   const float by = sum > 0.f ? 1.f / sum : sum;  // no key: zeros; a sum that is NaN stays one

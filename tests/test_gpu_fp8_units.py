@@ -132,3 +132,35 @@ def test_nan_in_cut_sequences(cuda, hq, hkv, d, n):
     whole = ~ref.isnan()
     assert_within(got[whole], ref[whole], bound.nan_to_num(float("inf"))[whole])
     assert _lib.read_status() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (14, 2, 64)])
+def test_nan_in_keys_in_parts(cuda, hq, hkv, d):
+    """Few queries behind a long prefix, whose keys go to several blocks: NaN queries, a head whose every key is NaN, and one whose
+    keys are NaN in a stretch that makes up whole parts."""
+    g = torch.Generator().manual_seed(d)
+    n, new = 4000, 5
+    planes, tables = random_planes(g, 16, hkv, d), tables_for(g, [n], 16)
+    cu_q, cu_k = torch.tensor([0, new], dtype=torch.int32), torch.tensor([0, n], dtype=torch.int32)
+    assert _lib.load().nvllm_prefill_fp8_workspace_bytes(1, new, n, hq, hkv, d) > 0  # in parts
+    for stretch in (0, 12):
+        k = planes[0].clone()
+        if stretch:
+            k[tables[0, 1:1 + stretch].long(), :, 1, 7] = 0xFF
+        q = torch.randn(new, hq, d, generator=g).bfloat16()
+        q[1, 0], q[3, hq - 1, 0] = float("nan"), float("inf")
+        args = (q, (k, *planes[1:]), cu_q, cu_k, tables, 0.1)
+        got = A.prefill_varlen_fp8(q.to(cuda), *planes_on(cuda, *args[1]), cu_q.to(cuda), cu_k.to(cuda), new, n, 0.1, tables.to(cuda)).cpu()
+        want = torch.zeros(got.shape, dtype=torch.bool)
+        want[1, 0] = want[3, hq - 1] = True
+        if stretch:
+            want[:, hq // 2:] = True
+        assert torch.equal(got.isnan(), want)
+        group = hq // hkv
+        for h in range(1 if stretch else hkv):
+            heads = slice(h * group, (h + 1) * group)
+            finite = torch.where(q[:, heads].isfinite(), q[:, heads], 0)
+            ref, bound = prefill_reference(finite, by_head(args[1], h), cu_q, cu_k, tables, 0.1)
+            whole = ~want[:, heads]
+            assert_within(got[:, heads][whole], ref[whole], bound[whole], f"KV head {h}")
+    assert _lib.read_status() == 0
