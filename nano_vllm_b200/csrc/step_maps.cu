@@ -177,7 +177,7 @@ extern "C" int nvllm_step_maps(const int32_t* seq_lens, const int32_t* cached_le
   static bool ready[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (smem > (48u << 10) && (dev < 0 || dev >= 64 || !ready[dev])) {
+  if (dev < 0 || dev >= 64 || !ready[dev]) {  // whatever this batch needs: the kernel's own arrays come on top of it
     const cudaError_t e = cudaFuncSetAttribute(step_maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kMapsMaxBatch + 1) * sizeof(int4));
     if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "step_maps: cannot reserve shared memory: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[dev] = true;
