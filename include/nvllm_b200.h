@@ -344,13 +344,14 @@ NVLLM_API int nvllm_prefill_varlen_fp8(const void* q, int64_t q_row_stride, cons
  * ceil(cached / 256) of them, are given.
  *   block_tables: the entries from there to ceil(seq / 256) are taken from free_blocks, in order, sequence after sequence;
  *       those behind become -1
- *   cu_seqlens_q, cu_seqlens_k [batch + 1]: prefix sums of max(seq - cached, 0) and of seq
+ *   cu_seqlens_q, cu_seqlens_k [batch + 1]: prefix sums of max(seq - cached, 0), no more than num_rows, and of seq
  *   slot_mapping (int32), positions (int64) [num_rows]: of the new tokens, packed sequence after sequence; rows behind the
  *       last one (the padding of a captured batch) get slot -1 and position 0
  *   blocks_taken [1]: how many free blocks the step needs.  More than num_free: the entries without a block are -1, and so
  *       are the slots in them.
  * Lengths outside 0 to 256 * max_blocks are cut to that and flagged NVLLM_STATUS_BAD_BLOCK; more new tokens than num_rows are
- * flagged NVLLM_STATUS_BAD_SLOT (the first num_rows are listed).  batch 1 to 4096; batch * max_blocks * 256 < 2^31.
+ * flagged NVLLM_STATUS_BAD_SLOT (the first num_rows are listed, and cu_seqlens_q ends there, so that what reads or writes
+ * num_rows rows by it stays within them).  batch 1 to 4096; batch * max_blocks * 256 < 2^31.
  * One launch; a second call with the same arguments leaves the same.
  */
 NVLLM_API int nvllm_step_maps(const int32_t* seq_lens, const int32_t* cached_lens, int32_t batch, int32_t* block_tables,

@@ -3,7 +3,7 @@
 // Sequence b has cached_lens[b] tokens in the cache and seq_lens[b] with this step.  With held = ceil(cached / 256), need =
 // ceil(seq / 256) and first[b] the sum of max(need - held, 0) over the sequences before it:
 //   block_tables[b][held .. need) = free_blocks[first[b] ...];  entries from need on: -1;  entries below held stay
-//   cu_seqlens_q, cu_seqlens_k: prefix sums of max(seq - cached, 0) and of seq
+//   cu_seqlens_q, cu_seqlens_k: prefix sums of max(seq - cached, 0), cut to the rows there are, and of seq
 //   packed token t of b: position cached + t, slot = table[position / 256] * 256 + position % 256
 //   rows behind the last token: slot -1 (stored nowhere), position 0
 //
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kMapsThreads) step_maps_kernel(const StepMapsP
     x.y += before[1];
     s_seq[b] = x;
     if (first_block) {
-      p.cu_q[b] = x.x;
+      p.cu_q[b] = min(x.x, p.rows);
       p.cu_k[b] = keys;
     }
     keys += x.w;
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kMapsThreads) step_maps_kernel(const StepMapsP
     const int total = before[0] + sum[0], taken = before[1] + sum[1];
     s_seq[p.batch] = make_int4(total, taken, 0, 0);
     if (first_block) {
-      p.cu_q[p.batch] = total;
+      p.cu_q[p.batch] = min(total, p.rows);
       p.cu_k[p.batch] = keys;
       *p.taken = taken;
       if (total > p.rows) atomicOr(p.status, NVLLM_STATUS_BAD_SLOT);

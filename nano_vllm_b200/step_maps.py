@@ -15,7 +15,7 @@ from .attention import _native
 
 
 class StepMaps(NamedTuple):
-    cu_seqlens_q: torch.Tensor  # int32 [B + 1]: offsets of the sequences' new tokens
+    cu_seqlens_q: torch.Tensor  # int32 [B + 1]: offsets of the sequences' new tokens, no more than num_tokens
     cu_seqlens_k: torch.Tensor  # int32 [B + 1]: and of all their tokens
     slot_mapping: torch.Tensor  # int32 [num_tokens]: cache slot of every new token, -1 behind the last one
     positions: torch.Tensor     # int64 [num_tokens]: its position in its sequence, 0 behind the last one

@@ -4,6 +4,10 @@ import sys
 from pathlib import Path
 
 import pytest
+import torch
+
+from nano_vllm_b200 import _lib, attention as A
+from nano_vllm_b200.step_maps import step_maps
 
 pytestmark = pytest.mark.gpu
 ROOT = Path(__file__).resolve().parents[1]
@@ -36,3 +40,20 @@ def test_first_batch_of_a_process(cuda, batch):
     """16 bytes a sequence reach the 48 KB that a launch has without asking for more, beside what the kernel has of its own."""
     r = subprocess.run([sys.executable, "-c", SCRIPT % {"root": str(ROOT), "batch": batch}], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "as listed" in r.stdout, r.stderr[-2000:]
+
+
+def test_more_tokens_than_rows_stay_within_the_rows(cuda):
+    """Offsets end at the rows there are: a prefill over them leaves what lies behind its output as it was."""
+    i32 = dict(dtype=torch.int32, device=cuda)
+    hq, hkv, d, rows = 4, 2, 64, 100
+    codes, scales = torch.zeros(8, 256, hkv, d, device=cuda).to(torch.float8_e4m3fn), torch.ones(8, hkv, 16, device=cuda)
+    q = torch.randn(rows, hq, d, device=cuda).bfloat16()
+    for lens, want in (([300, 500], [0, 100, 100]), ([60, 500], [0, 60, 100]), ([60, 40], [0, 60, 100])):
+        table = torch.full((2, 2), -1, **i32)
+        _lib.read_status()
+        m = step_maps(torch.tensor(lens, **i32), torch.zeros(2, **i32), table, torch.arange(8, **i32), rows)
+        assert _lib.read_status() == (1 if sum(lens) > rows else 0)
+        assert m.cu_seqlens_q.tolist() == want and m.cu_seqlens_k.tolist() == [0, lens[0], sum(lens)]
+        out = torch.full((rows + 700, hq, d), 3.0, dtype=torch.bfloat16, device=cuda)
+        A.prefill_varlen_fp8(q, codes, codes, scales, scales, m.cu_seqlens_q, m.cu_seqlens_k, max(lens), max(lens), 0.1, table, out=out[:rows])
+        assert (out[rows:] == 3).all() and (out[:rows] == 0).all()
