@@ -274,14 +274,14 @@ NVLLM_API int nvllm_attention_prefill(const void* q, int64_t q_row_stride,
  *   codes   k_cache / v_cache: e4m3 (1 byte), [num_blocks, 256, Hkv, D] contiguous, addressed as the bf16 planes are;
  *   scales  k_scale / v_scale: fp32, [num_blocks, Hkv, 16] contiguous: one for every group of NVLLM_SCALE_GROUP slots of a
  *           block and KV head.  Slot s, head h holds  code * scale[s / 256][h][s % 256 / 16].
- * All four 16-byte aligned; num_blocks * 256 < 2^31.  D in {64,128}.  The readers take any positive finite scales, the stores
- * write powers of two from 2^-64 to 2^120.
+ * All four 16-byte aligned; num_blocks * 256 < 2^31.  D in {64,128}.  The readers take any finite scales from 0 on (results
+ * below 2^-126 may be zero; sums of |V| over the keys end where fp32 does, at 2^128), the stores write powers of two from 2^-64 to 2^120.
  *
  * nvllm_store_kvcache_fp8 stores rows as nvllm_store_kvcache does (row strides, skipped and flagged slots as there).  For every
  * group that rows go to, and each head: f = the lowest offset in the group that is written, a = the largest finite magnitude
  * of the rows written,
  *     need  = the smallest power of two (from 2^-64 on) with a <= 448 * need
- *     scale = need where f == 0, else max(need, the group's scale so far (rounded up to a power of two))
+ *     scale = need where f == 0, else max(need, the group's scale so far (rounded up to a power of two from 2^-64 to 2^120))
  *     rows written: code = x / scale rounded to e4m3, nearest even;  infinities and NaN become NaN
  *     rows of the group below f, if the scale has grown: code = code * old / scale, rounded likewise
  * i.e. a group is filled from its first slot on, as sequences grow: a row at offset 0 starts it afresh, and rows above f that are

@@ -403,14 +403,17 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
   // What O is held in (the same for all lanes of the warp): a group's P goes into its product times vscale / unit.  It is the
   // largest scale of the first tile, changed where a tile's largest is more than 8 times larger or 4 times smaller, so that P,
   // up to 2^12, stays below f16's end and loses two bits of its range at most; not below 2^-60 of what it has been, which keeps
-  // O finite whatever the scales.
+  // O finite whatever the scales; and not below 2^-114, so that it is normal when the 2^12 is taken off: smaller scales,
+  // subnormal ones too, leave P to f16's lower end.
+  constexpr float least_unit = 0x1p-114f;
   float unit, most_unit;
   auto reset_state = [&]() {
 #pragma unroll
     for (int c = 0; c < C::KS; ++c) o[c][0] = o[c][1] = o[c][2] = o[c][3] = 0.f;
     m0 = m1 = -INFINITY;
     l0 = l1 = 0.f;
-    unit = most_unit = 0.f;
+    unit = least_unit;
+    most_unit = 0.f;
   };
   reset_state();
 
@@ -438,12 +441,16 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       l0 += __shfl_xor_sync(ALL, l0, sh);
       l1 += __shfl_xor_sync(ALL, l1, sh);
     }
+    // without the 2^12: the sums of large values end where fp32 does as it is
+    constexpr float back = 1.f / (1 << static_cast<int>(kFp8WeightBits));
+    l0 *= back, l1 *= back;
+    const float by = unit * back;
     sync_warps();  // the previous merge has been read by everyone
 #pragma unroll
     for (int c = 0; c < C::KS; ++c) {
       float* dst = sm_o + (warp * 8 + 2 * tig) * OROW + c * 16 + 2 * gid;
-      *reinterpret_cast<float2*>(dst) = make_float2(o[c][0] * unit, o[c][2] * unit);
-      *reinterpret_cast<float2*>(dst + OROW) = make_float2(o[c][1] * unit, o[c][3] * unit);
+      *reinterpret_cast<float2*>(dst) = make_float2(o[c][0] * by, o[c][2] * by);
+      *reinterpret_cast<float2*>(dst + OROW) = make_float2(o[c][1] * by, o[c][3] * by);
     }
     if (gid == 0) {
       float* dst = sm_o + (warp * 8 + 2 * tig) * OROW + D;
@@ -720,17 +727,17 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     float alpha0 = fast_exp2(m0 - mn0), alpha1 = fast_exp2(m1 - mn1);
     l0 *= alpha0;
     l1 *= alpha1;
-    if (most_vs > unit * kFp8UnitUp || (most_vs > 0.f && most_vs * kFp8UnitDown < unit)) {
-      const float next = fmaxf(most_vs, most_unit * 0x1p-60f), change = unit > 0.f ? unit / next : 0.f;
+    if (most_vs > unit * kFp8UnitUp || (most_vs * kFp8UnitDown < unit && unit > least_unit && most_vs > 0.f)) {
+      const float next = fminf(fmaxf(fmaxf(most_vs, most_unit * 0x1p-60f), least_unit), kLargestUnit), change = unit / next;
       alpha0 *= change;
       alpha1 *= change;
       unit = next;
       most_unit = fmaxf(most_unit, next);
     }
-    const float per_unit = unit > 0.f ? 1.f / unit : 0.f;
+    const float per_unit = 1.f / unit;
     m0 = mn0;
     m1 = mn1;
-    const float top0 = mn0 - kFp8WeightBits, top1 = mn1 - kFp8WeightBits;  // sums of P carry 2^12 as O does: nothing to take off again
+    const float top0 = mn0 - kFp8WeightBits, top1 = mn1 - kFp8WeightBits;  // sums of P carry 2^12 as O does
     uint32_t pb[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -740,7 +747,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       s[mt][3] = fast_exp2(s[mt][3] - top1);
       l0 += s[mt][0] + s[mt][2];  // per-lane partial sums; reduced over the token lanes at the flush
       l1 += s[mt][1] + s[mt][3];
-      const float f = vs[mt] * per_unit;
+      const float f = mul_subnormal(vs[mt], per_unit);
       pb[mt][0] = movmatrix_trans(pack_f16x2(s[mt][0] * f, s[mt][1] * f));
       pb[mt][1] = movmatrix_trans(pack_f16x2(s[mt][2] * f, s[mt][3] * f));
     }

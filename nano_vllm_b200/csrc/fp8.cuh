@@ -3,7 +3,8 @@
 // A code c of slot s, head h stands for value(c) * scale[s / 256][h][s % 256 / 16].  Scales that the stores write are powers
 // of two: a floating-point code loses nothing by that (the same four significant bits in every binade, 448 / 2^-6 from end to
 // end), the quotient x / scale is exact, so that a row is rounded once, by its code, and a group whose scale has to grow is
-// coded anew without a second rounding except of values that fall below 2^-6 of the new scale.  Readers take any finite scale.
+// coded anew without a second rounding except of values that fall below 2^-6 of the new scale.  Readers take any finite scale from
+// 0 on; their results below 2^-126 may be zero.
 #pragma once
 
 #include "common.cuh"
@@ -65,6 +66,16 @@ __device__ __forceinline__ uint2 ld_shared8(uint32_t a) {
 }
 __device__ __forceinline__ void st_shared8(uint32_t a, const uint2& v) {
   asm volatile("st.shared.v2.u32 [%0], {%1,%2};\n" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// What sums over V are held in stays between these, whatever the scales: so does its reciprocal, which the build's fast arithmetic
+// flushes to zero behind 2^126, as it does subnormal operands.
+constexpr float kLargestUnit = 0x1p126f;
+// a * b with subnormal operands as they are.
+__device__ __forceinline__ float mul_subnormal(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 __device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }

@@ -69,7 +69,7 @@ struct Geo {
   static constexpr int OFF_MISC = OFF_SLOTS + 64;                  // TMEM address, abort flag
   static constexpr int OFF_TILES = OFF_MISC + 64;                  // 4 tiles: see Fp8Tile
   static constexpr int OFF_ROW = OFF_TILES + 256;                  // 2 items x 128 rows: the query row's power of two
-  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: O's last unit / row sum
+  static constexpr int OFF_INV = OFF_ROW + 2 * 128 * 4;            // 2 items x 128 rows: 1 / row sum
   static constexpr int SMEM = OFF_INV + 2 * 128 * 4 + 1024;
   static constexpr int SBO = D == 128 ? 1024 : 512;                // eight rows of codes
   static constexpr int OCH = D / 32;
@@ -178,6 +178,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
   volatile int* parts_of_item = reinterpret_cast<volatile int*>(base_ptr + G::OFF_MISC + 16);  // SPLIT: whose part this block has
   float* row_factor = reinterpret_cast<float*>(base_ptr + G::OFF_ROW);
   float* inv_buf = reinterpret_cast<float*>(base_ptr + G::OFF_INV);
+  float* unit_buf = reinterpret_cast<float*>(base_ptr + G::OFF_MISC + 24);  // 2 items: what O is held in at its end
   const int pack = p.pack, BMT = p.tile_tokens;
   auto token_of = [&](int row) { return row * p.inv_pack >> 16; };  // row / pack, row < 128
 
@@ -262,12 +263,13 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           float most = fmaxf(v, __shfl_xor_sync(ALL, v, 1));
           most = fmaxf(most, __shfl_xor_sync(ALL, most, 2));
           const float before = unit;
-          if (j == 0) unit = most_unit = most;
+          if (j == 0) unit = most, most_unit = 0.f;
           else if (most > unit * 128.f || (most > 0.f && most * 0x1p14f < unit)) unit = fmaxf(most, most_unit * 0x1p-60f);
+          unit = fminf(fmaxf(unit, 0x1p-126f), kLargestUnit);
           most_unit = fmaxf(most_unit, unit);
           Fp8Tile& tile = *reinterpret_cast<Fp8Tile*>(base_ptr + G::OFF_TILES + (t & 3) * sizeof(Fp8Tile));
           if (lane < 4) {
-            const float ratio = unit > 0.f ? v / unit : 0.f;
+            const float ratio = mul_subnormal(v, 1.f / unit);
             tile.k[g] = k;
             asm("cvt.rn.f16x2.f32 %0, %1, %1;" : "=r"(tile.v[g]) : "f"(ratio));
             if (g == 0) {
@@ -521,7 +523,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         float ks[4];
         *reinterpret_cast<float4*>(ks) = *reinterpret_cast<const float4*>(tile.k);
         const float change = tile.change;
-        unit = tile.unit;  // goes on with the row's sum: the record is the next tiles' once P is reported
+        unit = tile.unit;  // goes on with the rows' sums: the record is the next tiles' once P is reported
 #pragma unroll
         for (int g = 0; g < 4; ++g) ks[g] = fmaxf(ks[g] * factor, 0x1p-126f);  // not zero, which -inf of a masked score must not meet
         const int j0 = (x.first + j) * BN;
@@ -600,10 +602,11 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       // what takes O to the result, or to its part of it, goes to the row warps; no key: zeros; a sum that is NaN stays one
       float by = l > 0.f ? 1.f / l : l;
       if (SPLIT && *parts_of_item > 1) {
-        p.ws_ml[static_cast<int64_t>(blockIdx.x) * BM + r] = make_float2(m_used, l);
-        by = 1.f;
+        by = 1.f / (1 << static_cast<int>(kWeightBits));  // sums of large values end where fp32 does as it is
+        p.ws_ml[static_cast<int64_t>(blockIdx.x) * BM + r] = make_float2(m_used, l * by);
       }
-      inv_buf[(it & 1) * 128 + r] = by * unit;
+      inv_buf[(it & 1) * 128 + r] = by;
+      if (r == 0) unit_buf[it & 1] = unit;
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(bar(EPI_FULL0 + (it & 1)));
@@ -716,7 +719,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
       return true;
     };
     // A part of an item's keys: O in 32 bits goes to the workspace, four columns of all rows side by side.
-    auto set_aside = [&](const Fp8Item& x, float unit) {
+    auto set_aside = [&](const Fp8Item& x, float by, float unit) {
       const int rows = min(BMT, x.Lq - x.m0) * pack;
       float4* mine = p.ws_o + static_cast<int64_t>(blockIdx.x) * (D / 4) * BM + r;
 #pragma unroll 1
@@ -727,8 +730,8 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         if (r < rows) {
 #pragma unroll
           for (int k = 0; k < 32; k += 4)
-            mine[(c * 8 + k / 4) * BM] = make_float4(__uint_as_float(o[k]) * unit, __uint_as_float(o[k + 1]) * unit,
-                                                     __uint_as_float(o[k + 2]) * unit, __uint_as_float(o[k + 3]) * unit);
+            mine[(c * 8 + k / 4) * BM] = make_float4(__uint_as_float(o[k]) * by * unit, __uint_as_float(o[k + 1]) * by * unit,
+                                                     __uint_as_float(o[k + 2]) * by * unit, __uint_as_float(o[k + 3]) * by * unit);
         }
       }
       return true;
@@ -737,10 +740,10 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
     // with the row's sum.
     auto results = [&](const Fp8Item& x, int done, int last) {
       if (!wait_or_abort(bar(EPI_FULL0 + (done & 1)), (done >> 1) & 1, abort_flag)) return false;
-      const float inv = inv_buf[(done & 1) * 128 + r];
+      const float inv = inv_buf[(done & 1) * 128 + r], unit = unit_buf[done & 1];  // one after the other: their product may be subnormal
       if (!wait_or_abort(bar(PV_DONE0 + (last & 1)), (last >> 1) & 1, abort_flag)) return false;
       tc_fence_after();
-      if (SPLIT && *parts_of_item > 1) return set_aside(x, inv);
+      if (SPLIT && *parts_of_item > 1) return set_aside(x, inv, unit);
       // O / l -> bf16, 32 columns at a time through this warp's patch of shared memory
       const int srow = lane >> 2, spiece = lane & 3;
       __nv_bfloat16* out_tile = p.out + static_cast<int64_t>(x.q0 + x.m0) * p.out_stride + x.h * D;
@@ -758,10 +761,10 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint4 v;
-          v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv);
-          v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv);
-          v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv);
-          v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv);
+          v.x = pack_bf16x2(__uint_as_float(o[8 * k]) * inv * unit, __uint_as_float(o[8 * k + 1]) * inv * unit);
+          v.y = pack_bf16x2(__uint_as_float(o[8 * k + 2]) * inv * unit, __uint_as_float(o[8 * k + 3]) * inv * unit);
+          v.z = pack_bf16x2(__uint_as_float(o[8 * k + 4]) * inv * unit, __uint_as_float(o[8 * k + 5]) * inv * unit);
+          v.w = pack_bf16x2(__uint_as_float(o[8 * k + 6]) * inv * unit, __uint_as_float(o[8 * k + 7]) * inv * unit);
           *reinterpret_cast<uint4*>(stage + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = v;
         }
         __syncwarp();

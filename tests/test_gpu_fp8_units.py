@@ -164,3 +164,33 @@ def test_nan_in_keys_in_parts(cuda, hq, hkv, d):
             whole = ~want[:, heads]
             assert_within(got[:, heads][whole], ref[whole], bound[whole], f"KV head {h}")
     assert _lib.read_status() == 0
+
+
+@pytest.mark.parametrize("n", [70, 900, 4000])
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (14, 2, 64)])
+def test_scales_from_the_smallest_to_the_largest(cuda, hq, hkv, d, n):
+    """V's scales anywhere in fp32's range, subnormal ones too, in decode and in prefill with keys whole and in parts; results that
+    are normal numbers are as right as any."""
+    g = torch.Generator().manual_seed(n)
+    blocks = 2 * -(-n // 256)
+    planes, tables = random_planes(g, blocks, hkv, d, spread=0.3), tables_for(g, [n, n], blocks)
+    k, v, ks, vs = planes
+    vs = vs.double() / vs.max()
+    q = torch.randn(2, hq, d, generator=g).bfloat16()
+    ctx, cu_q = torch.tensor([n, n], dtype=torch.int32), torch.arange(3, dtype=torch.int32)
+    few = (v & 0x87)  # the smallest codes, for the largest scales
+    for exponent, codes in [(e, v) for e in (0, -64, -100, -118, -126, -130, -140, 64, 100, 110)] + [(127, few)]:
+        now = (k, codes, ks, (vs * 2.0 ** exponent).float())
+        ref, bound = prefill_reference(q, now, cu_q, cu_q * n, tables, 0.1)
+        # a few terms and the result may be flushed to zero, 2^-126 each; V over a unit with a scale that is no power of two
+        # is rounded twice
+        bound = bound * (1 + 4 / 3) + 2.0 ** -123
+        dev = planes_on(cuda, *now)
+        outs = [A.decode_paged_fp8(q.to(cuda), *dev, ctx.to(cuda), tables.to(cuda), 0.1)]
+        for batch in (1, 150):  # 150 of them, of the same two sequences: keys whole
+            rows = torch.arange(2).repeat(batch)
+            many = torch.arange(2 * batch + 1, dtype=torch.int32)
+            outs.append(A.prefill_varlen_fp8(q[rows].to(cuda), *dev, many.to(cuda), (many * n).to(cuda), 1, n, 0.1, tables[rows].to(cuda))[-2:])
+        for out in outs:
+            assert_within(out.double().cpu() * 2.0 ** -exponent, ref * 2.0 ** -exponent, bound * 2.0 ** -exponent, f"2^{exponent}")
+    assert _lib.read_status() == 0
