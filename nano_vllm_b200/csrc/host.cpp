@@ -10,17 +10,19 @@
 // include/nvllm_b200.h from the library that the ctypes loader opened (bind), raises what the
 // Python code raised (AssertionError for layout, RuntimeError for device and dtype, NvllmError for
 // an argument the library refused), and never touches the device except through those functions,
-// torch's allocator, and one event per staged decode step.
+// torch's allocator, one event per staged decode step, and a user object on a graph that holds decode scratch.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <cuda_runtime_api.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <atomic>
 #include <cstring>
 #include <limits>
 #include <memory>
@@ -148,38 +150,89 @@ int64_t rows_in(const at::Tensor& t, int64_t row_elems) { return row_elems > 0 ?
 PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }
 
 // ---- decode scratch ---------------------------------------------------------------------
-// One buffer per device, grown on demand and zero-filled when it is made: its head holds the
-// arrival counters of the decode kernel, which must start at zero and which every completed
-// call leaves at zero.  Outgrown buffers are kept alive because CUDA graphs captured earlier
-// still hold their addresses.
-std::vector<at::Tensor> g_workspaces, g_retired;
+// Zero-filled when it is made: its head holds the arrival counters of the decode kernels, which must start at zero and which
+// every completed call leaves at zero.  Launches that may run at the same time must not meet in one buffer, so every stream
+// has one, grown on demand, and so has every stream of a capture: graphs run when and where their owner launches them.  A
+// graph's buffers go to later captures once the last of it is gone.
+struct Scratch {
+  at::Tensor buffer;
+  c10::DeviceIndex device;
+  cudaStream_t stream;
+  unsigned long long capture;  // 0: of the stream's own launches; else 1 + the capture's id
+  std::atomic<bool>* held;     // of a capture: whether its graph lives
+};
+std::vector<Scratch> g_scratch;
 
-void workspace(const at::Tensor& like, int64_t nbytes, void** p, int64_t* size) {
-  *p = nullptr;
-  *size = 0;
-  if (nbytes == 0) return;
-  const size_t dev = static_cast<size_t>(like.device().index());
-  if (g_workspaces.size() <= dev) g_workspaces.resize(dev + 1);
-  auto enough = [&] { return g_workspaces[dev].defined() && g_workspaces[dev].numel() >= nbytes; };
-  if (!enough()) {
-    at::Tensor fresh = unlocked([&] { return at::zeros({std::max<int64_t>(nbytes, 1 << 20)}, like.options().dtype(at::kByte)); });
-    if (!enough()) {  // not grown by another thread meanwhile
-      if (g_workspaces[dev].defined()) g_retired.push_back(g_workspaces[dev]);
-      g_workspaces[dev] = std::move(fresh);
-    }
-  }
-  const at::Tensor& ws = g_workspaces[dev];
-  *p = ws.data_ptr();
-  *size = ws.numel();
+// `held` is true until `graph` and all that is instantiated from it have been destroyed and have finished; for good if the
+// driver cannot tell.
+void hold(cudaGraph_t graph, std::atomic<bool>* held) {
+  held->store(true);
+  cudaUserObject_t object;
+  const auto gone = [](void* p) { static_cast<std::atomic<bool>*>(p)->store(false); };
+  if (graph && cudaUserObjectCreate(&object, held, gone, 1, cudaUserObjectNoDestructorSync) == cudaSuccess)
+    (void)cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  (void)cudaGetLastError();
 }
 
-// Zeroes the current device's buffers, outgrown ones too (after a launch whose waits ran out), and waits for that.
+// Zeros that a graph is given while it is captured: filled now and outside of it, by a stream that nobody captures.
+at::Tensor zeros_beside_capture(int64_t nbytes, const at::TensorOptions& options, c10::DeviceIndex device) {
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  c10::cuda::CUDAStream side = c10::cuda::getStreamFromPool(false, device);
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  for (int i = 0; i < 64 && cudaStreamIsCapturing(side.stream(), &status) == cudaSuccess && status != cudaStreamCaptureStatusNone; ++i)
+    side = c10::cuda::getStreamFromPool(false, device);
+  const c10::cuda::CUDAStreamGuard on(side);
+  at::Tensor t = at::zeros({nbytes}, options);
+  side.synchronize();
+  return t;
+}
+
+at::Tensor workspace(const at::Tensor& like, int64_t nbytes) {
+  if (nbytes == 0) return {};
+  const c10::DeviceIndex device = like.device().index();
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_of(like));
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long capture = 0;
+  cudaGraph_t graph = nullptr;
+  if (cudaStreamGetCaptureInfo(stream, &status, &capture, &graph) != cudaSuccess) (void)cudaGetLastError();  // 0.1 us
+  const bool captured = status != cudaStreamCaptureStatusNone;
+  capture = captured ? capture + 1 : 0;
+  auto mine = [&](const Scratch& s) { return s.device == device && s.stream == stream && s.capture == capture; };
+  auto find = [&]() -> Scratch* {
+    for (Scratch& s : g_scratch)
+      if (mine(s) && s.buffer.numel() >= nbytes) return &s;
+    return nullptr;
+  };
+  if (Scratch* s = find()) return s->buffer;
+  if (captured)
+    for (Scratch& s : g_scratch)
+      if (s.held && !s.held->load() && s.device == device && s.buffer.numel() >= nbytes) {
+        s.stream = stream;
+        s.capture = capture;
+        hold(graph, s.held);
+        return s.buffer;
+      }
+  const int64_t size = std::max<int64_t>(nbytes, 1 << 20);
+  const at::TensorOptions bytes = like.options().dtype(at::kByte);
+  at::Tensor fresh = unlocked([&] { return captured ? zeros_beside_capture(size, bytes, device) : at::zeros({size}, bytes); });
+  if (captured) {
+    g_scratch.push_back({fresh, device, stream, capture, new std::atomic<bool>(true)});
+    hold(graph, g_scratch.back().held);
+    return fresh;
+  }
+  if (Scratch* s = find()) return s->buffer;  // another thread has grown it meanwhile
+  for (Scratch& s : g_scratch)
+    if (mine(s)) return s.buffer = fresh;  // what it outgrew was the stream's, and launches on it come before any other use
+  g_scratch.push_back({fresh, device, stream, 0, nullptr});
+  return fresh;
+}
+
+// Zeroes the current device's buffers (after a launch whose waits ran out), and waits for that.
 PyObject* clear_workspaces(PyObject* const*) {
   const c10::DeviceIndex dev = c10::cuda::current_device();
-  std::vector<at::Tensor> all = g_workspaces;
-  all.insert(all.end(), g_retired.begin(), g_retired.end());
-  for (const at::Tensor& ws : all)
-    if (ws.defined() && ws.device().index() == dev) ws.zero_();
+  const std::vector<Scratch> all = g_scratch;
+  for (const Scratch& s : all)
+    if (s.device == dev) at::Tensor(s.buffer).zero_();
   const c10::cuda::CUDAStream st = c10::cuda::getCurrentCUDAStream(dev);
   unlocked([&] { st.synchronize(); });
   Py_RETURN_NONE;
@@ -233,9 +286,9 @@ void decode(const Rows& q, int64_t hq, int64_t d, const at::Tensor& k_cache, con
   const int64_t need = api.decode_workspace_bytes(static_cast<int32_t>(q.n), width, static_cast<int32_t>(hq),
                                                   static_cast<int32_t>(hkv), static_cast<int32_t>(d));
   check(need);
-  void* ws;
-  int64_t ws_size;
-  workspace(k_cache, need, &ws, &ws_size);
+  const at::Tensor scratch = workspace(k_cache, need);
+  void* const ws = scratch.data_ptr();
+  const int64_t ws_size = scratch.numel();
   const int32_t B = static_cast<int32_t>(q.n), HQ = static_cast<int32_t>(hq), HKV = static_cast<int32_t>(hkv),
                 D = static_cast<int32_t>(d);
   void* st = stream_of(k_cache);
@@ -464,9 +517,9 @@ void decode_fp8(const Rows& q, int64_t hq, const Fp8Planes& c, const at::Tensor&
                 D = static_cast<int32_t>(c.d), width = static_cast<int32_t>(block_tables.size(1));
   const int64_t need = api.decode_workspace_bytes(B, width, HQ, HKV, D);
   check(need);
-  void* ws;
-  int64_t ws_size;
-  workspace(like, need, &ws, &ws_size);
+  const at::Tensor scratch = workspace(like, need);
+  void* const ws = scratch.data_ptr();
+  const int64_t ws_size = scratch.numel();
   void* st = stream_of(like);
   launch([&] {
     if (step)
