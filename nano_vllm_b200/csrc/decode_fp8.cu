@@ -315,8 +315,9 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     };
     int64_t blk = block_at(0);
     float scale = scale_of(blk, (u0 - cc.first) * UNIT);
+    int j = 0;
 #pragma unroll 1
-    for (int j = 0; j < n_units; ++j) {
+    for (; j < n_units; ++j) {
       const int unit0 = (u0 + j - cc.first) * UNIT;
       if (j >= NST && !__all_sync(ALL, sm100::mbar_wait(free(j), (j / NST - 1) & 1))) {
         bad |= NVLLM_STATUS_TIMEOUT;
@@ -344,6 +345,10 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(full(j));
     }
+    // No copy is in flight when the block ends, whether or not the others have waited for it.
+#pragma unroll 1
+    for (int i = max(j - NST, 0); i < j; ++i)
+      if (!sm100::mbar_wait(full(i), (i / NST) & 1)) bad |= NVLLM_STATUS_TIMEOUT;
     if (bad && lane == 0) atomicOr(p.status, bad);
     return;
   }
@@ -620,12 +625,12 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       load_q(qn, qn_b);
       if (STEP) next_row = load_new(qn_b);
     }
-    // A wait that ran out: nothing more is waited for or stored, but all barriers that the other warps count on are met.  (A vote
-    // here, to skip the tiles too, costs 3 % of the launch.)
+    // A wait that ran out: nothing more is waited for or stored, and no stage is given back, so that the loading warp stops too; but all
+    // barriers that the other warps count on are met.  (A vote here, to skip the tiles too, costs 3 % of the launch.)
     if (!(bad & NVLLM_STATUS_TIMEOUT) && !sm100::mbar_wait(full(i), (i / NST) & 1)) bad |= NVLLM_STATUS_TIMEOUT;
     const int t0 = (u - cc.first) * UNIT + warp * TT;
     if (t0 >= cc.ctx) {
-      if (lane == 0) sm100::mbar_arrive(free(i));
+      if (lane == 0 && !(bad & NVLLM_STATUS_TIMEOUT)) sm100::mbar_arrive(free(i));
       continue;
     }
     const uint32_t kbase = warp_tile + (i % NST) * C::STAGE_BYTES, vbase = kbase + C::UNIT_BYTES;
@@ -777,7 +782,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       }
     }
     __syncwarp();  // everything of the unit is in registers
-    if (lane == 0) sm100::mbar_arrive(free(i));
+    if (lane == 0 && !(bad & NVLLM_STATUS_TIMEOUT)) sm100::mbar_arrive(free(i));
   }
   bad = __reduce_or_sync(ALL, bad);
   if (bad && lane == 0) atomicOr(p.status, bad);

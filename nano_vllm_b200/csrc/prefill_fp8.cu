@@ -298,11 +298,10 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         T += x.n_kv;
         if (lane == 0) mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
       }
-      if (!ok) {  // gave up: no copy is in flight when the block ends
+      // no copy is in flight when the block ends, whoever gave up
 #pragma unroll 1
-        for (int t = max(loaded - 2, 0); t < loaded; ++t) (void)mbar_wait(bar(K_FULL0 + (t & 1)), (t >> 1) & 1);
-        if (rows_loaded > 0) (void)mbar_wait(bar(ROWS_FULL), (rows_loaded - 1) & 1);
-      }
+      for (int t = max(loaded - 2, 0); t < loaded; ++t) (void)mbar_wait(bar(K_FULL0 + (t & 1)), (t >> 1) & 1);
+      if (rows_loaded > 0) (void)mbar_wait(bar(ROWS_FULL), (rows_loaded - 1) & 1);
     } else if (warp == 10) {
       // ---------------------------------------------------------------- TMA of V
       if (elect_one()) {
@@ -329,10 +328,8 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
           T += x.n_kv;
           mbar_arrive(bar(ITEM_FREE0 + (it & 1)));
         }
-        if (!ok) {
 #pragma unroll 1
-          for (int t = max(loaded - 2, 0); t < loaded; ++t) (void)mbar_wait(bar(RAW_FULL0 + (t & 1)), (t >> 1) & 1);
-        }
+        for (int t = max(loaded - 2, 0); t < loaded; ++t) (void)mbar_wait(bar(RAW_FULL0 + (t & 1)), (t >> 1) & 1);
       }
     } else if (warp == 9) {
       // ---------------------------------------------------------------- MMA issuer
