@@ -42,11 +42,11 @@ constexpr int NTHREADS = 384;
 constexpr int REGS_LAUNCH = 80, REGS_SOFTMAX = 136, REGS_ROWS = 64, REGS_OTHER = 40;
 static_assert(128 * (REGS_SOFTMAX + REGS_ROWS + REGS_OTHER) <= NTHREADS * REGS_LAUNCH, "register pool of a block");
 constexpr int TMEM_COLS = 256, TMEM_O = 128;  // S / P buffers [0,64) and [64,128), O [128,256)
-// Log2 units: P is 2^8 where a score is the maximum in use, which is kept until one is 2^7 times larger; f16 goes to 2^16.  (P from 1 on,
-// and 2^14, lost all that 131072 keys 18 nats below a first one have.)  Where a row outgrows its maximum, its warp's other rows go to
-// theirs too: 4 x 4096 tokens (16 heads over 8 of 128, scores of 2.2 nats) one call after the other 380 -> 365 us; thresholds of 8, 6 and 5
-// are 362, 370 and 367, 14 is 349.  (14 for an item's first 1024 keys alone is 358, and loses 2^-26 of the largest on each of those.)
-constexpr float kWeightBits = 8.f, kRescaleThreshold = 7.f;
+// Log2 units: P is 2^8 where a score is the maximum in use, which is kept until one is 2^7.9 times larger; f16 goes to 2^16.  (P from 1
+// on, and 2^14, lost all that 131072 keys 18 nats below a first one have.)  Where a row outgrows its maximum, its warp's other rows go
+// to theirs too.  4 x 4096 tokens (16 heads over 8 of 128, scores of 2.2 nats), one call after the other: 367 us; rows each for itself
+// 380; 2^7 370, 2^5 371, 2^14 355.  (2^14 for an item's first 512 keys alone is 361, and loses 2^-26 of the largest on each of those.)
+constexpr float kWeightBits = 8.f, kRescaleThreshold = 7.9f;
 enum Bar {
   Q_FULL, K_FULL0, K_FULL1, RAW_FULL0, RAW_FULL1, RAW_FREE0, RAW_FREE1, V_FULL0, V_FULL1, QK_DONE0, QK_DONE1, PV_DONE0, PV_DONE1,
   P_FULL0, P_FULL1, ITEM_FULL0, ITEM_FULL1, ITEM_FREE0, ITEM_FREE1, O_FREE, EPI_FULL0, EPI_FULL1,
