@@ -208,7 +208,10 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     // No more ranges than units, and where sequences are few no more than balance the two costs of a cut: a range streams
     // total / n units and a sequence's merge reads n / batch partials.
     n_ranges = max(1, min(min(p.n_ranges, total), static_cast<int>(sqrtf(kFp8SplitBalance * total * p.batch))));
-    if (p.batch == 1 && total <= 4) n_ranges = 1;  // a unit more takes less than a merge: 317 tokens 6.7 -> 6.4 us
+    // Two units one after the other take less than a merge, three and four do not: one sequence of 200 tokens (16 / 8 heads of 128) 4.35 us,
+    // cut 5.3; 317 5.3, 5.35; 512 6.5, 5.35; its step 5.0, 5.6; 6.0, 5.6; 7.15, 5.75.  Of 512, 600, 900 (14 / 2 of 64) 4.1, 5.05; 5.0, 5.15; 5.95,
+    // 5.2.
+    if (p.batch == 1 && total <= 2) n_ranges = 1;
     if (range >= n_ranges || total == 0) return false;  // block-uniform
     per_range = total / n_ranges, longer = total - per_range * n_ranges;  // the first `longer` ranges hold one more
     u0 = range * per_range + min(range, longer), u1 = u0 + per_range + (range < longer ? 1 : 0);
