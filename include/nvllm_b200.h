@@ -295,7 +295,8 @@ NVLLM_API int nvllm_store_kvcache_fp8(const void* key, int64_t key_row_stride, c
 
 /*
  * nvllm_decode_paged over an 8-bit cache: same arguments, limits, workspace and rules, with the scales beside the codes.  Query
- * and P are rounded to f16 (the query scaled by a power of two per head), sums are fp32.
+ * and P are rounded to f16 (the query scaled by a power of two per head, P to an upper end of 2^15), sums are fp32: a weight is off by
+ * 2^-11 of itself, or by 2^-35 of the largest where that is more.
  */
 NVLLM_API int nvllm_decode_paged_fp8(const void* q, int64_t q_row_stride, const void* k_cache, const void* v_cache,
                            const float* k_scale, const float* v_scale, const int32_t* context_lens,
@@ -322,7 +323,9 @@ NVLLM_API int nvllm_decode_step_fp8(const void* q, int64_t q_row_stride, const v
  * nvllm_prefill_varlen over an 8-bit cache, through the block table: same masks, same rules for rows without a key and for what lies
  * behind a sequence's end.  total_q: rows of q and out.  max_seqlen_q / max_seqlen_k: at least the longest.  Queries are
  * taken as sums of two e4m3 numbers (all of bf16's bits down to 2^-10 of a row's largest value, an error of at most 2^-17 of
- * that below), P is rounded to f16, sums are fp32.  batch <= 1024; scale >= 0.
+ * that below), P is rounded to f16 (a weight is off by 2^-11 of itself, or by 2^-33 of the largest where that is more), sums are fp32.
+ * NaN in V of one of a sequence's tokens may reach, in its column, rows of a query tile that do not see the token.
+ * batch <= 1024; scale >= 0.
  * `workspace`: nvllm_prefill_fp8_workspace_bytes(...) bytes for the same sizes on the current device, 16-byte aligned; it may be
  * nvllm_decode_paged's (calls that share one must not overlap).  With it, few new tokens behind long prefixes have their keys
  * split over the GPU; without (NULL) they have not, and the results are as good.

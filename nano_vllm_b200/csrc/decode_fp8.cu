@@ -4,13 +4,14 @@
 //
 // The step variant also does what store_kvcache_fp8 does for the one new token of every sequence.
 //
-// Bound by the cached bytes, half of a bf16 cache's: 128 sequences of 1024-8192 tokens (32 / 8 heads of 128) 184 us, 6.4 TB/s
-// (bf16: 363), 180 with nothing computed.  The launch is cut as the bf16 decode's is (decode_paged.cu): all sequences' work units
+// Bound by the cached bytes, half of a bf16 cache's: 128 sequences of 1024-8192 tokens (32 / 8 heads of 128) 185 us, 6.4 TB/s
+// (bf16: 363), 180 with nothing computed; launch after launch, with the power cap on the clocks, 204.  The launch is cut as the bf16 decode's is (decode_paged.cu): all sequences' work units
 // in one list, an equal stretch of it to each of two resident blocks per SM, partial results of sequences that a cut
 // divides merged by the last block to arrive.  What differs is what a tile costs:
 //   * A warp of its own loads: table entries, tiles by TMA (a box for every warp's tile that holds a token), scales.  When the
 //     four others did that themselves, with cp.async, they spent half of their instructions on it; a barrier of the block
-//     for every unit instead was slower (128 sequences 199 -> 214 us, loading warp 184; 60 of 100-1024 21.5, 23.3, 18.3).
+//     for every unit instead was slower (128 sequences 199 -> 214 us, loading warp 184; 60 of 100-1024 21.5, 23.3, 18.3,
+//     all before merges of few parts had code of their own).
 //   * K codes go from shared memory to registers 16 bytes a lane and become f16 pairs there (cvt, exact, two cycles).  The four
 //     codes of a word are columns k = 2 tig .. and k = 2 tig + 8 .. of one m16n8k16 product: the order of the summed index
 //     is free, the query's columns follow it.
@@ -28,7 +29,7 @@
 // Small batches are bound by trips one after the other: lengths and split (0.7 us), table entry, tiles, the products of a tile
 // (0.7), flush (0.6), arrival (0.8), merge (of two to four parts 1.5 us by short code of its own, by that for any number 3).  The
 // first three run ahead of the wait for the previous kernel and are verified behind it (a sequence of 317 tokens 7.1 -> 6.7 us
-// in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6; now 5.9, 17.6 and 18.2).
+// in a chain, 60 of 100-1024 23.1 -> 22.4, two of 100000 (head_dim 64) 20 -> 18.6; with all that came later 5.5, 17.6 and 18.2).
 #include "fp8.cuh"
 #include "sm100.cuh"
 
@@ -736,7 +737,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     l0 *= alpha0;
     l1 *= alpha1;
     if (most_vs > unit * kFp8UnitUp || (most_vs * kFp8UnitDown < unit && unit > least_unit && most_vs > 0.f)) {
-      const float next = fminf(fmaxf(fmaxf(most_vs, most_unit * 0x1p-60f), least_unit), kLargestUnit), change = unit / next;
+      const float next = fminf(fmaxf(fmaxf(most_vs, most_unit * 0x1p-60f), least_unit), kLargestUnit), change = next != unit ? unit / next : 1.f;
       alpha0 *= change;
       alpha1 *= change;
       unit = next;

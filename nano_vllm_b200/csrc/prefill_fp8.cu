@@ -23,9 +23,10 @@
 // counter in memory, so nothing is shared by launches.  Where there are two blocks or more to an item (few new tokens behind a
 // long prefix) an item's keys go to several of them (SPLIT), and prefill_fp8_join sums the parts up from the workspace.
 //
-// 4 x 4096 tokens (16 heads over 8 of 128): 318 us at full clocks, 860 TFLOP/s; 12 sequences of 100-2000 tokens behind 256-4096 (14
-// over 2 of 64): 200.  Bound by the chain scores - softmax - P - product of a block, of which two to an SM overlap: without
-// the exponentials 8 % less, without V's conversion 11 and 9, without rescaling O 5 and 6; the tensor cores are busy 42 % of the time.
+// 4 x 4096 tokens (16 heads over 8 of 128) at full clocks: 299 us, 920 TFLOP/s, where scores are nearly flat, 353 where they spread by
+// 2.2 nats with long tails; 12 sequences of 100-2000 tokens behind 256-4096 (14 over 2 of 64) 217 us.  Bound by the chain scores -
+// softmax - P - product of a block, of which two to an SM overlap: of the 353 and 217, leaving out V's conversion saves 40 and 20, rescaling
+// O 27 and 15, the exponentials 18 and 14; the tensor cores are busy 41 % of the time.
 #include <algorithm>
 
 #include "fp8.cuh"
