@@ -325,6 +325,7 @@ NVLLM_API int nvllm_decode_step_fp8(const void* q, int64_t q_row_stride, const v
  * taken as sums of two e4m3 numbers (all of bf16's bits down to 2^-10 of a row's largest value, an error of at most 2^-17 of
  * that below), P is rounded to f16 (a weight is off by 2^-11 of itself, or by 2^-33 of the largest where that is more), sums are fp32.
  * NaN in V of one of a sequence's tokens may reach, in its column, rows of a query tile that do not see the token.
+ * |scale * q . K| up to 2^26: beyond, results are finite but may be too small.
  * batch <= 1024; scale >= 0.
  * `workspace`: nvllm_prefill_fp8_workspace_bytes(...) bytes for the same sizes on the current device, 16-byte aligned; it may be
  * nvllm_decode_paged's (calls that share one must not overlap).  With it, few new tokens behind long prefixes have their keys

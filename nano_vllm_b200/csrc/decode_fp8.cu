@@ -133,8 +133,8 @@ struct Fp8Cut {  // a sequence whose units lie in several ranges: n of them, fro
 // 8192 tokens (32 / 8 heads of 128) 9.9, 9.6, 8.8, 9.4 us, two of 2000 (16 / 8) 7.4, 7.5, 6.6, 6.6, two of 110000 (14 / 2 of 64) 20, 16.6,
 // 16.1, 16.1.
 constexpr float kFp8SplitBalance = 16.f;
-// P's largest in log2 units, and how far V's scales may go from the unit of O: their product stays in f16, which ends at 2^16.
-constexpr float kFp8WeightBits = 12.f, kFp8UnitUp = 8.f, kFp8UnitDown = 4.f;
+// What goes on P, and how far V's scales may go from the unit of O: their product stays in f16, which ends at 2^16.
+constexpr float kFp8Weight = 0x1p12f, kFp8UnitUp = 8.f, kFp8UnitDown = 4.f;
 
 template <class C, bool STEP>
 __global__ void __launch_bounds__(C::NTHREADS, C::BLOCKS)
@@ -450,10 +450,7 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       l0 += __shfl_xor_sync(ALL, l0, sh);
       l1 += __shfl_xor_sync(ALL, l1, sh);
     }
-    // without the 2^12: the sums of large values end where fp32 does as it is
-    constexpr float back = 1.f / (1 << static_cast<int>(kFp8WeightBits));
-    l0 *= back, l1 *= back;
-    const float by = unit * back;
+    const float by = unit * (1.f / kFp8Weight);
     sync_warps();  // the previous merge has been read by everyone
 #pragma unroll
     for (int c = 0; c < C::KS; ++c) {
@@ -715,10 +712,10 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
       vs[mt] = t0 + mt * 16 < cc.ctx ? ld_shared_f32(scales + (C::UNIT_GROUPS + mt) * 4) : 0.f;  // a group past the end: whatever is there
       most_vs = fmaxf(most_vs, vs[mt]);
       const float f0 = qk0 * ks, f1 = qk1 * ks;
-      s[mt][0] *= f0;
-      s[mt][1] *= f1;
-      s[mt][2] *= f0;
-      s[mt][3] *= f1;
+      s[mt][0] = __fmul_rn(s[mt][0], f0);  // rounded here: the largest minus the maximum is zero, however large the scores are
+      s[mt][1] = __fmul_rn(s[mt][1], f1);
+      s[mt][2] = __fmul_rn(s[mt][2], f0);
+      s[mt][3] = __fmul_rn(s[mt][3], f1);
       if (tail) {
         const int tr = t0 + mt * 16 + token_of_row<D>(gid);
         if (tr >= cc.ctx) s[mt][0] = s[mt][1] = -INFINITY;
@@ -746,17 +743,16 @@ decode_fp8_kernel(const DecodeFp8Params p, const __grid_constant__ CUtensorMap t
     const float per_unit = 1.f / unit;
     m0 = mn0;
     m1 = mn1;
-    const float top0 = mn0 - kFp8WeightBits, top1 = mn1 - kFp8WeightBits;  // sums of P carry 2^12 as O does
     uint32_t pb[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      s[mt][0] = fast_exp2(s[mt][0] - top0);
-      s[mt][1] = fast_exp2(s[mt][1] - top1);
-      s[mt][2] = fast_exp2(s[mt][2] - top0);
-      s[mt][3] = fast_exp2(s[mt][3] - top1);
+      s[mt][0] = fast_exp2(s[mt][0] - mn0);
+      s[mt][1] = fast_exp2(s[mt][1] - mn1);
+      s[mt][2] = fast_exp2(s[mt][2] - mn0);
+      s[mt][3] = fast_exp2(s[mt][3] - mn1);
       l0 += s[mt][0] + s[mt][2];  // per-lane partial sums; reduced over the token lanes at the flush
       l1 += s[mt][1] + s[mt][3];
-      const float f = mul_subnormal(vs[mt], per_unit);
+      const float f = mul_subnormal(vs[mt], per_unit) * kFp8Weight;
       pb[mt][0] = movmatrix_trans(pack_f16x2(s[mt][0] * f, s[mt][1] * f));
       pb[mt][1] = movmatrix_trans(pack_f16x2(s[mt][2] * f, s[mt][3] * f));
     }

@@ -45,9 +45,11 @@ static_assert(128 * (REGS_SOFTMAX + REGS_ROWS + REGS_OTHER) <= NTHREADS * REGS_L
 constexpr int TMEM_COLS = 256, TMEM_O = 128;  // S / P buffers [0,64) and [64,128), O [128,256)
 // Log2 units: P is 2^8 where a score is the maximum in use, which is kept until one is 2^7.9 times larger; f16 goes to 2^16.  (P from 1
 // on, and 2^14, lost all that 131072 keys 18 nats below a first one have.)  Where a row outgrows its maximum, its warp's other rows go
-// to theirs too.  4 x 4096 tokens (16 heads over 8 of 128, scores of 2.2 nats), one call after the other: 367 us; rows each for itself
+// to theirs too.  4 x 4096 tokens (16 heads over 8 of 128, scores of 2.2 nats), one call after the other: 366 us; rows each for itself
 // 380; 2^7 370, 2^5 371, 2^14 355.  (2^14 for an item's first 512 keys alone is 361, and loses 2^-26 of the largest on each of those.)
-constexpr float kWeightBits = 8.f, kRescaleThreshold = 7.9f;
+// The multiply-subtract below does not round a score as the maximum was, so a large score's rounding comes off the threshold: P
+// stays within f16 for scores up to 2^27, and is cut to its end beyond.  (Scores rounded alike where they are that large: 371 us.)
+constexpr float kWeightBits = 8.f, kRescaleThreshold = 7.9f, kScoreRounding = 0x1p-23f;
 enum Bar {
   Q_FULL, K_FULL0, K_FULL1, RAW_FULL0, RAW_FULL1, RAW_FREE0, RAW_FREE1, V_FULL0, V_FULL1, QK_DONE0, QK_DONE1, PV_DONE0, PV_DONE1,
   P_FULL0, P_FULL1, ITEM_FULL0, ITEM_FULL1, ITEM_FREE0, ITEM_FREE1, O_FREE, EPI_FULL0, EPI_FULL1,
@@ -545,7 +547,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
         }
         const float m_new = fmaxf(m_used, mx);
         // lazy rescale: the old reference maxima stay until one of the warp has been outgrown by the threshold; then all follow
-        if (change != 1.f || __any_sync(ALL, m_new > m_used + kRescaleThreshold)) {
+        if (change != 1.f || __any_sync(ALL, m_new - m_used > fmaf(fabsf(m_new), -kScoreRounding, kRescaleThreshold))) {
           float alpha = 1.f;
           if (m_new > m_used) {
             alpha = (m_used == -INFINITY) ? 0.f : fast_exp2(m_used - m_new);
@@ -580,7 +582,7 @@ prefill_fp8_kernel(const PrefillFp8Params p, const __grid_constant__ CUtensorMap
             unpack2(fma2(pack2(__uint_as_float(s[2 * c]), __uint_as_float(s[2 * c + 1])), scale2, nmsub2), a0, a1);
             const float p0 = fast_exp2(a0), p1 = fast_exp2(a1);
             sum2[c & 1] = add2(sum2[c & 1], pack2(p0, p1));
-            asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(s[c]) : "f"(p1), "f"(p0));
+            asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(s[c]) : "f"(p1), "f"(p0));
           }
         }
         {

@@ -194,3 +194,39 @@ def test_scales_from_the_smallest_to_the_largest(cuda, hq, hkv, d, n):
         for out in outs:
             assert_within(out.double().cpu() * 2.0 ** -exponent, ref * 2.0 ** -exponent, bound * 2.0 ** -exponent, f"2^{exponent}")
     assert _lib.read_status() == 0
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(4, 2, 128), (14, 2, 64)])
+def test_scores_of_millions(cuda, hq, hkv, d):
+    """Scores so large that their own rounding is a good part of a binade of a weight, and more: results stay within the values attended,
+    and are the value of a key that is clearly above all others."""
+    g = torch.Generator().manual_seed(hq)
+    n, rows, group = 1700, 40, hq // hkv
+    planes, tables = random_planes(g, 7, hkv, d), tables_for(g, [n], 7)
+    dev, table = planes_on(cuda, *planes), tables.to(cuda)
+    keys, values = (F8.gather(planes[i], planes[2 + i], tables[0], n).repeat_interleave(group, 1) for i in (0, 1))
+    low, high = values.amin(0), values.amax(0)  # [hq, d]
+    slack = 2.0 ** -7 * torch.maximum(low.abs(), high.abs())  # weights and the result are rounded, sums too
+    ctx = torch.full((rows,), n, dtype=torch.int32, device=cuda)
+    seen = torch.arange(n) <= torch.arange(rows)[:, None] + n - rows
+    for exponent in range(8, 19):
+        q = (torch.randn(rows, hq, d, generator=g) * 2.0 ** exponent).bfloat16()  # scores up to 2^(exponent + 10)
+        outs = [(torch.ones(rows, n, dtype=torch.bool), A.decode_paged_fp8(q.to(cuda), *dev, ctx, table.expand(rows, -1).contiguous(), 1.0))]
+        for batch in (1, 20):  # keys in parts; keys whole
+            cu = torch.arange(batch + 1, dtype=torch.int32, device=cuda)
+            out = A.prefill_varlen_fp8(q.repeat(batch, 1, 1).to(cuda), *dev, cu * rows, cu * n, rows, n, 1.0, table.expand(batch, -1).contiguous())
+            outs += [(seen, part) for part in out.view(batch, rows, hq, d)]
+        scores = torch.einsum("qhd,khd->qhk", q.double(), keys)
+        # 32-bit sums and products: 2^-20 of the terms' magnitudes; the prefill's query in two parts: 2^-17 of its largest value
+        error = 2.0 ** -20 * torch.einsum("qhd,khd->qhk", q.double().abs(), keys.abs()).amax(-1)
+        error += 2.0 ** -17 * q.double().abs().amax(-1) * keys.abs().sum(-1).amax(0)
+        for mask, out in outs:
+            out = out.double().cpu()
+            assert ((out >= low - slack) & (out <= high + slack)).all(), f"2^{exponent}"
+            two = scores.masked_fill(~mask[:, None], -torch.inf).topk(2)
+            clear = two.values[..., 0] - two.values[..., 1] > 2 * error + 30
+            clear &= two.values.abs().amax(-1) < 2.0 ** 26
+            assert clear.sum() > rows or exponent > 16
+            want = values.permute(1, 0, 2)[torch.arange(hq), two.indices[..., 0]]
+            assert ((out - want).abs() <= 2.0 ** -7 * want.abs())[clear].all(), f"2^{exponent}"
+    assert _lib.read_status() == 0
