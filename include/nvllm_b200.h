@@ -64,6 +64,7 @@ extern "C" {
 #define NVLLM_STATUS_BAD_BLOCK 2 /* a block_tables entry in use was outside [0,num_blocks) */
 #define NVLLM_STATUS_TIMEOUT 4   /* a bounded in-kernel wait expired; that launch's output is invalid, and a
                                   * decode workspace that it used has to be zero-filled again */
+#define NVLLM_STATUS_BAD_TOKEN 8 /* token_logprobs / head_logprobs saw a token >= vocab (its result is NaN) */
 
 /*
  * Scatter the new tokens' K and V rows into the paged cache.
@@ -432,6 +433,21 @@ NVLLM_API int nvllm_sample_plan(int32_t batch, int32_t vocab, int32_t num_sms, i
 #define NVLLM_SAMPLE_FORMS 6
 NVLLM_API int nvllm_sample_layout(int32_t batch, int32_t vocab, int64_t vocab_offset, int32_t logits_are_fp32, int32_t num_sms,
                                   const int32_t* clusters, int32_t* blocks, int32_t* threads);
+
+/*
+ * Log probabilities of given tokens, entropy and top alternatives of softmax(logits / T), in one pass over the logits
+ * [rows, vocab] (bf16 or fp32, unit inner stride).  No counterpart in the reference.
+ *   logprobs[r]: of tokens[r] (int64); 0 where that is negative, NaN and NVLLM_STATUS_BAD_TOKEN where it is >= vocab
+ *   entropy[r]: in nats;  top_tokens / top_logprobs [rows, top] contiguous: the largest logits in order, ties to the lowest index
+ * All statistics are fp32.  temperatures: fp32 [rows] or NULL; one that is not above 0 counts as 1.  -infinity in a row is a
+ * masked token; a row with a NaN, with +infinity or with nothing but -infinity has NaN for results (its alternatives go by the
+ * logits, NaN like -infinity; subnormal logits order like 0).  0 <= top <= NVLLM_LOGPROBS_MAX_TOP.  No alignment beyond the
+ * element's is required; the rest of the 16-byte pieces that a row's first and last elements lie in may be read.
+ */
+#define NVLLM_LOGPROBS_MAX_TOP 64
+NVLLM_API int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32, int64_t row_stride, const int64_t* tokens,
+                         const float* temperatures, int32_t rows, int32_t vocab, int32_t top, float* logprobs, float* entropy,
+                         int64_t* top_tokens, float* top_logprobs, void* stream);
 
 /*
  * Decode-step inputs for a captured CUDA graph, in one launch.  `staged` is a device copy of

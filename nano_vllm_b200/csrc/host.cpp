@@ -62,6 +62,7 @@ struct Api {
   decltype(&nvllm_prefill_varlen_fp8) prefill_varlen_fp8;
   decltype(&nvllm_prefill_fp8_workspace_bytes) prefill_fp8_workspace_bytes;
   decltype(&nvllm_step_maps) step_maps;
+  decltype(&nvllm_token_logprobs) token_logprobs;
 } api;
 PyObject* g_check = nullptr;  // _lib.check: raises NvllmError for a negative code
 
@@ -894,6 +895,81 @@ PyObject* sample(PyObject* const* a, bool candidates) {
 PyObject* sample_tokens(PyObject* const* a) { return sample(a, false); }
 PyObject* sample_candidates(PyObject* const* a) { return sample(a, true); }
 
+// ---- log probabilities ----------------------------------------------------------------------
+
+// The n result tensors of a call: made, or the caller's own (checked by the caller of this).
+void results(PyObject* given, int n, const char* what, at::Tensor* out, const char* const* names) {
+  if (!PySequence_Check(given) || PySequence_Size(given) != n) raise(PyExc_ValueError, what);
+  for (int i = 0; i < n; ++i) {
+    Ref item(PySequence_GetItem(given, i));
+    out[i] = tensor(item.o, names[i]);
+  }
+}
+PyObject* as_tuple(const at::Tensor* out, int n) {
+  PyObject* result = PyTuple_New(n);
+  if (!result) throw PyErrorSet{};
+  for (int i = 0; i < n; ++i) PyTuple_SET_ITEM(result, i, wrap(out[i]));
+  return result;
+}
+void require_result(const char* name, const at::Tensor& t, at::ScalarType type, at::IntArrayRef sizes, const at::Tensor& like) {
+  if (!t.is_cuda() || t.scalar_type() != type || !t.is_contiguous() || t.sizes() != sizes)
+    raise(PyExc_RuntimeError, std::string(name) + " must be a contiguous CUDA " + c10::toString(type) + " tensor of the documented shape");
+  require_on(name, t, like);
+}
+const float* row_temperatures(const at::Tensor* t, int64_t rows, const at::Tensor& like) {
+  if (!t) return nullptr;
+  if (!t->is_cuda() || t->scalar_type() != at::kFloat || !t->is_contiguous())
+    raise(PyExc_RuntimeError, "temperatures must be contiguous CUDA float32");
+  require(t->numel() == rows, "temperatures has one entry per row");
+  require_on("temperatures", *t, like);
+  return ptr<float>(*t);
+}
+
+// logits, tokens, top, temperatures, out
+PyObject* token_logprobs(PyObject* const* a) {
+  const at::Tensor &logits = tensor(a[0], "logits"), &tokens = tensor(a[1], "tokens");
+  const int64_t top = as_i64(a[2]);
+  const at::Tensor* temps = maybe_tensor(a[3], "temperatures");
+  if (!logits.is_cuda()) raise(PyExc_RuntimeError, "logits must be a CUDA tensor (nano_vllm_b200 has no CPU path)");
+  if (logits.scalar_type() != at::kBFloat16 && logits.scalar_type() != at::kFloat)
+    raise(PyExc_RuntimeError, "logits must be bfloat16 or float32, got " + std::string(c10::toString(logits.scalar_type())));
+  require(logits.dim() == 2 && logits.stride(1) == 1, "logits.dim() == 2 and logits.stride(1) == 1");
+  const int64_t rows = logits.size(0), vocab = logits.size(1);
+  constexpr int64_t most = std::numeric_limits<int32_t>::max();
+  require(rows <= most && vocab <= most, "sizes must fit 32 bits");
+  require(tokens.is_cuda() && tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.numel() == rows,
+          "tokens must be a contiguous CUDA int64 tensor, one per row");
+  require_on("tokens", tokens, logits);
+  const float* t = row_temperatures(temps, rows, logits);
+  if (top < 0 || top > NVLLM_LOGPROBS_MAX_TOP || top > vocab)
+    raise(PyExc_ValueError, "top must be 0 to " + std::to_string(NVLLM_LOGPROBS_MAX_TOP) + " and no more than the vocabulary");
+  at::Tensor out[4];
+  if (a[4] == Py_None) {
+    unlocked([&] {
+      const at::TensorOptions f32 = logits.options().dtype(at::kFloat);
+      out[0] = at::empty({rows}, f32);
+      out[1] = at::empty({rows}, f32);
+      out[2] = at::empty({rows, top}, f32.dtype(at::kLong));
+      out[3] = at::empty({rows, top}, f32);
+      return 0;
+    });
+  } else {
+    const char* const of[4] = {"logprobs", "entropy", "top_tokens", "top_logprobs"};
+    results(a[4], 4, "out must be the four tensors of an earlier call", out, of);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t shape[2] = {rows, top};
+      require_result(of[i], out[i], i == 2 ? at::kLong : at::kFloat, at::IntArrayRef(shape, i < 2 ? 1 : 2), logits);
+    }
+  }
+  const c10::cuda::CUDAGuard guard(logits.device());
+  launch([&] {
+    return api.token_logprobs(logits.data_ptr(), logits.scalar_type() == at::kFloat, rows > 1 ? logits.stride(0) : std::max<int64_t>(logits.stride(0), vocab),
+                              ptr<int64_t>(tokens), t, static_cast<int32_t>(rows), static_cast<int32_t>(vocab), static_cast<int32_t>(top),
+                              ptr<float>(out[0]), ptr<float>(out[1]), ptr<int64_t>(out[2]), ptr<float>(out[3]), stream_of(logits));
+  });
+  return as_tuple(out, 4);
+}
+
 // ---- decode-step inputs ---------------------------------------------------------------------
 
 struct Sections {  // byte offsets of the staging block (decode_inputs.layout)
@@ -1087,6 +1163,7 @@ PyObject* bind(PyObject* const* a) {  // library path, check
   RESOLVE(prefill_varlen_fp8);
   RESOLVE(prefill_fp8_workspace_bytes);
   RESOLVE(step_maps);
+  RESOLVE(token_logprobs);
 #undef RESOLVE
   Py_INCREF(a[1]);
   Py_XSETREF(g_check, a[1]);
@@ -1142,6 +1219,7 @@ PyMethodDef methods[] = {
     METHOD(decode_step_fp8, 12),
     METHOD(prefill_varlen_fp8, 12),
     METHOD(step_maps, 6),
+    METHOD(token_logprobs, 5),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of nano_vllm_b200's entry points.", -1, methods,

@@ -1,0 +1,453 @@
+// Log probabilities of given tokens, entropy and top alternatives from rows of logits, in one pass.
+//
+// For a row of V logits x, temperature T (one that is not above 0 counts as 1), m = max x:
+//   Z = sum exp((x_i - m) / T)            logprob of token k = (x_k - m) / T - ln Z
+//   entropy = ln Z - sum exp((x_i - m) / T) (x_i - m) / T / Z
+//   top alternatives: the `top` largest logits, ties to the lowest index, with their log probabilities
+// The pass carries the running maximum and both sums, rescaled when the maximum grows.  A row with a NaN, with +infinity or
+// with nothing but -infinity has no distribution: all its results are NaN (its alternatives go by the logits, NaN like -infinity).
+//
+// Alternatives without a second pass: a thread keeps the largest of its 16-byte pieces' maxima and the first piece that has it.
+// Of 128 groups of threads the top-th largest (maximum, piece) is a bound that `top` elements reach, so every alternative lies
+// in a thread whose own (maximum, piece) reaches it: about `top` threads, whose pieces are read again (from L2) and compared
+// with the bound.  Pieces break ties of values, so rows of equal values (masks) leave no more of them than others.
+//
+// A row is read by a cluster of 1 to 8 blocks.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <utility>
+
+#include "common.cuh"
+
+namespace nvllm {
+
+constexpr int kLpThreads = 256;
+constexpr int kLpMaxCluster = 8;
+constexpr int kLpMaxTop = NVLLM_LOGPROBS_MAX_TOP;
+constexpr int kLpGroups = 128;   // of threads, whose maxima give the bound
+constexpr int kLpCands = 1024;   // elements that reach the bound; more go the slow way
+
+struct LogprobParams {
+  const void* logits;
+  int64_t row_stride;
+  const int64_t* tokens;
+  const float* temperatures;  // nullable
+  int vocab, top;
+  float* logprobs;
+  float* entropy;
+  int64_t* top_tokens;
+  float* top_logprobs;
+  int* status;
+};
+
+// Float as an unsigned number of the same order; NaN like -infinity, one zero, subnormal numbers (to which comparisons are
+// blind, as this is compiled) like it.
+__device__ __forceinline__ uint32_t lp_order(float x) {
+  uint32_t u = __float_as_uint(x);
+  if ((u & 0x7fffffffu) > 0x7f800000u) u = 0xff800000u;
+  if (!(u & 0x7f800000u)) u = 0;
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float lp_value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+// Orders by value, then lower place first.  Never 0.
+__device__ __forceinline__ uint64_t lp_key(float x, uint32_t place) { return (static_cast<uint64_t>(lp_order(x)) << 32) | (0xffffffffu - place); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 16 bytes of a row.
+template <typename T>
+struct LpPiece;
+template <>
+struct LpPiece<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[N]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(u[i] << 16);
+      x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float max(const uint4& w) {  // NaN ignored
+    auto h = [](uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); };
+    const __nv_bfloat162 m = __hmax2(__hmax2(h(w.x), h(w.y)), __hmax2(h(w.z), h(w.w)));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  // -infinity in the places below lo and from hi on
+  static __device__ __forceinline__ uint4 cut(uint4 w, int lo, int hi) {
+    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k < lo || k >= hi) u[k / 2] = k % 2 ? (u[k / 2] & 0xffffu) | 0xff800000u : (u[k / 2] & 0xffff0000u) | 0xff80u;
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+template <>
+struct LpPiece<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(const uint4& w, float (&x)[N]) {
+    x[0] = __uint_as_float(w.x);
+    x[1] = __uint_as_float(w.y);
+    x[2] = __uint_as_float(w.z);
+    x[3] = __uint_as_float(w.w);
+  }
+  static __device__ __forceinline__ float max(const uint4& w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static __device__ __forceinline__ uint4 cut(uint4 w, int lo, int hi) {
+    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (k < lo || k >= hi) u[k] = 0xff800000u;
+    return make_uint4(u[0], u[1], u[2], u[3]);
+  }
+};
+
+// Maximum m (no less than the smallest finite number), s = sum exp2(c (x - m)), t = sum exp2(c (x - m)) (x - m).
+struct LpSums {
+  float m, s, t;
+  // Differences of -infinity: no weight, and 0 and not NaN times that.
+  static __device__ __forceinline__ float diff(float a, float m) { return max_nan(a - m, -3e38f); }
+  __device__ __forceinline__ void rescale(float to, float c) {
+    const float d = diff(m, to), f = fast_exp2(d * c);
+    s *= f;
+    t = fmaf(s, d, f * t);  // s first: times d it may not overflow
+    m = to;
+  }
+  __device__ __forceinline__ void join(float m2, float s2, float t2, float c) {
+    LpSums o{m2, s2, t2};
+    const float to = fmaxf(m, m2);
+    rescale(to, c);
+    o.rescale(to, c);
+    s += o.s;
+    t += o.t;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobParams p) {
+  using P = LpPiece<T>;
+  constexpr int N = P::N, C = 4;
+  namespace cg = cooperative_groups;
+  __shared__ uint64_t s_bounds[kLpGroups];
+  __shared__ uint64_t s_cand[kLpCands];
+  __shared__ uint64_t s_list[kLpMaxCluster][kLpMaxTop];  // of the first block: every block's alternatives in order, 0 behind the last
+  __shared__ float s_sums[kLpMaxCluster][3];
+  __shared__ float s_warp[kLpThreads / 32][3];
+  __shared__ uint16_t s_slot[kLpThreads];
+  __shared__ uint64_t s_tau;
+  __shared__ int s_slots, s_cands;
+  __shared__ uint64_t s_most[kLpThreads / 32];
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  auto started = cluster.barrier_arrive();  // waited for before another block's shared memory is written
+  const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank());
+  const int row = blockIdx.x / csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int me = crank * kLpThreads + tid, all = csize * kLpThreads;  // of the row's threads
+  const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
+  const float temperature = p.temperatures ? p.temperatures[row] : 1.f;
+  const float inv_t = temperature > 0.f ? fminf(__frcp_rn(temperature), 1e38f) : 1.f;
+  const float c = inv_t * 1.4426950408889634f;
+  int64_t token = -1;
+  float given = 0.f;
+  if (me == 0) {
+    token = p.tokens[row];
+    if (token >= 0 && token < p.vocab) given = static_cast<float>(x[token]);
+  }
+  if (tid == 0) {
+    s_tau = 0;
+    s_slots = s_cands = 0;
+  }
+
+  // Pieces start on 16-byte boundaries: what lies before and behind the row in the first and last one counts as -infinity.
+  const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
+  const uint4* base = reinterpret_cast<const uint4*>(x - shift);
+  const int pieces = static_cast<int>((static_cast<int64_t>(shift) + p.vocab + N - 1) / N);
+  const int last_hi = shift + p.vocab - (pieces - 1) * N;  // places of the last piece
+  const int head = shift > 0 || pieces == 1 ? 1 : 0;       // piece 0 is cut: the row's first thread has it
+  const int tail = pieces > 1 && last_hi < N ? 1 : 0;      // and the last one
+  const int whole = pieces - head - tail;
+  auto cut_piece = [&](int g) { return P::cut(__ldg(base + g), g == 0 ? shift : 0, g == pieces - 1 ? last_hi : N); };
+
+  LpSums sum{-FLT_MAX, 0.f, 0.f};
+  float best = -INFINITY;
+  const bool any = me == 0 || me < whole;
+  int at = me == 0 ? 0 : head + me;  // the first piece of this thread
+  uint64_t s2 = 0, t2 = 0;  // of pairs of elements
+  auto add = [&](const uint4& w) {
+    float e[N];
+    P::unpack(w, e);
+    const uint64_t minus_m = pack2(-sum.m, -sum.m), c2 = pack2(c, c);
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      float a, b, ya, yb;
+      const uint64_t y = add2(pack2(e[k], e[k + 1]), minus_m);
+      unpack2(y, ya, yb);
+      const uint64_t y2 = pack2(max_nan(ya, -3e38f), max_nan(yb, -3e38f));
+      unpack2(mul2(y2, c2), a, b);
+      const uint64_t w2 = pack2(fast_exp2(a), fast_exp2(b));
+      s2 = add2(s2, w2);
+      t2 = fma2(w2, y2, t2);
+    }
+  };
+  auto fold = [&]() {  // the pairs' sums into sum
+    float a, b;
+    unpack2(s2, a, b);
+    sum.s += a + b;
+    unpack2(t2, a, b);
+    sum.t += a + b;
+    s2 = t2 = 0;
+  };
+  auto grow = [&](float to) {
+    to = fmaxf(to, sum.m);
+    const float d = LpSums::diff(sum.m, to), f = fast_exp2(d * c);
+    const uint64_t f2 = pack2(f, f), d2 = pack2(d, d);
+    s2 = mul2(s2, f2);
+    t2 = fma2(s2, d2, mul2(t2, f2));
+    sum.m = to;
+  };
+  auto note = [&](float most, int g) {
+    if (most > best) {
+      best = most;
+      at = g;
+    }
+  };
+  auto one = [&](const uint4& w, int g) {
+    const float most = P::max(w);
+    note(most, g);
+    grow(best);
+    add(w);
+  };
+  if (me == 0 && head) one(cut_piece(0), 0);
+  {
+    const uint4* from = base + head;
+    uint4 next[C];
+    int i = me;
+    const int step = C * all;
+    auto load = [&](int j) {
+#pragma unroll
+      for (int k = 0; k < C; ++k) next[k] = __ldg(from + j + k * all);
+    };
+    const bool first = i + (C - 1) * all < whole;
+    if (first) load(i);
+    while (i + (C - 1) * all < whole) {
+      uint4 raw[C];
+#pragma unroll
+      for (int k = 0; k < C; ++k) raw[k] = next[k];
+      if (i + step + (C - 1) * all < whole) load(i + step);
+#pragma unroll
+      for (int k = 0; k < C; ++k) note(P::max(raw[k]), head + i + k * all);
+      grow(best);
+#pragma unroll
+      for (int k = 0; k < C; ++k) add(raw[k]);
+      i += step;
+    }
+    for (; i < whole; i += all) one(__ldg(from + i), head + i);
+  }
+  if (me == 0 && tail) one(cut_piece(pieces - 1), pieces - 1);
+  fold();
+
+  // ---- sums of the block
+#pragma unroll
+  for (int sh = 16; sh > 0; sh >>= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, sum.m, sh), a = __shfl_xor_sync(0xffffffffu, sum.s, sh), b = __shfl_xor_sync(0xffffffffu, sum.t, sh);
+    sum.join(m2, a, b, c);
+  }
+  if (lane == 0) {
+    s_warp[warp][0] = sum.m;
+    s_warp[warp][1] = sum.s;
+    s_warp[warp][2] = sum.t;
+  }
+
+  // ---- the block's alternatives, in order
+  const int top = p.top;
+  uint64_t mine = 0;
+  if (top > 0) {
+    constexpr int G = kLpThreads / kLpGroups;  // threads of a group
+    mine = any ? lp_key(best, static_cast<uint32_t>(at)) : 0;
+    uint64_t most = mine;
+#pragma unroll
+    for (int sh = 1; sh < G; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
+    if (tid % G == 0) s_bounds[tid / G] = most;
+    __syncthreads();
+    int above = 0;
+#pragma unroll 8
+    for (int k = tid % G; k < kLpGroups; k += G) above += s_bounds[k] > most;
+#pragma unroll
+    for (int sh = 1; sh < G; sh <<= 1) above += __shfl_xor_sync(0xffffffffu, above, sh);
+    if (tid % G == 0 && above == top - 1 && most) s_tau = most;  // one group: keys differ
+    __syncthreads();
+    const uint64_t tau = s_tau;
+    if (mine && mine >= tau) s_slot[atomicAdd(&s_slots, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    const int each = (whole + all - 1) / all + 2;  // pieces of a thread, the cut ones counted
+    const int total = s_slots * each;
+    // calls f(element's key) for the elements of piece n of the listed threads that reach the bound
+    auto look = [&](int n, auto&& f) {
+      const int who = crank * kLpThreads + s_slot[n / each], i = n % each;
+      int g = head + who + i * all;
+      uint4 w;
+      if (i >= each - 2) {
+        if (who != 0 || !(i == each - 1 ? tail : head)) return;
+        g = i == each - 1 ? pieces - 1 : 0;
+        w = cut_piece(g);
+      } else {
+        if (g >= head + whole) return;
+        w = __ldg(base + g);
+      }
+      float e[N];
+      P::unpack(w, e);
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const int id = g * N + k - shift;
+        if (id >= 0 && id < p.vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) f(lp_key(e[k], static_cast<uint32_t>(id)));
+      }
+    };
+    for (int n = tid; n < total; n += kLpThreads)
+      look(n, [&](uint64_t key) {
+        const int k = atomicAdd(&s_cands, 1);
+        if (k < kLpCands) s_cand[k] = key;
+      });
+    __syncthreads();
+    const int cands = s_cands;
+    uint64_t* list = s_list[0];
+    if (cands <= kLpCands) {
+      for (int n = tid; n < max(cands, top); n += kLpThreads) {
+        if (n >= cands) {
+          list[n] = 0;
+          continue;
+        }
+        const uint64_t key = s_cand[n];
+        int rank = 0;
+        for (int k = 0; k < cands; ++k) rank += s_cand[k] > key;
+        if (rank < top) list[rank] = key;
+      }
+    } else {  // the largest ones stand close together in few threads: one after the other
+      uint64_t before = ~0ull;
+      for (int r = 0; r < top; ++r) {
+        uint64_t most = 0;
+        for (int n = tid; n < total; n += kLpThreads)
+          look(n, [&](uint64_t key) {
+            if (key < before && key > most) most = key;
+          });
+#pragma unroll
+        for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
+        if (lane == 0) s_most[warp] = most;
+        __syncthreads();
+        for (int k = 0; k < kLpThreads / 32; ++k) most = max(most, s_most[k]);
+        before = most;
+        if (tid == 0) list[r] = most;
+        __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+  pdl_trigger();
+  cluster.barrier_wait(std::move(started));
+  if (tid == 0) {
+    for (int k = 1; k < kLpThreads / 32; ++k) sum.join(s_warp[k][0], s_warp[k][1], s_warp[k][2], c);
+    float* to = cluster.map_shared_rank(&s_sums[0][0], 0) + 3 * crank;
+    to[0] = sum.m;
+    to[1] = sum.s;
+    to[2] = sum.t;
+  }
+  if (crank != 0) {
+    uint64_t* to = cluster.map_shared_rank(&s_list[0][0], 0) + crank * kLpMaxTop;
+    for (int k = tid; k < top; k += kLpThreads) to[k] = s_list[0][k];
+  }
+  cluster.sync();
+  if (crank != 0) return;
+
+  // ---- results of the row
+  sum = {s_sums[0][0], s_sums[0][1], s_sums[0][2]};
+  for (int k = 1; k < csize; ++k) sum.join(s_sums[k][0], s_sums[k][1], s_sums[k][2], c);
+  const float log_z = static_cast<float>(log(static_cast<double>(sum.s)));
+  if (tid == 0) {
+    float lp = 0.f;
+    if (token >= p.vocab) {
+      lp = NAN;
+      atomicOr(p.status, NVLLM_STATUS_BAD_TOKEN);
+    } else if (token >= 0) {
+      lp = (given - sum.m) * inv_t - log_z;
+    }
+    p.logprobs[row] = lp;
+    p.entropy[row] = log_z - inv_t * __fdiv_rn(sum.t, sum.s);
+  }
+  const int keys = csize * top;
+  for (int n = tid; n < keys; n += kLpThreads) {
+    const uint64_t key = s_list[n / top][n % top];
+    if (!key) continue;
+    int rank = n;
+    if (csize > 1) {
+      rank = 0;
+      for (int b = 0; b < csize; ++b)
+        for (int k = 0; k < top && s_list[b][k] > key; ++k) ++rank;
+      if (rank >= top) continue;
+    }
+    const int64_t to = static_cast<int64_t>(row) * top + rank;
+    p.top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
+    p.top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - sum.m) * inv_t - log_z;
+  }
+}
+
+}  // namespace nvllm
+
+extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32, int64_t row_stride, const int64_t* tokens,
+                                    const float* temperatures, int32_t rows, int32_t vocab, int32_t top, float* logprobs,
+                                    float* entropy, int64_t* top_tokens, float* top_logprobs, void* stream) {
+  using namespace nvllm;
+  if (rows < 0 || vocab <= 0 || vocab > 0x7fffff00) return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d vocab=%d invalid", rows, vocab);
+  if (top < 0 || top > kLpMaxTop || top > vocab)
+    return fail(NVLLM_E_GEOMETRY, "token_logprobs: top=%d outside 0 to %d (vocab=%d)", top, kLpMaxTop, vocab);
+  if (rows == 0) return NVLLM_OK;
+  if (!logits || !tokens || !logprobs || !entropy || (top > 0 && (!top_tokens || !top_logprobs)))
+    return fail(NVLLM_E_NULL, "token_logprobs: NULL pointer argument");
+  if (row_stride < vocab) return fail(NVLLM_E_GEOMETRY, "token_logprobs: the row stride is smaller than vocab");
+  auto off = [](const void* q, size_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
+  if (off(logits, logits_are_fp32 ? 4 : 2) || off(tokens, 8) || off(temperatures, 4) || off(logprobs, 4) || off(entropy, 4) ||
+      off(top_tokens, 8) || off(top_logprobs, 4))
+    return fail(NVLLM_E_ALIGN, "token_logprobs: a pointer is not aligned to its element size");
+  LogprobParams p;
+  p.status = status_word();
+  const int sms = num_sms();
+  if (!p.status || sms <= 0) return fail(NVLLM_E_NO_DEVICE, "token_logprobs: no CUDA device is usable");
+  p.logits = logits;
+  p.row_stride = row_stride;
+  p.tokens = tokens;
+  p.temperatures = temperatures;
+  p.vocab = vocab;
+  p.top = top;
+  p.logprobs = logprobs;
+  p.entropy = entropy;
+  p.top_tokens = top_tokens;
+  p.top_logprobs = top_logprobs;
+  const int64_t pieces = (static_cast<int64_t>(vocab) + (logits_are_fp32 ? 3 : 7)) / (logits_are_fp32 ? 4 : 8);
+  int csize = kLpMaxCluster;
+  while (csize > 1 && (static_cast<int64_t>(rows) * csize > 4ll * sms || pieces < 2ll * csize * kLpThreads)) csize /= 2;
+  if (static_cast<int64_t>(rows) * csize > 0x7fffffff) return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d too many", rows);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * csize), 1, 1);
+  cfg.blockDim = dim3(kLpThreads, 1, 1);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = csize;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, logits_are_fp32 ? logprobs_kernel<float> : logprobs_kernel<__nv_bfloat16>, p);
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(NVLLM_E_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
+  }
+  count_launch();
+  return NVLLM_OK;
+}

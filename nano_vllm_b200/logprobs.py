@@ -1,0 +1,31 @@
+"""Log probabilities of tokens: what an engine answers with beside the tokens themselves, and what a search over several
+answers goes by.  nano-vllm's ``Sampler`` (nanovllm/layers/sampler.py:10-26) returns tokens only.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Sequence
+
+import torch
+
+from .attention import _native
+
+
+class TokenLogprobs(NamedTuple):
+    logprobs: torch.Tensor      # fp32 [N]: of the given tokens
+    entropy: torch.Tensor       # fp32 [N]: of the rows' distributions, in nats
+    top_tokens: torch.Tensor    # int64 [N, top]: the most probable tokens in order, ties to the lowest index
+    top_logprobs: torch.Tensor  # fp32 [N, top]: theirs
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperatures: torch.Tensor | None = None,
+                   out: Sequence[torch.Tensor] | None = None) -> TokenLogprobs:
+    """Under ``softmax(logits / T)`` of every row of ``logits`` ``[N, V]`` (bf16 or fp32): the log probability of its token of
+    ``tokens`` (int64 ``[N]``), the entropy, and the ``top`` (0 to 64) most probable tokens with theirs.  One launch, one read
+    of the logits; all statistics in fp32.
+
+    ``temperatures``: fp32 ``[N]`` as for ``sample_tokens``, where 1 stands for any that is not above 0 (greedy rows); without
+    them T is 1.  A negative token asks for none: 0 (rows of a padded batch); one beyond the vocabulary gives NaN and sets bit 8
+    of ``_lib.read_status()``.  Logits of -infinity are masked tokens.  A row with a NaN, with +infinity or with nothing but
+    -infinity has no distribution and NaN for results; its ``top_tokens`` go by the logits, NaN like -infinity.
+    ``out``: the four result tensors of an earlier call or of a graph, else they are made."""
+    return TokenLogprobs._make(_native(logits).token_logprobs(logits, tokens, top, temperatures, out))
