@@ -450,6 +450,56 @@ NVLLM_API int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32, 
                          int64_t* top_tokens, float* top_logprobs, void* stream);
 
 /*
+ * Blocks of a cache: copied, forked with their sequences, compacted, the free ones listed.  No counterpart on the reference's
+ * GPU side (its BlockManager, nanovllm/engine/block_manager.py:26-113, counts references on the host and copies nothing).
+ *
+ * A cache is up to NVLLM_CACHE_MAX_PARTS tensors, each of `planes` planes (of layers, of K and V) of num_blocks blocks:
+ * [256, Hkv, D] values of slot_bytes bytes a slot, or, for the scales of a cache in 8 bits, [scale_heads, 16] floats (slot_bytes
+ * 0).  A block is contiguous; planes and blocks lie at the given BYTE strides.  Bases, strides and slot_bytes are multiples of
+ * 16 bytes.
+ */
+#define NVLLM_CACHE_MAX_PARTS 160
+#define NVLLM_PAGES_MAX_BLOCKS 400000 /* of a cache that free_list / compact_blocks count */
+#define NVLLM_FORK_MAX_ROWS 4096      /* sequences of a fork, before and after */
+typedef struct {
+  void* base;
+  int64_t planes, plane_stride, block_stride;
+  int32_t slot_bytes, scale_heads;
+} nvllm_cache_part;
+
+/* Block dst_blocks[i] = block src_blocks[i] in every plane of every part, one launch; with num_slots only the first
+ * num_slots[i] slots (and the scales of their groups).  Pairs with a negative block are left out, ones beyond num_blocks too, and
+ * flagged.  A block that is copied to is in no other pair. */
+NVLLM_API int nvllm_copy_blocks(const nvllm_cache_part* parts, int32_t num_parts, int64_t num_blocks, const int32_t* src_blocks,
+                      const int32_t* dst_blocks, const int32_t* num_slots, int64_t num_copies, void* stream);
+
+/* num_rows sequences that go on from sequences parents[i] of a batch (negative: an empty row, length 0, entries -1), one launch.
+ * Row i of new_tables has the entries of its parent's row below ceil(len / 256), -1 behind them; new_lens[i] its length.  Whole
+ * blocks are shared.  A begun last block (len % 256 slots) stays with the parent's first new row; every other one gets the next of
+ * free_blocks in its place, in order of the rows, and a copy of the begun slots.  blocks_taken: how many that are; rows for which
+ * there is none left have -1 there.  new_tables may not overlap block_tables. */
+NVLLM_API int nvllm_fork_sequences(const nvllm_cache_part* parts, int32_t num_parts, int64_t num_blocks, const int32_t* block_tables,
+                         int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens, int32_t batch, const int32_t* parents,
+                         int32_t num_rows, const int32_t* free_blocks, int32_t num_free, int32_t* new_tables, int64_t new_row_stride,
+                         int32_t* new_lens, int32_t* blocks_taken, void* stream);
+
+/* ref_counts[i] = max(held[i], 0) (held NULL: 0) + how often the entries in use of the tables (columns below ceil(len / 256)) name
+ * block i; free_blocks: the ids with none in order, -1 behind them; num_free: how many.  One launch.  Negative entries name no
+ * block, ones beyond num_blocks are left out and flagged. */
+NVLLM_API int nvllm_free_list(const int32_t* block_tables, int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens, int32_t batch,
+                    const int32_t* held, int64_t num_blocks, int32_t* ref_counts, int32_t* free_blocks, int32_t* num_free, void* stream);
+
+/* Moves the n live blocks (those with a count in the sense of nvllm_free_list) to ids below n: the live ones from n on go to the
+ * free ones below it, in order.  moved_to[num_blocks]: the new id of every live block, -1 of the others; new_tables: the tables
+ * with the new ids, -1 where none is in use (may be block_tables); num_live: n.  Two launches.  workspace: of
+ * nvllm_compact_workspace_bytes(num_blocks) bytes, uninitialised. */
+NVLLM_API int64_t nvllm_compact_workspace_bytes(int64_t num_blocks);
+NVLLM_API int nvllm_compact_blocks(const nvllm_cache_part* parts, int32_t num_parts, int64_t num_blocks, const int32_t* block_tables,
+                         int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens, int32_t batch, const int32_t* held,
+                         int32_t* new_tables, int64_t new_row_stride, int32_t* moved_to, int32_t* num_live, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/*
  * Decode-step inputs for a captured CUDA graph, in one launch.  `staged` is a device copy of
  * one host staging block holding, at the given BYTE offsets: tokens int64[batch] (last token of
  * each sequence), lens int32[batch] (sequence lengths, the new token included), offsets

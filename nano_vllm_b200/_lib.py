@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int32, c_int64, c_uint64, c_void_p, POINTER
+from ctypes import c_char_p, c_float, c_int32, c_int64, c_uint64, c_void_p, POINTER, Structure
 from pathlib import Path
 
 # NVLLM_B200_LIB points the loader at another build of the same library (e.g. one compiled
@@ -53,6 +53,14 @@ SIGNATURES = {
     "nvllm_sample_layout": (c_int32, [c_int32, c_int32, c_int64, c_int32, c_int32, POINTER(c_int32), POINTER(c_int32), POINTER(c_int32)]),
     "nvllm_token_logprobs": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p]),
+    "nvllm_copy_blocks": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
+    "nvllm_fork_sequences": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_int32,
+                                       c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
+    "nvllm_free_list": (c_int32, [c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                  c_void_p]),
+    "nvllm_compact_workspace_bytes": (c_int64, [c_int64]),
+    "nvllm_compact_blocks": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+                                       c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "nvllm_decode_step_inputs": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32,
                                            c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "nvllm_decode_step_inputs_pinned": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int32,
@@ -99,6 +107,12 @@ SIGNATURES = {
 
 _lib = None
 _host = None
+
+
+class CachePart(Structure):
+    """nvllm_cache_part: one tensor of a cache, its planes and blocks at byte strides."""
+    _fields_ = [("base", c_void_p), ("planes", c_int64), ("plane_stride", c_int64), ("block_stride", c_int64),
+                ("slot_bytes", c_int32), ("scale_heads", c_int32)]
 
 
 class NvllmError(RuntimeError):

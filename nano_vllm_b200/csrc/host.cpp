@@ -63,6 +63,11 @@ struct Api {
   decltype(&nvllm_prefill_fp8_workspace_bytes) prefill_fp8_workspace_bytes;
   decltype(&nvllm_step_maps) step_maps;
   decltype(&nvllm_token_logprobs) token_logprobs;
+  decltype(&nvllm_copy_blocks) copy_blocks;
+  decltype(&nvllm_fork_sequences) fork_sequences;
+  decltype(&nvllm_free_list) free_list;
+  decltype(&nvllm_compact_workspace_bytes) compact_workspace_bytes;
+  decltype(&nvllm_compact_blocks) compact_blocks;
 } api;
 PyObject* g_check = nullptr;  // _lib.check: raises NvllmError for a negative code
 
@@ -970,6 +975,210 @@ PyObject* token_logprobs(PyObject* const* a) {
   return as_tuple(out, 4);
 }
 
+// ---- blocks of a cache ----------------------------------------------------------------------
+
+// The tensors of a cache: values [..., blocks, 256, Hkv, D] (bf16 or e4m3) and scales [..., blocks, Hkv, 16] (fp32).
+struct Cache {
+  std::vector<nvllm_cache_part> parts;
+  int64_t blocks = -1;
+  at::Tensor like;
+};
+Cache cache_parts(PyObject* o) {
+  Cache c;
+  Ref all(PySequence_Fast(o, "caches must be a sequence of tensors"));
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(all.o);
+  if (n < 1 || n > NVLLM_CACHE_MAX_PARTS) raise(PyExc_ValueError, "caches must be 1 to " + std::to_string(NVLLM_CACHE_MAX_PARTS) + " tensors");
+  for (Py_ssize_t k = 0; k < n; ++k) {
+    const at::Tensor& t = tensor(PySequence_Fast_GET_ITEM(all.o, k), "a cache");
+    if (!t.is_cuda()) raise(PyExc_RuntimeError, "caches must be CUDA tensors (nano_vllm_b200 has no CPU path)");
+    const bool scales = t.scalar_type() == at::kFloat;
+    if (!scales && t.scalar_type() != at::kBFloat16 && t.scalar_type() != at::kFloat8_e4m3fn)
+      raise(PyExc_RuntimeError, "caches must be bfloat16 or float8_e4m3fn values, or float32 scales, got " + std::string(c10::toString(t.scalar_type())));
+    const int64_t inner = scales ? 2 : 3, d = t.dim() - 1 - inner;  // of a block's dimensions; the blocks' dimension
+    require(d >= 0 && (scales ? t.size(-1) == NVLLM_BLOCK_SIZE / NVLLM_SCALE_GROUP : t.size(-3) == NVLLM_BLOCK_SIZE),
+            "a cache is [..., blocks, 256, Hkv, D], its scales [..., blocks, Hkv, 16]");
+    int64_t step = 1;
+    for (int64_t i = t.dim() - 1; i > d; --i) {
+      require(t.stride(i) == step || t.size(i) == 1, "a block of a cache must be contiguous");
+      step *= t.size(i);
+    }
+    int64_t planes = 1, stride = 0;  // the dimensions before the blocks', which must lie like one
+    for (int64_t i = d - 1; i >= 0; --i) {
+      if (t.size(i) == 1) continue;
+      if (planes == 1) stride = t.stride(i);
+      require(planes == 1 || t.stride(i) == stride * planes, "the planes of a cache must lie at one stride");
+      planes *= t.size(i);
+    }
+    require(planes > 0 && step > 0 && t.size(d) > 0, "a cache has blocks");
+    require(step <= std::numeric_limits<int32_t>::max(), "sizes must fit 32 bits");
+    const int64_t size = t.element_size();
+    if (k == 0) {
+      c.blocks = t.size(d);
+      c.like = t;
+    }
+    require(t.size(d) == c.blocks, "all tensors of a cache have the same number of blocks");
+    require_on("a cache", t, c.like);
+    c.parts.push_back({t.data_ptr(), planes, stride * size, (t.size(d) > 1 ? t.stride(d) : step) * size,
+                       scales ? 0 : static_cast<int32_t>(step / NVLLM_BLOCK_SIZE * size), scales ? static_cast<int32_t>(t.size(-2)) : 0});
+  }
+  return c;
+}
+
+void require_i32_on(const char* name, const at::Tensor& t, int64_t n, const at::Tensor& like) {
+  require_i32(name, t);
+  require_on(name, t, like);
+  if (t.dim() != 1 || (n >= 0 && t.numel() != n)) raise(PyExc_AssertionError, std::string(name) + " has one entry for each");
+}
+struct Tables {
+  int64_t batch, width;
+};
+Tables require_tables(const at::Tensor& table, const at::Tensor& lens, const at::Tensor& like) {
+  require_i32("block_tables", table);
+  require_on("block_tables", table, like);
+  require(table.dim() == 2 && table.size(1) > 0, "block_tables.dim() == 2, a column or more");
+  require(table.size(0) <= std::numeric_limits<int32_t>::max() && table.size(1) <= std::numeric_limits<int32_t>::max(), "sizes must fit 32 bits");
+  require_i32_on("seq_lens", lens, table.size(0), like);
+  return {table.size(0), table.size(1)};
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
+bool overlap(const at::Tensor& a, const at::Tensor& b) {  // of the memory between first and last elements
+  auto span = [](const at::Tensor& t) {
+    const char* p = static_cast<const char*>(t.data_ptr());
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return std::pair<const char*, const char*>(p, t.numel() ? p + (last + 1) * t.element_size() : p);
+  };
+  const auto [a0, a1] = span(a);
+  const auto [b0, b1] = span(b);
+  return a0 < b1 && b0 < a1;
+}
+
+PyObject* copy_blocks(PyObject* const* a) {  // caches, src_blocks, dst_blocks, num_slots
+  const Cache c = cache_parts(a[0]);
+  const at::Tensor &src = tensor(a[1], "src_blocks"), &dst = tensor(a[2], "dst_blocks");
+  const at::Tensor* slots = maybe_tensor(a[3], "num_slots");
+  require_i32_on("src_blocks", src, -1, c.like);
+  require_i32_on("dst_blocks", dst, src.numel(), c.like);
+  if (slots) require_i32_on("num_slots", *slots, src.numel(), c.like);
+  const c10::cuda::CUDAGuard guard(c.like.device());
+  launch([&] {
+    return api.copy_blocks(c.parts.data(), static_cast<int32_t>(c.parts.size()), c.blocks, ptr<int32_t>(src), ptr<int32_t>(dst),
+                           slots ? ptr<int32_t>(*slots) : nullptr, src.numel(), stream_of(c.like));
+  });
+  Py_RETURN_NONE;
+}
+
+PyObject* fork_sequences(PyObject* const* a) {  // caches, block_tables, seq_lens, parents, free_blocks, out
+  const Cache c = cache_parts(a[0]);
+  const at::Tensor &table = tensor(a[1], "block_tables"), &lens = tensor(a[2], "seq_lens"), &parents = tensor(a[3], "parents"),
+                   &free = tensor(a[4], "free_blocks");
+  const Tables t = require_tables(table, lens, c.like);
+  require_i32_on("parents", parents, -1, c.like);
+  require_i32_on("free_blocks", free, -1, c.like);
+  const int64_t rows = parents.numel();
+  constexpr int64_t most = std::numeric_limits<int32_t>::max();
+  require(rows <= most && free.numel() <= most, "sizes must fit 32 bits");
+  at::Tensor out[3];
+  if (a[5] == Py_None) {
+    unlocked([&] {
+      out[0] = at::empty({rows, t.width}, table.options());
+      out[1] = at::empty({rows}, table.options());
+      out[2] = at::empty({1}, table.options());
+      return 0;
+    });
+  } else {
+    const char* const of[3] = {"block_tables", "seq_lens", "blocks_taken"};
+    results(a[5], 3, "out must be the three tensors of an earlier call", out, of);
+    require_i32("out's block_tables", out[0]);
+    require_on("out's block_tables", out[0], c.like);
+    require(out[0].dim() == 2 && out[0].size(0) == rows && out[0].size(1) == t.width, "out's block_tables is [rows, blocks]");
+    require_i32_on("out's seq_lens", out[1], rows, c.like);
+    require_i32_on("out's blocks_taken", out[2], 1, c.like);
+    for (const at::Tensor& o : out)
+      for (const at::Tensor* in : {&table, &lens, &parents, &free}) require(!overlap(o, *in), "the results may not lie on the arguments");
+  }
+  const c10::cuda::CUDAGuard guard(c.like.device());
+  launch([&] {
+    return api.fork_sequences(c.parts.data(), static_cast<int32_t>(c.parts.size()), c.blocks, ptr<int32_t>(table), row_stride(table),
+                              static_cast<int32_t>(t.width), ptr<int32_t>(lens), static_cast<int32_t>(t.batch), ptr<int32_t>(parents),
+                              static_cast<int32_t>(rows), ptr<int32_t>(free), static_cast<int32_t>(free.numel()), ptr<int32_t>(out[0]),
+                              row_stride(out[0]), ptr<int32_t>(out[1]), ptr<int32_t>(out[2]), stream_of(c.like));
+  });
+  return as_tuple(out, 3);
+}
+
+PyObject* free_list(PyObject* const* a) {  // block_tables, seq_lens, num_blocks, held, out
+  const at::Tensor &table = tensor(a[0], "block_tables"), &lens = tensor(a[1], "seq_lens");
+  const int64_t blocks = as_i64(a[2]);
+  const at::Tensor* held = maybe_tensor(a[3], "held");
+  if (!table.is_cuda()) raise(PyExc_RuntimeError, "block_tables must be a CUDA tensor (nano_vllm_b200 has no CPU path)");
+  const Tables t = require_tables(table, lens, table);
+  require(blocks > 0 && blocks <= NVLLM_PAGES_MAX_BLOCKS, "num_blocks is 1 to 400000");
+  if (held) require_i32_on("held", *held, blocks, table);
+  at::Tensor out[3];
+  if (a[4] == Py_None) {
+    unlocked([&] {
+      out[0] = at::empty({blocks}, table.options());
+      out[1] = at::empty({blocks}, table.options());
+      out[2] = at::empty({1}, table.options());
+      return 0;
+    });
+  } else {
+    const char* const of[3] = {"ref_counts", "free_blocks", "num_free"};
+    results(a[4], 3, "out must be the three tensors of an earlier call", out, of);
+    for (int i = 0; i < 3; ++i) require_i32_on(of[i], out[i], i < 2 ? blocks : 1, table);
+  }
+  const c10::cuda::CUDAGuard guard(table.device());
+  launch([&] {
+    return api.free_list(ptr<int32_t>(table), row_stride(table), static_cast<int32_t>(t.width), ptr<int32_t>(lens), static_cast<int32_t>(t.batch),
+                         held ? ptr<int32_t>(*held) : nullptr, blocks, ptr<int32_t>(out[0]), ptr<int32_t>(out[1]), ptr<int32_t>(out[2]),
+                         stream_of(table));
+  });
+  return as_tuple(out, 3);
+}
+
+PyObject* compact_blocks(PyObject* const* a) {  // caches, block_tables, seq_lens, held, out
+  const Cache c = cache_parts(a[0]);
+  const at::Tensor &table = tensor(a[1], "block_tables"), &lens = tensor(a[2], "seq_lens");
+  const at::Tensor* held = maybe_tensor(a[3], "held");
+  const Tables t = require_tables(table, lens, c.like);
+  if (held) require_i32_on("held", *held, c.blocks, c.like);
+  const int64_t need = api.compact_workspace_bytes(c.blocks);
+  check(need);
+  at::Tensor out[3], scratch;
+  unlocked([&] {
+    scratch = at::empty({need}, table.options().dtype(at::kByte));  // of the call
+    if (a[4] == Py_None) {
+      out[0] = at::empty({t.batch, t.width}, table.options());
+      out[1] = at::empty({c.blocks}, table.options());
+      out[2] = at::empty({1}, table.options());
+    }
+    return 0;
+  });
+  if (a[4] != Py_None) {
+    const char* const of[3] = {"block_tables", "moved_to", "num_live"};
+    results(a[4], 3, "out must be the three tensors of an earlier call", out, of);
+    require_i32("out's block_tables", out[0]);
+    require_on("out's block_tables", out[0], c.like);
+    require(out[0].dim() == 2 && out[0].size(0) == t.batch && out[0].size(1) == t.width, "out's block_tables is [sequences, blocks]");
+    require_i32_on("out's moved_to", out[1], c.blocks, c.like);
+    require_i32_on("out's num_live", out[2], 1, c.like);
+    const bool same = out[0].data_ptr() == table.data_ptr() && row_stride(out[0]) == row_stride(table);
+    require(same || !overlap(out[0], table), "out's block_tables is the tables themselves or lies elsewhere");
+    for (const at::Tensor& o : out)
+      for (const at::Tensor* in : {&lens, held}) require(!in || !overlap(o, *in), "the results may not lie on the arguments");
+    for (int i = 1; i < 3; ++i) require(!overlap(out[i], table), "the results may not lie on the arguments");
+  }
+  const c10::cuda::CUDAGuard guard(c.like.device());
+  launch([&] {
+    return api.compact_blocks(c.parts.data(), static_cast<int32_t>(c.parts.size()), c.blocks, ptr<int32_t>(table), row_stride(table),
+                              static_cast<int32_t>(t.width), ptr<int32_t>(lens), static_cast<int32_t>(t.batch), held ? ptr<int32_t>(*held) : nullptr,
+                              ptr<int32_t>(out[0]), row_stride(out[0]), ptr<int32_t>(out[1]), ptr<int32_t>(out[2]), scratch.data_ptr(), need,
+                              stream_of(c.like));
+  });
+  return as_tuple(out, 3);
+}
+
 // ---- decode-step inputs ---------------------------------------------------------------------
 
 struct Sections {  // byte offsets of the staging block (decode_inputs.layout)
@@ -1164,6 +1373,11 @@ PyObject* bind(PyObject* const* a) {  // library path, check
   RESOLVE(prefill_fp8_workspace_bytes);
   RESOLVE(step_maps);
   RESOLVE(token_logprobs);
+  RESOLVE(copy_blocks);
+  RESOLVE(fork_sequences);
+  RESOLVE(free_list);
+  RESOLVE(compact_workspace_bytes);
+  RESOLVE(compact_blocks);
 #undef RESOLVE
   Py_INCREF(a[1]);
   Py_XSETREF(g_check, a[1]);
@@ -1220,6 +1434,10 @@ PyMethodDef methods[] = {
     METHOD(prefill_varlen_fp8, 12),
     METHOD(step_maps, 6),
     METHOD(token_logprobs, 5),
+    METHOD(copy_blocks, 4),
+    METHOD(fork_sequences, 6),
+    METHOD(free_list, 5),
+    METHOD(compact_blocks, 5),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "Host path of nano_vllm_b200's entry points.", -1, methods,
