@@ -450,6 +450,18 @@ NVLLM_API int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32, 
                          int64_t* top_tokens, float* top_logprobs, void* stream);
 
 /*
+ * The same log probabilities and entropy from hidden states [rows, hidden] and the LM head's weight [vocab, hidden] (bf16, row
+ * strides multiples of 8; hidden too), of logits = hidden_states weight^T in fp32 that are never written: stands where
+ * ParallelLMHead.forward (nanovllm/layers/embed_head.py:68-88) would be followed by nvllm_token_logprobs, for all rows of a prompt.
+ * Two launches.  workspace: of nvllm_head_logprobs_workspace_bytes() on the same device, 16-byte aligned, uninitialised.
+ * A wait inside that runs out sets NVLLM_STATUS_TIMEOUT; the results are then invalid.
+ */
+NVLLM_API int64_t nvllm_head_logprobs_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab);
+NVLLM_API int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row_stride, const void* weight, int64_t weight_row_stride,
+                        const int64_t* tokens, const float* temperatures, int64_t rows, int64_t hidden, int64_t vocab,
+                        float* logprobs, float* entropy, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Blocks of a cache: copied, forked with their sequences, compacted, the free ones listed.  No counterpart on the reference's
  * GPU side (its BlockManager, nanovllm/engine/block_manager.py:26-113, counts references on the host and copies nothing).
  *

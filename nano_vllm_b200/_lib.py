@@ -53,6 +53,9 @@ SIGNATURES = {
     "nvllm_sample_layout": (c_int32, [c_int32, c_int32, c_int64, c_int32, c_int32, POINTER(c_int32), POINTER(c_int32), POINTER(c_int32)]),
     "nvllm_token_logprobs": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                                        c_void_p, c_void_p, c_void_p]),
+    "nvllm_head_logprobs_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "nvllm_head_logprobs": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,
+                                      c_void_p, c_void_p, c_int64, c_void_p]),
     "nvllm_copy_blocks": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p]),
     "nvllm_fork_sequences": (c_int32, [c_void_p, c_int32, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_int32,
                                        c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),

@@ -1,0 +1,399 @@
+// Log probabilities of given tokens and entropy from hidden states: the LM head's product whose epilogue is the softmax.
+//
+// logits = hidden [N, H] weight [V, H]^T are never written: a tile of 128 rows x up to 256 columns is accumulated in tensor
+// memory by tcgen05 and reduced there to three numbers for each row (maximum, sum of exponentials, their sum times the
+// logits: the statistics of token_logprobs), which a second launch joins over the vocabulary's tiles.
+//
+// Sums over H stay fp32: the tensor core cuts its running sum towards zero at every step, which over long rows is a systematic
+// loss (H = 4096: logits 3.7e-6 too small on average, log probabilities 2e-6 off), so a product is cut after kChunk elements
+// and the parts are added in registers (one part up to there; 4.6e-7 at 1024).
+#include <algorithm>
+
+#include "logprobs.cuh"
+#include "prefill_tc.cuh"
+
+namespace nvllm {
+namespace hlp {
+using namespace sm100;
+
+constexpr int BM = 128, BN = 256, BK = 64, NST = 4;
+constexpr int kEpilogueWarps = 8, kThreads = (kEpilogueWarps + 4) * 32;  // registers come by fours of warps
+constexpr int kRegs = 168, kRegsEpilogue = 216, kRegsOther = 72;         // at launch, and as the groups share them (LONG)
+static_assert(kEpilogueWarps * kRegsEpilogue + 4 * kRegsOther <= (kEpilogueWarps + 4) * kRegs, "no more than the block has");
+constexpr int kChunk = 1024;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int CTRL_BYTES = 1024, SMEM = CTRL_BYTES + NST * STAGE_BYTES + 1024;  // + alignment slack
+constexpr int TMEM_COLS = 512;  // two accumulators
+enum Bar { FULL0 = 0, EMPTY0 = NST, ACC_FULL0 = 2 * NST, ACC_FREE0 = 2 * NST + 2, DRAIN = 2 * NST + 4, NUM_BARS };
+
+struct Params {
+  const int64_t* tokens;
+  const float* temperatures;
+  int rows, vocab;
+  int bn;         // columns of a tile
+  int mt, nt;     // tiles of rows and of columns
+  int group, ng;  // column tiles that a unit of work has one after the other, and how many such groups
+  int mb;         // row tiles whose units take turns
+  int kb;         // blocks of 64 elements of a row
+  int keep;       // a thread block has one row tile all along
+  float4* partial;  // [slot][half][mt * 128]: maximum, sum, sum times logits
+  float* given;     // [mt * 128]: logit of the row's token
+  int* status;
+};
+
+struct Unit {
+  int m, g;
+};
+__device__ __forceinline__ Unit unit_of(const Params& p, int i) {
+  const int full = p.mb * p.ng, sb = i / full, r = i - sb * full, cnt = min(p.mb, p.mt - sb * p.mb);
+  return {sb * p.mb + r % cnt, r / cnt};
+}
+
+template <bool LONG>
+__global__ void __launch_bounds__(kThreads, 1) head_logprobs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
+  auto bar = [&](int i) { return base + 8u * i; };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(base_ptr + 512);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(base_ptr + 520);
+  const uint32_t ring = base + CTRL_BYTES;
+  if (tid == 0) {
+    *abort_flag = 0;
+    for (int i = 0; i < NUM_BARS; ++i) mbar_init(bar(i), i == ACC_FREE0 || i == ACC_FREE0 + 1 ? kEpilogueWarps : 1u);
+    mbar_fence_init();
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_b);
+  }
+  if (warp == kEpilogueWarps + 1) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  const int units = p.mt * p.ng, chunks = LONG ? (p.kb * BK + kChunk - 1) / kChunk : 1, per_chunk = LONG ? kChunk / BK : p.kb;
+
+  if (warp >= kEpilogueWarps) {
+    if constexpr (LONG) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kEpilogueWarps) {
+      // ------------------------------------------------------------------ TMA producer
+      if (elect_one()) {
+        const uint32_t bytes = A_BYTES + p.bn * BK * 2;
+        int s = 0, use = 0;
+        bool ok = true;
+        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+          const Unit u = unit_of(p, i);
+          for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n)
+            for (int kb = 0; kb < p.kb; ++kb) {
+              if (use > 0 && !(ok = wait_or_abort(bar(EMPTY0 + s), (use - 1) & 1, abort_flag))) break;
+              mbar_expect_tx(bar(FULL0 + s), bytes);
+              const uint32_t dst = ring + s * STAGE_BYTES;
+              tma_load_3d(dst, &map_a, bar(FULL0 + s), kb * BK, 0, u.m * BM);
+              tma_load_3d(dst + A_BYTES, &map_b, bar(FULL0 + s), kb * BK, 0, n * p.bn);
+              if (++s == NST) {
+                s = 0;
+                ++use;
+              }
+            }
+        }
+        if (!ok)  // no copy is in flight when the block ends
+          for (int k = 0; k < NST; ++k) {
+            const int uses = k < s ? use + 1 : use;
+            if (uses > 0) (void)mbar_wait(bar(FULL0 + k), (uses - 1) & 1);
+          }
+      }
+    } else if (warp == kEpilogueWarps + 1) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (elect_one()) {
+        const uint32_t idesc = umma_idesc(BM, p.bn, 0, 0);
+        const uint64_t desc0 = umma_desc(ring, 16, 1024);
+        int s = 0, use = 0, it = 0;
+        bool ok = true;
+        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+          const Unit u = unit_of(p, i);
+          for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n)
+            for (int c = 0; c < chunks && ok; ++c, ++it) {
+              const int b = it & 1;
+              if (it >= 2 && !(ok = wait_or_abort(bar(ACC_FREE0 + b), ((it >> 1) - 1) & 1, abort_flag))) break;
+              tc_fence_after();
+              const int first = c * per_chunk, last = min(first + per_chunk, p.kb);
+              for (int kb = first; kb < last; ++kb) {
+                if (!(ok = wait_or_abort(bar(FULL0 + s), use & 1, abort_flag))) break;
+                tc_fence_after();
+                const uint64_t da = desc0 + static_cast<uint64_t>((s * STAGE_BYTES) >> 4), db = da + (A_BYTES >> 4);
+  #pragma unroll
+                for (int ks = 0; ks < BK / 16; ++ks) umma_ss(tmem + b * BN, da + 2 * ks, db + 2 * ks, idesc, kb > first || ks > 0);
+                umma_commit(bar(EMPTY0 + s));
+                if (++s == NST) {
+                  s = 0;
+                  ++use;
+                }
+              }
+              if (ok) umma_commit(bar(ACC_FULL0 + b));
+            }
+        }
+        if (!ok) {  // nothing may still be running on tensor memory when it is freed
+          umma_commit(bar(DRAIN));
+          (void)mbar_wait(bar(DRAIN), 0);
+        }
+      }
+    }
+  } else {
+    if constexpr (LONG) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
+    // ------------------------------------------------------------------ epilogue: a row and half of the columns to a thread
+    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * (BN / 2);
+    const int64_t rows_padded = static_cast<int64_t>(p.mt) * BM;
+    LpSums sum{-FLT_MAX, 0.f, 0.f};
+    int it = 0, m = -1, slot = 0;
+    float c = 0.f;
+    int64_t token = -1;
+    bool ok = true;
+    auto flush = [&]() { p.partial[(static_cast<int64_t>(slot) * 2 + half) * rows_padded + m * BM + r] = make_float4(sum.m, sum.s, sum.t, 0.f); };
+    auto add = [&](float* v, int col, int n) {  // columns col to col + 31 of the vocabulary, of which the first n count
+      if (n < 32) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (k >= n) v[k] = -INFINITY;
+      }
+      float most = v[0];
+#pragma unroll
+      for (int k = 1; k < 31; k += 2) most = fmax3(most, v[k], v[k + 1]);
+      most = fmaxf(most, v[31]);
+      sum.rescale(fmaxf(most, sum.m), c);
+      const uint64_t minus_m = pack2(-sum.m, -sum.m), c2 = pack2(c, c);
+      uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+      for (int k = 0; k < 32; k += 2) {
+        float a, b, ya, yb;
+        unpack2(add2(pack2(v[k], v[k + 1]), minus_m), ya, yb);
+        const uint64_t y2 = pack2(max_nan(ya, -3e38f), max_nan(yb, -3e38f));
+        unpack2(mul2(y2, c2), a, b);
+        const uint64_t w2 = pack2(fast_exp2(a), fast_exp2(b));
+        s2 = add2(s2, w2);
+        t2 = fma2(w2, y2, t2);
+      }
+      float a, b;
+      unpack2(s2, a, b);
+      sum.s += a + b;
+      unpack2(t2, a, b);
+      sum.t += a + b;
+      const int64_t d = token - col;
+      if (d >= 0 && d < 32 && d < n) {
+        float x = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k)
+          if (k == d) x = v[k];
+        p.given[m * BM + r] = x;
+      }
+    };
+    for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+      const Unit u = unit_of(p, i);
+      if (m < 0 || !p.keep) {
+        m = u.m;
+        slot = u.g;
+        sum = {-FLT_MAX, 0.f, 0.f};
+        const int64_t row = static_cast<int64_t>(m) * BM + r;
+        token = row < p.rows ? p.tokens[row] : -1;
+        if (token >= p.vocab) token = -1;
+        c = (row < p.rows ? lp_inverse(p.temperatures, row) : 1.f) * 1.4426950408889634f;
+      }
+      for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n) {
+        const int first = n * p.bn + half * (BN / 2), end = min(p.vocab, (n + 1) * p.bn) - first;  // columns of this thread
+        float acc[LONG ? BN / 2 : 32];
+        for (int ch = 0; ch < chunks && ok; ++ch, ++it) {
+          const int b = it & 1;
+          if (!(ok = wait_or_abort(bar(ACC_FULL0 + b), (it >> 1) & 1, abort_flag))) break;
+          __syncwarp();
+          tc_fence_after();
+          if constexpr (LONG) {
+#pragma unroll
+            for (int j = 0; j < BN / 2; j += 32) {
+              uint32_t v[32];
+              tmem_ld32(at + b * BN + j, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) acc[j + k] = ch == 0 ? __uint_as_float(v[k]) : acc[j + k] + __uint_as_float(v[k]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(ACC_FREE0 + b));
+          } else {
+#pragma unroll 1
+            for (int j = 0; j < end && j < BN / 2; j += 32) {
+              uint32_t v[32];
+              tmem_ld32(at + b * BN + j, v);
+              tmem_wait_ld();
+#pragma unroll
+              for (int k = 0; k < 32; ++k) acc[k] = __uint_as_float(v[k]);
+              add(acc, first + j, end - j);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(ACC_FREE0 + b));
+          }
+        }
+        if constexpr (LONG) {
+          if (ok) {
+#pragma unroll
+            for (int j = 0; j < BN / 2; j += 32)
+              if (j < end) add(acc + j, first + j, end - j);
+          }
+        }
+      }
+      if (!p.keep) flush();
+    }
+    if (p.keep && m >= 0) flush();
+  }
+
+  pdl_trigger();
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag) atomicOr(p.status, NVLLM_STATUS_TIMEOUT);
+  if (warp == kEpilogueWarps + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, TMEM_COLS);
+  }
+}
+
+// Joins the partial statistics of `slots` slots for every row: 32 rows to a block, 8 threads a row.
+struct JoinParams {
+  const float4* partial;
+  const float* given;
+  const int64_t* tokens;
+  const float* temperatures;
+  int rows, vocab, slots;  // halves counted
+  int64_t rows_padded;
+  float *logprobs, *entropy;
+  int* status;
+};
+constexpr int kJoinRows = 32, kJoinWarps = 8;
+
+__global__ void __launch_bounds__(kJoinRows * kJoinWarps) join_kernel(const JoinParams p) {
+  __shared__ float s_sums[kJoinWarps][kJoinRows][3];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + lane;
+  const bool live = row < p.rows;
+  const float inv_t = live ? lp_inverse(p.temperatures, row) : 1.f, c = inv_t * 1.4426950408889634f;
+  const int64_t token = live ? p.tokens[row] : -1;
+  pdl_prologue();
+  LpSums sum{-FLT_MAX, 0.f, 0.f};
+  if (live)
+#pragma unroll 4
+    for (int k = warp; k < p.slots; k += kJoinWarps) {
+      const float4 v = p.partial[k * p.rows_padded + row];
+      sum.join(v.x, v.y, v.z, c);
+    }
+  s_sums[warp][lane][0] = sum.m;
+  s_sums[warp][lane][1] = sum.s;
+  s_sums[warp][lane][2] = sum.t;
+  __syncthreads();
+  if (warp != 0 || !live) return;
+  for (int k = 1; k < kJoinWarps; ++k) sum.join(s_sums[k][lane][0], s_sums[k][lane][1], s_sums[k][lane][2], c);
+  sum.results(row, token, token >= 0 && token < p.vocab ? p.given[row] : 0.f, inv_t, sum.log_z(), p.vocab, p.logprobs, p.entropy, p.status);
+}
+
+// How a problem is laid out over `sms` thread blocks.
+struct Plan {
+  int bn, mt, nt, group, ng, mb, kb, keep, grid, slots;
+  int64_t rows_padded, bytes;
+};
+static Plan plan_of(int rows, int hidden, int vocab, int sms) {
+  Plan pl;
+  pl.kb = (hidden + BK - 1) / BK;
+  pl.mt = (rows + BM - 1) / BM;
+  // the widest tile that leaves the fullest thread block as few columns as any
+  int64_t least = 0;
+  pl.bn = BN;
+  for (int bn = BN; bn >= BN / 2; bn -= 16) {
+    const int64_t tiles = static_cast<int64_t>(pl.mt) * ((vocab + bn - 1) / bn), cost = (tiles + sms - 1) / sms * bn;
+    if (bn == BN || cost < least) least = cost, pl.bn = bn;
+  }
+  pl.nt = (vocab + pl.bn - 1) / pl.bn;
+  pl.keep = pl.mt <= sms && sms % pl.mt == 0;
+  pl.group = 1;
+  while (!pl.keep && pl.group < 16 && static_cast<int64_t>(pl.mt) * ((pl.nt + 2 * pl.group - 1) / (2 * pl.group)) >= 48ll * sms) pl.group *= 2;
+  pl.ng = (pl.nt + pl.group - 1) / pl.group;
+  pl.mb = pl.keep ? pl.mt : static_cast<int>(std::min<int64_t>(pl.mt, std::max<int64_t>(1, (32ll << 20) / (BM * 2ll * hidden))));
+  pl.grid = static_cast<int>(std::min<int64_t>(sms, static_cast<int64_t>(pl.mt) * pl.ng));
+  pl.slots = 2 * (pl.keep ? std::min(sms / pl.mt, pl.ng) : pl.ng);
+  pl.rows_padded = static_cast<int64_t>(pl.mt) * BM;
+  pl.bytes = pl.slots * pl.rows_padded * 16 + pl.rows_padded * 4;
+  return pl;
+}
+
+static int check(int64_t rows, int64_t hidden, int64_t vocab) {
+  if (rows < 0 || rows > (1 << 24) || vocab <= 0 || vocab > (1 << 24) || hidden <= 0 || hidden > 65536 || hidden % 8)
+    return fail(NVLLM_E_GEOMETRY, "head_logprobs: rows=%lld hidden=%lld (a multiple of 8) vocab=%lld not supported", (long long)rows, (long long)hidden,
+                (long long)vocab);
+  return NVLLM_OK;
+}
+
+}  // namespace hlp
+}  // namespace nvllm
+
+extern "C" int64_t nvllm_head_logprobs_workspace_bytes(int64_t rows, int64_t hidden, int64_t vocab) {
+  using namespace nvllm;
+  if (const int e = hlp::check(rows, hidden, vocab)) return e;
+  if (rows == 0) return 0;
+  const int sms = num_sms();
+  return hlp::plan_of(static_cast<int>(rows), static_cast<int>(hidden), static_cast<int>(vocab), sms > 0 ? sms : 148).bytes;
+}
+
+extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row_stride, const void* weight, int64_t weight_row_stride,
+                                   const int64_t* tokens, const float* temperatures, int64_t rows, int64_t hidden, int64_t vocab,
+                                   float* logprobs, float* entropy, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace nvllm;
+  if (const int e = hlp::check(rows, hidden, vocab)) return e;
+  if (rows == 0) return NVLLM_OK;
+  if (!hidden_states || !weight || !tokens || !logprobs || !entropy) return fail(NVLLM_E_NULL, "head_logprobs: NULL pointer argument");
+  if (hidden_row_stride < hidden || weight_row_stride < hidden) return fail(NVLLM_E_GEOMETRY, "head_logprobs: a row stride is smaller than a row");
+  auto off = [](const void* q, size_t n) { return reinterpret_cast<uintptr_t>(q) % n != 0; };
+  if (!aligned16(hidden_states) || !aligned16(weight) || hidden_row_stride % 8 || weight_row_stride % 8 || off(tokens, 8) || off(temperatures, 4) ||
+      off(logprobs, 4) || off(entropy, 4))
+    return fail(NVLLM_E_ALIGN, "head_logprobs: rows must be 16-byte aligned, the other pointers aligned to their elements");
+  const int sms = num_sms();
+  int* status = status_word();
+  if (!status || sms <= 0) return fail(NVLLM_E_NO_DEVICE, "head_logprobs: no CUDA device is usable");
+  const hlp::Plan pl = hlp::plan_of(static_cast<int>(rows), static_cast<int>(hidden), static_cast<int>(vocab), sms);
+  if (!workspace || workspace_bytes < pl.bytes)
+    return fail(NVLLM_E_WORKSPACE, "head_logprobs: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)pl.bytes);
+  if (!aligned16(workspace)) return fail(NVLLM_E_ALIGN, "head_logprobs: the workspace must be 16-byte aligned");
+  CUtensorMap a, b;
+  if (!sm100::make_tmap_3d(&a, hidden_states, hidden, 1, rows, hidden_row_stride, hidden_row_stride, hlp::BM)) return NVLLM_E_CUDA;
+  if (!sm100::make_tmap_3d(&b, weight, hidden, 1, vocab, weight_row_stride, weight_row_stride, pl.bn)) return NVLLM_E_CUDA;
+  const bool is_long = hidden > hlp::kChunk;
+  static bool ready[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(hlp::head_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(hlp::head_logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
+    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "head_logprobs: cannot reserve shared memory: %s", cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  hlp::Params p{};
+  p.tokens = tokens;
+  p.temperatures = temperatures;
+  p.rows = static_cast<int>(rows);
+  p.vocab = static_cast<int>(vocab);
+  p.bn = pl.bn;
+  p.mt = pl.mt;
+  p.nt = pl.nt;
+  p.group = pl.group;
+  p.ng = pl.ng;
+  p.mb = pl.mb;
+  p.kb = pl.kb;
+  p.keep = pl.keep;
+  p.partial = static_cast<float4*>(workspace);
+  p.given = reinterpret_cast<float*>(p.partial + pl.slots * pl.rows_padded);
+  p.status = status;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (const int e = launch_kernel("head_logprobs", is_long ? hlp::head_logprobs_kernel<true> : hlp::head_logprobs_kernel<false>, dim3(pl.grid),
+                                  dim3(hlp::kThreads), hlp::SMEM, st, a, b, p))
+    return e;
+  const hlp::JoinParams j{p.partial, p.given, tokens, temperatures, p.rows, p.vocab, pl.slots, pl.rows_padded, logprobs, entropy, status};
+  return launch_kernel("head_logprobs", hlp::join_kernel, dim3(static_cast<unsigned>((rows + hlp::kJoinRows - 1) / hlp::kJoinRows)),
+                       dim3(hlp::kJoinRows * hlp::kJoinWarps), 0, st, j);
+}

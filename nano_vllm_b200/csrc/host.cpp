@@ -63,6 +63,8 @@ struct Api {
   decltype(&nvllm_prefill_fp8_workspace_bytes) prefill_fp8_workspace_bytes;
   decltype(&nvllm_step_maps) step_maps;
   decltype(&nvllm_token_logprobs) token_logprobs;
+  decltype(&nvllm_head_logprobs) head_logprobs;
+  decltype(&nvllm_head_logprobs_workspace_bytes) head_logprobs_workspace_bytes;
   decltype(&nvllm_copy_blocks) copy_blocks;
   decltype(&nvllm_fork_sequences) fork_sequences;
   decltype(&nvllm_free_list) free_list;
@@ -975,6 +977,46 @@ PyObject* token_logprobs(PyObject* const* a) {
   return as_tuple(out, 4);
 }
 
+// hidden_states, weight, tokens, temperatures, out
+PyObject* head_logprobs(PyObject* const* a) {
+  const at::Tensor &x = tensor(a[0], "hidden_states"), &w = tensor(a[1], "weight"), &tokens = tensor(a[2], "tokens");
+  const at::Tensor* temps = maybe_tensor(a[3], "temperatures");
+  require_cuda_bf16("hidden_states", x);
+  require_cuda_bf16("weight", w);
+  require_on("weight", w, x);
+  require(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "hidden_states [N, H] and weight [V, H]");
+  const int64_t rows = x.size(0), hidden = x.size(1), vocab = w.size(0);
+  require((x.stride(1) == 1 || hidden == 1) && (w.stride(1) == 1 || hidden == 1), "unit inner strides");
+  require(tokens.is_cuda() && tokens.scalar_type() == at::kLong && tokens.is_contiguous() && tokens.numel() == rows,
+          "tokens must be a contiguous CUDA int64 tensor, one per row");
+  require_on("tokens", tokens, x);
+  const float* t = row_temperatures(temps, rows, x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t need = api.head_logprobs_workspace_bytes(rows, hidden, vocab);
+  check(need);
+  at::Tensor out[2], scratch;
+  unlocked([&] {
+    const at::TensorOptions f32 = x.options().dtype(at::kFloat);
+    scratch = at::empty({need}, x.options().dtype(at::kByte));  // of the call
+    if (a[4] == Py_None) {
+      out[0] = at::empty({rows}, f32);
+      out[1] = at::empty({rows}, f32);
+    }
+    return 0;
+  });
+  if (a[4] != Py_None) {
+    const char* const of[2] = {"logprobs", "entropy"};
+    results(a[4], 2, "out must be the two tensors of an earlier call", out, of);
+    for (int i = 0; i < 2; ++i) require_result(of[i], out[i], at::kFloat, {rows}, x);
+  }
+  auto stride = [&](const at::Tensor& m) { return m.size(0) > 1 ? m.stride(0) : (hidden + 7) / 8 * 8; };
+  launch([&] {
+    return api.head_logprobs(x.data_ptr(), stride(x), w.data_ptr(), stride(w), ptr<int64_t>(tokens), t, rows, hidden, vocab,
+                             ptr<float>(out[0]), ptr<float>(out[1]), need > 0 ? scratch.data_ptr() : nullptr, need, stream_of(x));
+  });
+  return as_tuple(out, 2);
+}
+
 // ---- blocks of a cache ----------------------------------------------------------------------
 
 // The tensors of a cache: values [..., blocks, 256, Hkv, D] (bf16 or e4m3) and scales [..., blocks, Hkv, 16] (fp32).
@@ -1373,6 +1415,8 @@ PyObject* bind(PyObject* const* a) {  // library path, check
   RESOLVE(prefill_fp8_workspace_bytes);
   RESOLVE(step_maps);
   RESOLVE(token_logprobs);
+  RESOLVE(head_logprobs);
+  RESOLVE(head_logprobs_workspace_bytes);
   RESOLVE(copy_blocks);
   RESOLVE(fork_sequences);
   RESOLVE(free_list);
@@ -1434,6 +1478,7 @@ PyMethodDef methods[] = {
     METHOD(prefill_varlen_fp8, 12),
     METHOD(step_maps, 6),
     METHOD(token_logprobs, 5),
+    METHOD(head_logprobs, 5),
     METHOD(copy_blocks, 4),
     METHOD(fork_sequences, 6),
     METHOD(free_list, 5),

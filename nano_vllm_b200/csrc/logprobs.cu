@@ -16,10 +16,9 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <cfloat>
 #include <utility>
 
-#include "common.cuh"
+#include "logprobs.cuh"
 
 namespace nvllm {
 
@@ -53,12 +52,6 @@ __device__ __forceinline__ uint32_t lp_order(float x) {
 __device__ __forceinline__ float lp_value(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 // Orders by value, then lower place first.  Never 0.
 __device__ __forceinline__ uint64_t lp_key(float x, uint32_t place) { return (static_cast<uint64_t>(lp_order(x)) << 32) | (0xffffffffu - place); }
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 
 // 16 bytes of a row.
 template <typename T>
@@ -109,27 +102,6 @@ struct LpPiece<float> {
   }
 };
 
-// Maximum m (no less than the smallest finite number), s = sum exp2(c (x - m)), t = sum exp2(c (x - m)) (x - m).
-struct LpSums {
-  float m, s, t;
-  // Differences of -infinity: no weight, and 0 and not NaN times that.
-  static __device__ __forceinline__ float diff(float a, float m) { return max_nan(a - m, -3e38f); }
-  __device__ __forceinline__ void rescale(float to, float c) {
-    const float d = diff(m, to), f = fast_exp2(d * c);
-    s *= f;
-    t = fmaf(s, d, f * t);  // s first: times d it may not overflow
-    m = to;
-  }
-  __device__ __forceinline__ void join(float m2, float s2, float t2, float c) {
-    LpSums o{m2, s2, t2};
-    const float to = fmaxf(m, m2);
-    rescale(to, c);
-    o.rescale(to, c);
-    s += o.s;
-    t += o.t;
-  }
-};
-
 template <typename T>
 __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobParams p) {
   using P = LpPiece<T>;
@@ -151,8 +123,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   const int row = blockIdx.x / csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int me = crank * kLpThreads + tid, all = csize * kLpThreads;  // of the row's threads
   const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
-  const float temperature = p.temperatures ? p.temperatures[row] : 1.f;
-  const float inv_t = temperature > 0.f ? fminf(__frcp_rn(temperature), 1e38f) : 1.f;
+  const float inv_t = lp_inverse(p.temperatures, row);
   const float c = inv_t * 1.4426950408889634f;
   int64_t token = -1;
   float given = 0.f;
@@ -367,18 +338,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   // ---- results of the row
   sum = {s_sums[0][0], s_sums[0][1], s_sums[0][2]};
   for (int k = 1; k < csize; ++k) sum.join(s_sums[k][0], s_sums[k][1], s_sums[k][2], c);
-  const float log_z = static_cast<float>(log(static_cast<double>(sum.s)));
-  if (tid == 0) {
-    float lp = 0.f;
-    if (token >= p.vocab) {
-      lp = NAN;
-      atomicOr(p.status, NVLLM_STATUS_BAD_TOKEN);
-    } else if (token >= 0) {
-      lp = (given - sum.m) * inv_t - log_z;
-    }
-    p.logprobs[row] = lp;
-    p.entropy[row] = log_z - inv_t * __fdiv_rn(sum.t, sum.s);
-  }
+  const float log_z = sum.log_z();
+  if (tid == 0) sum.results(row, token, given, inv_t, log_z, p.vocab, p.logprobs, p.entropy, p.status);
   const int keys = csize * top;
   for (int n = tid; n < keys; n += kLpThreads) {
     const uint64_t key = s_list[n / top][n % top];

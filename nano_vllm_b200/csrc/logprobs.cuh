@@ -1,0 +1,57 @@
+// Running softmax statistics of a row with its entropy, shared by the kernels that score tokens.
+#pragma once
+
+#include <cfloat>
+
+#include "common.cuh"
+
+namespace nvllm {
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// 1 / T of a row; a temperature that is not above 0, or none, counts as 1.
+__device__ __forceinline__ float lp_inverse(const float* temperatures, int64_t row) {
+  const float t = temperatures ? temperatures[row] : 1.f;
+  return t > 0.f ? fminf(__frcp_rn(t), 1e38f) : 1.f;
+}
+
+// Maximum m (no less than the smallest finite number), s = sum exp2(c (x - m)), t = sum exp2(c (x - m)) (x - m).
+struct LpSums {
+  float m, s, t;
+  // Differences of -infinity: no weight, and 0 and not NaN times that.
+  static __device__ __forceinline__ float diff(float a, float m) { return max_nan(a - m, -3e38f); }
+  __device__ __forceinline__ void rescale(float to, float c) {
+    const float d = diff(m, to), f = fast_exp2(d * c);
+    s *= f;
+    t = fmaf(s, d, f * t);  // s first: times d it may not overflow
+    m = to;
+  }
+  __device__ __forceinline__ void join(float m2, float s2, float t2, float c) {
+    LpSums o{m2, s2, t2};
+    const float to = fmaxf(m, m2);
+    rescale(to, c);
+    o.rescale(to, c);
+    s += o.s;
+    t += o.t;
+  }
+  // ln of the sum, in 64 bits: where one token has nearly all of it the logarithm is what is left of 1.
+  __device__ __forceinline__ float log_z() const { return static_cast<float>(log(static_cast<double>(s))); }
+  __device__ __forceinline__ void results(int64_t row, int64_t token, float given, float inv_t, float log_z, int vocab, float* logprobs,
+                                          float* entropy, int* status) const {
+    float lp = 0.f;
+    if (token >= vocab) {
+      lp = NAN;
+      atomicOr(status, NVLLM_STATUS_BAD_TOKEN);
+    } else if (token >= 0) {
+      lp = (given - m) * inv_t - log_z;
+    }
+    logprobs[row] = lp;
+    entropy[row] = log_z - inv_t * __fdiv_rn(t, s);
+  }
+};
+
+}  // namespace nvllm

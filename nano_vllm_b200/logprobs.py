@@ -17,6 +17,11 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: torch.Tensor  # fp32 [N, top]: theirs
 
 
+class HeadLogprobs(NamedTuple):
+    logprobs: torch.Tensor  # fp32 [N]
+    entropy: torch.Tensor   # fp32 [N]
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, temperatures: torch.Tensor | None = None,
                    out: Sequence[torch.Tensor] | None = None) -> TokenLogprobs:
     """Under ``softmax(logits / T)`` of every row of ``logits`` ``[N, V]`` (bf16 or fp32): the log probability of its token of
@@ -29,3 +34,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     -infinity has no distribution and NaN for results; its ``top_tokens`` go by the logits, NaN like -infinity.
     ``out``: the four result tensors of an earlier call or of a graph, else they are made."""
     return TokenLogprobs._make(_native(logits).token_logprobs(logits, tokens, top, temperatures, out))
+
+
+def head_logprobs(hidden_states: torch.Tensor, weight: torch.Tensor, tokens: torch.Tensor, temperatures: torch.Tensor | None = None,
+                  out: Sequence[torch.Tensor] | None = None) -> HeadLogprobs:
+    """``token_logprobs`` of ``hidden_states @ weight.T`` (bf16 ``[N, H]`` and ``[V, H]``, H a multiple of 8), without those logits: they
+    are summed in fp32, not rounded, and never written.  For scoring what has been given: all positions of a prompt, answers
+    of another engine, the reference side of a comparison of two models; nano-vllm computes logits of a prompt's last position only
+    (``ParallelLMHead.forward``, nanovllm/layers/embed_head.py:68-88).  Tokens, temperatures and ``out`` (two tensors) as there."""
+    return HeadLogprobs._make(_native(hidden_states).head_logprobs(hidden_states, weight, tokens, temperatures, out))
