@@ -16,7 +16,6 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
-#include <utility>
 
 #include "logprobs.cuh"
 
@@ -107,19 +106,19 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   using P = LpPiece<T>;
   constexpr int N = P::N, C = 4;
   namespace cg = cooperative_groups;
-  __shared__ uint64_t s_bounds[kLpGroups];
-  __shared__ uint64_t s_cand[kLpCands];
-  __shared__ uint64_t s_list[kLpMaxCluster][kLpMaxTop];  // of the first block: every block's alternatives in order, 0 behind the last
+  __shared__ __align__(16) uint64_t s_bounds[kLpGroups];
+  __shared__ uint64_t s_cand[kLpCands];  // of the first block
   __shared__ float s_sums[kLpMaxCluster][3];
   __shared__ float s_warp[kLpThreads / 32][3];
   __shared__ uint16_t s_slot[kLpThreads];
   __shared__ uint64_t s_tau;
   __shared__ int s_slots, s_cands;
-  __shared__ uint64_t s_most[kLpThreads / 32];
+  __shared__ uint64_t s_most[kLpThreads / 32], s_all[2 * kLpMaxCluster];
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
-  auto started = cluster.barrier_arrive();  // waited for before another block's shared memory is written
   const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank());
+  const bool several = csize > 1;
+  if (several) cluster.barrier_arrive();  // waited for before another block's shared memory is written
   const int row = blockIdx.x / csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int me = crank * kLpThreads + tid, all = csize * kLpThreads;  // of the row's threads
   const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
@@ -224,7 +223,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   if (me == 0 && tail) one(cut_piece(pieces - 1), pieces - 1);
   fold();
 
-  // ---- sums of the block
+  // ---- sums of the block, and the largest (maximum, piece) of every group of threads
 #pragma unroll
   for (int sh = 16; sh > 0; sh >>= 1) {
     const float m2 = __shfl_xor_sync(0xffffffffu, sum.m, sh), a = __shfl_xor_sync(0xffffffffu, sum.s, sh), b = __shfl_xor_sync(0xffffffffu, sum.t, sh);
@@ -235,126 +234,137 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
     s_warp[warp][1] = sum.s;
     s_warp[warp][2] = sum.t;
   }
-
-  // ---- the block's alternatives, in order
   const int top = p.top;
-  uint64_t mine = 0;
+  const uint64_t mine = any ? lp_key(best, static_cast<uint32_t>(at)) : 0;
+  auto sync = [&]() {
+    if (several) cluster.sync();
+    else __syncthreads();
+  };
+  if (several) cluster.barrier_wait();
   if (top > 0) {
-    constexpr int G = kLpThreads / kLpGroups;  // threads of a group
-    mine = any ? lp_key(best, static_cast<uint32_t>(at)) : 0;
+    const int size = csize * kLpThreads / kLpGroups;  // threads of a group: 2 to 16
     uint64_t most = mine;
-#pragma unroll
-    for (int sh = 1; sh < G; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
-    if (tid % G == 0) s_bounds[tid / G] = most;
-    __syncthreads();
-    int above = 0;
-#pragma unroll 8
-    for (int k = tid % G; k < kLpGroups; k += G) above += s_bounds[k] > most;
-#pragma unroll
-    for (int sh = 1; sh < G; sh <<= 1) above += __shfl_xor_sync(0xffffffffu, above, sh);
-    if (tid % G == 0 && above == top - 1 && most) s_tau = most;  // one group: keys differ
-    __syncthreads();
-    const uint64_t tau = s_tau;
-    if (mine && mine >= tau) s_slot[atomicAdd(&s_slots, 1)] = static_cast<uint16_t>(tid);
-    __syncthreads();
-    const int each = (whole + all - 1) / all + 2;  // pieces of a thread, the cut ones counted
-    const int total = s_slots * each;
-    // calls f(element's key) for the elements of piece n of the listed threads that reach the bound
-    auto look = [&](int n, auto&& f) {
-      const int who = crank * kLpThreads + s_slot[n / each], i = n % each;
-      int g = head + who + i * all;
-      uint4 w;
-      if (i >= each - 2) {
-        if (who != 0 || !(i == each - 1 ? tail : head)) return;
-        g = i == each - 1 ? pieces - 1 : 0;
-        w = cut_piece(g);
-      } else {
-        if (g >= head + whole) return;
-        w = __ldg(base + g);
-      }
-      float e[N];
-      P::unpack(w, e);
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        const int id = g * N + k - shift;
-        if (id >= 0 && id < p.vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) f(lp_key(e[k], static_cast<uint32_t>(id)));
-      }
-    };
-    for (int n = tid; n < total; n += kLpThreads)
-      look(n, [&](uint64_t key) {
-        const int k = atomicAdd(&s_cands, 1);
-        if (k < kLpCands) s_cand[k] = key;
-      });
-    __syncthreads();
-    const int cands = s_cands;
-    uint64_t* list = s_list[0];
-    if (cands <= kLpCands) {
-      for (int n = tid; n < max(cands, top); n += kLpThreads) {
-        if (n >= cands) {
-          list[n] = 0;
-          continue;
-        }
-        const uint64_t key = s_cand[n];
-        int rank = 0;
-        for (int k = 0; k < cands; ++k) rank += s_cand[k] > key;
-        if (rank < top) list[rank] = key;
-      }
-    } else {  // the largest ones stand close together in few threads: one after the other
-      uint64_t before = ~0ull;
-      for (int r = 0; r < top; ++r) {
-        uint64_t most = 0;
-        for (int n = tid; n < total; n += kLpThreads)
-          look(n, [&](uint64_t key) {
-            if (key < before && key > most) most = key;
-          });
-#pragma unroll
-        for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
-        if (lane == 0) s_most[warp] = most;
-        __syncthreads();
-        for (int k = 0; k < kLpThreads / 32; ++k) most = max(most, s_most[k]);
-        before = most;
-        if (tid == 0) list[r] = most;
-        __syncthreads();
-      }
-    }
+    for (int sh = 1; sh < size; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
+    // every block of the row gets all groups' (a lane for each)
+    const int to = tid % size, group = me / size;
+    if (to < csize) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[group] = most;
   }
   __syncthreads();
-  pdl_trigger();
-  cluster.barrier_wait(std::move(started));
   if (tid == 0) {
     for (int k = 1; k < kLpThreads / 32; ++k) sum.join(s_warp[k][0], s_warp[k][1], s_warp[k][2], c);
-    float* to = cluster.map_shared_rank(&s_sums[0][0], 0) + 3 * crank;
+    float* to = (several ? cluster.map_shared_rank(&s_sums[0][0], 0) : &s_sums[0][0]) + 3 * crank;
     to[0] = sum.m;
     to[1] = sum.s;
     to[2] = sum.t;
   }
-  if (crank != 0) {
-    uint64_t* to = cluster.map_shared_rank(&s_list[0][0], 0) + crank * kLpMaxTop;
-    for (int k = tid; k < top; k += kLpThreads) to[k] = s_list[0][k];
-  }
-  cluster.sync();
-  if (crank != 0) return;
+  pdl_trigger();
+  sync();
 
-  // ---- results of the row
-  sum = {s_sums[0][0], s_sums[0][1], s_sums[0][2]};
-  for (int k = 1; k < csize; ++k) sum.join(s_sums[k][0], s_sums[k][1], s_sums[k][2], c);
-  const float log_z = sum.log_z();
-  if (tid == 0) sum.results(row, token, given, inv_t, log_z, p.vocab, p.logprobs, p.entropy, p.status);
-  const int keys = csize * top;
-  for (int n = tid; n < keys; n += kLpThreads) {
-    const uint64_t key = s_list[n / top][n % top];
-    if (!key) continue;
-    int rank = n;
-    if (csize > 1) {
-      rank = 0;
-      for (int b = 0; b < csize; ++b)
-        for (int k = 0; k < top && s_list[b][k] > key; ++k) ++rank;
-      if (rank >= top) continue;
+  // ---- the bound that `top` elements of the row reach, and the elements that do: to the first block's list
+  int* cands_at = several ? cluster.map_shared_rank(&s_cands, 0) : &s_cands;
+  uint64_t* cand_at = several ? cluster.map_shared_rank(s_cand, 0) : s_cand;
+  uint64_t tau = 0;
+  int each = 0, total = 0;
+  // calls f(element's key) for the elements that reach the bound in piece n of the listed threads
+  auto look = [&](int n, auto&& f) {
+    const int who = crank * kLpThreads + s_slot[n / each], i = n % each;
+    int g = head + who + i * all;
+    uint4 w;
+    if (i >= each - 2) {
+      if (who != 0 || !(i == each - 1 ? tail : head)) return;
+      g = i == each - 1 ? pieces - 1 : 0;
+      w = cut_piece(g);
+    } else {
+      if (g >= head + whole) return;
+      w = __ldg(base + g);
     }
+    float e[N];
+    P::unpack(w, e);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int id = g * N + k - shift;
+      if (id >= 0 && id < p.vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) f(lp_key(e[k], static_cast<uint32_t>(id)));
+    }
+  };
+  if (top > 0) {
+    {  // of two threads a group each: how many groups are above it
+      const ulonglong2* bounds = reinterpret_cast<const ulonglong2*>(s_bounds);
+      const uint64_t it = s_bounds[tid / 2];
+      int above = 0;
+#pragma unroll 8
+      for (int k = tid % 2; k < kLpGroups / 2; k += 2) {
+        const ulonglong2 v = bounds[k];
+        above += (v.x > it) + (v.y > it);
+      }
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      if (tid % 2 == 0 && above == top - 1 && it) s_tau = it;  // one group: keys differ
+    }
+    __syncthreads();
+    tau = s_tau;
+    if (mine && mine >= tau) s_slot[atomicAdd(&s_slots, 1)] = static_cast<uint16_t>(tid);
+    __syncthreads();
+    each = (whole + all - 1) / all + 2;  // pieces of a thread, the cut ones counted
+    total = s_slots * each;
+    for (int n = tid; n < total; n += kLpThreads)
+      look(n, [&](uint64_t key) {
+        const int k = atomicAdd(cands_at, 1);
+        if (k < kLpCands) cand_at[k] = key;
+      });
+  }
+  sum = {s_sums[0][0], s_sums[0][1], s_sums[0][2]};
+  float log_z = 0.f;
+  if (crank == 0) {
+    for (int k = 1; k < csize; ++k) sum.join(s_sums[k][0], s_sums[k][1], s_sums[k][2], c);
+    log_z = sum.log_z();
+    if (tid == 0) sum.results(row, token, given, inv_t, log_z, p.vocab, p.logprobs, p.entropy, p.status);
+  }
+  if (top == 0) return;
+  sync();
+  const int cands = *cands_at;
+  auto put = [&](int rank, uint64_t key) {
     const int64_t to = static_cast<int64_t>(row) * top + rank;
     p.top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
     p.top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - sum.m) * inv_t - log_z;
+  };
+  if (cands <= kLpCands) {
+    if (several) cluster.barrier_arrive();  // the first block's counter has been read
+    if (crank != 0) {
+      cluster.barrier_wait();
+      return;
+    }
+    // ranks by counting, eight threads a candidate
+    for (int n = tid / 8; n < ((cands + 3) & ~3); n += kLpThreads / 8) {
+      const uint64_t key = n < cands ? s_cand[n] : 0;
+      int rank = 0;
+      for (int k = tid % 8; k < cands; k += 8) rank += s_cand[k] > key;
+#pragma unroll
+      for (int sh = 1; sh < 8; sh <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, sh);
+      if (tid % 8 == 0 && n < cands && rank < top) put(rank, key);
+    }
+    if (several) cluster.barrier_wait();
+    return;
   }
+  // The largest ones stand close together in few threads: one after the other.
+  uint64_t before = ~0ull;
+  for (int r = 0; r < top; ++r) {
+    uint64_t most = 0;
+    for (int n = tid; n < total; n += kLpThreads)
+      look(n, [&](uint64_t key) {
+        if (key < before && key > most) most = key;
+      });
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
+    if (lane == 0) s_most[warp] = most;
+    __syncthreads();
+    for (int k = 0; k < kLpThreads / 32; ++k) most = max(most, s_most[k]);
+    if (tid < csize) (several ? cluster.map_shared_rank(s_all, tid) : s_all)[(r & 1) * kLpMaxCluster + crank] = most;
+    sync();
+    most = 0;
+    for (int k = 0; k < csize; ++k) most = max(most, s_all[(r & 1) * kLpMaxCluster + k]);
+    before = most;
+    if (crank == 0 && tid == 0) put(r, most);
+  }
+  sync();
 }
 
 }  // namespace nvllm
