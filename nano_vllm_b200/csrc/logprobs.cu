@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "logprobs.cuh"
 
@@ -33,6 +34,7 @@ struct LogprobParams {
   const int64_t* tokens;
   const float* temperatures;  // nullable
   int vocab, top;
+  int groups;  // of the threads that read a row, whose maxima give the bound: 32 to 128
   float* logprobs;
   float* entropy;
   int64_t* top_tokens;
@@ -71,6 +73,13 @@ struct LpPiece<__nv_bfloat16> {
     const __nv_bfloat162 m = __hmax2(__hmax2(h(w.x), h(w.y)), __hmax2(h(w.z), h(w.w)));
     return fmaxf(__low2float(m), __high2float(m));
   }
+  static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
+    auto f = [](uint32_t u, uint32_t v) {
+      const __nv_bfloat162 m = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&u), *reinterpret_cast<__nv_bfloat162*>(&v));
+      return *reinterpret_cast<const uint32_t*>(&m);
+    };
+    return make_uint4(f(a.x, b.x), f(a.y, b.y), f(a.z, b.z), f(a.w, b.w));
+  }
   // -infinity in the places below lo and from hi on
   static __device__ __forceinline__ uint4 cut(uint4 w, int lo, int hi) {
     uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -92,6 +101,10 @@ struct LpPiece<float> {
   static __device__ __forceinline__ float max(const uint4& w) {
     return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
   }
+  static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
+    auto f = [](uint32_t u, uint32_t v) { return __float_as_uint(fmaxf(__uint_as_float(u), __uint_as_float(v))); };
+    return make_uint4(f(a.x, b.x), f(a.y, b.y), f(a.z, b.z), f(a.w, b.w));
+  }
   static __device__ __forceinline__ uint4 cut(uint4 w, int lo, int hi) {
     uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
@@ -101,10 +114,10 @@ struct LpPiece<float> {
   }
 };
 
-template <typename T>
+template <typename T, bool TOP>
 __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobParams p) {
   using P = LpPiece<T>;
-  constexpr int N = P::N, C = 4;
+  constexpr int N = P::N, C = TOP ? 3 : 4;
   namespace cg = cooperative_groups;
   __shared__ __align__(16) uint64_t s_bounds[kLpGroups];
   __shared__ uint64_t s_cand[kLpCands];  // of the first block
@@ -112,6 +125,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   __shared__ float s_warp[kLpThreads / 32][3];
   __shared__ uint16_t s_slot[kLpThreads];
   __shared__ uint64_t s_tau;
+  __shared__ float s_m, s_log_z;
   __shared__ int s_slots, s_cands;
   __shared__ uint64_t s_most[kLpThreads / 32], s_all[2 * kLpMaxCluster];
   pdl_wait();
@@ -119,21 +133,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank());
   const bool several = csize > 1;
   if (several) cluster.barrier_arrive();  // waited for before another block's shared memory is written
-  const int row = blockIdx.x / csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int me = crank * kLpThreads + tid, all = csize * kLpThreads;  // of the row's threads
+  const int row = blockIdx.x / csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+  const int me = crank * threads + tid, all = csize * threads;  // of the row's threads
   const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
-  const float inv_t = lp_inverse(p.temperatures, row);
-  const float c = inv_t * 1.4426950408889634f;
-  int64_t token = -1;
-  float given = 0.f;
-  if (me == 0) {
-    token = p.tokens[row];
-    if (token >= 0 && token < p.vocab) given = static_cast<float>(x[token]);
-  }
-  if (tid == 0) {
-    s_tau = 0;
-    s_slots = s_cands = 0;
-  }
 
   // Pieces start on 16-byte boundaries: what lies before and behind the row in the first and last one counts as -infinity.
   const int shift = static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15u) / sizeof(T));
@@ -145,90 +147,143 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   const int whole = pieces - head - tail;
   auto cut_piece = [&](int g) { return P::cut(__ldg(base + g), g == 0 ? shift : 0, g == pieces - 1 ? last_hi : N); };
 
+  // A thread takes C pieces at a time, loaded one step ahead.
+  const uint4* from = base + head;
+  const uint4 nothing = P::cut(make_uint4(0, 0, 0, 0), 0, 0);
+  uint4 next[C];
+  const int step = C * all;
+  auto load = [&](int j) {
+#pragma unroll
+    for (int k = 0; k < C; ++k) next[k] = j + k * all < whole ? __ldg(from + j + k * all) : nothing;
+  };
+  int i = me;
+  load(i);
+  const float inv_t = lp_inverse(p.temperatures, row);
+  const float c = inv_t * 1.4426950408889634f;
+  int64_t token = -1;
+  float given = 0.f;
+  if (crank == 0 && tid == threads - 32) {  // which writes the results
+    token = p.tokens[row];
+    if (token >= 0 && token < p.vocab) given = static_cast<float>(x[token]);
+  }
+  if (tid == 0) {
+    s_tau = 0;
+    s_slots = s_cands = 0;
+  }
+
   LpSums sum{-FLT_MAX, 0.f, 0.f};
   float best = -INFINITY;
   const bool any = me == 0 || me < whole;
-  int at = me == 0 ? 0 : head + me;  // the first piece of this thread
-  uint64_t s2 = 0, t2 = 0;  // of pairs of elements
-  auto add = [&](const uint4& w) {
+  int at = head + me;  // the first piece with the largest element so far
+  const uint64_t c2 = pack2(c, c);
+  // Sums over pieces.  A masked element's difference is -infinity, whose product with its weight of 0 is NaN: such pieces are
+  // read and summed again with the differences kept finite (which costs the others an instruction an element).
+  auto add = [&](const uint4& w, auto finite, uint64_t& s2, uint64_t& t2) {
+    const uint64_t minus_m = pack2(-sum.m, -sum.m);
     float e[N];
     P::unpack(w, e);
-    const uint64_t minus_m = pack2(-sum.m, -sum.m), c2 = pack2(c, c);
 #pragma unroll
     for (int k = 0; k < N; k += 2) {
-      float a, b, ya, yb;
-      const uint64_t y = add2(pack2(e[k], e[k + 1]), minus_m);
-      unpack2(y, ya, yb);
-      const uint64_t y2 = pack2(max_nan(ya, -3e38f), max_nan(yb, -3e38f));
-      unpack2(mul2(y2, c2), a, b);
+      uint64_t y = add2(pack2(e[k], e[k + 1]), minus_m);
+      float a, b;
+      if constexpr (decltype(finite)::value) {
+        unpack2(y, a, b);
+        y = pack2(max_nan(a, -3e38f), max_nan(b, -3e38f));
+      }
+      unpack2(mul2(y, c2), a, b);
       const uint64_t w2 = pack2(fast_exp2(a), fast_exp2(b));
       s2 = add2(s2, w2);
-      t2 = fma2(w2, y2, t2);
+      t2 = fma2(w2, y, t2);
     }
   };
-  auto fold = [&]() {  // the pairs' sums into sum
+  auto finish = [&](uint64_t s2, uint64_t t2) {
+    float a, b, u, v;
+    unpack2(s2, a, b);
+    unpack2(t2, u, v);
+    if (u + v != u + v) return false;
+    sum.s += a + b;
+    sum.t += u + v;
+    return true;
+  };
+  auto slow = [&](const uint4& w) {
+    uint64_t s2 = 0, t2 = 0;
+    add(w, std::true_type{}, s2, t2);
     float a, b;
     unpack2(s2, a, b);
     sum.s += a + b;
     unpack2(t2, a, b);
     sum.t += a + b;
-    s2 = t2 = 0;
   };
-  auto grow = [&](float to) {
-    to = fmaxf(to, sum.m);
-    const float d = LpSums::diff(sum.m, to), f = fast_exp2(d * c);
-    const uint64_t f2 = pack2(f, f), d2 = pack2(d, d);
-    s2 = mul2(s2, f2);
-    t2 = fma2(s2, d2, mul2(t2, f2));
-    sum.m = to;
-  };
-  auto note = [&](float most, int g) {
-    if (most > best) {
-      best = most;
-      at = g;
+  // The maximum in use is the warp's: that grows a few times a row, a lane's in nearly every step of some lane.
+  auto grow = [&](float most) {
+    if (__any_sync(0xffffffffu, most > sum.m)) {
+      float m = fmaxf(most, sum.m);
+#pragma unroll
+      for (int sh = 16; sh > 0; sh >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
+      sum.rescale(m, c);
     }
   };
-  auto one = [&](const uint4& w, int g) {
-    const float most = P::max(w);
-    note(most, g);
-    grow(best);
-    add(w);
-  };
-  if (me == 0 && head) one(cut_piece(0), 0);
-  {
-    const uint4* from = base + head;
-    uint4 next[C];
-    int i = me;
-    const int step = C * all;
-    auto load = [&](int j) {
+  for (; i - lane < whole; i += step) {
+    uint4 raw[C];
 #pragma unroll
-      for (int k = 0; k < C; ++k) next[k] = __ldg(from + j + k * all);
-    };
-    const bool first = i + (C - 1) * all < whole;
-    if (first) load(i);
-    while (i + (C - 1) * all < whole) {
-      uint4 raw[C];
+    for (int k = 0; k < C; ++k) raw[k] = next[k];
+    if (i + step - lane < whole) load(i + step);
+    if constexpr (TOP) {
+      float largest = -INFINITY;
 #pragma unroll
-      for (int k = 0; k < C; ++k) raw[k] = next[k];
-      if (i + step + (C - 1) * all < whole) load(i + step);
+      for (int k = 0; k < C; ++k) {
+        const float most = P::max(raw[k]);
+        if (most > best) {
+          best = most;
+          at = head + i + k * all;
+        }
+        largest = fmaxf(largest, most);
+      }
+      grow(largest);
+    } else {
+      uint4 m = raw[0];
 #pragma unroll
-      for (int k = 0; k < C; ++k) note(P::max(raw[k]), head + i + k * all);
-      grow(best);
-#pragma unroll
-      for (int k = 0; k < C; ++k) add(raw[k]);
-      i += step;
+      for (int k = 1; k < C; ++k) m = P::larger(m, raw[k]);
+      grow(P::max(m));
     }
-    for (; i < whole; i += all) one(__ldg(from + i), head + i);
+    uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+    for (int k = 0; k < C; ++k) add(raw[k], std::false_type{}, s2, t2);
+    if (!finish(s2, t2)) {
+#pragma unroll 1
+      for (int k = 0; k < C; ++k)
+        if (i + k * all < whole) slow(__ldg(from + i + k * all));
+    }
   }
-  if (me == 0 && tail) one(cut_piece(pieces - 1), pieces - 1);
-  fold();
+  if (crank == 0 && warp == 0 && (head || tail)) {
+    const uint4 w0 = head && lane == 0 ? cut_piece(0) : nothing, w1 = tail && lane == 0 ? cut_piece(pieces - 1) : nothing;
+    const float first = P::max(w0), last = P::max(w1);
+    if (head && lane == 0 && !(first < best)) {  // the lowest piece, whenever it is looked at
+      best = fmaxf(first, -INFINITY);
+      at = 0;
+    }
+    if (last > best) {
+      best = last;
+      at = pieces - 1;
+    }
+    grow(fmaxf(first, last));
+    slow(w0);
+    slow(w1);
+  }
 
   // ---- sums of the block, and the largest (maximum, piece) of every group of threads
+  auto join_warp = [&](LpSums& v) {  // over the lanes
+    float m = v.m;
 #pragma unroll
-  for (int sh = 16; sh > 0; sh >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, sum.m, sh), a = __shfl_xor_sync(0xffffffffu, sum.s, sh), b = __shfl_xor_sync(0xffffffffu, sum.t, sh);
-    sum.join(m2, a, b, c);
-  }
+    for (int sh = 16; sh > 0; sh >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
+    v.rescale(m, c);
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) {
+      v.s += __shfl_xor_sync(0xffffffffu, v.s, sh);
+      v.t += __shfl_xor_sync(0xffffffffu, v.t, sh);
+    }
+  };
+  join_warp(sum);
   if (lane == 0) {
     s_warp[warp][0] = sum.m;
     s_warp[warp][1] = sum.s;
@@ -241,21 +296,24 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
     else __syncthreads();
   };
   if (several) cluster.barrier_wait();
-  if (top > 0) {
-    const int size = csize * kLpThreads / kLpGroups;  // threads of a group: 2 to 16
+  if constexpr (TOP) {
+    const int size = all / p.groups;  // threads of a group: 1 to 32
     uint64_t most = mine;
     for (int sh = 1; sh < size; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
-    // every block of the row gets all groups' (a lane for each)
-    const int to = tid % size, group = me / size;
-    if (to < csize) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[group] = most;
+    // every block of the row gets all groups'
+    for (int to = tid % size; to < csize; to += size) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[me / size] = most;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int k = 1; k < kLpThreads / 32; ++k) sum.join(s_warp[k][0], s_warp[k][1], s_warp[k][2], c);
-    float* to = (several ? cluster.map_shared_rank(&s_sums[0][0], 0) : &s_sums[0][0]) + 3 * crank;
-    to[0] = sum.m;
-    to[1] = sum.s;
-    to[2] = sum.t;
+  if (warp == 0) {
+    const int w = min(lane, threads / 32 - 1);
+    sum = {s_warp[w][0], lane == w ? s_warp[w][1] : 0.f, lane == w ? s_warp[w][2] : 0.f};
+    join_warp(sum);
+    if (lane == 0) {
+      float* to = (several ? cluster.map_shared_rank(&s_sums[0][0], 0) : &s_sums[0][0]) + 3 * crank;
+      to[0] = sum.m;
+      to[1] = sum.s;
+      to[2] = sum.t;
+    }
   }
   pdl_trigger();
   sync();
@@ -264,19 +322,20 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   int* cands_at = several ? cluster.map_shared_rank(&s_cands, 0) : &s_cands;
   uint64_t* cand_at = several ? cluster.map_shared_rank(s_cand, 0) : s_cand;
   uint64_t tau = 0;
-  int each = 0, total = 0;
+  float each_inv = 0.f;
+  int each = 0, total = 0, looked = 0;
   // calls f(element's key) for the elements that reach the bound in piece n of the listed threads
   auto look = [&](int n, auto&& f) {
-    const int who = crank * kLpThreads + s_slot[n / each], i = n % each;
-    int g = head + who + i * all;
+    int g;
     uint4 w;
-    if (i >= each - 2) {
-      if (who != 0 || !(i == each - 1 ? tail : head)) return;
-      g = i == each - 1 ? pieces - 1 : 0;
-      w = cut_piece(g);
-    } else {
+    if (n < total) {
+      const int nth = static_cast<int>((static_cast<float>(n) + 0.5f) * each_inv), who = crank * threads + s_slot[nth];
+      g = head + who + (n - nth * each) * all;
       if (g >= head + whole) return;
       w = __ldg(base + g);
+    } else {  // the cut pieces, whether they are in a listed thread or not
+      g = n == total && head ? 0 : pieces - 1;
+      w = cut_piece(g);
     }
     float e[N];
     P::unpack(w, e);
@@ -286,13 +345,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       if (id >= 0 && id < p.vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) f(lp_key(e[k], static_cast<uint32_t>(id)));
     }
   };
-  if (top > 0) {
-    {  // of two threads a group each: how many groups are above it
-      const ulonglong2* bounds = reinterpret_cast<const ulonglong2*>(s_bounds);
-      const uint64_t it = s_bounds[tid / 2];
+  if constexpr (TOP) {
+    // how many groups are above one: two threads count
+    const ulonglong2* bounds = reinterpret_cast<const ulonglong2*>(s_bounds);
+    for (int n = tid / 2; n < p.groups; n += threads / 2) {
+      const uint64_t it = s_bounds[n];
       int above = 0;
 #pragma unroll 8
-      for (int k = tid % 2; k < kLpGroups / 2; k += 2) {
+      for (int k = tid % 2; k < p.groups / 2; k += 2) {
         const ulonglong2 v = bounds[k];
         above += (v.x > it) + (v.y > it);
       }
@@ -303,28 +363,34 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
     tau = s_tau;
     if (mine && mine >= tau) s_slot[atomicAdd(&s_slots, 1)] = static_cast<uint16_t>(tid);
     __syncthreads();
-    each = (whole + all - 1) / all + 2;  // pieces of a thread, the cut ones counted
+    each = (whole + all - 1) / all;  // pieces of a thread
+    each_inv = __frcp_rn(static_cast<float>(each));
     total = s_slots * each;
-    for (int n = tid; n < total; n += kLpThreads)
+    looked = total + (crank == 0 ? head + tail : 0);
+    for (int n = tid; n < looked; n += threads)
       look(n, [&](uint64_t key) {
         const int k = atomicAdd(cands_at, 1);
         if (k < kLpCands) cand_at[k] = key;
       });
   }
-  sum = {s_sums[0][0], s_sums[0][1], s_sums[0][2]};
-  float log_z = 0.f;
-  if (crank == 0) {
-    for (int k = 1; k < csize; ++k) sum.join(s_sums[k][0], s_sums[k][1], s_sums[k][2], c);
-    log_z = sum.log_z();
-    if (tid == 0) sum.results(row, token, given, inv_t, log_z, p.vocab, p.logprobs, p.entropy, p.status);
+  if (crank == 0 && warp == threads / 32 - 1) {  // the warp with least to look at
+    const int b = min(lane, csize - 1);
+    sum = {s_sums[b][0], lane == b ? s_sums[b][1] : 0.f, lane == b ? s_sums[b][2] : 0.f};
+    join_warp(sum);
+    if (lane == 0) {
+      const float log_z = sum.log_z();
+      s_log_z = log_z;
+      s_m = sum.m;
+      sum.results(row, token, given, inv_t, log_z, p.vocab, p.logprobs, p.entropy, p.status);
+    }
   }
-  if (top == 0) return;
+  if constexpr (!TOP) return;
   sync();
   const int cands = *cands_at;
   auto put = [&](int rank, uint64_t key) {
     const int64_t to = static_cast<int64_t>(row) * top + rank;
     p.top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
-    p.top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - sum.m) * inv_t - log_z;
+    p.top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - s_m) * inv_t - s_log_z;
   };
   if (cands <= kLpCands) {
     if (several) cluster.barrier_arrive();  // the first block's counter has been read
@@ -333,7 +399,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       return;
     }
     // ranks by counting, eight threads a candidate
-    for (int n = tid / 8; n < ((cands + 3) & ~3); n += kLpThreads / 8) {
+    for (int n = tid / 8; n < ((cands + 3) & ~3); n += threads / 8) {
       const uint64_t key = n < cands ? s_cand[n] : 0;
       int rank = 0;
       for (int k = tid % 8; k < cands; k += 8) rank += s_cand[k] > key;
@@ -348,7 +414,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   uint64_t before = ~0ull;
   for (int r = 0; r < top; ++r) {
     uint64_t most = 0;
-    for (int n = tid; n < total; n += kLpThreads)
+    for (int n = tid; n < looked; n += threads)
       look(n, [&](uint64_t key) {
         if (key < before && key > most) most = key;
       });
@@ -356,7 +422,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
     for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
     if (lane == 0) s_most[warp] = most;
     __syncthreads();
-    for (int k = 0; k < kLpThreads / 32; ++k) most = max(most, s_most[k]);
+    for (int k = 0; k < threads / 32; ++k) most = max(most, s_most[k]);
     if (tid < csize) (several ? cluster.map_shared_rank(s_all, tid) : s_all)[(r & 1) * kLpMaxCluster + crank] = most;
     sync();
     most = 0;
@@ -399,22 +465,27 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   p.top_tokens = top_tokens;
   p.top_logprobs = top_logprobs;
   const int64_t pieces = (static_cast<int64_t>(vocab) + (logits_are_fp32 ? 3 : 7)) / (logits_are_fp32 ? 4 : 8);
-  int csize = kLpMaxCluster;
+  int csize = kLpMaxCluster, threads = kLpThreads;
   while (csize > 1 && (static_cast<int64_t>(rows) * csize > 4ll * sms || pieces < 2ll * csize * kLpThreads)) csize /= 2;
+  while (csize == 1 && threads > 64 && pieces < 8ll * threads) threads /= 2;
+  const int all = csize * threads;
+  p.groups = top <= 20 ? std::max(32, all / 32) : std::min(kLpGroups, all);
   if (static_cast<int64_t>(rows) * csize > 0x7fffffff) return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d too many", rows);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * csize), 1, 1);
-  cfg.blockDim = dim3(kLpThreads, 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = csize;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = csize;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, logits_are_fp32 ? logprobs_kernel<float> : logprobs_kernel<__nv_bfloat16>, p);
+  cfg.numAttrs = csize > 1 ? 2 : 1;
+  auto kernel = logits_are_fp32 ? (top > 0 ? logprobs_kernel<float, true> : logprobs_kernel<float, false>)
+                                : (top > 0 ? logprobs_kernel<__nv_bfloat16, true> : logprobs_kernel<__nv_bfloat16, false>);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return fail(NVLLM_E_CUDA, "token_logprobs launch: %s", cudaGetErrorString(e));
