@@ -16,15 +16,83 @@ namespace nvllm {
 namespace hlp {
 using namespace sm100;
 
-constexpr int BM = 128, BN = 256, BK = 64, NST = 4;
-constexpr int kEpilogueWarps = 8, kThreads = (kEpilogueWarps + 4) * 32;  // registers come by fours of warps
-constexpr int kRegs = 168, kRegsEpilogue = 216, kRegsOther = 72;         // at launch, and as the groups share them (LONG)
-static_assert(kEpilogueWarps * kRegsEpilogue + 4 * kRegsOther <= (kEpilogueWarps + 4) * kRegs, "no more than the block has");
+// Two blocks of a cluster work as a pair on 256 rows (PAIR): each has half of the rows and half of the columns' weights in its
+// shared memory, the first one's thread multiplies both with tcgen05 of two blocks, and each reduces its own rows.
+constexpr int BM = 128, BN = 256, BK = 64;
 constexpr int kChunk = 1024;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-constexpr int CTRL_BYTES = 1024, SMEM = CTRL_BYTES + NST * STAGE_BYTES + 1024;  // + alignment slack
+constexpr int CTRL_BYTES = 1024, RING_BYTES = 192 * 1024, SMEM = CTRL_BYTES + RING_BYTES + 1024;  // + alignment slack
+constexpr int A_BYTES = BM * BK * 2;
 constexpr int TMEM_COLS = 512;  // two accumulators
-enum Bar { FULL0 = 0, EMPTY0 = NST, ACC_FULL0 = 2 * NST, ACC_FREE0 = 2 * NST + 2, DRAIN = 2 * NST + 4, NUM_BARS };
+constexpr int MAX_NST = 6;
+enum Bar { FULL0 = 0, EMPTY0 = MAX_NST, ACC_FULL0 = 2 * MAX_NST, ACC_FREE0 = 2 * MAX_NST + 2, DRAIN = 2 * MAX_NST + 4, NUM_BARS };
+
+template <bool PAIR, bool LONG>
+struct Cfg {
+  static constexpr int STAGE_BYTES = A_BYTES + BN * BK * 2 / (PAIR ? 2 : 1), NST = RING_BYTES / STAGE_BYTES;
+  // Warps of the epilogue, columns of a thread.  The parts of long sums are added in registers: twice the warps hold them.
+  static constexpr int WARPS = LONG ? 16 : 8, COLS = BN / (WARPS / 4);
+  static constexpr int THREADS = (WARPS + 4) * 32;  // registers come by fours of warps
+  // registers at launch and as the groups share them
+  static constexpr int REGS = 96, REGS_EPILOGUE = 104, REGS_OTHER = 64;
+  static_assert(NST <= MAX_NST, "barriers");
+  static_assert(!LONG || WARPS * REGS_EPILOGUE + 4 * REGS_OTHER <= (WARPS + 4) * REGS, "no more than the block has");
+};
+
+#ifdef __CUDACC__
+// The same place in the shared memory of block `rank` of the cluster.
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+// A tile load of one block of a pair whose bytes are counted by a barrier of either.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap* map, uint32_t cluster_bar, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(map), "r"(cluster_bar), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+__device__ __forceinline__ void umma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// One arrival at the barrier of both blocks when the products issued so far are done.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3))
+               : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void alloc_tmem(uint32_t dst) {
+  if constexpr (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    tmem_alloc(dst, TMEM_COLS);
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void dealloc_tmem(uint32_t addr) {
+  if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(TMEM_COLS) : "memory");
+  else tmem_dealloc(addr, TMEM_COLS);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+#endif
 
 struct Params {
   const int64_t* tokens;
@@ -34,6 +102,7 @@ struct Params {
   int mt, nt;     // tiles of rows and of columns
   int group, ng;  // column tiles that a unit of work has one after the other, and how many such groups
   int mb;         // row tiles whose units take turns
+  int a_rows;     // rows of a tile that are loaded
   int kb;         // blocks of 64 elements of a row
   int keep;       // a thread block has one row tile all along
   float4* partial;  // [slot][half][mt * 128]: maximum, sum, sum times logits
@@ -49,10 +118,14 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int i) {
   return {sb * p.mb + r % cnt, r / cnt};
 }
 
-template <bool LONG>
-__global__ void __launch_bounds__(kThreads, 1) head_logprobs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+template <bool PAIR, bool LONG>
+__global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+  using G = Cfg<PAIR, LONG>;
+  constexpr int NST = G::NST, WARPS = G::WARPS, COLS = G::COLS, STAGE = G::STAGE_BYTES, CTAS = PAIR ? 2 : 1;
   extern __shared__ unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = PAIR ? blockIdx.x & 1 : 0;  // in the pair
+  const int first_unit = blockIdx.x / CTAS, unit_step = gridDim.x / CTAS;
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   unsigned char* base_ptr = smem_raw + (base - smem_u32(smem_raw));
   auto bar = [&](int i) { return base + 8u * i; };
@@ -61,56 +134,68 @@ __global__ void __launch_bounds__(kThreads, 1) head_logprobs_kernel(const __grid
   const uint32_t ring = base + CTRL_BYTES;
   if (tid == 0) {
     *abort_flag = 0;
-    for (int i = 0; i < NUM_BARS; ++i) mbar_init(bar(i), i == ACC_FREE0 || i == ACC_FREE0 + 1 ? kEpilogueWarps : 1u);
+    for (int i = 0; i < NUM_BARS; ++i) mbar_init(bar(i), i == ACC_FREE0 || i == ACC_FREE0 + 1 ? CTAS * WARPS : 1u);
     mbar_fence_init();
     prefetch_tmap(&map_a);
     prefetch_tmap(&map_b);
   }
-  if (warp == kEpilogueWarps + 1) tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+  if (warp == WARPS + 1) alloc_tmem<PAIR>(smem_u32(tmem_slot));
   tc_fence_before();
-  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // the other block's barriers are there
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   const int units = p.mt * p.ng, chunks = LONG ? (p.kb * BK + kChunk - 1) / kChunk : 1, per_chunk = LONG ? kChunk / BK : p.kb;
 
-  if (warp >= kEpilogueWarps) {
-    if constexpr (LONG) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == kEpilogueWarps) {
+  if (warp >= WARPS) {
+    if constexpr (LONG) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::REGS_OTHER));
+    if (warp == WARPS) {
       // ------------------------------------------------------------------ TMA producer
       if (elect_one()) {
-        const uint32_t bytes = A_BYTES + p.bn * BK * 2;
+        const int b_rows = p.bn / CTAS;
+        const uint32_t bytes = CTAS * (p.a_rows + b_rows) * BK * 2;  // of both blocks: the first one's barriers count them
         int s = 0, use = 0;
         bool ok = true;
-        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+        for (int i = first_unit; i < units && ok; i += unit_step) {
           const Unit u = unit_of(p, i);
           for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n)
             for (int kb = 0; kb < p.kb; ++kb) {
               if (use > 0 && !(ok = wait_or_abort(bar(EMPTY0 + s), (use - 1) & 1, abort_flag))) break;
-              mbar_expect_tx(bar(FULL0 + s), bytes);
-              const uint32_t dst = ring + s * STAGE_BYTES;
-              tma_load_3d(dst, &map_a, bar(FULL0 + s), kb * BK, 0, u.m * BM);
-              tma_load_3d(dst + A_BYTES, &map_b, bar(FULL0 + s), kb * BK, 0, n * p.bn);
+              const uint32_t dst = ring + s * STAGE;
+              if (rank == 0) mbar_expect_tx(bar(FULL0 + s), bytes);
+              if constexpr (PAIR) {
+                const uint32_t full = map_to(bar(FULL0 + s), 0);
+                tma_load_pair(dst, &map_a, full, kb * BK, 0, (u.m * 2 + rank) * BM);
+                tma_load_pair(dst + A_BYTES, &map_b, full, kb * BK, 0, n * p.bn + rank * b_rows);
+              } else {
+                tma_load_3d(dst, &map_a, bar(FULL0 + s), kb * BK, 0, u.m * BM);
+                tma_load_3d(dst + A_BYTES, &map_b, bar(FULL0 + s), kb * BK, 0, n * p.bn);
+              }
               if (++s == NST) {
                 s = 0;
                 ++use;
               }
             }
         }
-        if (!ok)  // no copy is in flight when the block ends
+        if (!ok && rank == 0)  // no copy is in flight when the block (the pair) ends
           for (int k = 0; k < NST; ++k) {
             const int uses = k < s ? use + 1 : use;
             if (uses > 0) (void)mbar_wait(bar(FULL0 + k), (uses - 1) & 1);
           }
       }
-    } else if (warp == kEpilogueWarps + 1) {
+    } else if (warp == WARPS + 1 && rank == 0) {
       // ------------------------------------------------------------------ MMA issuer
       if (elect_one()) {
-        const uint32_t idesc = umma_idesc(BM, p.bn, 0, 0);
+        const uint32_t idesc = umma_idesc(BM * CTAS, p.bn, 0, 0);
         const uint64_t desc0 = umma_desc(ring, 16, 1024);
+        auto commit = [&](int i) {
+          if constexpr (PAIR) commit_pair(bar(i));
+          else umma_commit(bar(i));
+        };
         int s = 0, use = 0, it = 0;
         bool ok = true;
-        for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+        for (int i = first_unit; i < units && ok; i += unit_step) {
           const Unit u = unit_of(p, i);
           for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n)
             for (int c = 0; c < chunks && ok; ++c, ++it) {
@@ -121,51 +206,64 @@ __global__ void __launch_bounds__(kThreads, 1) head_logprobs_kernel(const __grid
               for (int kb = first; kb < last; ++kb) {
                 if (!(ok = wait_or_abort(bar(FULL0 + s), use & 1, abort_flag))) break;
                 tc_fence_after();
-                const uint64_t da = desc0 + static_cast<uint64_t>((s * STAGE_BYTES) >> 4), db = da + (A_BYTES >> 4);
-  #pragma unroll
-                for (int ks = 0; ks < BK / 16; ++ks) umma_ss(tmem + b * BN, da + 2 * ks, db + 2 * ks, idesc, kb > first || ks > 0);
-                umma_commit(bar(EMPTY0 + s));
+                const uint64_t da = desc0 + static_cast<uint64_t>((s * STAGE) >> 4), db = da + (A_BYTES >> 4);
+#pragma unroll
+                for (int ks = 0; ks < BK / 16; ++ks) {
+                  if constexpr (PAIR) umma_pair(tmem + b * BN, da + 2 * ks, db + 2 * ks, idesc, kb > first || ks > 0);
+                  else umma_ss(tmem + b * BN, da + 2 * ks, db + 2 * ks, idesc, kb > first || ks > 0);
+                }
+                commit(EMPTY0 + s);
                 if (++s == NST) {
                   s = 0;
                   ++use;
                 }
               }
-              if (ok) umma_commit(bar(ACC_FULL0 + b));
+              if (ok) commit(ACC_FULL0 + b);
             }
         }
         if (!ok) {  // nothing may still be running on tensor memory when it is freed
-          umma_commit(bar(DRAIN));
+          commit(DRAIN);
           (void)mbar_wait(bar(DRAIN), 0);
         }
       }
     }
   } else {
-    if constexpr (LONG) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsEpilogue));
-    // ------------------------------------------------------------------ epilogue: a row and half of the columns to a thread
-    const int half = warp >> 2, r = (warp & 3) * 32 + lane;
-    const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + half * (BN / 2);
-    const int64_t rows_padded = static_cast<int64_t>(p.mt) * BM;
+    if constexpr (LONG) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::REGS_EPILOGUE));
+    // ------------------------------------------------------------------ epilogue: a row and COLS of the columns to a thread
+    const int part = warp >> 2, r = rank * BM + (warp & 3) * 32 + lane;
+    const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + part * COLS;
+    const int64_t rows_padded = static_cast<int64_t>(p.mt) * BM * CTAS;
     LpSums sum{-FLT_MAX, 0.f, 0.f};
-    int it = 0, m = -1, slot = 0;
+    int it = 0, slot = 0;
+    int64_t row = -1;
     float c = 0.f;
     int64_t token = -1;
     bool ok = true;
-    auto flush = [&]() { p.partial[(static_cast<int64_t>(slot) * 2 + half) * rows_padded + m * BM + r] = make_float4(sum.m, sum.s, sum.t, 0.f); };
-    auto add = [&](float* v, int col, int n) {  // columns col to col + 31 of the vocabulary, of which the first n count
-      if (n < 32) {
+    auto flush = [&]() { p.partial[(static_cast<int64_t>(slot) * (WARPS / 4) + part) * rows_padded + row] = make_float4(sum.m, sum.s, sum.t, 0.f); };
+    auto free_acc = [&](int b) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if (rank == 0) mbar_arrive(bar(ACC_FREE0 + b));
+        else arrive_at(map_to(bar(ACC_FREE0 + b), 0));
+      }
+    };
+    constexpr int W = LONG ? 16 : 32;  // columns at a time
+    auto add = [&](float (&v)[W], int col, int n) {  // from column col of the vocabulary, of which the first n count
+      if (n < W) {
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
+        for (int k = 0; k < W; ++k)
           if (k >= n) v[k] = -INFINITY;
       }
       float most = v[0];
 #pragma unroll
-      for (int k = 1; k < 31; k += 2) most = fmax3(most, v[k], v[k + 1]);
-      most = fmaxf(most, v[31]);
+      for (int k = 1; k < W - 1; k += 2) most = fmax3(most, v[k], v[k + 1]);
+      most = fmaxf(most, v[W - 1]);
       sum.rescale(fmaxf(most, sum.m), c);
       const uint64_t minus_m = pack2(-sum.m, -sum.m), c2 = pack2(c, c);
       uint64_t s2 = 0, t2 = 0;
 #pragma unroll
-      for (int k = 0; k < 32; k += 2) {
+      for (int k = 0; k < W; k += 2) {
         float a, b, ya, yb;
         unpack2(add2(pack2(v[k], v[k + 1]), minus_m), ya, yb);
         const uint64_t y2 = pack2(max_nan(ya, -3e38f), max_nan(yb, -3e38f));
@@ -180,80 +278,92 @@ __global__ void __launch_bounds__(kThreads, 1) head_logprobs_kernel(const __grid
       unpack2(t2, a, b);
       sum.t += a + b;
       const int64_t d = token - col;
-      if (d >= 0 && d < 32 && d < n) {
+      if (d >= 0 && d < W && d < n) {
         float x = 0.f;
 #pragma unroll
-        for (int k = 0; k < 32; ++k)
+        for (int k = 0; k < W; ++k)
           if (k == d) x = v[k];
-        p.given[m * BM + r] = x;
+        p.given[row] = x;
       }
     };
-    for (int i = blockIdx.x; i < units && ok; i += gridDim.x) {
+    for (int i = first_unit; i < units && ok; i += unit_step) {
       const Unit u = unit_of(p, i);
-      if (m < 0 || !p.keep) {
-        m = u.m;
+      if (row < 0 || !p.keep) {
         slot = u.g;
         sum = {-FLT_MAX, 0.f, 0.f};
-        const int64_t row = static_cast<int64_t>(m) * BM + r;
+        row = static_cast<int64_t>(u.m) * (BM * CTAS) + r;
         token = row < p.rows ? p.tokens[row] : -1;
         if (token >= p.vocab) token = -1;
         c = (row < p.rows ? lp_inverse(p.temperatures, row) : 1.f) * 1.4426950408889634f;
       }
       for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n) {
-        const int first = n * p.bn + half * (BN / 2), end = min(p.vocab, (n + 1) * p.bn) - first;  // columns of this thread
-        float acc[LONG ? BN / 2 : 32];
-        for (int ch = 0; ch < chunks && ok; ++ch, ++it) {
+        const int first = n * p.bn + part * COLS, end = min(p.vocab, (n + 1) * p.bn) - first;  // columns of this thread
+        if constexpr (!LONG) {
           const int b = it & 1;
           if (!(ok = wait_or_abort(bar(ACC_FULL0 + b), (it >> 1) & 1, abort_flag))) break;
+          ++it;
           __syncwarp();
           tc_fence_after();
-          if constexpr (LONG) {
-#pragma unroll
-            for (int j = 0; j < BN / 2; j += 32) {
-              uint32_t v[32];
-              tmem_ld32(at + b * BN + j, v);
-              tmem_wait_ld();
-#pragma unroll
-              for (int k = 0; k < 32; ++k) acc[j + k] = ch == 0 ? __uint_as_float(v[k]) : acc[j + k] + __uint_as_float(v[k]);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(ACC_FREE0 + b));
-          } else {
 #pragma unroll 1
-            for (int j = 0; j < end && j < BN / 2; j += 32) {
-              uint32_t v[32];
-              tmem_ld32(at + b * BN + j, v);
-              tmem_wait_ld();
+          for (int j = 0; j < end && j < COLS; j += 32) {
+            uint32_t v[32];
+            tmem_ld32(at + b * BN + j, v);
+            tmem_wait_ld();
+            float x[32];
 #pragma unroll
-              for (int k = 0; k < 32; ++k) acc[k] = __uint_as_float(v[k]);
-              add(acc, first + j, end - j);
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(ACC_FREE0 + b));
+            for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(v[k]);
+            add(x, first + j, end - j);
           }
-        }
-        if constexpr (LONG) {
-          if (ok) {
+          free_acc(b);
+        } else {
+          float acc[COLS];
+          for (int ch = 0; ch < chunks; ++ch, ++it) {
+            const int b = it & 1;
+            if (!(ok = wait_or_abort(bar(ACC_FULL0 + b), (it >> 1) & 1, abort_flag))) break;
+            __syncwarp();
+            tc_fence_after();
+            if (ch + 1 < chunks) {
 #pragma unroll
-            for (int j = 0; j < BN / 2; j += 32)
-              if (j < end) add(acc + j, first + j, end - j);
+              for (int j = 0; j < COLS; j += W) {
+                uint32_t v[W];
+                tmem_ld16(at + b * BN + j, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < W; ++k) acc[j + k] = ch == 0 ? __uint_as_float(v[k]) : acc[j + k] + __uint_as_float(v[k]);
+              }
+              free_acc(b);
+            } else {
+#pragma unroll
+              for (int j = 0; j < COLS; j += W) {
+                if (j < end) {
+                  uint32_t v[W];
+                  tmem_ld16(at + b * BN + j, v);
+                  tmem_wait_ld();
+                  float x[W];
+#pragma unroll
+                  for (int k = 0; k < W; ++k) x[k] = acc[j + k] + __uint_as_float(v[k]);
+                  add(x, first + j, end - j);
+                }
+              }
+              free_acc(b);
+            }
           }
         }
       }
       if (!p.keep) flush();
     }
-    if (p.keep && m >= 0) flush();
+    if (p.keep && row >= 0) flush();
   }
 
+  __syncwarp();
   pdl_trigger();
   tc_fence_before();
-  __syncthreads();
+  if constexpr (PAIR) cluster_sync();  // neither block's memory is in use any more
+  else __syncthreads();
   if (tid == 0 && *abort_flag) atomicOr(p.status, NVLLM_STATUS_TIMEOUT);
-  if (warp == kEpilogueWarps + 1) {
+  if (warp == WARPS + 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, TMEM_COLS);
+    dealloc_tmem<PAIR>(tmem);
   }
 }
 
@@ -294,31 +404,35 @@ __global__ void __launch_bounds__(kJoinRows * kJoinWarps) join_kernel(const Join
   sum.results(row, token, token >= 0 && token < p.vocab ? p.given[row] : 0.f, inv_t, sum.log_z(), p.vocab, p.logprobs, p.entropy, p.status);
 }
 
-// How a problem is laid out over `sms` thread blocks.
+// How a problem is laid out over the multiprocessors.
 struct Plan {
-  int bn, mt, nt, group, ng, mb, kb, keep, grid, slots;
+  int pair, bn, mt, nt, group, ng, mb, kb, keep, grid, slots, a_rows;
   int64_t rows_padded, bytes;
 };
 static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   Plan pl;
+  pl.pair = rows > BM;
+  const int bm = pl.pair ? 2 * BM : BM, workers = std::max(1, pl.pair ? sms / 2 : sms);
   pl.kb = (hidden + BK - 1) / BK;
-  pl.mt = (rows + BM - 1) / BM;
-  // the widest tile that leaves the fullest thread block as few columns as any
+  pl.mt = (rows + bm - 1) / bm;
+  pl.a_rows = pl.pair ? BM : std::min(BM, (rows + 7) / 8 * 8);
+  // the widest tile that leaves the worker with most tiles as few columns as any
   int64_t least = 0;
   pl.bn = BN;
   for (int bn = BN; bn >= BN / 2; bn -= 16) {
-    const int64_t tiles = static_cast<int64_t>(pl.mt) * ((vocab + bn - 1) / bn), cost = (tiles + sms - 1) / sms * bn;
+    const int64_t tiles = static_cast<int64_t>(pl.mt) * ((vocab + bn - 1) / bn), cost = (tiles + workers - 1) / workers * bn;
     if (bn == BN || cost < least) least = cost, pl.bn = bn;
   }
   pl.nt = (vocab + pl.bn - 1) / pl.bn;
-  pl.keep = pl.mt <= sms && sms % pl.mt == 0;
+  pl.keep = pl.mt <= workers && workers % pl.mt == 0;
   pl.group = 1;
-  while (!pl.keep && pl.group < 16 && static_cast<int64_t>(pl.mt) * ((pl.nt + 2 * pl.group - 1) / (2 * pl.group)) >= 48ll * sms) pl.group *= 2;
+  while (!pl.keep && pl.group < 16 && static_cast<int64_t>(pl.mt) * ((pl.nt + 2 * pl.group - 1) / (2 * pl.group)) >= 48ll * workers) pl.group *= 2;
   pl.ng = (pl.nt + pl.group - 1) / pl.group;
-  pl.mb = pl.keep ? pl.mt : static_cast<int>(std::min<int64_t>(pl.mt, std::max<int64_t>(1, (32ll << 20) / (BM * 2ll * hidden))));
-  pl.grid = static_cast<int>(std::min<int64_t>(sms, static_cast<int64_t>(pl.mt) * pl.ng));
-  pl.slots = 2 * (pl.keep ? std::min(sms / pl.mt, pl.ng) : pl.ng);
-  pl.rows_padded = static_cast<int64_t>(pl.mt) * BM;
+  pl.mb = pl.keep ? pl.mt : static_cast<int>(std::min<int64_t>(pl.mt, std::max<int64_t>(1, (32ll << 20) / (bm * 2ll * hidden))));
+  pl.grid = static_cast<int>(std::min<int64_t>(workers, static_cast<int64_t>(pl.mt) * pl.ng)) * (pl.pair ? 2 : 1);
+  const int parts = hidden > kChunk ? Cfg<false, true>::WARPS / 4 : Cfg<false, false>::WARPS / 4;
+  pl.slots = parts * (pl.keep ? std::min(workers / pl.mt, pl.ng) : pl.ng);
+  pl.rows_padded = static_cast<int64_t>(pl.mt) * bm;
   pl.bytes = pl.slots * pl.rows_padded * 16 + pl.rows_padded * 4;
   return pl;
 }
@@ -361,16 +475,20 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
     return fail(NVLLM_E_WORKSPACE, "head_logprobs: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)pl.bytes);
   if (!aligned16(workspace)) return fail(NVLLM_E_ALIGN, "head_logprobs: the workspace must be 16-byte aligned");
   CUtensorMap a, b;
-  if (!sm100::make_tmap_3d(&a, hidden_states, hidden, 1, rows, hidden_row_stride, hidden_row_stride, hlp::BM)) return NVLLM_E_CUDA;
-  if (!sm100::make_tmap_3d(&b, weight, hidden, 1, vocab, weight_row_stride, weight_row_stride, pl.bn)) return NVLLM_E_CUDA;
+  if (!sm100::make_tmap_3d(&a, hidden_states, hidden, 1, rows, hidden_row_stride, hidden_row_stride, pl.a_rows)) return NVLLM_E_CUDA;
+  if (!sm100::make_tmap_3d(&b, weight, hidden, 1, vocab, weight_row_stride, weight_row_stride, pl.pair ? pl.bn / 2 : pl.bn)) return NVLLM_E_CUDA;
   const bool is_long = hidden > hlp::kChunk;
+  using Kernel = decltype(&hlp::head_logprobs_kernel<false, false>);
+  static const Kernel kernels[2][2] = {{hlp::head_logprobs_kernel<false, false>, hlp::head_logprobs_kernel<false, true>},
+                                       {hlp::head_logprobs_kernel<true, false>, hlp::head_logprobs_kernel<true, true>}};
   static bool ready[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(hlp::head_logprobs_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(hlp::head_logprobs_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
-    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "head_logprobs: cannot reserve shared memory: %s", cudaGetErrorString(e));
+    for (int k = 0; k < 4; ++k) {
+      const cudaError_t e = cudaFuncSetAttribute(kernels[k / 2][k % 2], cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
+      if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "head_logprobs: cannot reserve shared memory: %s", cudaGetErrorString(e));
+    }
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
   hlp::Params p{};
@@ -384,15 +502,32 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   p.group = pl.group;
   p.ng = pl.ng;
   p.mb = pl.mb;
+  p.a_rows = pl.a_rows;
   p.kb = pl.kb;
   p.keep = pl.keep;
   p.partial = static_cast<float4*>(workspace);
   p.given = reinterpret_cast<float*>(p.partial + pl.slots * pl.rows_padded);
   p.status = status;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (const int e = launch_kernel("head_logprobs", is_long ? hlp::head_logprobs_kernel<true> : hlp::head_logprobs_kernel<false>, dim3(pl.grid),
-                                  dim3(hlp::kThreads), hlp::SMEM, st, a, b, p))
-    return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(pl.grid);
+  cfg.blockDim = dim3(is_long ? hlp::Cfg<false, true>::THREADS : hlp::Cfg<false, false>::THREADS);
+  cfg.dynamicSmemBytes = hlp::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pl.pair ? 2 : 1;
+  const cudaError_t launched = cudaLaunchKernelEx(&cfg, kernels[pl.pair][is_long], a, b, p);
+  count_launch();
+  if (launched != cudaSuccess) {
+    (void)cudaGetLastError();
+    return fail(NVLLM_E_CUDA, "head_logprobs launch: %s", cudaGetErrorString(launched));
+  }
   const hlp::JoinParams j{p.partial, p.given, tokens, temperatures, p.rows, p.vocab, pl.slots, pl.rows_padded, logprobs, entropy, status};
   return launch_kernel("head_logprobs", hlp::join_kernel, dim3(static_cast<unsigned>((rows + hlp::kJoinRows - 1) / hlp::kJoinRows)),
                        dim3(hlp::kJoinRows * hlp::kJoinWarps), 0, st, j);
