@@ -29,11 +29,10 @@ enum Bar { FULL0 = 0, EMPTY0 = MAX_NST, ACC_FULL0 = 2 * MAX_NST, ACC_FREE0 = 2 *
 template <bool PAIR, bool LONG>
 struct Cfg {
   static constexpr int STAGE_BYTES = A_BYTES + BN * BK * 2 / (PAIR ? 2 : 1), NST = RING_BYTES / STAGE_BYTES;
-  // Warps of the epilogue, columns of a thread.  The parts of long sums are added in registers: twice the warps hold them.
-  static constexpr int WARPS = LONG ? 16 : 8, COLS = BN / (WARPS / 4);
-  static constexpr int THREADS = (WARPS + 4) * 32;  // registers come by fours of warps
-  // registers at launch and as the groups share them
-  static constexpr int REGS = 96, REGS_EPILOGUE = 104, REGS_OTHER = 64;
+  static constexpr int WARPS = 8, COLS = BN / (WARPS / 4);  // of the epilogue; columns of a thread
+  static constexpr int THREADS = (WARPS + 4) * 32;          // registers come by fours of warps
+  // registers at launch and as the groups share them: the parts of long sums are added in those of the epilogue
+  static constexpr int REGS = 168, REGS_EPILOGUE = 216, REGS_OTHER = 72;
   static_assert(NST <= MAX_NST, "barriers");
   static_assert(!LONG || WARPS * REGS_EPILOGUE + 4 * REGS_OTHER <= (WARPS + 4) * REGS, "no more than the block has");
 };
