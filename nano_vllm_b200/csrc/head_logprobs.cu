@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
     int64_t row = -1;
     float c = 0.f;
     int64_t token = -1;
-    bool ok = true;
+    bool ok = true, live = true;  // live: of the warp's rows there is one
     auto flush = [&]() { p.partial[(static_cast<int64_t>(slot) * (WARPS / 4) + part) * rows_padded + row] = make_float4(sum.m, sum.s, sum.t, 0.f); };
     auto free_acc = [&](int b) {
       tc_fence_before();
@@ -291,6 +291,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
         slot = u.g;
         sum = {-FLT_MAX, 0.f, 0.f};
         row = static_cast<int64_t>(u.m) * (BM * CTAS) + r;
+        live = row - lane < p.rows;
         token = row < p.rows ? p.tokens[row] : -1;
         if (token >= p.vocab) token = -1;
         c = (row < p.rows ? lp_inverse(p.temperatures, row) : 1.f) * 1.4426950408889634f;
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (int j = 0; j < end && j < COLS; j += 32) {
+          for (int j = 0; j < end && j < COLS && live; j += 32) {
             uint32_t v[32];
             tmem_ld32(at + b * BN + j, v);
             tmem_wait_ld();
@@ -334,7 +335,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
             } else {
 #pragma unroll
               for (int j = 0; j < COLS; j += W) {
-                if (j < end) {
+                if (j < end && live) {
                   uint32_t v[W];
                   tmem_ld16(at + b * BN + j, v);
                   tmem_wait_ld();
@@ -366,41 +367,55 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
   }
 }
 
-// Joins the partial statistics of `slots` slots for every row: 32 rows to a block, 8 threads a row.
+// Joins the partial statistics of `slots` slots for every row: a block has `wide` rows and deals a row's slots out to 256 / wide
+// threads (one row to a block where there are few: 37 trips to memory one after the other in each of eight threads a row cost 6 us).
 struct JoinParams {
   const float4* partial;
   const float* given;
   const int64_t* tokens;
   const float* temperatures;
-  int rows, vocab, slots;  // halves counted
+  int rows, vocab, slots, wide;  // slots: halves counted
   int64_t rows_padded;
   float *logprobs, *entropy;
   int* status;
 };
-constexpr int kJoinRows = 32, kJoinWarps = 8;
+constexpr int kJoinThreads = 256;
 
-__global__ void __launch_bounds__(kJoinRows * kJoinWarps) join_kernel(const JoinParams p) {
-  __shared__ float s_sums[kJoinWarps][kJoinRows][3];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kJoinRows + lane;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) {
+  __shared__ float s_sums[3][kJoinThreads];
+  const int tid = threadIdx.x, part = tid / p.wide, parts = kJoinThreads / p.wide;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * p.wide + tid % p.wide;
   const bool live = row < p.rows;
   const float inv_t = live ? lp_inverse(p.temperatures, row) : 1.f, c = inv_t * 1.4426950408889634f;
   const int64_t token = live ? p.tokens[row] : -1;
   pdl_prologue();
   LpSums sum{-FLT_MAX, 0.f, 0.f};
-  if (live)
-#pragma unroll 4
-    for (int k = warp; k < p.slots; k += kJoinWarps) {
-      const float4 v = p.partial[k * p.rows_padded + row];
-      sum.join(v.x, v.y, v.z, c);
+  float given = 0.f;
+  if (live) {
+    if (part == 0 && token >= 0 && token < p.vocab) given = p.given[row];
+    constexpr int U = 8;
+    for (int k = part; k < p.slots; k += U * parts) {
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u * parts < p.slots) v[u] = p.partial[static_cast<int64_t>(k + u * parts) * p.rows_padded + row];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (k + u * parts < p.slots) sum.join(v[u].x, v[u].y, v[u].z, c);
     }
-  s_sums[warp][lane][0] = sum.m;
-  s_sums[warp][lane][1] = sum.s;
-  s_sums[warp][lane][2] = sum.t;
-  __syncthreads();
-  if (warp != 0 || !live) return;
-  for (int k = 1; k < kJoinWarps; ++k) sum.join(s_sums[k][lane][0], s_sums[k][lane][1], s_sums[k][lane][2], c);
-  sum.results(row, token, token >= 0 && token < p.vocab ? p.given[row] : 0.f, inv_t, sum.log_z(), p.vocab, p.logprobs, p.entropy, p.status);
+  }
+  for (int n = parts / 2; n > 0; n /= 2) {
+    s_sums[0][tid] = sum.m;
+    s_sums[1][tid] = sum.s;
+    s_sums[2][tid] = sum.t;
+    __syncthreads();
+    if (part < n) {
+      const int o = tid + n * p.wide;
+      sum.join(s_sums[0][o], s_sums[1][o], s_sums[2][o], c);
+    }
+    __syncthreads();
+  }
+  if (part == 0 && live) sum.results(row, token, given, inv_t, sum.log_z(), p.vocab, p.logprobs, p.entropy, p.status);
 }
 
 // How a problem is laid out over the multiprocessors.
@@ -427,7 +442,7 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   pl.group = 1;
   while (!pl.keep && pl.group < 16 && static_cast<int64_t>(pl.mt) * ((pl.nt + 2 * pl.group - 1) / (2 * pl.group)) >= 48ll * workers) pl.group *= 2;
   pl.ng = (pl.nt + pl.group - 1) / pl.group;
-  pl.mb = pl.keep ? pl.mt : static_cast<int>(std::min<int64_t>(pl.mt, std::max<int64_t>(1, (32ll << 20) / (bm * 2ll * hidden))));
+  pl.mb = pl.keep ? pl.mt : static_cast<int>(std::min<int64_t>(pl.mt, std::max<int64_t>(1, std::min<int64_t>(16, (32ll << 20) / (bm * 2ll * hidden)))));
   pl.grid = static_cast<int>(std::min<int64_t>(workers, static_cast<int64_t>(pl.mt) * pl.ng)) * (pl.pair ? 2 : 1);
   const int parts = hidden > kChunk ? Cfg<false, true>::WARPS / 4 : Cfg<false, false>::WARPS / 4;
   pl.slots = parts * (pl.keep ? std::min(workers / pl.mt, pl.ng) : pl.ng);
@@ -527,7 +542,8 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
     (void)cudaGetLastError();
     return fail(NVLLM_E_CUDA, "head_logprobs launch: %s", cudaGetErrorString(launched));
   }
-  const hlp::JoinParams j{p.partial, p.given, tokens, temperatures, p.rows, p.vocab, pl.slots, pl.rows_padded, logprobs, entropy, status};
-  return launch_kernel("head_logprobs", hlp::join_kernel, dim3(static_cast<unsigned>((rows + hlp::kJoinRows - 1) / hlp::kJoinRows)),
-                       dim3(hlp::kJoinRows * hlp::kJoinWarps), 0, st, j);
+  int wide = 1;
+  while (wide < 32 && rows > 4ll * sms * wide) wide *= 2;
+  const hlp::JoinParams j{p.partial, p.given, tokens, temperatures, p.rows, p.vocab, pl.slots, wide, pl.rows_padded, logprobs, entropy, status};
+  return launch_kernel("head_logprobs", hlp::join_kernel, dim3(static_cast<unsigned>((rows + wide - 1) / wide)), dim3(hlp::kJoinThreads), 0, st, j);
 }
