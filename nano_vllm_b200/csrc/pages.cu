@@ -17,6 +17,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace nvllm {
 
@@ -29,63 +30,99 @@ constexpr int64_t kLeastPiece = 4096;  // bytes of a plane's block that are wort
 template <int MOST>
 struct Parts {
   nvllm_cache_part part[MOST];
-  int n, planes;  // planes of all parts
+  int n, planes, value_planes;  // planes of all parts, and of those that are not scales
 };
 
-__device__ __forceinline__ uint4 ld_once(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
+// ---- copies: a thread keeps a ring of pieces of shared memory busy, bulk loads kLead pieces ahead of the bulk stores
+constexpr int kPiece = 16384, kStages = 8, kLead = 5;
+constexpr int kRingBytes = kPiece * kStages + 128;  // barriers behind the pieces
 
-// The first `slots` slots of block src to block dst: piece k of `pieces` of plane `plane` of all planes.
-template <int MOST>
-__device__ __forceinline__ void copy_piece(const Parts<MOST>& parts, int plane, int64_t src, int64_t dst, int slots, int k, int pieces) {
-  int i = 0;
-  while (plane >= static_cast<int>(parts.part[i].planes)) plane -= static_cast<int>(parts.part[i++].planes);
-  const nvllm_cache_part& c = parts.part[i];
-  unsigned char* base = static_cast<unsigned char*>(c.base) + plane * c.plane_stride;
-  const unsigned char* from = base + src * c.block_stride;
-  unsigned char* to = base + dst * c.block_stride;
-  if (c.scale_heads > 0) {
-    if (k != 0) return;
-    constexpr int groups = kBlockSize / NVLLM_SCALE_GROUP;
-    const int held = (slots + NVLLM_SCALE_GROUP - 1) / NVLLM_SCALE_GROUP;
-    for (int e = threadIdx.x; e < c.scale_heads * groups; e += kCopyThreads)
-      if (e % groups < held) reinterpret_cast<float*>(to)[e] = reinterpret_cast<const float*>(from)[e];
-    return;
-  }
-  const int64_t units = static_cast<int64_t>(slots) * c.slot_bytes / 16, each = (units + pieces - 1) / pieces;
-  const int64_t lo = k * each, hi = min(lo + each, units);
-  const uint4* f = reinterpret_cast<const uint4*>(from);
-  uint4* t = reinterpret_cast<uint4*>(to);
-  constexpr int U = 8;
-  int64_t o = lo + threadIdx.x;
-  for (; o + (U - 1) * kCopyThreads < hi; o += U * kCopyThreads) {
-    uint4 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = ld_once(f + o + u * kCopyThreads);
-#pragma unroll
-    for (int u = 0; u < U; ++u) t[o + u * kCopyThreads] = v[u];
-  }
-  for (; o < hi; o += kCopyThreads) t[o] = ld_once(f + o);
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;\n\tcp.async.bulk.commit_group;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
-// All copies: `of(c, src, dst, slots)` says what copy c is and whether there is anything to do.
+// All copies: `of(c, src, dst, slots)` says what copy c is and whether there is anything to do.  A (copy, plane) of values is cut
+// in `pieces` equal parts, an item each; items are dealt out to the blocks in turn.  Scales: threads 32 and on.
 template <int MOST, class F>
-__device__ __forceinline__ void copy_all(const Parts<MOST>& parts, int copies, F&& of) {
-  const int64_t pairs = static_cast<int64_t>(copies) * parts.planes;
-  if (pairs == 0) return;
-  int64_t largest = 0;
-  for (int i = 0; i < parts.n; ++i) largest = max(largest, static_cast<int64_t>(parts.part[i].slot_bytes) * kBlockSize);
-  const int64_t wanted = (int64_t{8} * gridDim.x + pairs - 1) / pairs, most = (largest + kLeastPiece - 1) / kLeastPiece;
-  const int pieces = static_cast<int>(max(int64_t{1}, min(wanted, most)));
-  for (int64_t item = blockIdx.x; item < pairs * pieces; item += gridDim.x) {
-    const int64_t pair = item / pieces;
-    const int c = static_cast<int>(pair / parts.planes);
-    int64_t src, dst;
-    int slots;
-    if (of(c, src, dst, slots)) copy_piece(parts, static_cast<int>(pair - static_cast<int64_t>(c) * parts.planes), src, dst, slots, static_cast<int>(item - pair * pieces), pieces);
+__device__ __forceinline__ void copy_all(const Parts<MOST>& parts, int copies, uint32_t ring, int* status, F&& of) {
+  if (copies == 0) return;
+  const uint32_t bars = ring + kPiece * kStages;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) sm100::mbar_init(bars + 8 * i, 1);
+    sm100::mbar_fence_init();
+    const int64_t pairs = static_cast<int64_t>(copies) * parts.value_planes;
+    int64_t largest = 0;
+    for (int i = 0; i < parts.n; ++i) largest = max(largest, static_cast<int64_t>(parts.part[i].slot_bytes) * kBlockSize);
+    const int64_t wanted = pairs ? (int64_t{8} * gridDim.x + pairs - 1) / pairs : 1, most = (largest + kLeastPiece - 1) / kLeastPiece;
+    const int pieces = static_cast<int>(max(int64_t{1}, min(wanted, most)));
+    __shared__ unsigned char* s_to[kStages];
+    __shared__ uint32_t s_bytes[kStages];
+    int64_t n = 0;  // pieces of shared memory loaded so far
+    bool ok = true;
+    auto store = [&](int64_t m) {
+      const int s = static_cast<int>(m % kStages);
+      if (!(ok = sm100::mbar_wait(bars + 8 * s, (m / kStages) & 1))) return;
+      bulk_store(s_to[s], ring + s * kPiece, s_bytes[s]);
+    };
+    for (int64_t item = blockIdx.x; item < pairs * pieces && ok; item += gridDim.x) {
+      const int64_t pair = item / pieces;
+      const int c = static_cast<int>(pair / parts.value_planes), k = static_cast<int>(item - pair * pieces);
+      int64_t src, dst;
+      int slots;
+      if (!of(c, src, dst, slots)) continue;
+      int plane = static_cast<int>(pair - static_cast<int64_t>(c) * parts.value_planes), i = 0;
+      while (parts.part[i].scale_heads > 0 || plane >= static_cast<int>(parts.part[i].planes)) {
+        if (parts.part[i].scale_heads == 0) plane -= static_cast<int>(parts.part[i].planes);
+        ++i;
+      }
+      const nvllm_cache_part& part = parts.part[i];
+      unsigned char* plane_at = static_cast<unsigned char*>(part.base) + plane * part.plane_stride;
+      const int64_t units = static_cast<int64_t>(slots) * part.slot_bytes / 16, each = (units + pieces - 1) / pieces;
+      const int64_t end = min((k + 1) * each, units) * 16;
+      for (int64_t at = k * each * 16; at < end && ok; at += kPiece) {
+        const uint32_t bytes = static_cast<uint32_t>(min(end - at, static_cast<int64_t>(kPiece)));
+        const int s = static_cast<int>(n % kStages);
+        bulk_wait_read<kStages - kLead - 1>();  // the store that had the stage before has read it
+        s_to[s] = plane_at + dst * part.block_stride + at;
+        s_bytes[s] = bytes;
+        sm100::mbar_expect_tx(bars + 8 * s, bytes);
+        bulk_load(ring + s * kPiece, plane_at + src * part.block_stride + at, bytes, bars + 8 * s);
+        if (++n > kLead) store(n - 1 - kLead);
+      }
+    }
+    for (int64_t m = max(int64_t{0}, n - kLead); m < n; ++m) {
+      if (ok) store(m);
+      else (void)sm100::mbar_wait(bars + 8 * (m % kStages), (m / kStages) & 1);  // no copy is in flight when the block ends
+    }
+    bulk_wait_all();
+    if (!ok) atomicOr(status, NVLLM_STATUS_TIMEOUT);
+  } else if (threadIdx.x >= 32) {
+    const int scale_planes = parts.planes - parts.value_planes;
+    for (int64_t item = blockIdx.x; item < static_cast<int64_t>(copies) * scale_planes; item += gridDim.x) {
+      const int c = static_cast<int>(item / scale_planes);
+      int64_t src, dst;
+      int slots;
+      if (!of(c, src, dst, slots)) continue;
+      int plane = static_cast<int>(item - static_cast<int64_t>(c) * scale_planes), i = 0;
+      while (parts.part[i].scale_heads == 0 || plane >= static_cast<int>(parts.part[i].planes)) {
+        if (parts.part[i].scale_heads > 0) plane -= static_cast<int>(parts.part[i].planes);
+        ++i;
+      }
+      const nvllm_cache_part& part = parts.part[i];
+      unsigned char* plane_at = static_cast<unsigned char*>(part.base) + plane * part.plane_stride;
+      const float* from = reinterpret_cast<const float*>(plane_at + src * part.block_stride);
+      float* to = reinterpret_cast<float*>(plane_at + dst * part.block_stride);
+      constexpr int groups = kBlockSize / NVLLM_SCALE_GROUP;
+      const int held = (slots + NVLLM_SCALE_GROUP - 1) / NVLLM_SCALE_GROUP;
+      for (int e = threadIdx.x - 32; e < part.scale_heads * groups; e += blockDim.x - 32)
+        if (e % groups < held) to[e] = from[e];
+    }
   }
 }
 
@@ -98,15 +135,16 @@ struct CopyParams {
 
 template <int MOST>
 __global__ void __launch_bounds__(kCopyThreads) copy_blocks_kernel(const __grid_constant__ Parts<MOST> parts, const CopyParams p) {
+  extern __shared__ __align__(128) unsigned char s_ring[];
   pdl_prologue();
   const int copies = p.count ? min(*p.count, p.copies) : p.copies;
-  copy_all(parts, copies, [&](int c, int64_t& src, int64_t& dst, int& slots) {
+  copy_all(parts, copies, smem_u32(s_ring), p.status, [&](int c, int64_t& src, int64_t& dst, int& slots) {
     src = p.src[c];
     dst = p.dst[c];
     slots = p.slots ? max(0, min(p.slots[c], kBlockSize)) : kBlockSize;
     if (src < 0 || dst < 0) return false;
     if (src >= p.num_blocks || dst >= p.num_blocks) {
-      if (threadIdx.x == 0) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
+      atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
       return false;
     }
     return src != dst;
@@ -152,8 +190,8 @@ struct ForkParams {
 
 template <int MOST>
 __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constant__ Parts<MOST> parts, const ForkParams p) {
-  extern __shared__ int4 s_mem4[];
-  int* s_mem = reinterpret_cast<int*>(s_mem4);
+  extern __shared__ __align__(128) unsigned char s_ring[];
+  int* s_mem = reinterpret_cast<int*>(s_ring + kRingBytes);
   int* s_first = s_mem;               // of every old sequence: its first new row
   int* s_fresh = s_first + p.batch;   // of every new row: the block of its own that it gets, -1 none left, -2 none needed
   int4* s_list = reinterpret_cast<int4*>(s_mem + ((p.batch + p.rows + 3) & ~3));  // copies: from, to, slots
@@ -208,14 +246,14 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constan
     if (col < need) id = col == need - 1 && fresh != -2 ? fresh : p.table[b * p.stride + col];
     p.new_table[i * p.new_stride + col] = id;
   }
-  copy_all(parts, total, [&](int c, int64_t& src, int64_t& dst, int& slots) {
+  copy_all(parts, total, smem_u32(s_ring), p.status, [&](int c, int64_t& src, int64_t& dst, int& slots) {
     const int4 x = s_list[c];
     src = x.x;
     dst = x.y;
     slots = x.z;
     if (src < 0 || dst < 0) return false;
     if (src >= p.num_blocks || dst >= p.num_blocks) {
-      if (threadIdx.x == 0) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
+      atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
       return false;
     }
     return src != dst;
@@ -372,14 +410,27 @@ static Parts<MOST> gather(const nvllm_cache_part* part, int n) {
   Parts<MOST> all{};
   std::copy(part, part + n, all.part);
   all.n = n;
-  for (int i = 0; i < n; ++i) all.planes += static_cast<int>(part[i].planes);
+  for (int i = 0; i < n; ++i) {
+    all.planes += static_cast<int>(part[i].planes);
+    if (part[i].scale_heads == 0) all.value_planes += static_cast<int>(part[i].planes);
+  }
   return all;
 }
 
 static int launch_copies(const char* what, const nvllm_cache_part* part, int n, const CopyParams& p, cudaStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(4 * num_sms()));
-  if (n <= kFewParts) return launch_kernel(what, copy_blocks_kernel<kFewParts>, grid, dim3(kCopyThreads), 0, stream, gather<kFewParts>(part, n), p);
-  return launch_kernel(what, copy_blocks_kernel<kManyParts>, grid, dim3(kCopyThreads), 0, stream, gather<kManyParts>(part, n), p);
+  static bool ready[2][64] = {};
+  const int many = n > kFewParts;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !ready[many][dev]) {
+    const cudaError_t e = many ? cudaFuncSetAttribute(copy_blocks_kernel<kManyParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes)
+                               : cudaFuncSetAttribute(copy_blocks_kernel<kFewParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "%s: cannot reserve shared memory: %s", what, cudaGetErrorString(e));
+    if (dev >= 0 && dev < 64) ready[many][dev] = true;
+  }
+  const dim3 grid(static_cast<unsigned>(num_sms()));
+  if (!many) return launch_kernel(what, copy_blocks_kernel<kFewParts>, grid, dim3(kCopyThreads), kRingBytes, stream, gather<kFewParts>(part, n), p);
+  return launch_kernel(what, copy_blocks_kernel<kManyParts>, grid, dim3(kCopyThreads), kRingBytes, stream, gather<kManyParts>(part, n), p);
 }
 
 static int check_tables(const char* what, const int32_t* table, int64_t stride, int32_t width, const int32_t* lens, int32_t batch) {
@@ -458,7 +509,7 @@ extern "C" int nvllm_fork_sequences(const nvllm_cache_part* parts, int32_t num_p
   const int many = num_parts > kFewParts;
   int dev = 0;
   cudaGetDevice(&dev);
-  auto bytes = [](int64_t old, int64_t rows) { return static_cast<size_t>(((old + rows + 3) & ~3ll) * 4 + rows * 16); };
+  auto bytes = [](int64_t old, int64_t rows) { return static_cast<size_t>(kRingBytes + ((old + rows + 3) & ~3ll) * 4 + rows * 16); };
   if (dev < 0 || dev >= 64 || !ready[many][dev]) {
     const int most = static_cast<int>(bytes(kForkMax, kForkMax));
     const cudaError_t e = many ? cudaFuncSetAttribute(fork_kernel<kManyParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)
@@ -466,7 +517,7 @@ extern "C" int nvllm_fork_sequences(const nvllm_cache_part* parts, int32_t num_p
     if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "fork_sequences: cannot reserve shared memory: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[many][dev] = true;
   }
-  const dim3 grid(static_cast<unsigned>(4 * num_sms()));
+  const dim3 grid(static_cast<unsigned>(num_sms()));
   const size_t smem = bytes(batch, num_rows);
   if (!many)
     return launch_kernel("fork_sequences", fork_kernel<kFewParts>, grid, dim3(kCopyThreads), smem, static_cast<cudaStream_t>(stream),
