@@ -33,9 +33,13 @@ struct Parts {
   int n, planes, value_planes;  // planes of all parts, and of those that are not scales
 };
 
-// ---- copies: a thread keeps a ring of pieces of shared memory busy, bulk loads kLead pieces ahead of the bulk stores
-constexpr int kPiece = 16384, kStages = 8, kLead = 5;
+// ---- copies: a thread keeps a ring of pieces of shared memory busy, bulk loads kLead pieces ahead of the bulk stores.  Two such
+// blocks to an SM with 6 pieces of 16 KB move 6.1-6.2 TB/s (the copy rate is 6.55): one with 8 pieces is as fast on large copies and
+// 1-2 us slower on small ones (three blocks of one layer 6.8 us, 4.5 so: room for the next launch beside it), pieces of 8 KB
+// 5.5 TB/s, threads with 16-byte loads and stores 5.2-5.4.
+constexpr int kPiece = 16384, kStages = 6, kLead = 2;
 constexpr int kRingBytes = kPiece * kStages + 128;  // barriers behind the pieces
+static_assert(kStages * 8 <= 128 && kLead < kStages, "barriers, and a stage whose store is being read");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -277,52 +281,86 @@ struct PlanParams {
   int* status;
 };
 
-template <bool COMPACT>
+template <bool COMPACT, bool SEVERAL>
 __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) {
   namespace cg = cooperative_groups;
   extern __shared__ int s_count[];  // of the ids [first, first + mine)
   __shared__ int s_warp[kPlanThreads / 32], s_free[kPlanMaxCluster], s_holes;
   cg::cluster_group cluster = cg::this_cluster();
-  const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank()), tid = threadIdx.x;
+  const int csize = SEVERAL ? static_cast<int>(cluster.num_blocks()) : 1, crank = SEVERAL ? static_cast<int>(cluster.block_rank()) : 0;
+  const int tid = threadIdx.x;
   const int share = (p.num_blocks + csize - 1) / csize, first = crank * share, mine = max(0, min(share, p.num_blocks - first));
   const int me = crank * kPlanThreads + tid, all = csize * kPlanThreads;
-  pdl_prologue();
-  for (int i = tid; i < mine; i += kPlanThreads) s_count[i] = p.held ? max(p.held[first + i], 0) : 0;
-  cluster.sync();
-
-  const int most = p.width * kBlockSize;
-  const int64_t entries = static_cast<int64_t>(p.batch) * p.width;
-  bool bad = false;
-  // the id at an entry in use, or a negative number
-  auto entry = [&](int64_t e) {
-    const int b = static_cast<int>(e / p.width), col = static_cast<int>(e - static_cast<int64_t>(b) * p.width);
-    const int id = p.table[b * p.stride + col], n = p.lens[b];
-    bad |= n < 0 || n > most;
-    if (col >= blocks_of(max(0, min(n, most)))) return -1;
-    bad |= id >= p.num_blocks;
-    return id < p.num_blocks ? id : -1;
+  auto sync = [&]() {
+    if constexpr (SEVERAL) cluster.sync();
+    else __syncthreads();
   };
-  for (int64_t e = me; e < entries; e += all) {
-    const int id = entry(e);
-    if (id >= 0) {
-      const int owner = id / share;
-      atomicAdd(cluster.map_shared_rank(s_count, owner) + (id - owner * share), 1);
+  auto at_rank = [&](int* mem, int r) {
+    if constexpr (SEVERAL) return cluster.map_shared_rank(mem, r);
+    else return mem;
+  };
+  auto count_of = [&](int id) {
+    const int owner = SEVERAL ? id / share : 0;
+    return at_rank(s_count, owner) + (id - owner * share);
+  };
+  pdl_prologue();
+
+  // The entries in use, a few of a thread in flight at a time: f(entry, id), a negative id where there is none.
+  const int most = p.width * kBlockSize, entries = p.batch * p.width;
+  constexpr int E = 8;
+  bool bad = false;
+  int id[E], len[E];
+  auto load = [&](int from) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const unsigned e = from + k * all;
+      if (e < static_cast<unsigned>(entries)) {
+        const int b = e / static_cast<unsigned>(p.width);
+        len[k] = p.lens[b];
+        id[k] = p.table[b * p.stride + (e - b * p.width)];
+      }
     }
+  };
+  auto each = [&](int from, auto&& f) {
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+      const unsigned e = from + k * all;
+      if (e >= static_cast<unsigned>(entries)) continue;
+      const int col = e % static_cast<unsigned>(p.width), n = len[k];
+      bad |= n < 0 || n > most;
+      const bool used = col < blocks_of(max(0, min(n, most)));
+      bad |= used && id[k] >= p.num_blocks;
+      f(e, used && id[k] < p.num_blocks ? id[k] : -1);
+    }
+  };
+  load(me);
+  for (int i = tid; i < mine; i += kPlanThreads) s_count[i] = p.held ? max(p.held[first + i], 0) : 0;
+  sync();
+  for (int from = me;;) {
+    each(from, [&](int, int i) {
+      if (i >= 0) atomicAdd(count_of(i), 1);
+    });
+    if (entries - from <= E * all) break;
+    from += E * all;
+    load(from);
   }
   if (bad) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
-  cluster.sync();
+  sync();
 
   // free ids before those of a thread, which has a run of them (odd: no two of a warp in one bank)
   const int run = ((mine + kPlanThreads - 1) / kPlanThreads) | 1, lo = min(tid * run, mine), hi = min(lo + run, mine);
   int sum = 0, total;
   for (int i = lo; i < hi; ++i) sum += s_count[i] == 0;
   int before = scan_block<kPlanThreads>(sum, s_warp, &total);
-  if (tid < csize) cluster.map_shared_rank(s_free, tid)[crank] = total;
-  cluster.sync();
-  int free_all = 0;
-  for (int r = 0; r < csize; ++r) {
-    if (r < crank) before += s_free[r];
-    free_all += s_free[r];
+  int free_all = total;
+  if constexpr (SEVERAL) {
+    if (tid < csize) cluster.map_shared_rank(s_free, tid)[crank] = total;
+    cluster.sync();
+    free_all = 0;
+    for (int r = 0; r < csize; ++r) {
+      if (r < crank) before += s_free[r];
+      free_all += s_free[r];
+    }
   }
   if constexpr (!COMPACT) {
     for (int i = lo; i < hi; ++i)
@@ -335,51 +373,49 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanParams p) 
     int f = before;
     for (int i = lo; i < hi; ++i) {  // free ids before id `live`: the holes, as many as blocks move
       if (first + i == live)
-        for (int r = 0; r < csize; ++r) cluster.map_shared_rank(&s_holes, r)[0] = f;
+        for (int r = 0; r < csize; ++r) at_rank(&s_holes, r)[0] = f;
       f += s_count[i] == 0;
     }
     if (live == p.num_blocks && tid == 0) s_holes = 0;
-    cluster.sync();
+    sync();
     const int holes = s_holes;
     f = before;
     for (int i = lo; i < hi; ++i) {
-      const int id = first + i;
+      const int b = first + i;
       if (s_count[i] == 0) {
-        if (id < live) p.holes[f] = id;
+        if (b < live) p.holes[f] = b;
         ++f;
-      } else if (id >= live) {
-        p.movers[id - f - (live - holes)] = id;
+      } else if (b >= live) {
+        p.movers[b - f - (live - holes)] = b;
       }
     }
-    cluster.sync();
+    sync();
     f = before;
     for (int i = lo; i < hi; ++i) {
-      const int id = first + i;
-      int to = id;
+      const int b = first + i;
+      int to = b;
       if (s_count[i] == 0) {
         ++f;
         to = -1;
-      } else if (id >= live) {
-        to = __ldcg(p.holes + (id - f - (live - holes)));
+      } else if (b >= live) {
+        to = __ldcg(p.holes + (b - f - (live - holes)));
       }
       s_count[i] = to;
     }
-    cluster.sync();
+    sync();
     for (int i = tid; i < mine; i += kPlanThreads) p.moved_to[first + i] = s_count[i];
-    for (int64_t e = me; e < entries; e += all) {
-      const int b = static_cast<int>(e / p.width), col = static_cast<int>(e - static_cast<int64_t>(b) * p.width), id = entry(e);
-      int to = -1;
-      if (id >= 0) {
-        const int owner = id / share;
-        to = cluster.map_shared_rank(s_count, owner)[id - owner * share];
-      }
-      p.new_table[b * p.new_stride + col] = to;
+    for (int from = me; from < entries; from += E * all) {
+      if (entries > E * all) load(from);  // else the thread still has its entries
+      each(from, [&](int e, int i) {
+        const int b = e / p.width;
+        p.new_table[b * p.new_stride + (e - b * p.width)] = i >= 0 ? *count_of(i) : -1;
+      });
     }
     if (me == 0) {
       *p.num_live = live;
       *p.moves = holes;
     }
-    cluster.sync();  // the others read this block's shared memory
+    if constexpr (SEVERAL) cluster.sync();  // the others read this block's shared memory
   }
 }
 
@@ -428,14 +464,15 @@ static int launch_copies(const char* what, const nvllm_cache_part* part, int n, 
     if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "%s: cannot reserve shared memory: %s", what, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[many][dev] = true;
   }
-  const dim3 grid(static_cast<unsigned>(num_sms()));
+  const dim3 grid(static_cast<unsigned>(2 * num_sms()));
   if (!many) return launch_kernel(what, copy_blocks_kernel<kFewParts>, grid, dim3(kCopyThreads), kRingBytes, stream, gather<kFewParts>(part, n), p);
   return launch_kernel(what, copy_blocks_kernel<kManyParts>, grid, dim3(kCopyThreads), kRingBytes, stream, gather<kManyParts>(part, n), p);
 }
 
 static int check_tables(const char* what, const int32_t* table, int64_t stride, int32_t width, const int32_t* lens, int32_t batch) {
-  if (batch < 0 || width <= 0 || stride < width || static_cast<int64_t>(width) * kBlockSize > 0x7fffffff)
-    return fail(NVLLM_E_GEOMETRY, "%s: batch=%d max_blocks=%d invalid or beyond the row stride", what, batch, width);
+  if (batch < 0 || width <= 0 || stride < width || static_cast<int64_t>(width) * kBlockSize > 0x7fffffff ||
+      static_cast<int64_t>(batch) * width > (1 << 28))
+    return fail(NVLLM_E_GEOMETRY, "%s: batch=%d max_blocks=%d invalid, beyond the row stride or too many entries", what, batch, width);
   if (batch > 0 && (!table || !lens)) return fail(NVLLM_E_NULL, "%s: NULL pointer argument", what);
   return NVLLM_OK;
 }
@@ -447,28 +484,29 @@ static int launch_plan(const char* what, const PlanParams& p, cudaStream_t strea
   cudaGetDevice(&dev);
   constexpr int most = (kPlanMaxBlocks + kPlanMaxCluster - 1) / kPlanMaxCluster * 4;
   if (dev < 0 || dev >= 64 || !ready[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(plan_kernel<COMPACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    cudaError_t e = cudaFuncSetAttribute(plan_kernel<COMPACT, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(plan_kernel<COMPACT, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "%s: cannot reserve shared memory: %s", what, cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
+  // One block up to four entries and blocks to a thread (64 x 16 entries 3.9 us, 256 x 16 entries of 2000 blocks 5.5, a cluster 6.1),
+  // then a cluster of eight (256 x 32 of 4200 6.4 us, two blocks 7.5, one 8.8; 512 x 32 of 8000 7.7, two 12).
   const int64_t items = std::max<int64_t>(p.num_blocks, static_cast<int64_t>(p.batch) * p.width);
-  int csize = 1;
-  while (csize < kPlanMaxCluster && (items > 4ll * csize * kPlanThreads)) csize *= 2;
-  while (csize < kPlanMaxCluster && (p.num_blocks + csize - 1) / csize * 4 > most) csize *= 2;
+  const int csize = items <= 4 * kPlanThreads ? 1 : kPlanMaxCluster;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(csize);
   cfg.blockDim = dim3(kPlanThreads);
   cfg.dynamicSmemBytes = static_cast<size_t>((p.num_blocks + csize - 1) / csize) * 4;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = csize;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = csize;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, plan_kernel<COMPACT>, p);
+  cfg.numAttrs = csize > 1 ? 2 : 1;
+  const cudaError_t e = csize > 1 ? cudaLaunchKernelEx(&cfg, plan_kernel<COMPACT, true>, p) : cudaLaunchKernelEx(&cfg, plan_kernel<COMPACT, false>, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();
     return fail(NVLLM_E_CUDA, "%s launch: %s", what, cudaGetErrorString(e));
@@ -517,7 +555,7 @@ extern "C" int nvllm_fork_sequences(const nvllm_cache_part* parts, int32_t num_p
     if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "fork_sequences: cannot reserve shared memory: %s", cudaGetErrorString(e));
     if (dev >= 0 && dev < 64) ready[many][dev] = true;
   }
-  const dim3 grid(static_cast<unsigned>(num_sms()));
+  const dim3 grid(static_cast<unsigned>(2 * num_sms()));
   const size_t smem = bytes(batch, num_rows);
   if (!many)
     return launch_kernel("fork_sequences", fork_kernel<kFewParts>, grid, dim3(kCopyThreads), smem, static_cast<cudaStream_t>(stream),
