@@ -197,27 +197,33 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constan
   extern __shared__ __align__(128) unsigned char s_ring[];
   int* s_mem = reinterpret_cast<int*>(s_ring + kRingBytes);
   int* s_first = s_mem;               // of every old sequence: its first new row
-  int* s_fresh = s_first + p.batch;   // of every new row: the block of its own that it gets, -1 none left, -2 none needed
-  int4* s_list = reinterpret_cast<int4*>(s_mem + ((p.batch + p.rows + 3) & ~3));  // copies: from, to, slots
+  int* s_len = s_first + p.batch;     // and its length
+  int* s_fresh = s_len + p.batch;     // of every new row: the block of its own that it gets, -1 none left, -2 none needed
+  int4* s_list = reinterpret_cast<int4*>(s_mem + ((2 * p.batch + p.rows + 3) & ~3));  // copies: from, to, slots
   __shared__ int s_warp[kCopyThreads / 32];
   const int tid = threadIdx.x;
   pdl_prologue();
-  for (int b = tid; b < p.batch; b += kCopyThreads) s_first[b] = 0x7fffffff;
-  __syncthreads();
-  bool bad_parent = false, bad_len = false;
-  for (int i = tid; i < p.rows; i += kCopyThreads) {
-    const int b = p.parents[i];
-    if (b >= 0 && b < p.batch) atomicMin(&s_first[b], i);
-    else bad_parent |= b >= p.batch;
+  const int most = p.width * kBlockSize;
+  bool bad = false;
+  int parent = tid < p.rows ? p.parents[tid] : -1;  // in flight with the lengths
+  for (int b = tid; b < p.batch; b += kCopyThreads) {
+    const int n = p.lens[b], len = max(0, min(n, most));
+    s_first[b] = 0x7fffffff;
+    s_len[b] = len;
+    if (n != len) s_len[b] = len | static_cast<int>(0x80000000u);  // marked: an error if a row goes on from it
   }
   __syncthreads();
-  const int most = p.width * kBlockSize;
-  auto length = [&](int b) {
-    if (b < 0 || b >= p.batch) return 0;
-    const int n = p.lens[b];
-    bad_len |= n < 0 || n > most;
-    return max(0, min(n, most));
-  };
+  for (int i = tid; i < p.rows; i += kCopyThreads) {
+    const int b = i == tid ? parent : p.parents[i];
+    if (b >= 0 && b < p.batch) {
+      atomicMin(&s_first[b], i);
+      bad |= s_len[b] < 0;
+    } else {
+      bad |= b >= p.batch;
+    }
+  }
+  __syncthreads();
+  auto length = [&](int b) { return b < 0 || b >= p.batch ? 0 : s_len[b] & 0x7fffffff; };
   const int per = (p.rows + kCopyThreads - 1) / kCopyThreads, lo = min(tid * per, p.rows), hi = min(lo + per, p.rows);
   int sum = 0;
   for (int i = lo; i < hi; ++i) {
@@ -239,12 +245,14 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(const __grid_constan
   }
   __syncthreads();
   if (blockIdx.x == 0) {
-    for (int i = tid; i < p.rows; i += kCopyThreads) p.new_lens[i] = length(p.parents[i]);
-    if (tid == 0) *p.taken = total;
-    if (bad_parent || bad_len) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
+    if (bad) atomicOr(p.status, NVLLM_STATUS_BAD_BLOCK);
+    for (int i = tid - 32; i >= 0 && i < p.rows; i += kCopyThreads - 32) p.new_lens[i] = length(p.parents[i]);
+    if (tid == 32) *p.taken = total;
   }
-  for (int64_t e = static_cast<int64_t>(blockIdx.x) * kCopyThreads + tid; e < static_cast<int64_t>(p.rows) * p.width; e += static_cast<int64_t>(gridDim.x) * kCopyThreads) {
-    const int i = static_cast<int>(e / p.width), col = static_cast<int>(e - static_cast<int64_t>(i) * p.width);
+  // the tables, while the first thread copies
+  constexpr int writers = kCopyThreads - 32;
+  for (unsigned e = blockIdx.x * writers + tid - 32; tid >= 32 && e < static_cast<unsigned>(p.rows) * p.width; e += gridDim.x * writers) {
+    const int i = static_cast<int>(e / p.width), col = static_cast<int>(e - i * p.width);
     const int b = p.parents[i], need = blocks_of(length(b)), fresh = s_fresh[i];
     int id = -1;
     if (col < need) id = col == need - 1 && fresh != -2 ? fresh : p.table[b * p.stride + col];
@@ -536,6 +544,7 @@ extern "C" int nvllm_fork_sequences(const nvllm_cache_part* parts, int32_t num_p
   using namespace nvllm;
   if (const int e = check_parts("fork_sequences", parts, num_parts, num_blocks)) return e;
   if (const int e = check_tables("fork_sequences", block_tables, bt_row_stride, max_blocks, seq_lens, batch)) return e;
+  if (static_cast<int64_t>(num_rows) * max_blocks > (1 << 28)) return fail(NVLLM_E_GEOMETRY, "fork_sequences: %d rows of %d blocks are too many", num_rows, max_blocks);
   if (batch > kForkMax || num_rows <= 0 || num_rows > kForkMax || num_free < 0 || new_row_stride < max_blocks)
     return fail(NVLLM_E_GEOMETRY, "fork_sequences: %d rows from %d outside 1 to %d, num_free=%d, or a short row stride", num_rows, batch, kForkMax, num_free);
   if (!parents || !new_tables || !new_lens || !blocks_taken || (num_free > 0 && !free_blocks))
@@ -547,7 +556,7 @@ extern "C" int nvllm_fork_sequences(const nvllm_cache_part* parts, int32_t num_p
   const int many = num_parts > kFewParts;
   int dev = 0;
   cudaGetDevice(&dev);
-  auto bytes = [](int64_t old, int64_t rows) { return static_cast<size_t>(kRingBytes + ((old + rows + 3) & ~3ll) * 4 + rows * 16); };
+  auto bytes = [](int64_t old, int64_t rows) { return static_cast<size_t>(kRingBytes + ((2 * old + rows + 3) & ~3ll) * 4 + rows * 16); };
   if (dev < 0 || dev >= 64 || !ready[many][dev]) {
     const int most = static_cast<int>(bytes(kForkMax, kForkMax));
     const cudaError_t e = many ? cudaFuncSetAttribute(fork_kernel<kManyParts>, cudaFuncAttributeMaxDynamicSharedMemorySize, most)
