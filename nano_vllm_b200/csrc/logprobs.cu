@@ -147,17 +147,22 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   const int whole = pieces - head - tail;
   auto cut_piece = [&](int g) { return P::cut(__ldg(base + g), g == 0 ? shift : 0, g == pieces - 1 ? last_hi : N); };
 
-  // A thread takes C pieces at a time, loaded one step ahead.
+  // A thread takes C pieces at a time; those of the next step are loaded before the current ones are looked at, into the other of
+  // two sets of registers (one set, copied, took 0.5 instructions an element).  The last step, which not all pieces may have, comes
+  // first, beside the first one.
   const uint4* from = base + head;
-  const uint4 nothing = P::cut(make_uint4(0, 0, 0, 0), 0, 0);
-  uint4 next[C];
   const int step = C * all;
-  auto load = [&](int j) {
+  const int steps = max(0, (whole - (me - lane) - 31 - (C - 1) * all + step - 1) / step);  // that all lanes have whole
+  const int rest = me + steps * step;                                                   // where the last one starts
+  uint4 x0[C], x1[C];
+  auto load = [&](uint4 (&to)[C], int j) {
 #pragma unroll
-    for (int k = 0; k < C; ++k) next[k] = j + k * all < whole ? __ldg(from + j + k * all) : nothing;
+    for (int k = 0; k < C; ++k) to[k] = __ldg(from + j + k * all);
   };
-  int i = me;
-  load(i);
+  if (steps > 0) load(x0, me);
+  const uint4 nothing = P::cut(make_uint4(0, 0, 0, 0), 0, 0);
+#pragma unroll
+  for (int k = 0; k < C; ++k) x1[k] = rest + k * all < whole ? __ldg(from + rest + k * all) : nothing;
   const float inv_t = lp_inverse(p.temperatures, row);
   const float c = inv_t * 1.4426950408889634f;
   int64_t token = -1;
@@ -174,7 +179,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   LpSums sum{-FLT_MAX, 0.f, 0.f};
   float best = -INFINITY;
   const bool any = me == 0 || me < whole;
-  int at = head + me;  // the first piece with the largest element so far
+  int at = 0;  // the first piece with the largest element so far
   const uint64_t c2 = pack2(c, c);
   // Sums over pieces.  A masked element's difference is -infinity, whose product with its weight of 0 is NaN: such pieces are
   // read and summed again with the differences kept finite (which costs the others an instruction an element).
@@ -223,11 +228,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       sum.rescale(m, c);
     }
   };
-  for (; i - lane < whole; i += step) {
-    uint4 raw[C];
-#pragma unroll
-    for (int k = 0; k < C; ++k) raw[k] = next[k];
-    if (i + step - lane < whole) load(i + step);
+  // Pieces i, i + all, ...
+  auto take = [&](const uint4 (&raw)[C], int i) {
     if constexpr (TOP) {
       float largest = -INFINITY;
 #pragma unroll
@@ -254,6 +256,27 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       for (int k = 0; k < C; ++k)
         if (i + k * all < whole) slow(__ldg(from + i + k * all));
     }
+  };
+  if (rest - lane < whole) {
+    at = head + rest;
+    take(x1, rest);
+  }
+  const float best_last = best;
+  const int at_last = at;
+  best = -INFINITY;
+  at = head + me;
+  for (int n = 0, i = me; n < steps; n += 2) {
+    if (n + 1 < steps) load(x1, i + step);
+    take(x0, i);
+    i += step;
+    if (n + 1 >= steps) break;
+    if (n + 2 < steps) load(x0, i + step);
+    take(x1, i);
+    i += step;
+  }
+  if (best_last > best || steps == 0) {
+    best = best_last;
+    at = at_last;
   }
   if (crank == 0 && warp == 0 && (head || tail)) {
     const uint4 w0 = head && lane == 0 ? cut_piece(0) : nothing, w1 = tail && lane == 0 ? cut_piece(pieces - 1) : nothing;
