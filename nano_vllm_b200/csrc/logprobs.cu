@@ -35,6 +35,7 @@ struct LogprobParams {
   const float* temperatures;  // nullable
   int vocab, top;
   int groups;  // of the threads that read a row, whose maxima give the bound: 32 to 128
+  int log_csize, log_all, log_size;  // blocks of a row, its threads, threads of a group: powers of two, divided by with shifts
   float* logprobs;
   float* entropy;
   int64_t* top_tokens;
@@ -130,11 +131,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   __shared__ uint64_t s_most[kLpThreads / 32], s_all[2 * kLpMaxCluster];
   pdl_wait();
   cg::cluster_group cluster = cg::this_cluster();
-  const int csize = static_cast<int>(cluster.num_blocks()), crank = static_cast<int>(cluster.block_rank());
+  const int csize = 1 << p.log_csize, crank = blockIdx.x & (csize - 1);
   const bool several = csize > 1;
   if (several) cluster.barrier_arrive();  // waited for before another block's shared memory is written
-  const int row = blockIdx.x / csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
-  const int me = crank * threads + tid, all = csize * threads;  // of the row's threads
+  const int row = blockIdx.x >> p.log_csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = 1 << (p.log_all - p.log_csize);
+  const int me = crank * threads + tid, all = 1 << p.log_all;  // of the row's threads
   const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
 
   // Pieces start on 16-byte boundaries: what lies before and behind the row in the first and last one counts as -infinity.
@@ -152,7 +153,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   // first, beside the first one.
   const uint4* from = base + head;
   const int step = C * all;
-  const int steps = max(0, (whole - (me - lane) - 31 - (C - 1) * all + step - 1) / step);  // that all lanes have whole
+  const int steps = max(0, ((whole - (me - lane) - 32 + all) >> p.log_all) / C);  // that all lanes have whole
   const int rest = me + steps * step;                                                   // where the last one starts
   uint4 x0[C], x1[C];
   auto load = [&](uint4 (&to)[C], int j) {
@@ -320,11 +321,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   };
   if (several) cluster.barrier_wait();
   if constexpr (TOP) {
-    const int size = all / p.groups;  // threads of a group: 1 to 32
+    const int size = 1 << p.log_size;  // threads of a group: 1 to 32
     uint64_t most = mine;
     for (int sh = 1; sh < size; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
     // every block of the row gets all groups'
-    for (int to = tid % size; to < csize; to += size) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[me / size] = most;
+    for (int to = tid & (size - 1); to < csize; to += size) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[me >> p.log_size] = most;
   }
   __syncthreads();
   if (warp == 0) {
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
     tau = s_tau;
     if (mine && mine >= tau) s_slot[atomicAdd(&s_slots, 1)] = static_cast<uint16_t>(tid);
     __syncthreads();
-    each = (whole + all - 1) / all;  // pieces of a thread
+    each = (whole + all - 1) >> p.log_all;  // pieces of a thread
     each_inv = __frcp_rn(static_cast<float>(each));
     total = s_slots * each;
     looked = total + (crank == 0 ? head + tail : 0);
@@ -493,6 +494,14 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   while (csize == 1 && threads > 64 && pieces < 8ll * threads) threads /= 2;
   const int all = csize * threads;
   p.groups = top <= 20 ? std::max(32, all / 32) : std::min(kLpGroups, all);
+  auto log2_of = [](int n) {
+    int l = 0;
+    while (n >> (l + 1)) ++l;
+    return l;
+  };
+  p.log_csize = log2_of(csize);
+  p.log_all = log2_of(all);
+  p.log_size = log2_of(all / p.groups);
   if (static_cast<int64_t>(rows) * csize > 0x7fffffff) return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d too many", rows);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * csize), 1, 1);
