@@ -20,20 +20,20 @@ using namespace sm100;
 // shared memory, the first one's thread multiplies both with tcgen05 of two blocks, and each reduces its own rows.
 constexpr int BM = 128, BN = 256, BK = 64;
 constexpr int kChunk = 1024;
-constexpr int CTRL_BYTES = 1024, RING_BYTES = 192 * 1024, SMEM = CTRL_BYTES + RING_BYTES + 1024;  // + alignment slack
-constexpr int A_BYTES = BM * BK * 2;
+// A stage holds what is loaded of a tile's rows and its columns for 64 elements of k.  The product reads 128 rows all the same:
+// behind the loaded ones whatever follows, which ends in accumulator rows that nobody reads (the last stage's lie in the slack).
+constexpr int CTRL_BYTES = 1024, RING_BYTES = 192 * 1024, SLACK_BYTES = BM * BK * 2;
+constexpr int SMEM = CTRL_BYTES + RING_BYTES + SLACK_BYTES + 1024;  // + alignment
 constexpr int TMEM_COLS = 512;  // two accumulators
-constexpr int MAX_NST = 6;
+constexpr int MAX_NST = 16;
 enum Bar { FULL0 = 0, EMPTY0 = MAX_NST, ACC_FULL0 = 2 * MAX_NST, ACC_FREE0 = 2 * MAX_NST + 2, DRAIN = 2 * MAX_NST + 4, NUM_BARS };
 
 template <bool PAIR, bool LONG>
 struct Cfg {
-  static constexpr int STAGE_BYTES = A_BYTES + BN * BK * 2 / (PAIR ? 2 : 1), NST = RING_BYTES / STAGE_BYTES;
   static constexpr int WARPS = 8, COLS = BN / (WARPS / 4);  // of the epilogue; columns of a thread
   static constexpr int THREADS = (WARPS + 4) * 32;          // registers come by fours of warps
   // registers at launch and as the groups share them: the parts of long sums are added in those of the epilogue
   static constexpr int REGS = 168, REGS_EPILOGUE = 216, REGS_OTHER = 72;
-  static_assert(NST <= MAX_NST, "barriers");
   static_assert(!LONG || WARPS * REGS_EPILOGUE + 4 * REGS_OTHER <= (WARPS + 4) * REGS, "no more than the block has");
 };
 
@@ -101,7 +101,8 @@ struct Params {
   int mt, nt;     // tiles of rows and of columns
   int group, ng;  // column tiles that a unit of work has one after the other, and how many such groups
   int mb;         // row tiles whose units take turns
-  int a_rows;     // rows of a tile that are loaded
+  int a_rows;     // rows of a tile that are loaded (of each block)
+  int nst;        // stages
   int kb;         // blocks of 64 elements of a row
   int keep;       // a thread block has one row tile all along
   float4* partial;  // [slot][half][mt * 128]: maximum, sum, sum times logits
@@ -120,7 +121,8 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int i) {
 template <bool PAIR, bool LONG>
 __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   using G = Cfg<PAIR, LONG>;
-  constexpr int NST = G::NST, WARPS = G::WARPS, COLS = G::COLS, STAGE = G::STAGE_BYTES, CTAS = PAIR ? 2 : 1;
+  constexpr int WARPS = G::WARPS, COLS = G::COLS, CTAS = PAIR ? 2 : 1;
+  const int a_bytes = p.a_rows * BK * 2, stage_bytes = a_bytes + p.bn / CTAS * BK * 2, nst = p.nst;
   extern __shared__ unsigned char smem_raw[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = PAIR ? blockIdx.x & 1 : 0;  // in the pair
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
       // ------------------------------------------------------------------ TMA producer
       if (elect_one()) {
         const int b_rows = p.bn / CTAS;
-        const uint32_t bytes = CTAS * (p.a_rows + b_rows) * BK * 2;  // of both blocks: the first one's barriers count them
+        const uint32_t bytes = CTAS * stage_bytes;  // of both blocks: the first one's barriers count them
         int s = 0, use = 0;
         bool ok = true;
         for (int i = first_unit; i < units && ok; i += unit_step) {
@@ -161,24 +163,24 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
           for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n)
             for (int kb = 0; kb < p.kb; ++kb) {
               if (use > 0 && !(ok = wait_or_abort(bar(EMPTY0 + s), (use - 1) & 1, abort_flag))) break;
-              const uint32_t dst = ring + s * STAGE;
+              const uint32_t dst = ring + s * stage_bytes;
               if (rank == 0) mbar_expect_tx(bar(FULL0 + s), bytes);
               if constexpr (PAIR) {
                 const uint32_t full = map_to(bar(FULL0 + s), 0);
                 tma_load_pair(dst, &map_a, full, kb * BK, 0, (u.m * 2 + rank) * BM);
-                tma_load_pair(dst + A_BYTES, &map_b, full, kb * BK, 0, n * p.bn + rank * b_rows);
+                tma_load_pair(dst + a_bytes, &map_b, full, kb * BK, 0, n * p.bn + rank * b_rows);
               } else {
                 tma_load_3d(dst, &map_a, bar(FULL0 + s), kb * BK, 0, u.m * BM);
-                tma_load_3d(dst + A_BYTES, &map_b, bar(FULL0 + s), kb * BK, 0, n * p.bn);
+                tma_load_3d(dst + a_bytes, &map_b, bar(FULL0 + s), kb * BK, 0, n * p.bn);
               }
-              if (++s == NST) {
+              if (++s == nst) {
                 s = 0;
                 ++use;
               }
             }
         }
         if (!ok && rank == 0)  // no copy is in flight when the block (the pair) ends
-          for (int k = 0; k < NST; ++k) {
+          for (int k = 0; k < nst; ++k) {
             const int uses = k < s ? use + 1 : use;
             if (uses > 0) (void)mbar_wait(bar(FULL0 + k), (uses - 1) & 1);
           }
@@ -205,14 +207,14 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
               for (int kb = first; kb < last; ++kb) {
                 if (!(ok = wait_or_abort(bar(FULL0 + s), use & 1, abort_flag))) break;
                 tc_fence_after();
-                const uint64_t da = desc0 + static_cast<uint64_t>((s * STAGE) >> 4), db = da + (A_BYTES >> 4);
+                const uint64_t da = desc0 + static_cast<uint64_t>((s * stage_bytes) >> 4), db = da + (a_bytes >> 4);
 #pragma unroll
                 for (int ks = 0; ks < BK / 16; ++ks) {
                   if constexpr (PAIR) umma_pair(tmem + b * BN, da + 2 * ks, db + 2 * ks, idesc, kb > first || ks > 0);
                   else umma_ss(tmem + b * BN, da + 2 * ks, db + 2 * ks, idesc, kb > first || ks > 0);
                 }
                 commit(EMPTY0 + s);
-                if (++s == NST) {
+                if (++s == nst) {
                   s = 0;
                   ++use;
                 }
@@ -420,7 +422,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
 
 // How a problem is laid out over the multiprocessors.
 struct Plan {
-  int pair, bn, mt, nt, group, ng, mb, kb, keep, grid, slots, a_rows;
+  int pair, bn, mt, nt, group, ng, mb, kb, keep, grid, slots, a_rows, nst;
   int64_t rows_padded, bytes;
 };
 static Plan plan_of(int rows, int hidden, int vocab, int sms) {
@@ -438,6 +440,7 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
     if (bn == BN || cost < least) least = cost, pl.bn = bn;
   }
   pl.nt = (vocab + pl.bn - 1) / pl.bn;
+  pl.nst = std::min(MAX_NST, RING_BYTES / ((pl.a_rows + pl.bn / (pl.pair ? 2 : 1)) * BK * 2));
   pl.keep = pl.mt <= workers && workers % pl.mt == 0;
   pl.group = 1;
   while (!pl.keep && pl.group < 16 && static_cast<int64_t>(pl.mt) * ((pl.nt + 2 * pl.group - 1) / (2 * pl.group)) >= 48ll * workers) pl.group *= 2;
@@ -517,6 +520,7 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   p.ng = pl.ng;
   p.mb = pl.mb;
   p.a_rows = pl.a_rows;
+  p.nst = pl.nst;
   p.kb = pl.kb;
   p.keep = pl.keep;
   p.partial = static_cast<float4*>(workspace);
