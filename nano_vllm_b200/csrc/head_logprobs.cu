@@ -324,30 +324,24 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
             if (!(ok = wait_or_abort(bar(ACC_FULL0 + b), (it >> 1) & 1, abort_flag))) break;
             __syncwarp();
             tc_fence_after();
-            if (ch + 1 < chunks) {
 #pragma unroll
-              for (int j = 0; j < COLS; j += W) {
-                uint32_t v[W];
-                tmem_ld16(at + b * BN + j, v);
-                tmem_wait_ld();
+            for (int j = 0; j < COLS; j += W) {
+              uint32_t v[W];
+              tmem_ld16(at + b * BN + j, v);
+              tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < W; ++k) acc[j + k] = ch == 0 ? __uint_as_float(v[k]) : acc[j + k] + __uint_as_float(v[k]);
-              }
-              free_acc(b);
-            } else {
+              for (int k = 0; k < W; ++k) acc[j + k] = ch == 0 ? __uint_as_float(v[k]) : acc[j + k] + __uint_as_float(v[k]);
+            }
+            free_acc(b);
+          }
+          if (!ok) break;
 #pragma unroll
-              for (int j = 0; j < COLS; j += W) {
-                if (j < end && live) {
-                  uint32_t v[W];
-                  tmem_ld16(at + b * BN + j, v);
-                  tmem_wait_ld();
-                  float x[W];
+          for (int j = 0; j < COLS; j += W) {
+            if (j < end && live) {
+              float x[W];
 #pragma unroll
-                  for (int k = 0; k < W; ++k) x[k] = acc[j + k] + __uint_as_float(v[k]);
-                  add(x, first + j, end - j);
-                }
-              }
-              free_acc(b);
+              for (int k = 0; k < W; ++k) x[k] = acc[j + k];
+              add(x, first + j, end - j);
             }
           }
         }

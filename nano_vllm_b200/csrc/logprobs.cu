@@ -81,6 +81,24 @@ struct LpPiece<__nv_bfloat16> {
     };
     return make_uint4(f(a.x, b.x), f(a.y, b.y), f(a.z, b.z), f(a.w, b.w));
   }
+  static __device__ __forceinline__ float max_or_nan(const uint4& w) {
+    auto f = [](uint32_t u, uint32_t v) {
+      uint32_t r;
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(v));
+      return r;
+    };
+    const uint32_t m = f(f(w.x, w.y), f(w.z, w.w));
+    return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+  }
+  // -infinity becomes the lowest finite number, NaN stays
+  static __device__ __forceinline__ uint4 lift(const uint4& w) {
+    auto f = [](uint32_t u) {
+      uint32_t r;
+      asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0xff7fff7fu));
+      return r;
+    };
+    return make_uint4(f(w.x), f(w.y), f(w.z), f(w.w));
+  }
   // -infinity in the places below lo and from hi on
   static __device__ __forceinline__ uint4 cut(uint4 w, int lo, int hi) {
     uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -101,6 +119,13 @@ struct LpPiece<float> {
   }
   static __device__ __forceinline__ float max(const uint4& w) {
     return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static __device__ __forceinline__ float max_or_nan(const uint4& w) {
+    return max_nan(max_nan(__uint_as_float(w.x), __uint_as_float(w.y)), max_nan(__uint_as_float(w.z), __uint_as_float(w.w)));
+  }
+  static __device__ __forceinline__ uint4 lift(const uint4& w) {
+    auto f = [](uint32_t u) { return __float_as_uint(max_nan(__uint_as_float(u), -FLT_MAX)); };
+    return make_uint4(f(w.x), f(w.y), f(w.z), f(w.w));
   }
   static __device__ __forceinline__ uint4 larger(const uint4& a, const uint4& b) {
     auto f = [](uint32_t u, uint32_t v) { return __float_as_uint(fmaxf(__uint_as_float(u), __uint_as_float(v))); };
@@ -182,8 +207,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   const bool any = me == 0 || me < whole;
   int at = 0;  // the first piece with the largest element so far
   const uint64_t c2 = pack2(c, c);
-  // Sums over pieces.  A masked element's difference is -infinity, whose product with its weight of 0 is NaN: such pieces are
-  // read and summed again with the differences kept finite (which costs the others an instruction an element).
+  // Sums over pieces.  A masked element's difference is -infinity, whose product with its weight of 0 is NaN.  A warp that comes upon
+  // one lifts -infinity to the lowest finite number first, from then on: half an instruction an element, pieces of which nothing is
+  // left are passed over, and the sums are right while the maximum is far above that number and differences do not overflow;
+  // otherwise the pieces are read again and summed one by one, with the differences kept finite.
+  bool masked = false;
   auto add = [&](const uint4& w, auto finite, uint64_t& s2, uint64_t& t2) {
     const uint64_t minus_m = pack2(-sum.m, -sum.m);
     float e[N];
@@ -202,16 +230,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       t2 = fma2(w2, y, t2);
     }
   };
-  auto finish = [&](uint64_t s2, uint64_t t2) {
-    float a, b, u, v;
-    unpack2(s2, a, b);
-    unpack2(t2, u, v);
-    if (u + v != u + v) return false;
-    sum.s += a + b;
-    sum.t += u + v;
-    return true;
-  };
-  auto slow = [&](const uint4& w) {
+  auto one = [&](const uint4& w) {
     uint64_t s2 = 0, t2 = 0;
     add(w, std::true_type{}, s2, t2);
     float a, b;
@@ -229,8 +248,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       sum.rescale(m, c);
     }
   };
-  // Pieces i, i + all, ...
-  auto take = [&](const uint4 (&raw)[C], int i) {
+  // Pieces i, i + all, ...; ragged: some of them may not be there.
+  auto take = [&](uint4 (&raw)[C], int i, bool ragged) {
     if constexpr (TOP) {
       float largest = -INFINITY;
 #pragma unroll
@@ -249,18 +268,38 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       for (int k = 1; k < C; ++k) m = P::larger(m, raw[k]);
       grow(P::max(m));
     }
-    uint64_t s2 = 0, t2 = 0;
+    bool lifted = masked || ragged;
+    while (true) {
+      if (lifted) {
+        float most = P::max_or_nan(raw[0]);
 #pragma unroll
-    for (int k = 0; k < C; ++k) add(raw[k], std::false_type{}, s2, t2);
-    if (!finish(s2, t2)) {
-#pragma unroll 1
-      for (int k = 0; k < C; ++k)
-        if (i + k * all < whole) slow(__ldg(from + i + k * all));
+        for (int k = 1; k < C; ++k) most = max_nan(most, P::max_or_nan(raw[k]));
+        if (__all_sync(0xffffffffu, most == -INFINITY)) return;  // nothing left of them
+#pragma unroll
+        for (int k = 0; k < C; ++k) raw[k] = P::lift(raw[k]);
+      }
+      uint64_t s2 = 0, t2 = 0;
+#pragma unroll
+      for (int k = 0; k < C; ++k) add(raw[k], std::false_type{}, s2, t2);
+      float a, b, u, v;
+      unpack2(s2, a, b);
+      unpack2(t2, u, v);
+      u += v;
+      if (!__any_sync(0xffffffffu, u != u || (lifted && sum.m < -3e38f))) {
+        sum.s += a + b;
+        sum.t += u;
+        return;
+      }
+      if (lifted) break;
+      lifted = masked = true;
     }
+#pragma unroll 1
+    for (int k = 0; k < C; ++k)
+      if (i + k * all < whole) one(__ldg(from + i + k * all));
   };
   if (rest - lane < whole) {
     at = head + rest;
-    take(x1, rest);
+    take(x1, rest, true);
   }
   const float best_last = best;
   const int at_last = at;
@@ -268,11 +307,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   at = head + me;
   for (int n = 0, i = me; n < steps; n += 2) {
     if (n + 1 < steps) load(x1, i + step);
-    take(x0, i);
+    take(x0, i, false);
     i += step;
     if (n + 1 >= steps) break;
     if (n + 2 < steps) load(x0, i + step);
-    take(x1, i);
+    take(x1, i, false);
     i += step;
   }
   if (best_last > best || steps == 0) {
@@ -291,8 +330,8 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
       at = pieces - 1;
     }
     grow(fmaxf(first, last));
-    slow(w0);
-    slow(w1);
+    one(w0);
+    one(w1);
   }
 
   // ---- sums of the block, and the largest (maximum, piece) of every group of threads
