@@ -140,25 +140,250 @@ struct LpPiece<float> {
   }
 };
 
+// From the threads' statistics to the row's results.
 template <typename T, bool TOP>
-__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobParams p) {
+__device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, const float sum_t, const uint64_t mine, const uint4* const base,
+                                       const int shift, const int pieces, const int head, const int tail, const float inv_t, const float given,
+                                       const int64_t token, const int vocab, const int top, const int groups, const int log_csize, const int log_all,
+                                       const int log_size, float* const logprobs, float* const entropy, int64_t* const top_tokens,
+                                       float* const top_logprobs, int* const status) {
   using P = LpPiece<T>;
-  constexpr int N = P::N, C = TOP ? 3 : 4;
+  constexpr int N = P::N;
   namespace cg = cooperative_groups;
   __shared__ __align__(16) uint64_t s_bounds[kLpGroups];
   __shared__ uint64_t s_cand[kLpCands];  // of the first block
   __shared__ float s_sums[kLpMaxCluster][3];
   __shared__ float s_warp[kLpThreads / 32][3];
   __shared__ uint16_t s_slot[kLpThreads];
+  __shared__ uint64_t s_key[kLpThreads];
   __shared__ uint64_t s_tau;
   __shared__ float s_m, s_log_z;
   __shared__ int s_slots, s_cands;
   __shared__ uint64_t s_most[kLpThreads / 32], s_all[2 * kLpMaxCluster];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int csize = 1 << log_csize, crank = blockIdx.x & (csize - 1), row = blockIdx.x >> log_csize;
+  const bool several = csize > 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = 1 << (log_all - log_csize), all = 1 << log_all, me = crank * threads + tid;
+  const int whole = pieces - head - tail;
+  const float c = inv_t * 1.4426950408889634f;
+  LpSums sum{sum_m, sum_s, sum_t};
+  if (tid == 0) {
+    s_tau = 0;
+    s_slots = s_cands = 0;
+  }
+  // ---- sums of the block, and the largest (maximum, piece) of every group of threads
+  auto join_warp = [&](LpSums& v) {  // over the lanes
+    float m = v.m;
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
+    v.rescale(m, c);
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) {
+      v.s += __shfl_xor_sync(0xffffffffu, v.s, sh);
+      v.t += __shfl_xor_sync(0xffffffffu, v.t, sh);
+    }
+  };
+  join_warp(sum);
+  if (lane == 0) {
+    s_warp[warp][0] = sum.m;
+    s_warp[warp][1] = sum.s;
+    s_warp[warp][2] = sum.t;
+  }
+  auto sync = [&]() {
+    if (several) cluster.sync();
+    else __syncthreads();
+  };
+  if (several) cluster.barrier_wait();
+  if constexpr (TOP) {
+    const int size = 1 << log_size;  // threads of a group: 1 to 32
+    uint64_t most = mine;
+    for (int sh = 1; sh < size; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
+    // every block of the row gets all groups'
+    for (int to = tid & (size - 1); to < csize; to += size) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[me >> log_size] = most;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    const int w = min(lane, threads / 32 - 1);
+    sum = {s_warp[w][0], lane == w ? s_warp[w][1] : 0.f, lane == w ? s_warp[w][2] : 0.f};
+    join_warp(sum);
+    if (lane == 0) {
+      float* to = (several ? cluster.map_shared_rank(&s_sums[0][0], 0) : &s_sums[0][0]) + 3 * crank;
+      to[0] = sum.m;
+      to[1] = sum.s;
+      to[2] = sum.t;
+    }
+  }
+  pdl_trigger();
+  sync();
+
+  // ---- the bound that `top` elements of the row reach, and the elements that do: to the first block's list
+  int* cands_at = several ? cluster.map_shared_rank(&s_cands, 0) : &s_cands;
+  uint64_t* cand_at = several ? cluster.map_shared_rank(s_cand, 0) : s_cand;
+  uint64_t tau = 0;
+  float each_inv = 0.f;
+  int each = 0, total = 0, looked = 0;
+  // The keys of the elements that reach the bound in piece n of the listed threads, 0 in the place of the others.
+  auto look = [&](int n, uint64_t (&keys)[N]) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) keys[k] = 0;
+    int g;
+    uint4 w;
+    if (n < total) {
+      const int nth = static_cast<int>((static_cast<float>(n) + 0.5f) * each_inv), who = crank * threads + s_slot[nth];
+      g = head + who + (n - nth * each) * all;
+      if (g >= head + whole) return;
+      w = __ldg(base + g);
+    } else if (n < looked) {  // the cut pieces, whether they are in a listed thread or not
+      g = n == total && head ? 0 : pieces - 1;
+      const int last_hi = shift + vocab - (pieces - 1) * N;
+      w = P::cut(__ldg(base + g), g == 0 ? shift : 0, g == pieces - 1 ? last_hi : N);
+    } else {
+      return;
+    }
+    float e[N];
+    P::unpack(w, e);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int id = g * N + k - shift;
+      if (id >= 0 && id < vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) keys[k] = lp_key(e[k], static_cast<uint32_t>(id));
+    }
+  };
+  if constexpr (TOP) {
+    // how many groups are above one: two threads count
+    const ulonglong2* bounds = reinterpret_cast<const ulonglong2*>(s_bounds);
+    for (int n = tid / 2; n < groups; n += threads / 2) {
+      const uint64_t it = s_bounds[n];
+      int above = 0;
+#pragma unroll 8
+      for (int k = tid % 2; k < groups / 2; k += 2) {
+        const ulonglong2 v = bounds[k];
+        above += (v.x > it) + (v.y > it);
+      }
+      above += __shfl_xor_sync(0xffffffffu, above, 1);
+      if (tid % 2 == 0 && above == top - 1 && it) s_tau = it;  // one group: keys differ
+    }
+    __syncthreads();
+    tau = s_tau;
+    auto list = [&]() {
+      if (mine && mine >= tau) {
+        const int k = atomicAdd(&s_slots, 1);
+        s_slot[k] = static_cast<uint16_t>(tid);
+        s_key[k] = mine;
+      }
+      __syncthreads();
+    };
+    list();
+    if (s_slots > 2 * top) {  // ties (a mask that leaves fewer than `top`): the block's own top-th thread is a closer bound
+      const int n = s_slots;
+      const uint64_t it = tid < n ? s_key[tid] : 0;
+      int above = 0;
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) above += s_key[k] > it;
+      if (it && above == top - 1) s_tau = it;
+      __syncthreads();
+      tau = s_tau;
+      if (tid == 0) s_slots = 0;
+      __syncthreads();
+      list();
+    }
+    each = (whole + all - 1) >> log_all;  // pieces of a thread
+    each_inv = __frcp_rn(static_cast<float>(each));
+    total = s_slots * each;
+    looked = total + (crank == 0 ? head + tail : 0);
+    for (int n = tid; n - lane < looked; n += threads) {  // a place in the list for what a warp has found, then the keys
+      uint64_t keys[N];
+      look(n, keys);
+      int found = 0;
+#pragma unroll
+      for (int k = 0; k < N; ++k) found += keys[k] != 0;
+      if (!__any_sync(0xffffffffu, found)) continue;
+      int upto = found;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      int place = lane == 31 ? atomicAdd(cands_at, upto) : 0;
+      place = __shfl_sync(0xffffffffu, place, 31) + upto - found;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (keys[k]) {
+          if (place < kLpCands) cand_at[place] = keys[k];
+          ++place;
+        }
+    }
+  }
+  if (crank == 0 && warp == threads / 32 - 1) {  // the warp with least to look at
+    const int b = min(lane, csize - 1);
+    sum = {s_sums[b][0], lane == b ? s_sums[b][1] : 0.f, lane == b ? s_sums[b][2] : 0.f};
+    join_warp(sum);
+    if (lane == 0) {
+      const float log_z = sum.log_z();
+      s_log_z = log_z;
+      s_m = sum.m;
+      sum.results(row, token, given, inv_t, log_z, vocab, logprobs, entropy, status);
+    }
+  }
+  if constexpr (!TOP) return;
+  sync();
+  const int cands = *cands_at;
+  auto put = [&](int rank, uint64_t key) {
+    const int64_t to = static_cast<int64_t>(row) * top + rank;
+    top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
+    top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - s_m) * inv_t - s_log_z;
+  };
+  if (cands <= kLpCands) {
+    if (several) cluster.barrier_arrive();  // the first block's counter has been read
+    if (crank != 0) {
+      cluster.barrier_wait();
+      return;
+    }
+    // ranks by counting, eight threads a candidate
+    for (int n = tid / 8; n < ((cands + 3) & ~3); n += threads / 8) {
+      const uint64_t key = n < cands ? s_cand[n] : 0;
+      int rank = 0;
+      for (int k = tid % 8; k < cands; k += 8) rank += s_cand[k] > key;
+#pragma unroll
+      for (int sh = 1; sh < 8; sh <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, sh);
+      if (tid % 8 == 0 && n < cands && rank < top) put(rank, key);
+    }
+    if (several) cluster.barrier_wait();
+    return;
+  }
+  // The largest ones stand close together in few threads: one after the other.
+  uint64_t before = ~0ull;
+  for (int r = 0; r < top; ++r) {
+    uint64_t most = 0;
+    for (int n = tid; n < looked; n += threads) {
+      uint64_t keys[N];
+      look(n, keys);
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (keys[k] < before) most = max(most, keys[k]);
+    }
+#pragma unroll
+    for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
+    if (lane == 0) s_most[warp] = most;
+    __syncthreads();
+    for (int k = 0; k < threads / 32; ++k) most = max(most, s_most[k]);
+    if (tid < csize) (several ? cluster.map_shared_rank(s_all, tid) : s_all)[(r & 1) * kLpMaxCluster + crank] = most;
+    sync();
+    most = 0;
+    for (int k = 0; k < csize; ++k) most = max(most, s_all[(r & 1) * kLpMaxCluster + k]);
+    before = most;
+    if (crank == 0 && tid == 0) put(r, most);
+  }
+  sync();
+}
+
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_constant__ LogprobParams p) {
+  using P = LpPiece<T>;
+  constexpr int N = P::N, C = TOP ? 3 : 4;
   pdl_wait();
-  cg::cluster_group cluster = cg::this_cluster();
   const int csize = 1 << p.log_csize, crank = blockIdx.x & (csize - 1);
   const bool several = csize > 1;
-  if (several) cluster.barrier_arrive();  // waited for before another block's shared memory is written
+  if (several) cooperative_groups::this_cluster().barrier_arrive();  // waited for before another block's shared memory is written
   const int row = blockIdx.x >> p.log_csize, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = 1 << (p.log_all - p.log_csize);
   const int me = crank * threads + tid, all = 1 << p.log_all;  // of the row's threads
   const T* x = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
@@ -196,10 +421,6 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
   if (crank == 0 && tid == threads - 32) {  // which writes the results
     token = p.tokens[row];
     if (token >= 0 && token < p.vocab) given = static_cast<float>(x[token]);
-  }
-  if (tid == 0) {
-    s_tau = 0;
-    s_slots = s_cands = 0;
   }
 
   LpSums sum{-FLT_MAX, 0.f, 0.f};
@@ -334,166 +555,9 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const LogprobPa
     one(w1);
   }
 
-  // ---- sums of the block, and the largest (maximum, piece) of every group of threads
-  auto join_warp = [&](LpSums& v) {  // over the lanes
-    float m = v.m;
-#pragma unroll
-    for (int sh = 16; sh > 0; sh >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, sh));
-    v.rescale(m, c);
-#pragma unroll
-    for (int sh = 16; sh > 0; sh >>= 1) {
-      v.s += __shfl_xor_sync(0xffffffffu, v.s, sh);
-      v.t += __shfl_xor_sync(0xffffffffu, v.t, sh);
-    }
-  };
-  join_warp(sum);
-  if (lane == 0) {
-    s_warp[warp][0] = sum.m;
-    s_warp[warp][1] = sum.s;
-    s_warp[warp][2] = sum.t;
-  }
-  const int top = p.top;
-  const uint64_t mine = any ? lp_key(best, static_cast<uint32_t>(at)) : 0;
-  auto sync = [&]() {
-    if (several) cluster.sync();
-    else __syncthreads();
-  };
-  if (several) cluster.barrier_wait();
-  if constexpr (TOP) {
-    const int size = 1 << p.log_size;  // threads of a group: 1 to 32
-    uint64_t most = mine;
-    for (int sh = 1; sh < size; sh <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
-    // every block of the row gets all groups'
-    for (int to = tid & (size - 1); to < csize; to += size) (several ? cluster.map_shared_rank(s_bounds, to) : s_bounds)[me >> p.log_size] = most;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    const int w = min(lane, threads / 32 - 1);
-    sum = {s_warp[w][0], lane == w ? s_warp[w][1] : 0.f, lane == w ? s_warp[w][2] : 0.f};
-    join_warp(sum);
-    if (lane == 0) {
-      float* to = (several ? cluster.map_shared_rank(&s_sums[0][0], 0) : &s_sums[0][0]) + 3 * crank;
-      to[0] = sum.m;
-      to[1] = sum.s;
-      to[2] = sum.t;
-    }
-  }
-  pdl_trigger();
-  sync();
-
-  // ---- the bound that `top` elements of the row reach, and the elements that do: to the first block's list
-  int* cands_at = several ? cluster.map_shared_rank(&s_cands, 0) : &s_cands;
-  uint64_t* cand_at = several ? cluster.map_shared_rank(s_cand, 0) : s_cand;
-  uint64_t tau = 0;
-  float each_inv = 0.f;
-  int each = 0, total = 0, looked = 0;
-  // calls f(element's key) for the elements that reach the bound in piece n of the listed threads
-  auto look = [&](int n, auto&& f) {
-    int g;
-    uint4 w;
-    if (n < total) {
-      const int nth = static_cast<int>((static_cast<float>(n) + 0.5f) * each_inv), who = crank * threads + s_slot[nth];
-      g = head + who + (n - nth * each) * all;
-      if (g >= head + whole) return;
-      w = __ldg(base + g);
-    } else {  // the cut pieces, whether they are in a listed thread or not
-      g = n == total && head ? 0 : pieces - 1;
-      w = cut_piece(g);
-    }
-    float e[N];
-    P::unpack(w, e);
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      const int id = g * N + k - shift;
-      if (id >= 0 && id < p.vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) f(lp_key(e[k], static_cast<uint32_t>(id)));
-    }
-  };
-  if constexpr (TOP) {
-    // how many groups are above one: two threads count
-    const ulonglong2* bounds = reinterpret_cast<const ulonglong2*>(s_bounds);
-    for (int n = tid / 2; n < p.groups; n += threads / 2) {
-      const uint64_t it = s_bounds[n];
-      int above = 0;
-#pragma unroll 8
-      for (int k = tid % 2; k < p.groups / 2; k += 2) {
-        const ulonglong2 v = bounds[k];
-        above += (v.x > it) + (v.y > it);
-      }
-      above += __shfl_xor_sync(0xffffffffu, above, 1);
-      if (tid % 2 == 0 && above == top - 1 && it) s_tau = it;  // one group: keys differ
-    }
-    __syncthreads();
-    tau = s_tau;
-    if (mine && mine >= tau) s_slot[atomicAdd(&s_slots, 1)] = static_cast<uint16_t>(tid);
-    __syncthreads();
-    each = (whole + all - 1) >> p.log_all;  // pieces of a thread
-    each_inv = __frcp_rn(static_cast<float>(each));
-    total = s_slots * each;
-    looked = total + (crank == 0 ? head + tail : 0);
-    for (int n = tid; n < looked; n += threads)
-      look(n, [&](uint64_t key) {
-        const int k = atomicAdd(cands_at, 1);
-        if (k < kLpCands) cand_at[k] = key;
-      });
-  }
-  if (crank == 0 && warp == threads / 32 - 1) {  // the warp with least to look at
-    const int b = min(lane, csize - 1);
-    sum = {s_sums[b][0], lane == b ? s_sums[b][1] : 0.f, lane == b ? s_sums[b][2] : 0.f};
-    join_warp(sum);
-    if (lane == 0) {
-      const float log_z = sum.log_z();
-      s_log_z = log_z;
-      s_m = sum.m;
-      sum.results(row, token, given, inv_t, log_z, p.vocab, p.logprobs, p.entropy, p.status);
-    }
-  }
-  if constexpr (!TOP) return;
-  sync();
-  const int cands = *cands_at;
-  auto put = [&](int rank, uint64_t key) {
-    const int64_t to = static_cast<int64_t>(row) * top + rank;
-    p.top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
-    p.top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - s_m) * inv_t - s_log_z;
-  };
-  if (cands <= kLpCands) {
-    if (several) cluster.barrier_arrive();  // the first block's counter has been read
-    if (crank != 0) {
-      cluster.barrier_wait();
-      return;
-    }
-    // ranks by counting, eight threads a candidate
-    for (int n = tid / 8; n < ((cands + 3) & ~3); n += threads / 8) {
-      const uint64_t key = n < cands ? s_cand[n] : 0;
-      int rank = 0;
-      for (int k = tid % 8; k < cands; k += 8) rank += s_cand[k] > key;
-#pragma unroll
-      for (int sh = 1; sh < 8; sh <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, sh);
-      if (tid % 8 == 0 && n < cands && rank < top) put(rank, key);
-    }
-    if (several) cluster.barrier_wait();
-    return;
-  }
-  // The largest ones stand close together in few threads: one after the other.
-  uint64_t before = ~0ull;
-  for (int r = 0; r < top; ++r) {
-    uint64_t most = 0;
-    for (int n = tid; n < looked; n += threads)
-      look(n, [&](uint64_t key) {
-        if (key < before && key > most) most = key;
-      });
-#pragma unroll
-    for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
-    if (lane == 0) s_most[warp] = most;
-    __syncthreads();
-    for (int k = 0; k < threads / 32; ++k) most = max(most, s_most[k]);
-    if (tid < csize) (several ? cluster.map_shared_rank(s_all, tid) : s_all)[(r & 1) * kLpMaxCluster + crank] = most;
-    sync();
-    most = 0;
-    for (int k = 0; k < csize; ++k) most = max(most, s_all[(r & 1) * kLpMaxCluster + k]);
-    before = most;
-    if (crank == 0 && tid == 0) put(r, most);
-  }
-  sync();
+  // What the end of a row wants of registers would cost the stream a tenth if it were part of it.
+  lp_finish<T, TOP>(sum.m, sum.s, sum.t, any ? lp_key(best, static_cast<uint32_t>(at)) : 0, base, shift, pieces, head, tail, inv_t, given, token, p.vocab, p.top,
+                    p.groups, p.log_csize, p.log_all, p.log_size, p.logprobs, p.entropy, p.top_tokens, p.top_logprobs, p.status);
 }
 
 }  // namespace nvllm
