@@ -438,6 +438,8 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   pl.keep = pl.mt <= workers && workers % pl.mt == 0;
   pl.group = 1;
   while (!pl.keep && pl.group < 16 && static_cast<int64_t>(pl.mt) * ((pl.nt + 2 * pl.group - 1) / (2 * pl.group)) >= 48ll * workers) pl.group *= 2;
+  // no more than 64 MB of partial statistics, as long as there is a longer group
+  while (!pl.keep && pl.group < pl.nt && 2ll * ((pl.nt + pl.group - 1) / pl.group) * pl.mt * bm * 16 > (64 << 20)) pl.group *= 2;
   pl.ng = (pl.nt + pl.group - 1) / pl.group;
   pl.mb = pl.keep ? pl.mt : static_cast<int>(std::min<int64_t>(pl.mt, std::max<int64_t>(1, std::min<int64_t>(16, (32ll << 20) / (bm * 2ll * hidden)))));
   pl.grid = static_cast<int>(std::min<int64_t>(workers, static_cast<int64_t>(pl.mt) * pl.ng)) * (pl.pair ? 2 : 1);
@@ -449,7 +451,7 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
 }
 
 static int check(int64_t rows, int64_t hidden, int64_t vocab) {
-  if (rows < 0 || rows > (1 << 24) || vocab <= 0 || vocab > (1 << 24) || hidden <= 0 || hidden > 65536 || hidden % 8)
+  if (rows < 0 || rows > (1 << 24) || vocab <= 0 || vocab > (1 << 21) || hidden <= 0 || hidden > 65536 || hidden % 8)
     return fail(NVLLM_E_GEOMETRY, "head_logprobs: rows=%lld hidden=%lld (a multiple of 8) vocab=%lld not supported", (long long)rows, (long long)hidden,
                 (long long)vocab);
   return NVLLM_OK;

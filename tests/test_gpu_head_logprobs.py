@@ -49,6 +49,18 @@ def test_more_row_tiles_than_multiprocessors(cuda):
     check(cuda, *some(g, 148 * 256 + 130, 16, 700))
 
 
+def test_rows_whose_statistics_are_kept_for_several_tiles(cuda):
+    """So many rows that column tiles go in groups; rows from everywhere against the reference."""
+    g = torch.Generator().manual_seed(8)
+    x, w, tokens = some(g, 150_000, 16, 5003)
+    got = head_logprobs(x.to(cuda), w.to(cuda), tokens.to(cuda))
+    rows = torch.cat([torch.arange(3), torch.randint(150_000, (300,), generator=g), torch.arange(149_990, 150_000)])
+    given, entropy, bounds = head_logprobs_ref(x[rows], w, tokens[rows])
+    assert_same(got.logprobs[rows.to(cuda)], given, bounds[0], "logprobs")
+    assert_same(got.entropy[rows.to(cuda)], entropy, bounds[1], "entropy")
+    assert _lib.read_status() == 0
+
+
 @pytest.mark.parametrize("hidden", [64, 1536])
 def test_temperatures_tokens_and_strides(cuda, hidden):
     g = torch.Generator().manual_seed(2)

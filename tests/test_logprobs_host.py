@@ -31,7 +31,7 @@ def test_token_logprobs_refuses(lib, change, code):
 
 @pytest.mark.parametrize("change,code", [
     ({}, -6), ({"rows": 0}, 0), ({"rows": -1}, -3), ({"rows": 1 << 25}, -3), ({"hidden": 0}, -3), ({"hidden": 68}, -3), ({"hidden": 1 << 17}, -3),
-    ({"vocab": 0}, -3), ({"vocab": 1 << 25}, -3), ({"x": NULL}, -1), ({"w": NULL}, -1), ({"tokens": NULL}, -1), ({"lp": NULL}, -1),
+    ({"vocab": 0}, -3), ({"vocab": (1 << 21) + 1}, -3), ({"x": NULL}, -1), ({"w": NULL}, -1), ({"tokens": NULL}, -1), ({"lp": NULL}, -1),
     ({"entropy": NULL}, -1), ({"x": P8}, -2), ({"w": P8}, -2), ({"x_stride": 132}, -2), ({"w_stride": 132}, -2), ({"x_stride": 120}, -3),
     ({"w_stride": 120}, -3), ({"tokens": P4}, -2), ({"lp": P2}, -2), ({"t": P2}, -2)])
 def test_head_logprobs_refuses(lib, change, code):
@@ -49,4 +49,5 @@ def test_head_logprobs_workspace_grows_with_rows_and_not_with_every_tile(lib):
     assert size(0, 1024, 151936) == 0
     assert 0 < size(1, 1024, 151936) < 1 << 20
     assert size(4096, 1024, 151936) < 128 << 20
-    assert size(32768, 4096, 151936) < 256 << 20
+    assert size(32768, 4096, 151936) < 80 << 20
+    assert size(1 << 20, 4096, 151936) < 160 << 20
