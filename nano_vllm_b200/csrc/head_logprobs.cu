@@ -4,9 +4,13 @@
 // memory by tcgen05 and reduced there to three numbers for each row (maximum, sum of exponentials, their sum times the
 // logits: the statistics of token_logprobs), which a second launch joins over the vocabulary's tiles.
 //
-// Sums over H stay fp32: the tensor core cuts its running sum towards zero at every step, which over long rows is a systematic
-// loss (H = 4096: logits 3.7e-6 too small on average, log probabilities 2e-6 off), so a product is cut after kChunk elements
-// and the parts are added in registers (one part up to there; 4.6e-7 at 1024).
+// Sums over H stay fp32, in a tensor core that cuts its running sum towards zero at every step of 16 products.  That is a systematic
+// loss: at H = 4096 logits come out 3.7e-6 too small, log probabilities 2e-6 off.  Two things are done about it.  A product is cut after
+// kChunk elements and the parts are added in registers.  And the logits' scale makes good what a step loses on average (kStepLoss, half a
+// last place of a sum that is still on its way, measured at 64 to 5120 elements, products of either sign and of one): at H = 1024
+// log probabilities 4.6e-7 -> 1.9e-7 and entropy 8.4e-7 -> 1.2e-7 off (relative, 512 rows of 151936), at 4096 4.6e-7 -> 1.7e-7 and
+// 9.1e-7 -> 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off at 1024.  Parts of 512 elements would halve the loss too, at 1195 us instead of
+// 933 for 4096 x 1024 x 151936.
 #include <algorithm>
 
 #include "logprobs.cuh"
@@ -20,6 +24,7 @@ using namespace sm100;
 // shared memory, the first one's thread multiplies both with tcgen05 of two blocks, and each reduces its own rows.
 constexpr int BM = 128, BN = 256, BK = 64;
 constexpr int kChunk = 1024;
+constexpr double kStepLoss = 1.5e-8;
 // A stage holds what is loaded of a tile's rows and its columns for 64 elements of k.  The product reads 128 rows all the same:
 // behind the loaded ones whatever follows, which ends in accumulator rows that nobody reads (the last stage's lie in the slack).
 constexpr int CTRL_BYTES = 1024, RING_BYTES = 192 * 1024, SLACK_BYTES = BM * BK * 2;
@@ -96,6 +101,7 @@ __device__ __forceinline__ void cluster_sync() {
 struct Params {
   const int64_t* tokens;
   const float* temperatures;
+  float scale;    // of the logits
   int rows, vocab;
   int bn;         // columns of a tile
   int mt, nt;     // tiles of rows and of columns
@@ -296,7 +302,7 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
         live = row - lane < p.rows;
         token = row < p.rows ? p.tokens[row] : -1;
         if (token >= p.vocab) token = -1;
-        c = (row < p.rows ? lp_inverse(p.temperatures, row) : 1.f) * 1.4426950408889634f;
+        c = (row < p.rows ? lp_inverse(p.temperatures, row) : 1.f) * p.scale * 1.4426950408889634f;
       }
       for (int n = u.g * p.group; n < min((u.g + 1) * p.group, p.nt) && ok; ++n) {
         const int first = n * p.bn + part * COLS, end = min(p.vocab, (n + 1) * p.bn) - first;  // columns of this thread
@@ -370,6 +376,7 @@ struct JoinParams {
   const float* given;
   const int64_t* tokens;
   const float* temperatures;
+  float scale;
   int rows, vocab, slots, wide;  // slots: halves counted
   int64_t rows_padded;
   float *logprobs, *entropy;
@@ -382,7 +389,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const JoinParams p) 
   const int tid = threadIdx.x, part = tid / p.wide, parts = kJoinThreads / p.wide;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * p.wide + tid % p.wide;
   const bool live = row < p.rows;
-  const float inv_t = live ? lp_inverse(p.temperatures, row) : 1.f, c = inv_t * 1.4426950408889634f;
+  const float inv_t = (live ? lp_inverse(p.temperatures, row) : 1.f) * p.scale, c = inv_t * 1.4426950408889634f;
   const int64_t token = live ? p.tokens[row] : -1;
   pdl_prologue();
   LpSums sum{-FLT_MAX, 0.f, 0.f};
@@ -507,6 +514,7 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   hlp::Params p{};
   p.tokens = tokens;
   p.temperatures = temperatures;
+  p.scale = static_cast<float>(1 + hlp::kStepLoss * static_cast<double>((std::min<int64_t>(hidden, hlp::kChunk) + 15) / 16 - 1));
   p.rows = static_cast<int>(rows);
   p.vocab = static_cast<int>(vocab);
   p.bn = pl.bn;
@@ -544,6 +552,6 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   }
   int wide = 1;
   while (wide < 32 && rows > 4ll * sms * wide) wide *= 2;
-  const hlp::JoinParams j{p.partial, p.given, tokens, temperatures, p.rows, p.vocab, pl.slots, wide, pl.rows_padded, logprobs, entropy, status};
+  const hlp::JoinParams j{p.partial, p.given, tokens, temperatures, p.scale, p.rows, p.vocab, pl.slots, wide, pl.rows_padded, logprobs, entropy, status};
   return launch_kernel("head_logprobs", hlp::join_kernel, dim3(static_cast<unsigned>((rows + wide - 1) / wide)), dim3(hlp::kJoinThreads), 0, st, j);
 }
