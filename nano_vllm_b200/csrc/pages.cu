@@ -11,7 +11,9 @@
 // The tables' side is a few trips to memory one after the other: a fork's is worked out by every thread block for itself, so
 // that one launch does it all; counts of all blocks lie in the shared memory of one cluster (ids dealt out in ranges), whose
 // barriers separate counting, summing and writing.  Copies are bound by memory alone: a (copy, plane) is cut in equal pieces, so
-// that few copies of few planes spread over all SMs.
+// that few copies of few planes spread over all SMs.  Measured: a fork of 12 sequences to 48 over 28 layers in 8 bits (520 MB read and
+// written) 84 us, 6.2 TB/s; two begun blocks of 28 layers 10.7 us, of which start and plan 4; a compaction of 2.2 GB 367, of which counting 6;
+// the free list of 256 x 32 entries 6.3.
 #include <cooperative_groups.h>
 
 #include <algorithm>
