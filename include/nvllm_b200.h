@@ -472,7 +472,7 @@ NVLLM_API int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row_
  */
 #define NVLLM_CACHE_MAX_PARTS 160
 #define NVLLM_PAGES_MAX_BLOCKS 400000 /* of a cache that free_list / compact_blocks count */
-#define NVLLM_FORK_MAX_ROWS 4096      /* sequences of a fork, before and after */
+#define NVLLM_FORK_MAX_ROWS 4096      /* sequences of a fork, before and after; of all calls, rows x max_blocks is 2^28 at most */
 typedef struct {
   void* base;
   int64_t planes, plane_stride, block_stride;

@@ -11,6 +11,11 @@
 // log probabilities 4.6e-7 -> 1.9e-7 and entropy 8.4e-7 -> 1.2e-7 off (relative, 512 rows of 151936), at 4096 4.6e-7 -> 1.7e-7 and
 // 9.1e-7 -> 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off at 1024.  Parts of 512 elements would halve the loss too, at 1195 us instead of
 // 933 for 4096 x 1024 x 151936.
+//
+// What bounds it.  Many rows: the tensor cores, busy 93 to 95 % of the time, and then the power cap (4096 x 1024 x 151936 933 us, 1366
+// TFLOP/s; 1000 x 4096 830-870; blocks of 128 rows by themselves, which feed the tensor cores twice the bytes, 1306 and 1248).  H below some
+// 900: the reduction of a tile (4096 x 512 644 us; 16 warps instead of 8 625, but 77 x 896 47.6 instead of 45.9).  Up to 128 rows: the weights' stream
+// (one row of 1024 53.5 us, 5.8 TB/s; of 4096 197.6, 6.3), with as many stages as fit on their way (four: 54.8 and 200.8).
 #include <algorithm>
 
 #include "logprobs.cuh"
@@ -506,8 +511,13 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
     for (int k = 0; k < 4; ++k) {
-      const cudaError_t e = cudaFuncSetAttribute(kernels[k / 2][k % 2], cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
+      cudaError_t e = cudaFuncSetAttribute(kernels[k / 2][k % 2], cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
       if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "head_logprobs: cannot reserve shared memory: %s", cudaGetErrorString(e));
+      cudaFuncAttributes attr;  // a block with fewer registers than its groups share would wait for them without end
+      if (k % 2 && (e = cudaFuncGetAttributes(&attr, kernels[k / 2][k % 2])) != cudaSuccess)
+        return fail(NVLLM_E_CUDA, "head_logprobs: %s", cudaGetErrorString(e));
+      if (k % 2 && attr.numRegs < hlp::Cfg<false, true>::REGS)
+        return fail(NVLLM_E_CUDA, "head_logprobs: compiled to %d registers, %d needed", attr.numRegs, hlp::Cfg<false, true>::REGS);
     }
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }

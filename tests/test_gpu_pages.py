@@ -138,6 +138,11 @@ def test_forks_of_many(cuda):
     check_fork(cuda, g, [5], [0] * 4096, layers=1, hkv=1, d=8)
 
 
+def test_forks_of_wide_tables(cuda):
+    g = torch.Generator().manual_seed(18)
+    check_fork(cuda, g, [100_000, 131_072, 77], [0, 1, 1, 0, 2, 2, 0], layers=1, hkv=1, d=8, wide=5)
+
+
 def test_forks_without_enough_free_blocks(cuda):
     g = torch.Generator().manual_seed(9)
     check_fork(cuda, g, [300, 5], [1, 1, 0, 1, 0], spare=1)
@@ -171,6 +176,15 @@ def test_free_lists(cuda, lens, num_blocks):
     check_free(cuda, g, lens, num_blocks)
     held = torch.randint(-2, 3, (num_blocks,), generator=g).tolist()
     check_free(cuda, g, lens, num_blocks, held, shared=3, width=max(map(R.blocks_of, lens)) + 5, wide=2)
+
+
+def test_free_list_and_compaction_of_more_entries_than_threads_hold(cuda):
+    """Tables whose entries take the cluster several trips."""
+    g = torch.Generator().manual_seed(4)
+    lens = torch.randint(0, 5 * 256, (5000,), generator=g).tolist()
+    num_blocks = 5000 * 5 + 77
+    check_free(cuda, g, lens, num_blocks, width=31, wide=1)
+    check_compact(cuda, g, lens, num_blocks, shared=2, layers=1, hkv=1, d=8)
 
 
 def test_free_list_of_nothing_and_of_what_is_not_there(cuda):
