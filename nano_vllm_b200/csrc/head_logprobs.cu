@@ -441,7 +441,7 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   // the widest tile that leaves the worker with most tiles as few columns as any
   int64_t least = 0;
   pl.bn = BN;
-  for (int bn = BN; bn >= BN / 2; bn -= 16) {
+  for (int bn = BN; bn >= BN / 2; bn -= pl.pair ? 32 : 16) {  // what tcgen05 of one block and of two take
     const int64_t tiles = static_cast<int64_t>(pl.mt) * ((vocab + bn - 1) / bn), cost = (tiles + workers - 1) / workers * bn;
     if (bn == BN || cost < least) least = cost, pl.bn = bn;
   }

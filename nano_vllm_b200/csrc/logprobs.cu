@@ -565,7 +565,9 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
                                     const float* temperatures, int32_t rows, int32_t vocab, int32_t top, float* logprobs,
                                     float* entropy, int64_t* top_tokens, float* top_logprobs, void* stream) {
   using namespace nvllm;
-  if (rows < 0 || vocab <= 0 || vocab > 0x7fffff00) return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d vocab=%d invalid", rows, vocab);
+  // a listed piece's thread is found by a product in fp32, which is right for up to 2^22 pieces of a block's 2 top listed threads
+  if (rows < 0 || vocab <= 0 || vocab > NVLLM_LOGPROBS_MAX_VOCAB)
+    return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d vocab=%d (1 to %d) not supported", rows, vocab, NVLLM_LOGPROBS_MAX_VOCAB);
   if (top < 0 || top > kLpMaxTop || top > vocab)
     return fail(NVLLM_E_GEOMETRY, "token_logprobs: top=%d outside 0 to %d (vocab=%d)", top, kLpMaxTop, vocab);
   if (rows == 0) return NVLLM_OK;
@@ -609,7 +611,6 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   p.log_csize = log2_of(csize);
   p.log_all = log2_of(all);
   p.log_size = log2_of(all / p.groups);
-  if (static_cast<int64_t>(rows) * csize > 0x7fffffff) return fail(NVLLM_E_GEOMETRY, "token_logprobs: rows=%d too many", rows);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * csize), 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);

@@ -69,7 +69,7 @@ def free_list(block_tables: torch.Tensor, seq_lens: torch.Tensor, num_blocks: in
               out: Sequence[torch.Tensor] | None = None) -> FreeList:
     """How often the sequences (``block_tables`` int32 ``[B, W]``, ``seq_lens`` int32 ``[B]``) refer to each of the ``num_blocks`` (up to
     400000) blocks of a cache, and which none of them does.  ``held`` (int32 ``[num_blocks]``) counts references from elsewhere, such as
-    prefixes that are kept.  Entries behind a sequence's last block are not looked at, negative ones name no block, and ones
+    prefixes that are kept (the sums have to fit 32 bits).  Entries behind a sequence's last block are not looked at, negative ones name no block, and ones
     beyond ``num_blocks`` set bit 2 of ``_lib.read_status()``.  One launch."""
     return FreeList._make(_native(block_tables).free_list(block_tables, seq_lens, num_blocks, held, out))
 

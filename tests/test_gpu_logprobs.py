@@ -127,6 +127,32 @@ def test_sizes_of_32_bits(cuda):
     check(cuda, logits, tokens, 9, on_gpu=wide[:, -3001:])
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_largest_vocabulary_of_equal_tokens(cuda, dtype):
+    logits = torch.zeros(2, 1 << 24, dtype=dtype, device=cuda)
+    got = token_logprobs(logits, torch.tensor([5, -1], device=cuda), 64)
+    # 2^24 equal weights: every sum is a whole number, ln 2^24 is off by 2^-23 of itself
+    want = 24 * math.log(2.0)
+    assert got.top_tokens.tolist() == [list(range(64))] * 2
+    for value, expected in ((got.logprobs[0], -want), (got.logprobs[1], 0.0), (got.entropy, want), (got.top_logprobs, -want)):
+        assert torch.all((value.double() - expected).abs() <= want * 2.0 ** -22)
+
+
+def test_temperatures_without_a_bound(cuda):
+    """Masked tokens have no weight at any temperature, the others one and the same."""
+    g = torch.Generator().manual_seed(12)
+    logits = torch.randn(6, 3001, generator=g)
+    logits[:, 1::2] = -torch.inf
+    t = torch.tensor([math.inf, 3e38, 1e36, 1e31, 1e30, 1e29])
+    tokens = torch.tensor([0, 2, 1, 4, 6, 8])
+    got = token_logprobs(logits.to(cuda), tokens.to(cuda), 5, t.to(cuda))
+    given, entropy, ids, alternatives, bounds = logprobs_ref(logits, tokens, 5, t.clamp(max=1e30))
+    assert torch.equal(got.top_tokens.cpu(), ids)
+    assert_same(got.logprobs, given, bounds[0], "logprobs")
+    assert_same(got.entropy, entropy, bounds[1], "entropy")
+    assert_same(got.top_logprobs, alternatives, bounds[2], "top_logprobs")
+
+
 def test_results_go_where_they_are_wanted(cuda):
     """``out``, a captured graph replayed on new logits, and another stream."""
     g = torch.Generator().manual_seed(4)

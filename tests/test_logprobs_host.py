@@ -18,6 +18,7 @@ def test_there_is_no_cpu_fallback():
 
 @pytest.mark.parametrize("change,code", [
     ({}, -6), ({"rows": 0}, 0), ({"rows": -1}, -3), ({"vocab": 0}, -3), ({"vocab": 0x7fffffff}, -3), ({"top": -1}, -3), ({"top": 65}, -3),
+    ({"vocab": (1 << 24) + 1}, -3),
     ({"vocab": 5, "top": 6}, -3), ({"stride": 999}, -3), ({"logits": NULL}, -1), ({"tokens": NULL}, -1), ({"lp": NULL}, -1),
     ({"entropy": NULL}, -1), ({"ids": NULL}, -1), ({"alternatives": NULL}, -1), ({"tokens": P4}, -2), ({"ids": P4}, -2), ({"lp": P2}, -2),
     ({"t": P2}, -2), ({"logits": ctypes.c_void_p(4097)}, -2), ({"fp32": 1, "logits": P2}, -2)])
