@@ -438,10 +438,13 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   pl.kb = (hidden + BK - 1) / BK;
   pl.mt = (rows + bm - 1) / bm;
   pl.a_rows = pl.pair ? BM : std::min(BM, (rows + 7) / 8 * 8);
-  // the widest tile that leaves the worker with most tiles as few columns as any
+  // The widest tile that leaves the worker with most tiles as few columns as any, in steps that tcgen05 of one block and of two take.
+  // A pair's are not below 192 columns, where the rows that are loaded again for each tile bound it: 4096 x 1024 x 151936 in tiles of 128
+  // columns 1138 us, 160 984, 192 908, 224 925, 256 931 (calls one after the other, at the power cap).  Up to 128 rows the weights are most of
+  // what is loaded: 77 x 896 in tiles of 128 columns 50.2 us, 176 49.6, 208 49.2, 256 53.8.
   int64_t least = 0;
   pl.bn = BN;
-  for (int bn = BN; bn >= BN / 2; bn -= pl.pair ? 32 : 16) {  // what tcgen05 of one block and of two take
+  for (int bn = BN; bn >= (pl.pair ? 192 : 128); bn -= pl.pair ? 32 : 16) {
     const int64_t tiles = static_cast<int64_t>(pl.mt) * ((vocab + bn - 1) / bn), cost = (tiles + workers - 1) / workers * bn;
     if (bn == BN || cost < least) least = cost, pl.bn = bn;
   }
