@@ -9,13 +9,13 @@
 // kChunk elements and the parts are added in registers.  And the logits' scale makes good what a step loses on average (kStepLoss, half a
 // last place of a sum that is still on its way, measured at 64 to 5120 elements, products of either sign and of one): at H = 1024
 // log probabilities 4.6e-7 -> 1.9e-7 and entropy 8.4e-7 -> 1.2e-7 off (relative, 512 rows of 151936), at 4096 4.6e-7 -> 1.7e-7 and
-// 9.1e-7 -> 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off at 1024.  Parts of 512 elements would halve the loss too, at 1195 us instead of
-// 933 for 4096 x 1024 x 151936.
+// 9.1e-7 -> 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off at 1024.  Parts of 512 elements would halve the loss too, at 1.28 times
+// the time for 4096 x 1024 x 151936.
 //
-// What bounds it.  Many rows: the tensor cores, busy 93 to 95 % of the time, and then the power cap (4096 x 1024 x 151936 933 us, 1366
-// TFLOP/s; 1000 x 4096 830-870; blocks of 128 rows by themselves, which feed the tensor cores twice the bytes, 1306 and 1248).  H below some
-// 900: the reduction of a tile (4096 x 512 644 us; 16 warps instead of 8 625, but 77 x 896 47.6 instead of 45.9).  Up to 128 rows: the weights' stream
-// (one row of 1024 53.5 us, 5.8 TB/s; of 4096 197.6, 6.3), with as many stages as fit on their way (four: 54.8 and 200.8).
+// What bounds it.  Many rows: the tensor cores, and then the power cap (4096 x 1024 x 151936 803 us, 1590 TFLOP/s, 908 in a long chain; 1000 x
+// 4096 830-870; blocks of 128 rows by themselves, which feed the tensor cores twice the bytes, 1306 and 1248).  H below some 900: the reduction
+// of a tile (4096 x 512 490 us of 393; tiles shared out evenly to the warps the same; 16 warps instead of 8 made 77 x 896 47.6 instead of 45.9).  Up to 128 rows: the weights' stream (one row of 1024
+// 53.5 us, 5.8 TB/s; of 4096 197.6, 6.3), with as many stages as fit on their way (four: 54.8 and 200.8).
 #include <algorithm>
 
 #include "logprobs.cuh"
@@ -439,7 +439,7 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   pl.mt = (rows + bm - 1) / bm;
   pl.a_rows = pl.pair ? BM : std::min(BM, (rows + 7) / 8 * 8);
   // The widest tile that leaves the worker with most tiles as few columns as any, in steps that tcgen05 of one block and of two take.
-  // A pair's are not below 192 columns, where the rows that are loaded again for each tile bound it: 4096 x 1024 x 151936 in tiles of 128
+  // A pair's are not below 192 columns, where a tile's operands take longer to come than their product: 4096 x 1024 x 151936 in tiles of 128
   // columns 1138 us, 160 984, 192 908, 224 925, 256 931 (calls one after the other, at the power cap).  Up to 128 rows the weights are most of
   // what is loaded: 77 x 896 in tiles of 128 columns 50.2 us, 176 49.6, 208 49.2, 256 53.8.
   int64_t least = 0;
