@@ -93,6 +93,16 @@ def test_rows_without_a_distribution(cuda, hidden):
     assert abs(got.entropy[2].item() - math.log(1500)) < 1e-5
 
 
+@pytest.mark.parametrize("hidden", [8, 64, 1024, 2056])
+def test_sums_of_one_product(cuda, hidden):
+    """Products that no sum cuts: what makes good the mean loss of long sums stays within the bound here too."""
+    g = torch.Generator().manual_seed(hidden)
+    _, w, tokens = some(g, 130, hidden, 700)
+    x = torch.zeros(130, hidden)
+    x[torch.arange(130), torch.randint(hidden, (130,), generator=g)] = 4.0
+    check(cuda, x.bfloat16(), w, tokens)
+
+
 def test_agrees_with_the_logits_that_it_does_not_write(cuda):
     g = torch.Generator().manual_seed(4)
     x, w, tokens = some(g, 33, 512, 9001)
