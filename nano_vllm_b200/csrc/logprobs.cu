@@ -10,15 +10,17 @@
 // Alternatives without a second pass: a thread keeps the largest of its 16-byte pieces' maxima and the first piece that has it.
 // Of 32 to 128 groups of threads the top-th largest (maximum, piece) is a bound that `top` elements reach, so every alternative lies
 // in a thread whose own (maximum, piece) reaches it: about `top` threads, whose pieces are read again (from L2) and compared
-// with the bound.  Pieces break ties of values, and where many threads tie (a mask that leaves fewer than `top`) a block takes its own
-// top-th thread for a closer bound.  More elements at the bound than the list holds are found one after the other.
+// with the bound.  Pieces break ties of values, and where many threads tie (a mask that leaves fewer than `top`) a block finds a closer
+// bound among its own threads, counting the ties within their pieces.  Where more elements reach the bound than the list holds (largest
+// ones that stand close together), each block keeps its own top ones.
 //
 // A row is read by a cluster of 1 to 8 blocks, four to a multiprocessor.
 //
 // What bounds it: 8 cycles of the unit for exponentials and about 7 issue slots an element and scheduler, beside 11 cycles of memory: of
 // 4096 rows of 151936 bf16 the loads alone take 181 us, the pass 205-225, with one alternative 218 (5.7 TB/s).  250 rows: 15.1, 20.8, with
 // five 24.5 (500 blocks on 592 places).  One row with 20 alternatives: 7.3, of which the end 3: bound 0.4, listed threads' pieces 1.7,
-// ranks and results 0.9, each a chain of short steps.
+// ranks and results 0.9, each a chain of short steps.  Rows of which a mask leaves 4 tokens, 20 alternatives: one 10.9, 64 23 (12.6 without a
+// mask), 250 33 (28.6); 64 alternatives: 2000 rows of 1000 28.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -32,7 +34,8 @@ constexpr int kLpThreads = 256;
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpMaxTop = NVLLM_LOGPROBS_MAX_TOP;
 constexpr int kLpGroups = 128;   // of threads, whose maxima give the bound
-constexpr int kLpCands = 1024;   // elements that reach the bound; more go the slow way
+constexpr int kLpTied = 8;       // threads at the bound's value that make a block look for a closer one (4 and 16 measured the same)
+constexpr int kLpCands = 1024;   // elements that reach the bound, as many as the list holds
 
 struct LogprobParams {
   const void* logits;
@@ -161,11 +164,10 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
   __shared__ float s_sums[kLpMaxCluster][3];
   __shared__ float s_warp[kLpThreads / 32][3];
   __shared__ uint16_t s_slot[kLpThreads];
-  __shared__ uint64_t s_key[kLpThreads];
+  __shared__ __align__(16) uint64_t s_key[kLpThreads];
   __shared__ uint64_t s_tau;
   __shared__ float s_m, s_log_z;
-  __shared__ int s_slots, s_cands;
-  __shared__ uint64_t s_most[kLpThreads / 32], s_all[2 * kLpMaxCluster];
+  __shared__ int s_slots, s_cands, s_reach[2][kLpThreads / 32];
   const cg::cluster_group cluster = cg::this_cluster();
   const int csize = 1 << log_csize, crank = blockIdx.x & (csize - 1), row = blockIdx.x >> log_csize;
   const bool several = csize > 1;
@@ -254,6 +256,27 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
       if (id >= 0 && id < vocab && lp_key(e[k], static_cast<uint32_t>(g)) >= tau) keys[k] = lp_key(e[k], static_cast<uint32_t>(id));
     }
   };
+  // Elements that reach the bound, and `least`, to the first block's list.
+  auto collect = [&](uint64_t least) {
+    for (int n = tid; n < looked; n += threads) {
+      uint64_t keys[N];
+      look(n, keys);
+      int found = 0;
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        if (keys[k] < least) keys[k] = 0;
+        found += keys[k] != 0;
+      }
+      if (!found) continue;
+      int place = atomicAdd(cands_at, found);  // one for a piece: 0.2 us each at another block
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (keys[k]) {
+          if (place < kLpCands) cand_at[place] = keys[k];
+          ++place;
+        }
+    }
+  };
   if constexpr (TOP) {
     // how many groups are above one: two threads count
     const ulonglong2* bounds = reinterpret_cast<const ulonglong2*>(s_bounds);
@@ -276,41 +299,51 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
         s_slot[k] = static_cast<uint16_t>(tid);
         s_key[k] = mine;
       }
-      __syncthreads();
+      return __syncthreads_count(mine && mine >= tau && mine >> 32 == tau >> 32);  // threads whose largest is the bound's value
     };
-    list();
-    if (s_slots > 2 * top) {  // ties (a mask that leaves fewer than `top`): the block's own top-th thread is a closer bound
+    const int tied = list();
+    if (s_slots > 2 * top || tied > kLpTied) {
+      // A closer bound among the block's own threads.  Of a thread with (value, piece), so many elements reach that: those of the value in
+      // the piece, of a masked one all.  The bound is where these numbers, from the largest key on, come to `top`.  (Without the numbers, each
+      // thread for one element: 250 rows of which 4 tokens are left, 20 alternatives, 53 us instead of 33; 64 of 64 alternatives 425 instead
+      // of 34; with 5 alternatives 21.8 instead of 22.4.)  Places are below 2^23: they move up four bits to make room.
       const int n = s_slots;
       const uint64_t it = tid < n ? s_key[tid] : 0;
-      int above = 0;
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) above += s_key[k] > it;
-      if (it && above == top - 1) s_tau = it;
+      uint64_t mark = 0;
+      int ties = 1;
+      if (it) {
+        const int g = static_cast<int>(0xffffffffu - static_cast<uint32_t>(it));
+        if (g >= head && g < head + whole) {
+          float e[N];
+          P::unpack(__ldg(base + g), e);
+          ties = 0;
+#pragma unroll
+          for (int k = 0; k < N; ++k) ties += lp_order(e[k]) == static_cast<uint32_t>(it >> 32);
+        }
+        mark = (it >> 32 << 32) | (static_cast<uint32_t>(it) << 4) | ties;
+      }
+      s_key[tid] = mark;
       __syncthreads();
-      tau = s_tau;
+      int above = 0;
+      const ulonglong2* marks = reinterpret_cast<const ulonglong2*>(s_key);
+      for (int k = 0; k < n; k += 8) {
+        ulonglong2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = marks[k / 2 + i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) above += (v[i].x > mark ? static_cast<int>(v[i].x & 15) : 0) + (v[i].y > mark ? static_cast<int>(v[i].y & 15) : 0);
+      }
+      if (it && above < top && above + ties >= top) s_tau = it;
       if (tid == 0) s_slots = 0;
       __syncthreads();
+      tau = s_tau;
       list();
     }
     each = (whole + all - 1) >> log_all;  // pieces of a thread
     each_inv = __frcp_rn(static_cast<float>(each));
     total = s_slots * each;
     looked = total + (crank == 0 ? head + tail : 0);
-    for (int n = tid; n < looked; n += threads) {
-      uint64_t keys[N];
-      look(n, keys);
-      int found = 0;
-#pragma unroll
-      for (int k = 0; k < N; ++k) found += keys[k] != 0;
-      if (!found) continue;
-      int place = atomicAdd(cands_at, found);  // one for a piece: 0.2 us each at another block
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (keys[k]) {
-          if (place < kLpCands) cand_at[place] = keys[k];
-          ++place;
-        }
-    }
+    collect(0);
   }
   if (crank == 0 && warp == threads / 32 - 1) {  // the warp with least to look at
     const int b = min(lane, csize - 1);
@@ -325,54 +358,57 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
   }
   if constexpr (!TOP) return;
   sync();
-  const int cands = *cands_at;
-  auto put = [&](int rank, uint64_t key) {
-    const int64_t to = static_cast<int64_t>(row) * top + rank;
-    top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
-    top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - s_m) * inv_t - s_log_z;
-  };
-  if (cands <= kLpCands) {
-    if (several) cluster.barrier_arrive();  // the first block's counter has been read
-    if (crank != 0) {
-      cluster.barrier_wait();
-      return;
+  int cands = *cands_at;
+  if (cands > kLpCands) {
+    // Of a block no more than `top` go on: those that reach the key that `top` of its keys reach, which is found bit by bit (places are
+    // below 2^24, so eight bits are known).  151936 ascending logits, 64 alternatives: 34 us.
+    uint64_t least = 0;
+    for (int bit = 63; bit >= 0; --bit) {
+      if (bit == 31) {
+        least |= 0xff000000u;
+        bit = 23;
+      }
+      const uint64_t to = least | 1ull << bit;
+      int count = 0;
+      for (int n = tid; n < looked; n += threads) {
+        uint64_t keys[N];
+        look(n, keys);
+#pragma unroll
+        for (int k = 0; k < N; ++k) count += keys[k] >= to;
+      }
+      count = __reduce_add_sync(0xffffffffu, count);
+      if (lane == 0) s_reach[bit & 1][warp] = count;
+      __syncthreads();
+      count = 0;
+      for (int w = 0; w < threads / 32; ++w) count += s_reach[bit & 1][w];
+      if (count >= top) least = to;
+      if (count == top) break;
     }
+    sync();
+    if (crank == 0 && tid == 0) s_cands = 0;
+    sync();
+    collect(least);
+    sync();
+    cands = *cands_at;
+  }
+  if (several) cluster.barrier_arrive();  // the first block's counter has been read
+  if (crank == 0) {
     // ranks by counting, eight threads a candidate
     for (int n = tid / 8; n < ((cands + 3) & ~3); n += threads / 8) {
       const uint64_t key = n < cands ? s_cand[n] : 0;
       int rank = 0;
+#pragma unroll 4
       for (int k = tid % 8; k < cands; k += 8) rank += s_cand[k] > key;
 #pragma unroll
       for (int sh = 1; sh < 8; sh <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, sh);
-      if (tid % 8 == 0 && n < cands && rank < top) put(rank, key);
+      if (tid % 8 == 0 && n < cands && rank < top) {
+        const int64_t to = static_cast<int64_t>(row) * top + rank;
+        top_tokens[to] = 0xffffffffu - static_cast<uint32_t>(key);
+        top_logprobs[to] = (lp_value(static_cast<uint32_t>(key >> 32)) - s_m) * inv_t - s_log_z;
+      }
     }
-    if (several) cluster.barrier_wait();
-    return;
   }
-  // The largest ones stand close together in few threads: one after the other.
-  uint64_t before = ~0ull;
-  for (int r = 0; r < top; ++r) {
-    uint64_t most = 0;
-    for (int n = tid; n < looked; n += threads) {
-      uint64_t keys[N];
-      look(n, keys);
-#pragma unroll
-      for (int k = 0; k < N; ++k)
-        if (keys[k] < before) most = max(most, keys[k]);
-    }
-#pragma unroll
-    for (int sh = 16; sh > 0; sh >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, sh));
-    if (lane == 0) s_most[warp] = most;
-    __syncthreads();
-    for (int k = 0; k < threads / 32; ++k) most = max(most, s_most[k]);
-    if (tid < csize) (several ? cluster.map_shared_rank(s_all, tid) : s_all)[(r & 1) * kLpMaxCluster + crank] = most;
-    sync();
-    most = 0;
-    for (int k = 0; k < csize; ++k) most = max(most, s_all[(r & 1) * kLpMaxCluster + k]);
-    before = most;
-    if (crank == 0 && tid == 0) put(r, most);
-  }
-  sync();
+  if (several) cluster.barrier_wait();
 }
 
 template <typename T, bool TOP>
@@ -595,10 +631,12 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   const int64_t pieces = (static_cast<int64_t>(vocab) + (logits_are_fp32 ? 3 : 7)) / (logits_are_fp32 ? 4 : 8);
   // Blocks of a row: as many as the device holds at a time with four to a multiprocessor, each thread with two pieces or more (one row
   // in one block 20.7 us, two 13.8, four 9.6, eight 8.4; 250 rows in one 33, two 28, four 35).  Threads of a row of its own block: eight
-  // pieces each (5000 rows of 100 in blocks of 64 threads 60 us, 256 79; 4096 of 32000 in 64 162, 256 110).
+  // pieces each (5000 rows of 100 in blocks of 64 threads 60 us, 256 79; 4096 of 32000 in 64 162, 256 110), but twice as many as there are
+  // alternatives, as long as they have a piece: with fewer the bound is loose (64 alternatives, 2000 rows of 1000 in 64 threads 81 us, 128 24;
+  // 4096 of 4000 161 and 60; with a mask that leaves 4 tokens 2000 of 1000 20.5 and 28).
   int csize = kLpMaxCluster, threads = kLpThreads;
   while (csize > 1 && (static_cast<int64_t>(rows) * csize > 4ll * sms || pieces < 2ll * csize * kLpThreads)) csize /= 2;
-  while (csize == 1 && threads > 64 && pieces < 8ll * threads) threads /= 2;
+  while (csize == 1 && threads > 64 && pieces < 8ll * threads && std::min<int64_t>(2 * top, pieces) <= threads / 2) threads /= 2;
   const int all = csize * threads;
   // Groups: enough of them that the bound lies close to the last alternative, counted against one another (64 rows with 32 alternatives
   // in 128 groups 16.0 us, in 64 17.8; with 20 alternatives 32 and 128 groups are the same in a row's own block and 0.2 us better).

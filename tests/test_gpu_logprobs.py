@@ -118,6 +118,27 @@ def test_alternatives_that_one_thread_reads(cuda, dtype, step, vocab):
     check(cuda, logits[:7], tokens[:7], 20)
 
 
+@pytest.mark.parametrize("top", [5, 20, 64])
+@pytest.mark.parametrize("rows,vocab", [(3, 743), (150, 1003), (700, 1000), (4, 8000), (2, 40001), (70, 16384)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_alternatives_among_ties_and_runs(cuda, dtype, rows, vocab, top):
+    """Masks that leave a few tokens here and there, in one place or before the end, equal logits and ones that ascend."""
+    g = torch.Generator().manual_seed(vocab + top)
+    x, tokens = some(g, rows, vocab, dtype)
+    kind = torch.arange(rows) % 6
+    few = torch.rand(rows, vocab, generator=g) * vocab < torch.tensor([3.0, 30.0])[torch.arange(rows) % 2][:, None]
+    few[:, 5] = True
+    x[(kind == 0)[:, None] & ~few] = -torch.inf
+    x[(kind == 1)[:, None] & ~few] = torch.finfo(dtype).min
+    at = torch.arange(vocab)
+    x[kind == 2] = x[kind == 2].masked_fill((at < vocab // 2) | (at > vocab // 2 + 12), -torch.inf)
+    x[kind == 3] = x[kind == 3].masked_fill(at < vocab - 9, -torch.inf)
+    x[kind == 4] = 1.5
+    x[kind == 5] = (at * 0.01).to(dtype)
+    tokens[:] = 5
+    check(cuda, x, torch.where(torch.isfinite(x[torch.arange(rows), tokens]), tokens, vocab - 1), top)
+
+
 def test_sizes_of_32_bits(cuda):
     """Rows further apart than 2^31 elements."""
     wide = torch.zeros(3, 1_500_000_000, dtype=torch.bfloat16, device=cuda)
