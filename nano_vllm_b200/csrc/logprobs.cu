@@ -10,7 +10,7 @@
 // Alternatives without a second pass: a thread keeps the largest of its 16-byte pieces' maxima and the first piece that has it.
 // Of 32 to 128 groups of threads the top-th largest (maximum, piece) is a bound that `top` elements reach, so every alternative lies
 // in a thread whose own (maximum, piece) reaches it: about `top` threads, whose pieces are read again (from L2) and compared
-// with the bound.  Pieces break ties of values, and where many threads tie (a mask that leaves fewer than `top`) a block finds a closer
+// with the bound; where those are many, a thread keeps these two for each segment of its pieces.  Pieces break ties of values, and where many threads tie (a mask that leaves fewer than `top`) a block finds a closer
 // bound among its own threads, counting the ties within their pieces.  Where more elements reach the bound than the list holds (largest
 // ones that stand close together), each block keeps its own top ones.
 //
@@ -31,10 +31,13 @@
 namespace nvllm {
 
 constexpr int kLpThreads = 256;
+template <bool TOP>
+constexpr int kLpStep = TOP ? 3 : 4;  // pieces that a thread takes at a time
 constexpr int kLpMaxCluster = 8;
 constexpr int kLpMaxTop = NVLLM_LOGPROBS_MAX_TOP;
 constexpr int kLpGroups = 128;   // of threads, whose maxima give the bound
 constexpr int kLpTied = 8;       // threads at the bound's value that make a block look for a closer one (4 and 16 measured the same)
+constexpr int kLpSegments = 8;   // of a thread's pieces, at most
 constexpr int kLpCands = 1024;   // elements that reach the bound, as many as the list holds
 
 struct LogprobParams {
@@ -45,6 +48,7 @@ struct LogprobParams {
   int vocab, top;
   int groups;  // of the threads that read a row, whose maxima give the bound: 32 to 128
   int log_csize, log_all, log_size;  // blocks of a row, its threads, threads of a group: powers of two, divided by with shifts
+  int log_seg;  // steps of a segment (PARTED)
   float* logprobs;
   float* entropy;
   int64_t* top_tokens;
@@ -149,25 +153,27 @@ struct LpPiece<float> {
   }
 };
 
+extern __shared__ uint64_t s_seg[];  // [kLpSegments][threads]: the largest (maximum, piece) of a segment
+
 // From the threads' statistics to the row's results.
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool PARTED>
 __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, const float sum_t, const uint64_t mine, const uint4* const base,
                                        const int shift, const int pieces, const int head, const int tail, const float inv_t, const float given,
                                        const int64_t token, const int vocab, const int top, const int groups, const int log_csize, const int log_all,
-                                       const int log_size, float* const logprobs, float* const entropy, int64_t* const top_tokens,
+                                       const int log_size, const int log_seg, float* const logprobs, float* const entropy, int64_t* const top_tokens,
                                        float* const top_logprobs, int* const status) {
   using P = LpPiece<T>;
-  constexpr int N = P::N;
+  constexpr int N = P::N, C = kLpStep<TOP>;
   namespace cg = cooperative_groups;
   __shared__ __align__(16) uint64_t s_bounds[kLpGroups];
   __shared__ uint64_t s_cand[kLpCands];  // of the first block
   __shared__ float s_sums[kLpMaxCluster][3];
   __shared__ float s_warp[kLpThreads / 32][3];
-  __shared__ uint16_t s_slot[kLpThreads];
+  __shared__ uint16_t s_slot[kLpThreads], s_part[PARTED ? 2 * kLpMaxTop * kLpSegments : 1];
   __shared__ __align__(16) uint64_t s_key[kLpThreads];
   __shared__ uint64_t s_tau;
   __shared__ float s_m, s_log_z;
-  __shared__ int s_slots, s_cands, s_reach[2][kLpThreads / 32];
+  __shared__ int s_slots, s_parts, s_cands, s_reach[2][kLpThreads / 32];
   const cg::cluster_group cluster = cg::this_cluster();
   const int csize = 1 << log_csize, crank = blockIdx.x & (csize - 1), row = blockIdx.x >> log_csize;
   const bool several = csize > 1;
@@ -177,7 +183,7 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
   LpSums sum{sum_m, sum_s, sum_t};
   if (tid == 0) {
     s_tau = 0;
-    s_slots = s_cands = 0;
+    s_slots = s_parts = s_cands = 0;
   }
   // ---- sums of the block, and the largest (maximum, piece) of every group of threads
   auto join_warp = [&](LpSums& v) {  // over the lanes
@@ -230,15 +236,16 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
   uint64_t tau = 0;
   float each_inv = 0.f;
   int each = 0, total = 0, looked = 0;
-  // The keys of the elements that reach the bound in piece n of the listed threads, 0 in the place of the others.
+  // The keys of the elements that reach the bound in piece n of what is listed (a thread, or a segment of one), 0 in the place of the others.
   auto look = [&](int n, uint64_t (&keys)[N]) {
 #pragma unroll
     for (int k = 0; k < N; ++k) keys[k] = 0;
     int g;
     uint4 w;
     if (n < total) {
-      const int nth = static_cast<int>((static_cast<float>(n) + 0.5f) * each_inv), who = crank * threads + s_slot[nth];
-      g = head + who + (n - nth * each) * all;
+      const int nth = static_cast<int>((static_cast<float>(n) + 0.5f) * each_inv);
+      if constexpr (PARTED) g = head + crank * threads + s_part[nth] % kLpThreads + (s_part[nth] / kLpThreads * each + n - nth * each) * all;
+      else g = head + crank * threads + s_slot[nth] + (n - nth * each) * all;
       if (g >= head + whole) return;
       w = __ldg(base + g);
     } else if (n < looked) {  // the cut pieces, whether they are in a listed thread or not
@@ -320,6 +327,7 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
 #pragma unroll
           for (int k = 0; k < N; ++k) ties += lp_order(e[k]) == static_cast<uint32_t>(it >> 32);
         }
+        ties = max(ties, 1);
         mark = (it >> 32 << 32) | (static_cast<uint32_t>(it) << 4) | ties;
       }
       s_key[tid] = mark;
@@ -339,9 +347,19 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
       tau = s_tau;
       list();
     }
+    int listed = s_slots;
     each = (whole + all - 1) >> log_all;  // pieces of a thread
+    if constexpr (PARTED) {               // of the listed threads the segments that reach the bound
+      each = C << log_seg;
+      for (int n = tid; n < listed * kLpSegments; n += threads) {
+        const int who = s_slot[n / kLpSegments], part = n % kLpSegments;
+        if (s_seg[part * threads + who] >= tau) s_part[atomicAdd(&s_parts, 1)] = static_cast<uint16_t>(part * kLpThreads + who);
+      }
+      __syncthreads();
+      listed = s_parts;
+    }
     each_inv = __frcp_rn(static_cast<float>(each));
-    total = s_slots * each;
+    total = listed * each;
     looked = total + (crank == 0 ? head + tail : 0);
     collect(0);
   }
@@ -411,10 +429,10 @@ __device__ __noinline__ void lp_finish(const float sum_m, const float sum_s, con
   if (several) cluster.barrier_wait();
 }
 
-template <typename T, bool TOP>
+template <typename T, bool TOP, bool PARTED>
 __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_constant__ LogprobParams p) {
   using P = LpPiece<T>;
-  constexpr int N = P::N, C = TOP ? 3 : 4;
+  constexpr int N = P::N, C = kLpStep<TOP>;
   pdl_wait();
   const int csize = 1 << p.log_csize, crank = blockIdx.x & (csize - 1);
   const bool several = csize > 1;
@@ -558,9 +576,11 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
     take(x1, rest, true);
   }
   const float best_last = best;
-  const int at_last = at;
+  const int at_last = !PARTED || rest < whole ? at : -1;
   best = -INFINITY;
   at = head + me;
+  if constexpr (PARTED)  // segments without a piece
+    for (int k = steps >> p.log_seg; k < kLpSegments; ++k) s_seg[k * threads + tid] = 0;
   for (int n = 0, i = me; n < steps; n += 2) {
     if (n + 1 < steps) load(x1, i + step);
     take(x0, i, false);
@@ -569,10 +589,24 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
     if (n + 2 < steps) load(x0, i + step);
     take(x1, i, false);
     i += step;
+    if constexpr (PARTED) {
+      if (((n + 2) >> p.log_seg) != (n >> p.log_seg)) {
+        s_seg[(n >> p.log_seg) * threads + tid] = lp_key(best, static_cast<uint32_t>(at));
+        best = -INFINITY;
+        at = head + i;
+      }
+    }
   }
-  if (best_last > best || steps == 0) {
+  bool open = steps > 0;  // the loop has left pieces that are in no segment yet
+  if constexpr (PARTED) open = steps >> p.log_seg << p.log_seg != steps;
+  if (best_last > best || !open) {
     best = best_last;
     at = at_last;
+  }
+  uint64_t others = 0;
+  if constexpr (PARTED) {
+    if (at >= 0) s_seg[(steps >> p.log_seg) * threads + tid] = lp_key(best, static_cast<uint32_t>(at));
+    for (int k = 0; k < steps >> p.log_seg; ++k) others = max(others, s_seg[k * threads + tid]);
   }
   if (crank == 0 && warp == 0 && (head || tail)) {
     const uint4 w0 = head && lane == 0 ? cut_piece(0) : nothing, w1 = tail && lane == 0 ? cut_piece(pieces - 1) : nothing;
@@ -591,8 +625,10 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
   }
 
   // What the end of a row wants of registers would cost the stream a tenth if it were part of it.
-  lp_finish<T, TOP>(sum.m, sum.s, sum.t, any ? lp_key(best, static_cast<uint32_t>(at)) : 0, base, shift, pieces, head, tail, inv_t, given, token, p.vocab, p.top,
-                    p.groups, p.log_csize, p.log_all, p.log_size, p.logprobs, p.entropy, p.top_tokens, p.top_logprobs, p.status);
+  uint64_t mine = any ? lp_key(best, static_cast<uint32_t>(at)) : 0;
+  if constexpr (PARTED) mine = at >= 0 ? max(others, mine) : others;
+  lp_finish<T, TOP, PARTED>(sum.m, sum.s, sum.t, mine, base, shift, pieces, head, tail, inv_t, given, token, p.vocab, p.top,
+                    p.groups, p.log_csize, p.log_all, p.log_size, p.log_seg, p.logprobs, p.entropy, p.top_tokens, p.top_logprobs, p.status);
 }
 
 }  // namespace nvllm
@@ -641,6 +677,7 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   // Groups: enough of them that the bound lies close to the last alternative, counted against one another (64 rows with 32 alternatives
   // in 128 groups 16.0 us, in 64 17.8; with 20 alternatives 32 and 128 groups are the same in a row's own block and 0.2 us better).
   p.groups = top <= 20 ? std::max(32, all / 32) : std::min(kLpGroups, all);
+  while (p.groups < std::min(kLpGroups, all) && pieces * p.groups < static_cast<int64_t>(top) * all) p.groups *= 2;
   auto log2_of = [](int n) {
     int l = 0;
     while (n >> (l + 1)) ++l;
@@ -649,9 +686,17 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   p.log_csize = log2_of(csize);
   p.log_all = log2_of(all);
   p.log_size = log2_of(all / p.groups);
+  // Segments of a thread's pieces, so that some and not all pieces of a listed thread are read again: where those would be more than two for
+  // each thread, of 32 or more (4096 rows of 151936 with 20 alternatives 320 us, in segments 280; with five 231 and 261; 300 rows with 64 76 and 47;
+  // 1003 fp32 rows with 64 219 and 147).  The pass itself takes 218 us without and 250 with them.
+  const int64_t each = (pieces + all) / all, steps = each / kLpStep<true> + 1;
+  const bool parted = each >= 32 && top * each > 2 * all;
+  p.log_seg = 1;
+  while (steps >> p.log_seg >= kLpSegments) ++p.log_seg;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * csize), 1, 1);
   cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = parted ? kLpSegments * threads * sizeof(uint64_t) : 0;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -661,8 +706,11 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = csize > 1 ? 2 : 1;
-  auto kernel = logits_are_fp32 ? (top > 0 ? logprobs_kernel<float, true> : logprobs_kernel<float, false>)
-                                : (top > 0 ? logprobs_kernel<__nv_bfloat16, true> : logprobs_kernel<__nv_bfloat16, false>);
+  auto of = [&](auto type) {
+    using T = decltype(type);
+    return parted ? logprobs_kernel<T, true, true> : top > 0 ? logprobs_kernel<T, true, false> : logprobs_kernel<T, false, false>;
+  };
+  auto kernel = logits_are_fp32 ? of(0.f) : of(__nv_bfloat16());
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) {
     (void)cudaGetLastError();

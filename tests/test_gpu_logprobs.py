@@ -139,6 +139,30 @@ def test_alternatives_among_ties_and_runs(cuda, dtype, rows, vocab, top):
     check(cuda, x, torch.where(torch.isfinite(x[torch.arange(rows), tokens]), tokens, vocab - 1), top)
 
 
+@pytest.mark.parametrize("dtype,rows,vocab,top", [
+    (torch.float32, 300, 33333, 20), (torch.bfloat16, 300, 65536 + 8 * 3 * 256, 20), (torch.bfloat16, 299, 71117, 64), (torch.float32, 160, 66000, 64),
+    (torch.float32, 297, 32768 + 4 * 256, 64)])
+def test_alternatives_of_threads_with_many_pieces(cuda, dtype, rows, vocab, top):
+    """Rows that few threads read: large logits early, late, everywhere, equal and masked ones."""
+    g = torch.Generator().manual_seed(vocab)
+    x, tokens = some(g, rows, vocab, dtype)
+    at, kind = torch.arange(vocab), torch.arange(rows) % 10
+    x[kind == 1] = x[kind == 1].masked_fill(torch.rand(vocab, generator=g) < 0.9999, -torch.inf)
+    x[kind == 2] = (at * 0.01).to(dtype)
+    x[kind == 3] = (at * -0.01).to(dtype)
+    x[kind == 4] = x[kind == 4].masked_fill(at < vocab - 5, -torch.inf)
+    x[kind == 5] = x[kind == 5].masked_fill(at >= 3, torch.finfo(dtype).min)
+    x[kind == 6] = 2.5
+    x[(kind == 7)[:, None] & (at % 4096 < 8)] += 20
+    x[(kind == 8)[:, None] & (torch.rand(vocab, generator=g) < 0.01)] = math.nan
+    tokens[kind == 1] = x[kind == 1].float().argmax(-1)
+    tokens[kind == 4], tokens[kind == 5] = vocab - 2, 1
+    wide = torch.full((rows, vocab + 3), math.nan, dtype=dtype, device=cuda)
+    wide[:, 1:vocab + 1] = x.to(cuda)
+    check(cuda, x, tokens, top, on_gpu=wide[:, 1:vocab + 1])
+    check(cuda, x, tokens, top)
+
+
 def test_sizes_of_32_bits(cuda):
     """Rows further apart than 2^31 elements."""
     wide = torch.zeros(3, 1_500_000_000, dtype=torch.bfloat16, device=cuda)
