@@ -19,6 +19,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "copy_ring.cuh"
 #include "sm100.cuh"
 
 namespace nvllm {
@@ -41,7 +42,7 @@ struct Parts {
 // 5.5 TB/s, threads with 16-byte loads and stores 5.2-5.4.
 constexpr int kPiece = 16384, kStages = 6, kLead = 2;
 constexpr int kRingBytes = kPiece * kStages + 128;  // barriers behind the pieces
-static_assert(kStages * 8 <= 128 && kLead < kStages, "barriers, and a stage whose store is being read");
+static_assert(kStages * 8 <= 128, "barriers");
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -52,6 +53,23 @@ __device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t byt
 template <int N>
 __device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
+struct RingIo {
+  uint32_t ring, bars;
+  unsigned char** to;  // of every stage: where its piece goes
+  uint32_t* bytes;     // and how much it is
+  template <int N>
+  __device__ __forceinline__ void read() { bulk_wait_read<N>(); }
+  __device__ __forceinline__ void load(int s, unsigned char* dst, const unsigned char* src, uint32_t n) {
+    to[s] = dst;
+    bytes[s] = n;
+    sm100::mbar_expect_tx(bars + 8 * s, n);
+    bulk_load(ring + s * kPiece, src, n, bars + 8 * s);
+  }
+  __device__ __forceinline__ bool wait(int s, uint32_t parity) { return sm100::mbar_wait(bars + 8 * s, parity); }
+  __device__ __forceinline__ void store(int s) { bulk_store(to[s], ring + s * kPiece, bytes[s]); }
+  __device__ __forceinline__ void finish() { bulk_wait_all(); }
+};
 
 // All copies: `of(c, src, dst, slots)` says what copy c is and whether there is anything to do.  A (copy, plane) of values is cut
 // in `pieces` equal parts, an item each; items are dealt out to the blocks in turn.  Scales: threads 32 and on.
@@ -69,14 +87,9 @@ __device__ __forceinline__ void copy_all(const Parts<MOST>& parts, int copies, u
     const int pieces = static_cast<int>(max(int64_t{1}, min(wanted, most)));
     __shared__ unsigned char* s_to[kStages];
     __shared__ uint32_t s_bytes[kStages];
-    int64_t n = 0;  // pieces of shared memory loaded so far
-    bool ok = true;
-    auto store = [&](int64_t m) {
-      const int s = static_cast<int>(m % kStages);
-      if (!(ok = sm100::mbar_wait(bars + 8 * s, (m / kStages) & 1))) return;
-      bulk_store(s_to[s], ring + s * kPiece, s_bytes[s]);
-    };
-    for (int64_t item = blockIdx.x; item < pairs * pieces && ok; item += gridDim.x) {
+    RingIo io{ring, bars, s_to, s_bytes};
+    CopyRing<kStages, kLead, RingIo> moving{io};
+    for (int64_t item = blockIdx.x; item < pairs * pieces && moving.ok; item += gridDim.x) {
       const int64_t pair = item / pieces;
       const int c = static_cast<int>(pair / parts.value_planes), k = static_cast<int>(item - pair * pieces);
       int64_t src, dst;
@@ -91,23 +104,11 @@ __device__ __forceinline__ void copy_all(const Parts<MOST>& parts, int copies, u
       unsigned char* plane_at = static_cast<unsigned char*>(part.base) + plane * part.plane_stride;
       const int64_t units = static_cast<int64_t>(slots) * part.slot_bytes / 16, each = (units + pieces - 1) / pieces;
       const int64_t end = min((k + 1) * each, units) * 16;
-      for (int64_t at = k * each * 16; at < end && ok; at += kPiece) {
-        const uint32_t bytes = static_cast<uint32_t>(min(end - at, static_cast<int64_t>(kPiece)));
-        const int s = static_cast<int>(n % kStages);
-        bulk_wait_read<kStages - kLead - 1>();  // the store that had the stage before has read it
-        s_to[s] = plane_at + dst * part.block_stride + at;
-        s_bytes[s] = bytes;
-        sm100::mbar_expect_tx(bars + 8 * s, bytes);
-        bulk_load(ring + s * kPiece, plane_at + src * part.block_stride + at, bytes, bars + 8 * s);
-        if (++n > kLead) store(n - 1 - kLead);
-      }
+      for (int64_t at = k * each * 16; at < end && moving.ok; at += kPiece)
+        moving.piece(plane_at + dst * part.block_stride + at, plane_at + src * part.block_stride + at,
+                     static_cast<uint32_t>(min(end - at, static_cast<int64_t>(kPiece))));
     }
-    for (int64_t m = max(int64_t{0}, n - kLead); m < n; ++m) {
-      if (ok) store(m);
-      else (void)sm100::mbar_wait(bars + 8 * (m % kStages), (m / kStages) & 1);  // no copy is in flight when the block ends
-    }
-    bulk_wait_all();
-    if (!ok) atomicOr(status, NVLLM_STATUS_TIMEOUT);
+    if (!moving.end()) atomicOr(status, NVLLM_STATUS_TIMEOUT);
   } else if (threadIdx.x >= 32) {
     const int scale_planes = parts.planes - parts.value_planes;
     for (int64_t item = blockIdx.x; item < static_cast<int64_t>(copies) * scale_planes; item += gridDim.x) {
