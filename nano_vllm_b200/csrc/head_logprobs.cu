@@ -190,11 +190,14 @@ __global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_ker
               }
             }
         }
-        if (!ok && rank == 0)  // no copy is in flight when the block (the pair) ends
-          for (int k = 0; k < nst; ++k) {
-            const int uses = k < s ? use + 1 : use;
-            if (uses > 0) (void)mbar_wait(bar(FULL0 + k), (uses - 1) & 1);
-          }
+        // Neither a copy nor an arrival is in flight when the block (the pair) ends: the last products that read a stage arrive at both
+        // blocks' barriers; where a wait ran out, the first block's barriers tell of the copies of both.
+        auto uses = [&](int k) { return k < s ? use + 1 : use; };
+        for (int k = 0; k < nst && ok; ++k)
+          if (uses(k) > 0) ok = wait_or_abort(bar(EMPTY0 + k), (uses(k) - 1) & 1, abort_flag);
+        if (!ok && rank == 0)
+          for (int k = 0; k < nst; ++k)
+            if (uses(k) > 0) (void)mbar_wait(bar(FULL0 + k), (uses(k) - 1) & 1);
       }
     } else if (warp == WARPS + 1 && rank == 0) {
       // ------------------------------------------------------------------ MMA issuer
