@@ -21,7 +21,7 @@ template <int STAGES, int LEAD, class Io>
 struct CopyRing {
   static_assert(LEAD < STAGES, "a stage whose store is being read");
   Io& io;
-  int64_t loaded = 0, stored = 0;
+  uint32_t loaded = 0, stored = 0;  // pieces: 2^32 of 16 KB are far more than a memory holds
   bool ok = true;
 
   template <class... From>
@@ -40,11 +40,11 @@ struct CopyRing {
   // flight when the block gives its shared memory up.
   NVLLM_RING bool end() {
     while (ok && stored < loaded) store();
-    for (int64_t m = stored; m < loaded; ++m) (void)io.wait(static_cast<int>(m % STAGES), phase(m));
+    for (uint32_t m = stored; m < loaded; ++m) (void)io.wait(static_cast<int>(m % STAGES), phase(m));
     io.finish();
     return ok;
   }
-  static NVLLM_RING uint32_t phase(int64_t m) { return static_cast<uint32_t>((m / STAGES) & 1); }
+  static NVLLM_RING uint32_t phase(uint32_t m) { return m / STAGES & 1; }
 };
 
 }  // namespace nvllm
