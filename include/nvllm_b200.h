@@ -439,11 +439,12 @@ NVLLM_API int nvllm_sample_layout(int32_t batch, int32_t vocab, int64_t vocab_of
  * [rows, vocab] (bf16 or fp32, unit inner stride).  No counterpart in the reference.
  *   logprobs[r]: of tokens[r] (int64); 0 where that is negative, NaN and NVLLM_STATUS_BAD_TOKEN where it is >= vocab
  *   entropy[r]: in nats;  top_tokens / top_logprobs [rows, top] contiguous: the largest logits in order, ties to the lowest index
- * All statistics are fp32.  temperatures: fp32 [rows] or NULL; one that is not above 0 counts as 1, one above
- * 1e30 as 1e30.  -infinity in a row is a masked token; a row with a NaN, with +infinity or with nothing but -infinity has NaN for
- * results (its alternatives go by the logits, NaN like -infinity; subnormal logits order like 0).  0 <= top <=
- * NVLLM_LOGPROBS_MAX_TOP, vocab <= NVLLM_LOGPROBS_MAX_VOCAB (a head_logprobs call: rows <= 2^24, hidden <= 65536).  No alignment beyond the
- * element's is required; the rest of the 16-byte pieces that a row's first and last elements lie in may be read.
+ * All statistics are fp32.  temperatures: fp32 [rows] or NULL; one that is not above 0 counts as 1, one above 1e30 as
+ * 1e30, one below 1e-38 as 1e-38.  -infinity in a row is a masked token; a row with a NaN, with +infinity or with nothing but
+ * -infinity has NaN for results (its alternatives go by the logits, NaN like -infinity; subnormal logits order like 0).
+ * 0 <= top <= NVLLM_LOGPROBS_MAX_TOP, vocab <= NVLLM_LOGPROBS_MAX_VOCAB (a head_logprobs call: rows <= 2^24, hidden <= 65536).
+ * No alignment beyond the element's is required; the rest of the 16-byte pieces that a row's first and last elements lie in may be
+ * read.
  */
 #define NVLLM_LOGPROBS_MAX_TOP 64
 #define NVLLM_LOGPROBS_MAX_VOCAB 16777216 /* head_logprobs: 2097152 */

@@ -14,10 +14,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 // 1 / T of a row; a temperature that is not above 0, or none, counts as 1.  Beyond 1e30 it counts as 1e30: every logit up to 1e22 is
-// uniform there already, and a masked one's difference, -3e38 at the least, still has no weight.
+// uniform there already, and a masked one's difference, -3e38 at the least, still has no weight.  Below 1e-38 it counts as 1e-38, whose
+// inverse is finite; a comparison, as this is compiled, would take subnormal ones for 0.
 __device__ __forceinline__ float lp_inverse(const float* temperatures, int64_t row) {
   const float t = temperatures ? temperatures[row] : 1.f;
-  return t > 0.f ? fminf(fmaxf(__frcp_rn(t), 1e-30f), 1e38f) : 1.f;
+  const int bits = __float_as_int(t);
+  return bits > 0 && bits <= 0x7f800000 ? fminf(fmaxf(__frcp_rn(t), 1e-30f), 1e38f) : 1.f;
 }
 
 // Maximum m (no less than the smallest finite number), s = sum exp2(c (x - m)), t = sum exp2(c (x - m)) (x - m).

@@ -29,9 +29,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     of the logits; all statistics in fp32.
 
     ``temperatures``: fp32 ``[N]`` as for ``sample_tokens``, where 1 stands for any that is not above 0 (greedy rows); without
-    them T is 1; above 1e30 it counts as 1e30.  V is up to 2^24 (2^21 in ``head_logprobs``).  A negative token asks for none: 0
-    (rows of a padded batch); one beyond the vocabulary gives NaN and sets bit 8 of ``_lib.read_status()``.  Logits of -infinity are masked tokens.  A row with a NaN, with +infinity or with nothing but
-    -infinity has no distribution and NaN for results; its ``top_tokens`` go by the logits, NaN like -infinity.
+    them T is 1; above 1e30 it counts as 1e30, below 1e-38 as 1e-38.  V is up to 2^24 (2^21 in ``head_logprobs``).  A negative token
+    asks for none: 0 (rows of a padded batch); one beyond the vocabulary gives NaN and sets bit 8 of ``_lib.read_status()``.
+    Logits of -infinity are masked tokens.  A row with a NaN, with +infinity or with nothing but -infinity has no distribution and
+    NaN for results; its ``top_tokens`` go by the logits, NaN like -infinity.
     ``out``: the four result tensors of an earlier call or of a graph, else they are made."""
     return TokenLogprobs._make(_native(logits).token_logprobs(logits, tokens, top, temperatures, out))
 
