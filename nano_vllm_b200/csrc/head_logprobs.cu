@@ -5,12 +5,13 @@
 // logits: the statistics of token_logprobs), which a second launch joins over the vocabulary's tiles.
 //
 // Sums over H stay fp32, in a tensor core that cuts its running sum towards zero at every step of 16 products.  That is a systematic
-// loss: at H = 4096 logits come out 3.7e-6 too small, log probabilities 2e-6 off.  Two things are done about it.  A product is cut after
-// kChunk elements and the parts are added in registers.  And the logits' scale makes good what a step loses on average (kStepLoss, half a
-// last place of a sum that is still on its way, measured at 64 to 5120 elements, products of either sign and of one): at H = 1024
-// log probabilities 4.6e-7 -> 1.9e-7 and entropy 8.4e-7 -> 1.2e-7 off (relative, 512 rows of 151936), at 4096 4.6e-7 -> 1.7e-7 and
-// 9.1e-7 -> 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off at 1024.  Parts of 512 elements would halve the loss too, at 1.28 times
-// the time for 4096 x 1024 x 151936.
+// loss: at H = 4096 logits come out 3.2e-6 too small, log probabilities 2e-6 off.  Two things are done about it.  A product is cut
+// after kChunk elements and the parts are added in registers.  And the logits' scale makes good what a step loses on average
+// (kStepLoss, half a last place of a sum that is still on its way, measured at 64 to 5120 elements, products of either sign and of
+// one): at H = 1024 logits are 1.0e-6 off on average without, 5e-8 with it, log probabilities 4.6e-7 and 1.9e-7, the entropy 8.4e-7 and
+// 1.2e-7 (relative, 512 rows of 151936); at 4096 4.6e-7 and 1.7e-7, 9.1e-7 and 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off
+// at 1024.  Sums that lose nothing, such as those of one product, come out too large by what is made good: 9.5e-7 of a difference
+// of logits at the most.  Parts of 512 elements would halve the loss too, at 1.28 times the time for 4096 x 1024 x 151936.
 //
 // What bounds it.  Many rows: the tensor cores, and then the power cap (4096 x 1024 x 151936 803 us, 1590 TFLOP/s, 908 in a long chain; 1000 x
 // 4096 830-870; blocks of 128 rows by themselves, which feed the tensor cores twice the bytes, 1306 and 1248).  H below some 900: the reduction
@@ -468,6 +469,17 @@ static Plan plan_of(int rows, int hidden, int vocab, int sms) {
   return pl;
 }
 
+// What makes good the mean loss of sums over `hidden` elements: of every part its own steps', the first of which has nothing to lose.
+// (All as if they were full ones: logits of 1472 elements 1.4e-7 too large on average.)
+static float scale_of(int64_t hidden) {
+  double lost = 0;
+  for (int64_t at = 0; at < hidden; at += kChunk) {
+    const int64_t n = std::min<int64_t>(kChunk, hidden - at);
+    lost += static_cast<double>(n) * static_cast<double>((n + 15) / 16 - 1);
+  }
+  return static_cast<float>(1 + kStepLoss * lost / static_cast<double>(hidden));
+}
+
 static int check(int64_t rows, int64_t hidden, int64_t vocab) {
   if (rows < 0 || rows > (1 << 24) || vocab <= 0 || vocab > (1 << 21) || hidden <= 0 || hidden > 65536 || hidden % 8)
     return fail(NVLLM_E_GEOMETRY, "head_logprobs: rows=%lld hidden=%lld (a multiple of 8) vocab=%lld not supported", (long long)rows, (long long)hidden,
@@ -530,7 +542,7 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   hlp::Params p{};
   p.tokens = tokens;
   p.temperatures = temperatures;
-  p.scale = static_cast<float>(1 + hlp::kStepLoss * static_cast<double>((std::min<int64_t>(hidden, hlp::kChunk) + 15) / 16 - 1));
+  p.scale = hlp::scale_of(hidden);
   p.rows = static_cast<int>(rows);
   p.vocab = static_cast<int>(vocab);
   p.bn = pl.bn;
