@@ -18,6 +18,7 @@
 // of a tile (4096 x 512 490 us of 393; tiles shared out evenly to the warps the same; 16 warps instead of 8 made 77 x 896 47.6 instead of 45.9).  Up to 128 rows: the weights' stream (one row of 1024
 // 53.5 us, 5.8 TB/s; of 4096 197.6, 6.3), with as many stages as fit on their way (four: 54.8 and 200.8).
 #include <algorithm>
+#include <atomic>
 
 #include "logprobs.cuh"
 #include "prefill_tc.cuh"
@@ -524,21 +525,25 @@ extern "C" int nvllm_head_logprobs(const void* hidden_states, int64_t hidden_row
   using Kernel = decltype(&hlp::head_logprobs_kernel<false, false>);
   static const Kernel kernels[2][2] = {{hlp::head_logprobs_kernel<false, false>, hlp::head_logprobs_kernel<false, true>},
                                        {hlp::head_logprobs_kernel<true, false>, hlp::head_logprobs_kernel<true, true>}};
-  static bool ready[64] = {false};
+  // All forms are made ready by the first call on a device, so that later ones can be captured whatever their sizes.
+  static std::atomic<bool> ready[64];
+  static std::atomic<int> registers[2][2];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !ready[dev]) {
     for (int k = 0; k < 4; ++k) {
       cudaError_t e = cudaFuncSetAttribute(kernels[k / 2][k % 2], cudaFuncAttributeMaxDynamicSharedMemorySize, hlp::SMEM);
       if (e != cudaSuccess) return fail(NVLLM_E_CUDA, "head_logprobs: cannot reserve shared memory: %s", cudaGetErrorString(e));
-      cudaFuncAttributes attr;  // a block with fewer registers than its groups share would wait for them without end
-      if (k % 2 && (e = cudaFuncGetAttributes(&attr, kernels[k / 2][k % 2])) != cudaSuccess)
+      cudaFuncAttributes attr;
+      if ((e = cudaFuncGetAttributes(&attr, kernels[k / 2][k % 2])) != cudaSuccess)
         return fail(NVLLM_E_CUDA, "head_logprobs: %s", cudaGetErrorString(e));
-      if (k % 2 && attr.numRegs < hlp::Cfg<false, true>::REGS)
-        return fail(NVLLM_E_CUDA, "head_logprobs: compiled to %d registers, %d needed", attr.numRegs, hlp::Cfg<false, true>::REGS);
+      registers[k / 2][k % 2] = attr.numRegs;
     }
     if (dev >= 0 && dev < 64) ready[dev] = true;
   }
+  // a block with fewer registers than its groups share would wait for them without end
+  if (is_long && registers[pl.pair][is_long] < hlp::Cfg<false, true>::REGS)
+    return fail(NVLLM_E_CUDA, "head_logprobs: compiled to %d registers, %d needed", registers[pl.pair][is_long].load(), hlp::Cfg<false, true>::REGS);
   hlp::Params p{};
   p.tokens = tokens;
   p.temperatures = temperatures;
