@@ -7,6 +7,10 @@ import pytest
 import torch
 from test_gpu_head_logprobs import check, some
 
+from nano_vllm_b200 import _lib
+from nano_vllm_b200.logprobs import head_logprobs
+from oracle.logprobs_ref import assert_same, head_logprobs_ref
+
 pytestmark = pytest.mark.gpu
 
 
@@ -37,3 +41,32 @@ assert all(torch.equal(i, j) for o, c in zip(out, cases) for i, j in zip(o, head
 """
     done = subprocess.run([sys.executable, "-c", script], cwd=Path(__file__).resolve().parents[1], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
+
+
+@pytest.mark.parametrize("rows,hidden,vocab", [(600, 1536, 30011), (300, 2056, 9001), (1500, 1032, 5003), (2000, 4096, 300), (769, 1040, 2000)])
+def test_pairs_with_long_sums(cuda, rows, hidden, vocab):
+    """Parts of more than 1024 elements by pairs of blocks, whose row tiles divide the multiprocessors (300 rows) and do not."""
+    g = torch.Generator().manual_seed(rows)
+    check(cuda, *some(g, rows, hidden, vocab))
+
+
+def test_long_sums_in_groups_of_tiles(cuda):
+    """So many rows that a unit of work has several column tiles; rows from everywhere against the reference."""
+    g = torch.Generator().manual_seed(9)
+    x, w, tokens = some(g, 20_000, 1040, 20_011)
+    got = head_logprobs(x.to(cuda), w.to(cuda), tokens.to(cuda))
+    rows = torch.cat([torch.arange(3), torch.randint(20_000, (60,), generator=g), torch.arange(19_990, 20_000)])
+    given, entropy, bounds = head_logprobs_ref(x[rows], w, tokens[rows])
+    assert_same(got.logprobs[rows.to(cuda)], given, bounds[0], "logprobs")
+    assert_same(got.entropy[rows.to(cuda)], entropy, bounds[1], "entropy")
+    assert _lib.read_status() == 0
+
+
+@pytest.mark.parametrize("rows,hidden", [(3, 64), (140, 8), (2, 1032)])
+def test_large_vocabularies(cuda, rows, hidden):
+    """The largest there is, and a ragged one: the last columns' tokens are scored too."""
+    g = torch.Generator().manual_seed(hidden)
+    for vocab in ((1 << 21, 151_643) if hidden < 1000 else (151_643,)):
+        x, w, tokens = some(g, rows, hidden, vocab)
+        tokens[0], tokens[1] = vocab - 1, 0
+        check(cuda, x, w, tokens)
