@@ -40,8 +40,9 @@ class Compaction(NamedTuple):
 
 
 def _host_of(caches):
-    first = next(iter(caches), None)
-    return _native(first) if isinstance(first, torch.Tensor) else _lib.host()
+    """The extension module, and the caches as a sequence (what can be gone through only once is)."""
+    caches = caches if isinstance(caches, (tuple, list)) else tuple(caches)
+    return _native(caches[0]) if caches and isinstance(caches[0], torch.Tensor) else _lib.host(), caches
 
 
 def copy_blocks(caches: Sequence[torch.Tensor], src_blocks: torch.Tensor, dst_blocks: torch.Tensor,
@@ -49,20 +50,22 @@ def copy_blocks(caches: Sequence[torch.Tensor], src_blocks: torch.Tensor, dst_bl
     """Block ``dst_blocks[i]`` becomes block ``src_blocks[i]`` (int32 ``[n]``) in all planes of all ``caches``, bit for bit, in one
     launch; with ``num_slots`` (int32 ``[n]``) only its first ``num_slots[i]`` slots, and the scales of their groups of 16.  Pairs with a
     negative block are left out (the padded size of a captured call).  A block that is copied to may be in no other pair."""
-    _host_of(caches).copy_blocks(caches, src_blocks, dst_blocks, num_slots)
+    host, caches = _host_of(caches)
+    host.copy_blocks(caches, src_blocks, dst_blocks, num_slots)
 
 
 def fork_sequences(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
                    free_blocks: torch.Tensor, out: Sequence[torch.Tensor] | None = None) -> Fork:
     """Sequences that go on from sequences of a batch: row ``i`` of the result is sequence ``parents[i]`` (int32 ``[rows]``) of
     ``block_tables`` (int32 ``[B, W]``) and ``seq_lens`` (int32 ``[B]``, tokens in the cache); a negative parent gives an empty row.  The
-    answers of a prompt, or the beams that survive a step.  Up to 4096 rows from up to 4096.
+    answers of a prompt, or the beams that survive a step.  1 to 4096 rows from up to 4096.
 
     Whole blocks are shared.  A begun last block stays with its parent's first new row; every other one gets a block of its own, the
     next of ``free_blocks`` (int32 ``[F]``, in order of the rows), with a copy of the slots in use.  More than there are shows in
     ``blocks_taken``; the rows without one have -1 in their tables.  Parents without a new row simply end: their blocks are free
     once the old tables are given up, not before.  One launch; the same call again leaves the same."""
-    return Fork._make(_host_of(caches).fork_sequences(caches, block_tables, seq_lens, parents, free_blocks, out))
+    host, caches = _host_of(caches)
+    return Fork._make(host.fork_sequences(caches, block_tables, seq_lens, parents, free_blocks, out))
 
 
 def free_list(block_tables: torch.Tensor, seq_lens: torch.Tensor, num_blocks: int, held: torch.Tensor | None = None,
@@ -80,4 +83,5 @@ def compact_blocks(caches: Sequence[torch.Tensor], block_tables: torch.Tensor, s
     with an id of ``n`` or more go to the free ids below ``n``, in order, contents and all.  The result's tables name the new ids
     (``out``'s may be ``block_tables`` themselves); what else names blocks (``held``, a prefix cache) goes by ``moved_to``.  Blocks that
     have been moved away keep their contents.  Two launches."""
-    return Compaction._make(_host_of(caches).compact_blocks(caches, block_tables, seq_lens, held, out))
+    host, caches = _host_of(caches)
+    return Compaction._make(host.compact_blocks(caches, block_tables, seq_lens, held, out))
