@@ -443,6 +443,7 @@ NVLLM_API int nvllm_sample_layout(int32_t batch, int32_t vocab, int64_t vocab_of
  * 1e30, one below 1e-38 as 1e-38.  -infinity in a row is a masked token; a row with a NaN, with +infinity or with nothing but
  * -infinity has NaN for results (its alternatives go by the logits, NaN like -infinity; subnormal logits order like 0).
  * 0 <= top <= NVLLM_LOGPROBS_MAX_TOP, vocab <= NVLLM_LOGPROBS_MAX_VOCAB (a head_logprobs call: rows <= 2^24, hidden <= 65536).
+ * The results lie apart from one another and from the logits; a row's result may replace its token or temperature (here and below).
  * No alignment beyond the element's is required; the rest of the 16-byte pieces that a row's first and last elements lie in may be
  * read.
  */

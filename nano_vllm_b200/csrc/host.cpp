@@ -24,6 +24,7 @@
 
 #include <atomic>
 #include <cstring>
+#include <initializer_list>
 #include <limits>
 #include <memory>
 #include <string>
@@ -923,6 +924,31 @@ void require_result(const char* name, const at::Tensor& t, at::ScalarType type, 
     raise(PyExc_RuntimeError, std::string(name) + " must be a contiguous CUDA " + c10::toString(type) + " tensor of the documented shape");
   require_on(name, t, like);
 }
+bool overlap(const at::Tensor& a, const at::Tensor& b) {  // of the memory between first and last elements
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  auto span = [](const at::Tensor& t) {
+    const char* p = static_cast<const char*>(t.data_ptr());
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    return std::pair<const char*, const char*>(p, p + (last + 1) * t.element_size());
+  };
+  const auto [a0, a1] = span(a);
+  const auto [b0, b1] = span(b);
+  return a0 < b1 && b0 < a1;
+}
+// Results lie on nothing that a call reads while it writes, nor on one another.
+void require_apart(const at::Tensor* out, int n, std::initializer_list<const at::Tensor*> in) {
+  for (int i = 0; i < n; ++i) {
+    for (int k = 0; k < i; ++k) require(!overlap(out[i], out[k]), "the results may not lie on one another");
+    for (const at::Tensor* t : in) require(!t || !overlap(out[i], *t), "the results may not lie on the arguments");
+  }
+}
+// What a row has one of may be replaced by the row's result.
+const at::Tensor* unless_in_place(const at::Tensor* t, const at::Tensor* out, int n) {
+  for (int i = 0; t && i < n; ++i)
+    if (out[i].data_ptr() == t->data_ptr() && out[i].numel() == t->numel() && out[i].element_size() == t->element_size()) return nullptr;
+  return t;
+}
 const float* row_temperatures(const at::Tensor* t, int64_t rows, const at::Tensor& like) {
   if (!t) return nullptr;
   if (!t->is_cuda() || t->scalar_type() != at::kFloat || !t->is_contiguous())
@@ -967,6 +993,7 @@ PyObject* token_logprobs(PyObject* const* a) {
       const int64_t shape[2] = {rows, top};
       require_result(of[i], out[i], i == 2 ? at::kLong : at::kFloat, at::IntArrayRef(shape, i < 2 ? 1 : 2), logits);
     }
+    require_apart(out, 4, {&logits, unless_in_place(&tokens, out, 4), unless_in_place(temps, out, 4)});
   }
   const c10::cuda::CUDAGuard guard(logits.device());
   launch([&] {
@@ -1008,6 +1035,7 @@ PyObject* head_logprobs(PyObject* const* a) {
     const char* const of[2] = {"logprobs", "entropy"};
     results(a[4], 2, "out must be the two tensors of an earlier call", out, of);
     for (int i = 0; i < 2; ++i) require_result(of[i], out[i], at::kFloat, {rows}, x);
+    require_apart(out, 2, {&x, &w, unless_in_place(&tokens, out, 2), unless_in_place(temps, out, 2)});
   }
   auto stride = [&](const at::Tensor& m) { return m.size(0) > 1 ? m.stride(0) : (hidden + 7) / 8 * 8; };
   launch([&] {
@@ -1083,17 +1111,6 @@ Tables require_tables(const at::Tensor& table, const at::Tensor& lens, const at:
   return {table.size(0), table.size(1)};
 }
 int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::max(t.stride(0), t.size(1)); }
-bool overlap(const at::Tensor& a, const at::Tensor& b) {  // of the memory between first and last elements
-  auto span = [](const at::Tensor& t) {
-    const char* p = static_cast<const char*>(t.data_ptr());
-    int64_t last = 0;
-    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
-    return std::pair<const char*, const char*>(p, t.numel() ? p + (last + 1) * t.element_size() : p);
-  };
-  const auto [a0, a1] = span(a);
-  const auto [b0, b1] = span(b);
-  return a0 < b1 && b0 < a1;
-}
 
 PyObject* copy_blocks(PyObject* const* a) {  // caches, src_blocks, dst_blocks, num_slots
   const Cache c = cache_parts(a[0]);
@@ -1136,8 +1153,7 @@ PyObject* fork_sequences(PyObject* const* a) {  // caches, block_tables, seq_len
     require(out[0].dim() == 2 && out[0].size(0) == rows && out[0].size(1) == t.width, "out's block_tables is [rows, blocks]");
     require_i32_on("out's seq_lens", out[1], rows, c.like);
     require_i32_on("out's blocks_taken", out[2], 1, c.like);
-    for (const at::Tensor& o : out)
-      for (const at::Tensor* in : {&table, &lens, &parents, &free}) require(!overlap(o, *in), "the results may not lie on the arguments");
+    require_apart(out, 3, {&table, &lens, &parents, &free});
   }
   const c10::cuda::CUDAGuard guard(c.like.device());
   launch([&] {
@@ -1169,6 +1185,7 @@ PyObject* free_list(PyObject* const* a) {  // block_tables, seq_lens, num_blocks
     const char* const of[3] = {"ref_counts", "free_blocks", "num_free"};
     results(a[4], 3, "out must be the three tensors of an earlier call", out, of);
     for (int i = 0; i < 3; ++i) require_i32_on(of[i], out[i], i < 2 ? blocks : 1, table);
+    require_apart(out, 3, {});  // all arguments have been read before the first is written
   }
   const c10::cuda::CUDAGuard guard(table.device());
   launch([&] {
@@ -1205,10 +1222,8 @@ PyObject* compact_blocks(PyObject* const* a) {  // caches, block_tables, seq_len
     require(out[0].dim() == 2 && out[0].size(0) == t.batch && out[0].size(1) == t.width, "out's block_tables is [sequences, blocks]");
     require_i32_on("out's moved_to", out[1], c.blocks, c.like);
     require_i32_on("out's num_live", out[2], 1, c.like);
-    const bool same = out[0].data_ptr() == table.data_ptr() && row_stride(out[0]) == row_stride(table);
-    require(same || !overlap(out[0], table), "out's block_tables is the tables themselves or lies elsewhere");
-    for (const at::Tensor& o : out)
-      for (const at::Tensor* in : {&lens, held}) require(!in || !overlap(o, *in), "the results may not lie on the arguments");
+    const bool same = out[0].data_ptr() == table.data_ptr() && row_stride(out[0]) == row_stride(table);  // or elsewhere
+    require_apart(out, 3, {&lens, held, same ? nullptr : &table});
     for (int i = 1; i < 3; ++i) require(!overlap(out[i], table), "the results may not lie on the arguments");
   }
   const c10::cuda::CUDAGuard guard(c.like.device());

@@ -33,7 +33,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: int = 0, tem
     asks for none: 0 (rows of a padded batch); one beyond the vocabulary gives NaN and sets bit 8 of ``_lib.read_status()``.
     Logits of -infinity are masked tokens.  A row with a NaN, with +infinity or with nothing but -infinity has no distribution and
     NaN for results; its ``top_tokens`` go by the logits, NaN like -infinity.
-    ``out``: the four result tensors of an earlier call or of a graph, else they are made."""
+    ``out``: the four result tensors of an earlier call or of a graph, else they are made.  They lie apart from one another and from
+    the logits; ``tokens`` and ``temperatures`` may be results' own places (one alternative for each token)."""
     return TokenLogprobs._make(_native(logits).token_logprobs(logits, tokens, top, temperatures, out))
 
 
