@@ -152,3 +152,34 @@ def test_answers_of_prompts_over_a_cache_in_8_bits(cuda, prompts, each):
             c = pages.compact_blocks(caches, tables, now)
             tables = c.block_tables
     assert _lib.read_status() == 0
+
+
+def test_beams_stay_apart(cuda):
+    """What each beam has, read from the cache, and the token chosen for it: no two are the same, as no two (parent, token) pairs are."""
+    model, beams = Model(cuda), 6
+    kv = torch.zeros(2, LAYERS, BLOCKS, 256, HKV, D, dtype=torch.bfloat16, device=cuda)
+    g = torch.Generator().manual_seed(3)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    prompt = torch.randint(VOCAB, (251,), generator=g).to(cuda)
+    tables, lens, tokens, scores = torch.full((1, 3), -1, dtype=torch.int32, device=cuda), i32([0]), prompt[-1:], torch.zeros(1, device=cuda)
+    m = step_maps(i32([250]), lens, tables, pages.free_list(tables, lens, BLOCKS).free_blocks, 250)
+    store(model, kv, prompt[:-1], m.slot_mapping)
+    lens = i32([250])
+    ids = {tuple(row): t for t, row in enumerate(model.k[0, :, 0, :8].view(torch.int16).tolist())}
+    assert len(ids) == VOCAB  # a token's key tells which it is
+    for step in range(9):
+        m = step_maps(lens + 1, lens, tables, pages.free_list(tables, lens, BLOCKS).free_blocks, len(tokens))
+        store(model, kv, tokens, m.slot_mapping)
+        lens = lens + 1
+        best = token_logprobs(model.hidden(tokens, kv, lens, tables) @ model.head.T, tokens, 2 * beams)
+        scores, which = torch.topk((scores[:, None] + best.top_logprobs).flatten(), beams)
+        parents, tokens = which // (2 * beams), best.top_tokens.flatten()[which]
+        f = pages.fork_sequences((kv,), tables, lens, parents.to(torch.int32), pages.free_list(tables, lens, BLOCKS).free_blocks)
+        tables, lens = f.block_tables, f.seq_lens
+        paths = set()
+        for row, n, token in zip(tables.tolist(), lens.tolist(), tokens.tolist()):
+            at = torch.tensor([row[t // 256] * 256 + t % 256 for t in range(n)], device=cuda)
+            had = [ids[tuple(k)] for k in kv[0, 0].view(-1, HKV, D)[at, 0, :8].view(torch.int16).tolist()]
+            assert had[:251] == prompt.tolist()
+            paths.add((*had, token))
+        assert len(paths) == beams, f"step {step}"
