@@ -674,10 +674,12 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   while (csize > 1 && (static_cast<int64_t>(rows) * csize > 4ll * sms || pieces < 2ll * csize * kLpThreads)) csize /= 2;
   while (csize == 1 && threads > 64 && pieces < 8ll * threads && std::min<int64_t>(2 * top, pieces) <= threads / 2) threads /= 2;
   const int all = csize * threads;
-  // Groups: enough of them that the bound lies close to the last alternative, counted against one another (64 rows with 32 alternatives
-  // in 128 groups 16.0 us, in 64 17.8; with 20 alternatives 32 and 128 groups are the same in a row's own block and 0.2 us better).
-  p.groups = top <= 20 ? std::max(32, all / 32) : std::min(kLpGroups, all);
-  while (p.groups < std::min(kLpGroups, all) && pieces * p.groups < static_cast<int64_t>(top) * all) p.groups *= 2;
+  // Groups: 2.5 for each alternative, so that the bound lies close to the last one; more take longer to be counted against one another.
+  // In 32, 64 and 128 groups: 250 rows of 151643 with 5 alternatives 24.4, 24.6, 25.5 us, 12 25.8, 25.9, 26.8, 16 27.1, 26.7, 27.3, 24 30.9,
+  // 28.5, 28.8, 40 -, 29.6, 29.3; 2000 of 32000 with 12 44.1, 43.3, 46.1, 24 55.3, 50.4, 51.8, 32 68, 56.2, 57.1, 40 -, 63.4, 60.1; a cluster's 64
+  // and 128: 64 fp32 rows with 24 15.3, 15.4, 32 16.6, 15.9.  And as many pieces to a group as there are alternatives to be told apart.
+  p.groups = std::max(32, all / 32);
+  while (p.groups < std::min(kLpGroups, all) && (2 * p.groups < 5 * top || pieces * p.groups < static_cast<int64_t>(top) * all)) p.groups *= 2;
   auto log2_of = [](int n) {
     int l = 0;
     while (n >> (l + 1)) ++l;
