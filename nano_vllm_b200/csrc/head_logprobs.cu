@@ -8,15 +8,16 @@
 // loss: at H = 4096 logits come out 3.2e-6 too small, log probabilities 2e-6 off.  Two things are done about it.  A product is cut
 // after kChunk elements and the parts are added in registers.  And the logits' scale makes good what a step loses on average
 // (kStepLoss, half a last place of a sum that is still on its way, measured at 64 to 5120 elements, products of either sign and of
-// one): at H = 1024 logits are 1.0e-6 off on average without, 5e-8 with it, log probabilities 4.6e-7 and 1.9e-7, the entropy 8.4e-7 and
-// 1.2e-7 (relative, 512 rows of 151936); at 4096 4.6e-7 and 1.7e-7, 9.1e-7 and 1.5e-7; fp32 sums without a tensor core are 1.9e-7 off
-// at 1024.  Sums that lose nothing, such as those of one product, come out too large by what is made good: 9.5e-7 of a difference
+// one): at H = 1024 logits are 1.0e-6 off on average without, 5e-8 with it, log probabilities 4.6e-7 and 1.9e-7, the entropy 8.4e-7
+// and 1.2e-7 (relative, 512 rows of 151936); at 4096 4.6e-7 and 1.7e-7, 9.1e-7 and 1.5e-7; fp32 sums without a tensor core are 1.9e-7
+// off at 1024.  Sums that lose nothing, such as those of one product, come out too large by what is made good: 9.5e-7 of a difference
 // of logits at the most.  Parts of 512 elements would halve the loss too, at 1.28 times the time for 4096 x 1024 x 151936.
 //
-// What bounds it.  Many rows: the tensor cores, and then the power cap (4096 x 1024 x 151936 803 us, 1590 TFLOP/s, 908 in a long chain; 1000 x
-// 4096 830-870; blocks of 128 rows by themselves, which feed the tensor cores twice the bytes, 1306 and 1248).  H below some 900: the reduction
-// of a tile (4096 x 512 490 us of 393; tiles shared out evenly to the warps the same; 16 warps instead of 8 made 77 x 896 47.6 instead of 45.9).  Up to 128 rows: the weights' stream (one row of 1024
-// 53.5 us, 5.8 TB/s; of 4096 197.6, 6.3), with as many stages as fit on their way (four: 54.8 and 200.8).
+// What bounds it.  Many rows: the tensor cores, and then the power cap (4096 x 1024 x 151936 803 us, 1590 TFLOP/s, 908 in a long chain;
+// 1000 x 4096 830-870; blocks of 128 rows by themselves, which feed the tensor cores twice the bytes, 1306 and 1248).  H below some
+// 900: the reduction of a tile (4096 x 512 490 us of 393; tiles shared out evenly to the warps the same; 16 warps instead of 8 made
+// 77 x 896 47.6 instead of 45.9).  Up to 128 rows: the weights' stream (one row of 1024 53.5 us, 5.8 TB/s; of 4096 197.6, 6.3), with as
+// many stages as fit on their way (four: 54.8 and 200.8).
 #include <algorithm>
 #include <atomic>
 
@@ -132,7 +133,8 @@ __device__ __forceinline__ Unit unit_of(const Params& p, int i) {
 }
 
 template <bool PAIR, bool LONG>
-__global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1) head_logprobs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
+__global__ void __launch_bounds__(Cfg<PAIR, LONG>::THREADS, 1)
+    head_logprobs_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const Params p) {
   using G = Cfg<PAIR, LONG>;
   constexpr int WARPS = G::WARPS, COLS = G::COLS, CTAS = PAIR ? 2 : 1;
   const int a_bytes = p.a_rows * BK * 2, stage_bytes = a_bytes + p.bn / CTAS * BK * 2, nst = p.nst;

@@ -9,18 +9,20 @@
 //
 // Alternatives without a second pass: a thread keeps the largest of its 16-byte pieces' maxima and the first piece that has it.
 // Of 32 to 128 groups of threads the top-th largest (maximum, piece) is a bound that `top` elements reach, so every alternative lies
-// in a thread whose own (maximum, piece) reaches it: about `top` threads, whose pieces are read again (from L2) and compared
-// with the bound; where those are many, a thread keeps these two for each segment of its pieces.  Pieces break ties of values, and where many threads tie (a mask that leaves fewer than `top`) a block finds a closer
-// bound among its own threads, counting the ties within their pieces.  Where more elements reach the bound than the list holds (largest
+// in a thread whose own (maximum, piece) reaches it: about `top` threads, whose pieces are read again and compared with the bound
+// (from L2 where the rows in flight fit in it; rows of 300 KB on every place of the device do not, and half of every sector of 32
+// bytes that comes again from memory is for nothing).  Where those pieces are many, a thread keeps its largest for each segment of
+// them.  Pieces break ties of values, and where many threads tie (a mask that leaves fewer than `top`) a block finds a closer bound
+// among its own threads, counting the ties within their pieces.  Where more elements reach the bound than the list holds (largest
 // ones that stand close together), each block keeps its own top ones.
 //
 // A row is read by a cluster of 1 to 8 blocks, four to a multiprocessor.
 //
-// What bounds it: 8 cycles of the unit for exponentials and about 7 issue slots an element and scheduler, beside 11 cycles of memory: of
-// 4096 rows of 151936 bf16 the loads alone take 181 us, the pass 205-225, with one alternative 218 (5.7 TB/s).  250 rows: 15.1, 20.8, with
-// five 24.5 (500 blocks on 592 places).  One row with 20 alternatives: 7.3, of which the end 3: bound 0.4, listed threads' pieces 1.7,
-// ranks and results 0.9, each a chain of short steps.  Rows of which a mask leaves 4 tokens, 20 alternatives: one 10.9, 64 23 (12.6 without a
-// mask), 250 33 (28.6); 64 alternatives: 2000 rows of 1000 28.
+// What bounds it: 8 cycles of the unit for exponentials and about 7 issue slots an element and scheduler, beside 11 cycles of
+// memory: of 4096 rows of 151936 bf16 the loads alone take 181 us, the pass 205-225, with one alternative 218 (5.7 TB/s; called one by
+// one 254).  250 rows: 15.1, 20.8, with five 24.4 (500 blocks on 592 places).  One row with 20 alternatives: 7.4, of which the end 3:
+// bound 0.4, listed threads' pieces 1.7, ranks and results 0.9, each a chain of short steps.  Rows of which a mask leaves 4 tokens,
+// 20 alternatives: one 10.3, 64 23 (13 without a mask), 250 28 (27.5); 64 alternatives: 2000 rows of 1000 26 (24).
 #include <cooperative_groups.h>
 
 #include <algorithm>
