@@ -691,7 +691,7 @@ extern "C" int nvllm_token_logprobs(const void* logits, int32_t logits_are_fp32,
   p.log_all = log2_of(all);
   p.log_size = log2_of(all / p.groups);
   // Segments of a thread's pieces, so that some and not all pieces of a listed thread are read again: where those would be more than two for
-  // each thread, of 32 or more (4096 rows of 151936 with 20 alternatives 320 us, in segments 280; with five 231 and 261; 300 rows with 64 76 and 47;
+  // each thread, of 32 or more (4096 rows of 151936 with 20 alternatives 320 us, in segments 272; with five 231 and 261; 300 rows with 64 76 and 47;
   // 1003 fp32 rows with 64 219 and 147).  The pass itself takes 218 us without and 250 with them.
   const int64_t each = (pieces + all) / all, steps = each / kLpStep<true> + 1;
   const bool parted = each >= 32 && top * each > 2 * all;
